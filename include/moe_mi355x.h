@@ -592,6 +592,92 @@ int moe_gather_rows(const void* src, int64_t n_src_rows, const int64_t* idx, int
 int moe_scatter_rows(const void* src, const int64_t* idx, int64_t n_rows, int32_t dim, int32_t dtype, void* dst,
                      int64_t n_dst_rows, moe_stream_t stream);
 
+/* ---------------------------------------------------------------------------
+ * bf16 experts whose activations are kept for the backward in MXFP8: e4m3
+ * elements, one e8m0 scale byte per 32 along the row, k + 127 with the least k in
+ * [-127, 127] for which max |x| <= 448 * 2^k (-127 for a block of zeros), 255
+ * for a block with an infinity or a NaN, whose values are then all NaN.
+ * ------------------------------------------------------------------------- */
+
+/* moe_grouped_gemm_gate_up with g and u, quantized from their fp32 sums, in g8,
+ * u8 [R,H] and their scales [R,H/32] instead of in bf16; h is the same. */
+int moe_grouped_gemm_gate_up_keep8(const uint16_t* x, const uint16_t* w1, const uint16_t* w3,
+                                   const int64_t* counts, int64_t n_rows, int32_t n_experts, int32_t dim,
+                                   int32_t hidden, uint8_t* g8, uint8_t* g8_scale, uint8_t* u8,
+                                   uint8_t* u8_scale, uint16_t* h, moe_stream_t stream);
+
+/* moe_grouped_gemm_bwd_dgu from the kept g and u, in fp32 between dh = dy.w2 and
+ * the rounding of dgu; h [R,H] = bf16(silu(g) * u) of the kept values for
+ * moe_grouped_gemm_bwd_dw2 (NULL: not written). */
+int moe_grouped_gemm_bwd_dgu_keep8(const uint16_t* dy, const uint16_t* w2, const uint8_t* g8,
+                                   const uint8_t* g8_scale, const uint8_t* u8, const uint8_t* u8_scale,
+                                   const int64_t* counts, int64_t n_rows, int32_t n_experts, int32_t dim,
+                                   int32_t hidden, uint16_t* dgu, uint16_t* h, moe_stream_t stream);
+
+/* x [rows, cols] bf16 (cols % 32 == 0) -> q [rows, cols], scale [rows, cols / 32],
+ * and back. */
+int moe_keep8_rows(const uint16_t* x, int64_t rows, int32_t cols, uint8_t* q, uint8_t* scale, moe_stream_t stream);
+int moe_restore8_rows(const uint8_t* q, const uint8_t* scale, int64_t rows, int32_t cols, uint16_t* x,
+                      moe_stream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * MXFP4 experts: e2m1 elements, two per byte along the contraction (the first in
+ * the low half), one e8m0 scale byte per 32: k + 127 with the least k in
+ * [-127, 127] for which max |x| <= 6 * 2^k (-127 for a block of zeros), 255
+ * for a block with an infinity or a NaN, whose values are then all NaN; elements
+ * x * 2^-k rounded to nearest, ties to the even code. Products accumulate in
+ * fp32 with both scales applied in the MFMA. D and H multiples of 32, E <= 1024;
+ * all pointers but the counts 16-byte aligned.
+ * ------------------------------------------------------------------------- */
+
+/* x [rows, cols] (dtype MOE_DTYPE_BF16 or MOE_DTYPE_FP32, cols % 32 == 0) ->
+ * q [rows, cols / 2], scale: row r's cols / 32 bytes at scale + r * scale_ld. */
+int moe_mxfp4_quant_rows(const void* x, int64_t rows, int32_t cols, int32_t dtype, int32_t scale_ld,
+                         uint8_t* q, uint8_t* scale, moe_stream_t stream);
+
+/* The values back: q [rows, cols / 2], row r's scales at scale + r * scale_ld ->
+ * x [rows, cols]; values past the dtype's range become infinities. */
+int moe_mxfp4_dequant_rows(const uint8_t* q, const uint8_t* scale, int64_t rows, int32_t cols,
+                           int32_t scale_ld, int32_t dtype, void* x, moe_stream_t stream);
+
+/* The row stride of the scales that the products' row operands take: cols / 32
+ * rounded up to 8 (weights' scales are dense). */
+int moe_mxfp4_scale_ld(int32_t cols);
+
+/* Bytes of workspace of moe_mxfp4_swiglu_fwd and moe_mxfp4_oss_fwd. */
+int64_t moe_mxfp4_workspace_bytes(int64_t n_rows, int32_t dim, int32_t hidden);
+
+/* The experts' forward on packed weights: x [R,D] bf16 in expert order, counts
+ * [E]; qw1, qw3 [E,H,D/2], qw2 [E,D,H/2] with scales [E,H,D/32], [E,D,H/32]:
+ * h = MXFP4(silu(xq.w1^T) * (xq.w3^T)), y = bf16(h.w2^T) [R,D]; rows past
+ * sum(counts) are zero. x is quantized on the way. */
+int moe_mxfp4_swiglu_fwd(const uint16_t* x, const uint8_t* qw1, const uint8_t* sw1, const uint8_t* qw2,
+                         const uint8_t* sw2, const uint8_t* qw3, const uint8_t* sw3, const int64_t* counts,
+                         int64_t n_rows, int32_t n_experts, int32_t dim, int32_t hidden, uint8_t* workspace,
+                         int64_t workspace_bytes, uint16_t* y, moe_stream_t stream);
+
+/* The same with gpt-oss's experts (gpt_oss/moe.py:43-122): qmlp1 [E,2H,D/2] (glu
+ * row 2j, linear row 2j + 1), biases bf16 [E,2H] and [E,D], all in fp32 between
+ * the products: g = min(glu + b, L), u = clamp(linear + b, -L, L),
+ * h = MXFP4(g * sigmoid(1.702 g) * (u + 1)), y = bf16(h.mlp2^T + b2). */
+int moe_mxfp4_oss_fwd(const uint16_t* x, const uint8_t* qmlp1, const uint8_t* smlp1, const uint16_t* mlp1_bias,
+                      const uint8_t* qmlp2, const uint8_t* smlp2, const uint16_t* mlp2_bias,
+                      const int64_t* counts, int64_t n_rows, int32_t n_experts, int32_t dim, int32_t hidden,
+                      float swiglu_limit, uint8_t* workspace, int64_t workspace_bytes, uint16_t* y,
+                      moe_stream_t stream);
+
+/* The training step's products, one launch each. gate_up_keep: qx [R,D/2] with
+ * scales of stride moe_mxfp4_scale_ld(D) -> qh [R,H/2] with scales of stride
+ * moe_mxfp4_scale_ld(H), and g, u in MXFP8 [R,H] with scales [R,H/32]. Rows past
+ * sum(counts) are left alone; down zeroes them in y. */
+int moe_mxfp4_gemm_gate_up_keep(const uint8_t* qx, const uint8_t* sx, const uint8_t* qw1, const uint8_t* sw1,
+                                const uint8_t* qw3, const uint8_t* sw3, const int64_t* counts, int64_t n_rows,
+                                int32_t n_experts, int32_t dim, int32_t hidden, uint8_t* qh, uint8_t* sh,
+                                uint8_t* g8, uint8_t* gs, uint8_t* u8, uint8_t* us, moe_stream_t stream);
+int moe_mxfp4_gemm_down(const uint8_t* qh, const uint8_t* sh, const uint8_t* qw2, const uint8_t* sw2,
+                        const int64_t* counts, int64_t n_rows, int32_t n_experts, int32_t dim, int32_t hidden,
+                        uint16_t* y, moe_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

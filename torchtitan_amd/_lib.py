@@ -91,6 +91,18 @@ SIGNATURES: dict[str, list] = {
     "moe_mxfp8_gemm_bwd_dx": [P, P, P, P, P, I64, I32, I32, I32, P, P],
     "moe_mxfp8_gemm_bwd_dw13": [P, P, P, P, P, I64, I64, I32, I32, I32, P, P, P],
     "moe_mxfp8_gemm_bwd_dw2": [P, P, P, P, P, I64, I64, I32, I32, I32, P, P],
+    "moe_grouped_gemm_gate_up_keep8": [P, P, P, P, I64, I32, I32, I32, P, P, P, P, P, P],
+    "moe_grouped_gemm_bwd_dgu_keep8": [P, P, P, P, P, P, P, I64, I32, I32, I32, P, P, P],
+    "moe_keep8_rows": [P, I64, I32, P, P, P],
+    "moe_restore8_rows": [P, P, I64, I32, P, P],
+    "moe_mxfp4_quant_rows": [P, I64, I32, I32, I32, P, P, P],
+    "moe_mxfp4_dequant_rows": [P, P, I64, I32, I32, I32, P, P],
+    "moe_mxfp4_scale_ld": [I32],
+    "moe_mxfp4_workspace_bytes": [I64, I32, I32],
+    "moe_mxfp4_swiglu_fwd": [P, P, P, P, P, P, P, P, I64, I32, I32, I32, P, I64, P, P],
+    "moe_mxfp4_oss_fwd": [P, P, P, P, P, P, P, P, I64, I32, I32, I32, F32, P, I64, P, P],
+    "moe_mxfp4_gemm_gate_up_keep": [P, P, P, P, P, P, P, I64, I32, I32, I32, P, P, P, P, P, P, P],
+    "moe_mxfp4_gemm_down": [P, P, P, P, P, I64, I32, I32, I32, P, P],
     "moe_expert_bias_update": [P, P, P, P, I32, I32, P],
     "moe_ep_permute_indices": [P, I32, I32, I64, P, P, P],
     "moe_ep_permute_pad_indices": [P, I32, I32, I32, I64, P, P, P, P],
@@ -98,7 +110,7 @@ SIGNATURES: dict[str, list] = {
     "moe_scatter_rows": [P, P, I64, I32, I32, P, I64, P],
 }
 _RESTYPES = {"moe_reorder_workspace_bytes": ctypes.c_int64, "moe_fp8_padded_rows": ctypes.c_int64,
-             "moe_mxfp8_padded_rows": ctypes.c_int64}
+             "moe_mxfp8_padded_rows": ctypes.c_int64, "moe_mxfp4_workspace_bytes": ctypes.c_int64}
 
 _ERRORS = {
     -1: "invalid argument",

@@ -57,7 +57,7 @@
 #include <type_traits>
 
 #include "common.h"
-
+#include "mx.h"
 
 namespace moe {
 
@@ -106,11 +106,22 @@ struct GemmParams {
   const uint16_t* b2;  // mlp2_bias [E, D] bf16
   float limit;         // swiglu_limit as bf16
   float alpha;         // 1.702
+  // the activations kept in 8 bits: g and u [R, H] e4m3 and their scales [R, H / 32],
+  // written by gate_up, read by dgu
+  uint8_t* g8;
+  uint8_t* g8s;
+  uint8_t* u8;
+  uint8_t* u8s;
 };
 
 // Expert epilogue variants: the SwiGLU of moe.py:53-70 and gpt-oss's biased,
-// clamped SwiGLU with interleaved mlp1 rows (gpt_oss/moe.py:43-52, 92-122).
-enum ExpertAct : int { kSwiGLU = 0, kOssGLU = 1 };
+// clamped SwiGLU with interleaved mlp1 rows (gpt_oss/moe.py:43-52, 92-122), and the SwiGLU
+// whose g and u are kept for the backward in MXFP8 instead of bf16: gate_up writes the same
+// h, bit for bit, and quantizes g and u from the fp32 sums (a rounding to bf16 before it
+// would move 3 % of the e4m3 roundings to a neighbour); dgu reads them back, computes in fp32
+// with one rounding per output, and writes h = silu(g) u of the kept values beside dgu, which
+// dw2 multiplies (keeping h too would be half as many bytes again).
+enum ExpertAct : int { kSwiGLU = 0, kOssGLU = 1, kSwiGLUKeep8 = 2 };
 
 // gpt-oss activation on pairs of bf16 values g (glu), u (linear), every op rounded to
 // bf16 as the reference's bf16 tensor ops: xg = clamp(g, max=L), xl = clamp(u, -L, L),
@@ -691,13 +702,33 @@ __global__ __launch_bounds__(NW * 64, OCC) void grouped_gemm_kernel(GemmParams p
                         sh = span64(ph[0], ph[1], lane);
             if (TAIL && hc >= H) continue;
             const int64_t off = (int64_t)r * H + hc;
-            *(uint4*)(p.out_g + off) = sg;
-            *(uint4*)(p.out_u + off) = su;
             *(uint4*)(p.out_h + off) = sh;
+            if constexpr (ACT == kSwiGLUKeep8) {
+              float ga[4], gb[4], ua[4], ub[4];
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                ga[q] = acc[i][4 * jp][q];
+                ua[q] = acc[i][4 * jp + 1][q];
+                gb[q] = acc[i][4 * jp + 2][q];
+                ub[q] = acc[i][4 * jp + 3][q];
+              }
+              uint2 qg, qu;
+              const uint32_t eg = mx::block8(ga, gb, qg), eu = mx::block8(ua, ub, qu);
+              *(uint2*)(p.g8 + off) = qg;
+              *(uint2*)(p.u8 + off) = qu;
+              if (g8 == 0) {
+                const int64_t so = (int64_t)r * (H / 32) + hc / 32;
+                p.g8s[so] = (uint8_t)eg;
+                p.u8s[so] = (uint8_t)eu;
+              }
+            } else {
+              *(uint4*)(p.out_g + off) = sg;
+              *(uint4*)(p.out_u + off) = su;
+            }
           }
         };
         if (r < seg1) {
-          if constexpr (ACT == kSwiGLU) {
+          if constexpr (ACT != kOssGLU) {
             // the range of the block's gate values, taken before their rounding to
             // bf16, which keeps them inside it
             float g_min = acc[i][0][0], g_max = acc[i][0][0];
@@ -771,6 +802,58 @@ __global__ __launch_bounds__(NW * 64, OCC) void grouped_gemm_kernel(GemmParams p
             const uint4 sv = span64(pv[0], pv[1], lane);
             if (TAIL && n >= D) continue;
             *(uint4*)(outp + (int64_t)r * D + n) = sv;
+          }
+        }
+      }
+    } else if constexpr (MODE == kBwdDgu && ACT == kSwiGLUKeep8) {
+      // s = sigmoid(g): du = dh g s, dg = dh u s (1 + g (1 - s)), h = g s u, from the kept
+      // values and the fp32 dh, each in the accumulators' layout; a block's four lanes share
+      // its scales. Loaded per 16 rows before the stores, as below.
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        const int r = row0 + wm * WM + i * 16 + ml;
+        uint32_t gq[TN], uq[TN];
+        float gsc[TN / 2], usc[TN / 2];
+        if (r < seg1) {
+#pragma unroll
+          for (int j = 0; j < TN; ++j) {
+            const int hh = nt * BN + wn * WN + j * 16 + nq;
+            if (TAIL && hh >= H) continue;
+            gq[j] = *(const uint32_t*)(p.g8 + (int64_t)r * H + hh);
+            uq[j] = *(const uint32_t*)(p.u8 + (int64_t)r * H + hh);
+            if (j % 2 == 0) {
+              gsc[j / 2] = mx::scale_value(p.g8s[(int64_t)r * (H / 32) + hh / 32]);
+              usc[j / 2] = mx::scale_value(p.u8s[(int64_t)r * (H / 32) + hh / 32]);
+            }
+          }
+#pragma unroll
+          for (int jp = 0; jp < TN / 2; ++jp) {
+            const int hh = nt * BN + wn * WN + jp * 32 + g8;
+            if (TAIL && hh >= H) continue;
+            uint2 pg[2], pu[2], ph[2];
+#pragma unroll
+            for (int h2 = 0; h2 < 2; ++h2) {
+              const int j = 2 * jp + h2;
+              float g[4], u[4], dg[4], du[4], h[4];
+              mx::from_e4m3x4(gq[j], gsc[jp], g);
+              mx::from_e4m3x4(uq[j], usc[jp], u);
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                const float dh = acc[i][j][q], sg = mx::sigmoid(g[q]), sl = g[q] * sg;
+                h[q] = sl * u[q];
+                du[q] = dh * sl;
+                dg[q] = dh * u[q] * sg * (1.0f + g[q] * (1.0f - sg));
+              }
+              pg[h2] = pack4(dg);
+              pu[h2] = pack4(du);
+              ph[h2] = pack4(h);
+            }
+            const uint4 sdg = span64(pg[0], pg[1], lane), sdu = span64(pu[0], pu[1], lane),
+                        sh = span64(ph[0], ph[1], lane);
+            const int64_t o2 = (int64_t)r * (2 * H) + hh;
+            *(uint4*)(p.out_dgu + o2) = sdg;
+            *(uint4*)(p.out_dgu + o2 + H) = sdu;
+            if (p.out_h) *(uint4*)(p.out_h + (int64_t)r * H + hh) = sh;
           }
         }
       }
@@ -1095,6 +1178,37 @@ MOE_API int moe_grouped_gemm_gate_up(const uint16_t* x, const uint16_t* w1, cons
   if (!x || !w1 || !w3 || !g || !u || !h) return kErrInvalidArgument;
   p.x = x; p.w1 = w1; p.w3 = w3; p.out_g = g; p.out_u = u; p.out_h = h;
   launch_mode<kFwdGateUp>(p, n_rows, stream);
+  return launch_status();
+}
+
+MOE_API int moe_grouped_gemm_gate_up_keep8(const uint16_t* x, const uint16_t* w1, const uint16_t* w3,
+                                           const int64_t* counts, int64_t n_rows, int32_t n_experts, int32_t dim,
+                                           int32_t hidden, uint8_t* g8, uint8_t* g8_scale, uint8_t* u8,
+                                           uint8_t* u8_scale, uint16_t* h, hipStream_t stream) {
+  GemmParams p;
+  int st = gemm_params(p, counts, n_rows, n_experts, dim, hidden);
+  if (st) return st;
+  if (n_rows == 0) return kOk;
+  if (!x || !w1 || !w3 || !g8 || !g8_scale || !u8 || !u8_scale || !h) return kErrInvalidArgument;
+  p.x = x; p.w1 = w1; p.w3 = w3; p.out_h = h;
+  p.g8 = g8; p.g8s = g8_scale; p.u8 = u8; p.u8s = u8_scale;
+  launch_mode<kFwdGateUp, kSwiGLUKeep8>(p, n_rows, stream);
+  return launch_status();
+}
+
+MOE_API int moe_grouped_gemm_bwd_dgu_keep8(const uint16_t* dy, const uint16_t* w2, const uint8_t* g8,
+                                           const uint8_t* g8_scale, const uint8_t* u8, const uint8_t* u8_scale,
+                                           const int64_t* counts, int64_t n_rows, int32_t n_experts, int32_t dim,
+                                           int32_t hidden, uint16_t* dgu, uint16_t* h, hipStream_t stream) {
+  GemmParams p;
+  int st = gemm_params(p, counts, n_rows, n_experts, dim, hidden);
+  if (st) return st;
+  if (n_rows == 0) return kOk;
+  if (!dy || !w2 || !g8 || !g8_scale || !u8 || !u8_scale || !dgu) return kErrInvalidArgument;
+  p.dy = dy; p.w2 = w2; p.out_dgu = dgu; p.out_h = h;
+  p.g8 = const_cast<uint8_t*>(g8); p.g8s = const_cast<uint8_t*>(g8_scale);
+  p.u8 = const_cast<uint8_t*>(u8); p.u8s = const_cast<uint8_t*>(u8_scale);
+  launch_mode<kBwdDgu, kSwiGLUKeep8>(p, n_rows, stream);
   return launch_status();
 }
 

@@ -13,6 +13,8 @@ when the library is missing.
 
 from __future__ import annotations
 
+from contextlib import nullcontext
+
 import torch
 from torch import Tensor
 
@@ -23,6 +25,7 @@ SCORE_FUNCS = {"softmax": 0, "sigmoid": 1}
 # and K <= 64, the histogram and reorder K <= 32 (and E <= 1024).
 MAX_EXPERTS = 512
 MAX_TOP_K = 32
+MAX_GEMM_EXPERTS = 1024  # of the grouped GEMMs
 DTYPE_CODES = {torch.bfloat16: 0, torch.float32: 1}
 
 # Gradient of x[token_idx] accumulates a token's K rows with a rounding to the
@@ -1147,6 +1150,451 @@ def _gsmx_bwd(ctx, dy, *_unused):
 
 
 grouped_swiglu_mxfp8.register_autograd(_gsmx_bwd, setup_context=_gsmx_setup)
+
+
+# ---------------------------------------------------------------------------
+# bf16 grouped SwiGLU experts whose activations are kept for the backward in
+# MXFP8, and MXFP4 experts (32-element blocks along each contraction)
+# ---------------------------------------------------------------------------
+def _guard(t: Tensor):
+    """Makes t's device the current one for the launches of an op, where it is not."""
+    return nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def _check_experts(op: str, x: Tensor, w1: Tensor, w2: Tensor, w3: Tensor, counts: Tensor, multiple: int) -> None:
+    """The arguments of experts with separate bf16 weights: x [R, D], w1 and w3 [E, H, D],
+    w2 [E, D, H], counts [E] integers, all on one device."""
+    require_gpu(x, w1, w2, w3, counts)
+    _check_bf16(op, x=x, w1=w1, w2=w2, w3=w3)
+    if x.dim() != 2 or w1.dim() != 3 or counts.dim() != 1:
+        raise ValueError(f"{op} expects x [R, D], weights [E, .., ..] and counts [E], got {tuple(x.shape)}, "
+                         f"{tuple(w1.shape)}, {tuple(counts.shape)}")
+    e, h, d = w1.shape
+    if x.shape[1] != d or w3.shape != (e, h, d) or w2.shape != (e, d, h) or counts.shape[0] != e:
+        raise ValueError(f"{op}: shapes do not agree: x {tuple(x.shape)}, w1 {tuple(w1.shape)}, w2 {tuple(w2.shape)}, "
+                         f"w3 {tuple(w3.shape)}, counts {tuple(counts.shape)}")
+    _check_dims(op, e, d, h, multiple)
+    _check_counts(op, counts, x, w1, w2, w3)
+
+
+def _check_dims(op: str, e: int, d: int, h: int, multiple: int) -> None:
+    if e < 1 or e > MAX_GEMM_EXPERTS:
+        raise ValueError(f"{op} takes 1 to {MAX_GEMM_EXPERTS} experts, got {e}")
+    if d < multiple or h < multiple or d % multiple or h % multiple:
+        raise ValueError(f"{op} takes dims that are multiples of {multiple}, got {d} and {h}")
+
+
+def _check_counts(op: str, counts: Tensor, *others: Tensor) -> None:
+    if counts.is_floating_point() or counts.is_complex() or counts.dtype == torch.bool:
+        raise TypeError(f"{op} expects integer counts, got {counts.dtype}")
+    if any(t.device != counts.device for t in others):
+        raise ValueError(f"{op}: tensors on more than one device")
+
+
+def _zero_rows_past(counts: Tensor, r: int, e: int, t: Tensor, s: int) -> None:
+    # (pairs of bf16 as one word; the dims of the bf16 GEMMs are even)
+    call("moe_zero_rows_past_f32", ptr(counts), r, e, ptr(t), t.shape[1] // 2, None, 0, None, 0, None, 0, s)
+
+
+@torch.library.custom_op("moe_mi355x::grouped_swiglu_ckpt8", mutates_args=())
+def grouped_swiglu_ckpt8(
+    x: Tensor, w1: Tensor, w2: Tensor, w3: Tensor, num_tokens_per_expert: Tensor
+) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor]:
+    """grouped_swiglu whose backward works from 8-bit activations: y [R, D], bit for bit
+    grouped_swiglu's on the experts' rows and zero on rows past sum(counts), then what is
+    kept: x [R, D], g and u [R, H] in MXFP8 (e4m3, one e8m0 scale per 32 along the row),
+    each followed by its scales. That is (D + 2H) 33/32 bytes a row instead of 2D + 6H.
+    The gradients are those at the kept values: the activation's at g and u, dw1 and dw3
+    with x, dw2 with h = silu(g) u. An infinity or NaN makes its block of 32 kept values NaN."""
+    op = "grouped_swiglu_ckpt8"
+    _check_experts(op, x, w1, w2, w3, num_tokens_per_expert, 64)
+    x, w1, w2, w3 = (_aligned(t.contiguous()) for t in (x, w1, w2, w3))
+    counts = num_tokens_per_expert.to(torch.int64).contiguous()
+    r, d = x.shape
+    e, h_dim, _ = w1.shape
+    u8 = lambda *shape: torch.empty(*shape, dtype=torch.uint8, device=x.device)  # noqa: E731
+    x8, xs = u8(r, d), u8(r, d // MX_BLOCK)
+    g8, gs, up8, us = u8(r, h_dim), u8(r, h_dim // MX_BLOCK), u8(r, h_dim), u8(r, h_dim // MX_BLOCK)
+    h = x.new_empty(r, h_dim)
+    y = x.new_empty(r, d)
+    with _guard(x):
+        s = stream_of(x)
+        call("moe_keep8_rows", ptr(x), r, d, ptr(x8), ptr(xs), s)
+        call("moe_grouped_gemm_gate_up_keep8", ptr(x), ptr(w1), ptr(w3), ptr(counts), r, e, d, h_dim, ptr(g8), ptr(gs),
+             ptr(up8), ptr(us), ptr(h), s)
+        call("moe_grouped_gemm_down", ptr(h), ptr(w2), ptr(counts), r, e, d, h_dim, ptr(y), s)
+        _zero_rows_past(counts, r, e, y, s)
+    return y, x8, xs, g8, gs, up8, us
+
+
+@grouped_swiglu_ckpt8.register_fake
+def _(x, w1, w2, w3, num_tokens_per_expert):
+    r, d = x.shape
+    h_dim = w1.shape[1]
+    u8 = lambda *shape: x.new_empty(*shape, dtype=torch.uint8)  # noqa: E731
+    return (x.new_empty(r, d), u8(r, d), u8(r, d // 32), u8(r, h_dim), u8(r, h_dim // 32), u8(r, h_dim),
+            u8(r, h_dim // 32))
+
+
+def _narrow_backward(dy: Tensor, w1: Tensor, w2: Tensor, w3: Tensor, counts: Tensor, g8: Tensor, gs: Tensor, up8: Tensor,
+                     us: Tensor, rows, hidden: Tensor | None, need_dx: bool, need_dw13: bool,
+                     need_dw2: bool) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+    """dx, dw1, dw2, dw3 of experts with bf16 weight values and g, u kept in MXFP8; rows()
+    gives the forward's x in bf16, `hidden` its h (None: silu(g) u of the kept values).
+    What is not needed comes back empty."""
+    r, d = dy.shape
+    e, h_dim, _ = w1.shape
+    s = stream_of(dy)
+    dgu = dy.new_empty(r, 2 * h_dim)
+    h = dy.new_empty(r, h_dim) if hidden is None and need_dw2 else hidden
+    if need_dx or need_dw13 or hidden is None:
+        call("moe_grouped_gemm_bwd_dgu_keep8", ptr(dy), ptr(w2), ptr(g8), ptr(gs), ptr(up8), ptr(us), ptr(counts), r, e,
+             d, h_dim, ptr(dgu), ptr(h) if hidden is None else None, s)
+    dx = dy.new_empty(r, d) if need_dx else dy.new_empty(0)
+    if need_dx:
+        call("moe_grouped_gemm_bwd_dx", ptr(dgu), ptr(w1), ptr(w3), ptr(counts), r, e, d, h_dim, ptr(dx), s)
+        _zero_rows_past(counts, r, e, dx, s)
+    dw1, dw3 = (torch.empty_like(w1) if need_dw13 else dy.new_empty(0) for _ in range(2))
+    if need_dw13:
+        x = rows()
+        call("moe_grouped_gemm_bwd_dw13", ptr(dgu), ptr(x), ptr(counts), r, e, d, h_dim, ptr(dw1), ptr(dw3), s)
+    dw2 = torch.empty_like(w2) if need_dw2 else dy.new_empty(0)
+    if need_dw2:
+        call("moe_grouped_gemm_bwd_dw2", ptr(dy), ptr(h), ptr(counts), r, e, d, h_dim, ptr(dw2), s)
+    return dx, dw1, dw2, dw3
+
+
+def _check_dy(op: str, dy: Tensor, r: int, d: int, like: Tensor) -> Tensor:
+    require_gpu(dy)
+    if tuple(dy.shape) != (r, d) or dy.device != like.device:
+        raise ValueError(f"{op} expects a gradient [{r}, {d}] on {like.device}, got {tuple(dy.shape)} on {dy.device}")
+    return _aligned(dy.to(torch.bfloat16).contiguous())
+
+
+@torch.library.custom_op("moe_mi355x::grouped_swiglu_ckpt8_backward", mutates_args=())
+def grouped_swiglu_ckpt8_backward(
+    dy: Tensor, w1: Tensor, w2: Tensor, w3: Tensor, num_tokens_per_expert: Tensor, x8: Tensor, xs: Tensor, g8: Tensor,
+    gs: Tensor, u8: Tensor, us: Tensor, need_dx: bool = True, need_dw13: bool = True, need_dw2: bool = True,
+) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+    """(dx, dw1, dw2, dw3) of grouped_swiglu_ckpt8 from what it kept; dx is zero on rows past
+    sum(counts), weights of experts without rows get zeros. What is not needed is empty."""
+    r, d = x8.shape
+    dy = _check_dy("grouped_swiglu_ckpt8_backward", dy, r, d, x8)
+    w1, w2, w3 = (_aligned(t.contiguous()) for t in (w1, w2, w3))
+    counts = num_tokens_per_expert.to(torch.int64).contiguous()
+
+    def rows() -> Tensor:
+        x = dy.new_empty(r, d)
+        call("moe_restore8_rows", ptr(x8), ptr(xs), r, d, ptr(x), stream_of(dy))
+        return x
+
+    with _guard(dy):
+        return _narrow_backward(dy, w1, w2, w3, counts, g8, gs, u8, us, rows, None, need_dx, need_dw13, need_dw2)
+
+
+@grouped_swiglu_ckpt8_backward.register_fake
+def _(dy, w1, w2, w3, num_tokens_per_expert, x8, xs, g8, gs, u8, us, need_dx=True, need_dw13=True, need_dw2=True):
+    empty = lambda: w1.new_empty(0)  # noqa: E731
+    return (w1.new_empty(x8.shape) if need_dx else empty(), torch.empty_like(w1) if need_dw13 else empty(),
+            torch.empty_like(w2) if need_dw2 else empty(), torch.empty_like(w3) if need_dw13 else empty())
+
+
+def _ckpt8_setup(ctx, inputs, output):
+    _x, w1, w2, w3, counts = inputs
+    _y, *kept = output
+    ctx.save_for_backward(w1, w2, w3, counts, *kept)
+    ctx.mark_non_differentiable(*kept)
+    ctx.set_materialize_grads(False)
+
+
+def _needed(need, grads) -> tuple:
+    """(dx, dw1, dw2, dw3, None) with None for inputs that take no gradient."""
+    return tuple(g if n else None for n, g in zip(need[:4], grads)) + (None,)
+
+
+def _ckpt8_bwd(ctx, dy, *_unused):
+    if dy is None:
+        return None, None, None, None, None
+    need = ctx.needs_input_grad
+    return _needed(need, grouped_swiglu_ckpt8_backward(dy, *ctx.saved_tensors, need[0], need[1] or need[3], need[2]))
+
+
+grouped_swiglu_ckpt8.register_autograd(_ckpt8_bwd, setup_context=_ckpt8_setup)
+
+
+def _check_mx_matrix(op: str, cols: int) -> None:
+    if cols < MX_BLOCK or cols % MX_BLOCK:
+        raise ValueError(f"{op} takes rows of whole blocks of {MX_BLOCK} elements, got {cols}")
+
+
+@torch.library.custom_op("moe_mi355x::mxfp4_quantize", mutates_args=())
+def mxfp4_quantize(x: Tensor) -> tuple[Tensor, Tensor]:
+    """x [.., K] (bf16 or fp32, K a multiple of 32) in MXFP4: (q [.., K / 2] uint8, two e2m1
+    codes a byte, the first in the low half; scale [.., K / 32] uint8, e8m0). A block's scale is
+    the least power of two 2^k, k in [-127, 127], with max |x| <= 6 * 2^k; elements are rounded
+    to nearest, ties to the even code. A block with an infinity or a NaN gets the NaN scale 255."""
+    require_gpu(x)
+    code = _mx_dtype("mxfp4_quantize", x.dtype)
+    if x.dim() < 1:
+        raise ValueError("mxfp4_quantize expects rows, got a scalar")
+    cols = x.shape[-1]
+    _check_mx_matrix("mxfp4_quantize", cols)
+    x = _aligned(x.contiguous())
+    q = torch.empty(*x.shape[:-1], cols // 2, dtype=torch.uint8, device=x.device)
+    scale = torch.empty(*x.shape[:-1], cols // MX_BLOCK, dtype=torch.uint8, device=x.device)
+    with _guard(x):
+        call("moe_mxfp4_quant_rows", ptr(x), x.numel() // cols, cols, code, cols // MX_BLOCK, ptr(q), ptr(scale),
+             stream_of(x))
+    return q, scale
+
+
+def _mx_dtype(op: str, dtype: torch.dtype) -> int:
+    if dtype not in DTYPE_CODES:
+        raise TypeError(f"{op} supports bfloat16 and float32, got {dtype}")
+    return DTYPE_CODES[dtype]
+
+
+@mxfp4_quantize.register_fake
+def _(x):
+    u8 = lambda n: x.new_empty(*x.shape[:-1], n, dtype=torch.uint8)  # noqa: E731
+    return u8(x.shape[-1] // 2), u8(x.shape[-1] // MX_BLOCK)
+
+
+@torch.library.custom_op("moe_mi355x::mxfp4_dequantize", mutates_args=())
+def mxfp4_dequantize(q: Tensor, scale: Tensor, dtype: torch.dtype = torch.bfloat16) -> Tensor:
+    """The values [.., K] of an MXFP4 matrix (q [.., K / 2], scale [.., K / 32] uint8) in bf16 or
+    fp32, which hold each of them exactly within their range (past it: infinities)."""
+    require_gpu(q, scale)
+    code = _mx_dtype("mxfp4_dequantize", dtype)
+    _check_packed("mxfp4_dequantize", "q", q, scale)
+    cols = 2 * q.shape[-1]
+    q, scale = _aligned(q.contiguous()), scale.contiguous()
+    x = torch.empty(*q.shape[:-1], cols, dtype=dtype, device=q.device)
+    with _guard(q):
+        call("moe_mxfp4_dequant_rows", ptr(q), ptr(scale), q.numel() // (cols // 2), cols, cols // MX_BLOCK, code, ptr(x),
+             stream_of(q))
+    return x
+
+
+@mxfp4_dequantize.register_fake
+def _(q, scale, dtype=torch.bfloat16):
+    return q.new_empty(*q.shape[:-1], 2 * q.shape[-1], dtype=dtype)
+
+
+def _check_packed(op: str, name: str, q: Tensor, scale: Tensor, shape: tuple | None = None) -> None:
+    """An MXFP4 matrix: q [.., K / 2] and scale [.., K / 32] bytes on one device, of the values'
+    `shape` where one is given."""
+    if q.dtype != torch.uint8 or scale.dtype != torch.uint8:
+        raise TypeError(f"{op} expects uint8 {name} and scales, got {q.dtype} and {scale.dtype}")
+    if q.dim() < 1 or scale.dim() != q.dim() or scale.shape[:-1] != q.shape[:-1] or q.device != scale.device:
+        raise ValueError(f"{op}: {name} {tuple(q.shape)} on {q.device} and its scales {tuple(scale.shape)} on "
+                         f"{scale.device} do not belong together")
+    _check_mx_matrix(op, 2 * q.shape[-1])
+    if scale.shape[-1] * 16 != q.shape[-1]:
+        raise ValueError(f"{op}: {name} of {2 * q.shape[-1]} columns takes {q.shape[-1] // 16} scales a row, "
+                         f"got {scale.shape[-1]}")
+    if shape is not None and tuple(q.shape[:-1]) + (2 * q.shape[-1],) != shape:
+        raise ValueError(f"{op} expects {name} of {list(shape)} values, got {[*q.shape[:-1], 2 * q.shape[-1]]}")
+
+
+def _mxfp4_workspace(r: int, d: int, h_dim: int, device: torch.device) -> Tensor:
+    return torch.empty(max(int(lib().moe_mxfp4_workspace_bytes(r, d, h_dim)), 16), dtype=torch.uint8, device=device)
+
+
+@torch.library.custom_op("moe_mi355x::grouped_swiglu_mxfp4", mutates_args=())
+def grouped_swiglu_mxfp4(
+    x: Tensor, qw1: Tensor, sw1: Tensor, qw2: Tensor, sw2: Tensor, qw3: Tensor, sw3: Tensor,
+    num_tokens_per_expert: Tensor,
+) -> Tensor:
+    """The SwiGLU experts on weights packed in MXFP4 (mxfp4_quantize of w1, w3 [E, H, D] and
+    w2 [E, D, H]): x [R, D] bf16 in expert order is quantized on the way, h = silu(x w1^T)
+    (x w3^T) is taken in fp32 and quantized, y = h w2^T [R, D] is rounded to bf16 once. Rows past
+    sum(counts) are zero. For inference: no gradients. D and H are multiples of 32."""
+    op = "grouped_swiglu_mxfp4"
+    require_gpu(x, qw1, sw1, qw2, sw2, qw3, sw3, num_tokens_per_expert)
+    r, d, e, h_dim = _check_mxfp4_rows(op, x, qw1, num_tokens_per_expert)
+    _check_packed(op, "w1", qw1, sw1, (e, h_dim, d))
+    _check_packed(op, "w2", qw2, sw2, (e, d, h_dim))
+    _check_packed(op, "w3", qw3, sw3, (e, h_dim, d))
+    _check_counts(op, num_tokens_per_expert, x, qw1, qw2, qw3)
+    x, qw1, sw1, qw2, sw2, qw3, sw3 = (_aligned(t.contiguous()) for t in (x, qw1, sw1, qw2, sw2, qw3, sw3))
+    counts = num_tokens_per_expert.to(torch.int64).contiguous()
+    ws = _mxfp4_workspace(r, d, h_dim, x.device)
+    y = x.new_empty(r, d)
+    with _guard(x):
+        call("moe_mxfp4_swiglu_fwd", ptr(x), ptr(qw1), ptr(sw1), ptr(qw2), ptr(sw2), ptr(qw3), ptr(sw3), ptr(counts), r, e,
+             d, h_dim, ptr(ws), ws.numel(), ptr(y), stream_of(x))
+    return y
+
+
+def _check_mxfp4_rows(op: str, x: Tensor, qw1: Tensor, counts: Tensor, glu: int = 1) -> tuple[int, int, int, int]:
+    _check_bf16(op, x=x)
+    if x.dim() != 2 or qw1.dim() != 3 or counts.dim() != 1 or counts.shape[0] != qw1.shape[0] or qw1.shape[1] % glu:
+        raise ValueError(f"{op} expects x [R, D], packed weights [E, .., ..] and counts [E], got {tuple(x.shape)}, "
+                         f"{tuple(qw1.shape)}, {tuple(counts.shape)}")
+    r, d = x.shape
+    e, h_dim = qw1.shape[0], qw1.shape[1] // glu
+    _check_dims(op, e, d, h_dim, MX_BLOCK)
+    return r, d, e, h_dim
+
+
+@grouped_swiglu_mxfp4.register_fake
+def _(x, qw1, sw1, qw2, sw2, qw3, sw3, num_tokens_per_expert):
+    return x.new_empty(x.shape)
+
+
+@torch.library.custom_op("moe_mi355x::grouped_swiglu_oss_mxfp4", mutates_args=())
+def grouped_swiglu_oss_mxfp4(
+    x: Tensor, qmlp1: Tensor, smlp1: Tensor, mlp1_bias: Tensor, qmlp2: Tensor, smlp2: Tensor, mlp2_bias: Tensor,
+    num_tokens_per_expert: Tensor, swiglu_limit: float,
+) -> Tensor:
+    """grouped_swiglu_mxfp4 for gpt-oss's experts (gpt_oss/moe.py:43-122): mlp1 [E, 2H, D] (glu row
+    2j, linear row 2j + 1) and mlp2 [E, D, H] packed in MXFP4, biases [E, 2H] and [E, D] taken in
+    bf16; biases, clamps and activation in fp32 between the products."""
+    op = "grouped_swiglu_oss_mxfp4"
+    require_gpu(x, qmlp1, smlp1, mlp1_bias, qmlp2, smlp2, mlp2_bias, num_tokens_per_expert)
+    r, d, e, h_dim = _check_mxfp4_rows(op, x, qmlp1, num_tokens_per_expert, 2)
+    _check_packed(op, "mlp1", qmlp1, smlp1, (e, 2 * h_dim, d))
+    _check_packed(op, "mlp2", qmlp2, smlp2, (e, d, h_dim))
+    if tuple(mlp1_bias.shape) != (e, 2 * h_dim) or tuple(mlp2_bias.shape) != (e, d):
+        raise ValueError(f"{op} expects biases [{e}, {2 * h_dim}] and [{e}, {d}], got {tuple(mlp1_bias.shape)} and "
+                         f"{tuple(mlp2_bias.shape)}")
+    if not swiglu_limit >= 0:
+        raise ValueError(f"{op} expects a clamp limit of at least 0, got {swiglu_limit}")
+    _check_counts(op, num_tokens_per_expert, x, qmlp1, mlp1_bias, qmlp2, mlp2_bias)
+    x, qmlp1, smlp1, qmlp2, smlp2 = (_aligned(t.contiguous()) for t in (x, qmlp1, smlp1, qmlp2, smlp2))
+    b1, b2 = (_aligned(t.to(torch.bfloat16).contiguous()) for t in (mlp1_bias, mlp2_bias))
+    counts = num_tokens_per_expert.to(torch.int64).contiguous()
+    ws = _mxfp4_workspace(r, d, h_dim, x.device)
+    y = x.new_empty(r, d)
+    with _guard(x):
+        call("moe_mxfp4_oss_fwd", ptr(x), ptr(qmlp1), ptr(smlp1), ptr(b1), ptr(qmlp2), ptr(smlp2), ptr(b2), ptr(counts), r,
+             e, d, h_dim, float(swiglu_limit), ptr(ws), ws.numel(), ptr(y), stream_of(x))
+    return y
+
+
+@grouped_swiglu_oss_mxfp4.register_fake
+def _(x, qmlp1, smlp1, mlp1_bias, qmlp2, smlp2, mlp2_bias, num_tokens_per_expert, swiglu_limit):
+    return x.new_empty(x.shape)
+
+
+def _mxfp4_rows(x: Tensor, s: int) -> tuple[Tensor, Tensor]:
+    """x [R, C] bf16 in MXFP4 as the products take their rows: the scales' row stride is
+    moe_mxfp4_scale_ld(C)."""
+    r, c = x.shape
+    ld = int(lib().moe_mxfp4_scale_ld(c))
+    q = torch.empty(r, c // 2, dtype=torch.uint8, device=x.device)
+    scale = torch.empty(r, ld, dtype=torch.uint8, device=x.device)
+    call("moe_mxfp4_quant_rows", ptr(x), r, c, 0, ld, ptr(q), ptr(scale), s)
+    return q, scale
+
+
+def _mxfp4_values(q: Tensor, scale: Tensor, s: int) -> Tensor:
+    """The bf16 values of rows [.., C / 2] whose scales have the row stride scale.shape[-1]."""
+    cols = 2 * q.shape[-1]
+    x = torch.empty(*q.shape[:-1], cols, dtype=torch.bfloat16, device=q.device)
+    call("moe_mxfp4_dequant_rows", ptr(q), ptr(scale), x.numel() // cols, cols, scale.shape[-1], 0, ptr(x), s)
+    return x
+
+
+@torch.library.custom_op("moe_mi355x::grouped_swiglu_mxfp4_train", mutates_args=())
+def grouped_swiglu_mxfp4_train(
+    x: Tensor, w1: Tensor, w2: Tensor, w3: Tensor, num_tokens_per_expert: Tensor
+) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor,
+           Tensor, Tensor]:
+    """The SwiGLU experts in MXFP4 from bf16 weights, with gradients: y [R, D] is
+    grouped_swiglu_mxfp4's on the packed weights. The backward passes the quantizations
+    straight through: it takes the products' gradients at their quantized operands (in bf16,
+    which holds them exactly) and the activation's at g and u kept in MXFP8. Returns y, then
+    what is kept: x and h, w1, w2, w3 in MXFP4 and g, u in MXFP8, each with its scales. D and
+    H are multiples of 64."""
+    op = "grouped_swiglu_mxfp4_train"
+    _check_experts(op, x, w1, w2, w3, num_tokens_per_expert, 64)
+    x, w1, w2, w3 = (_aligned(t.contiguous()) for t in (x, w1, w2, w3))
+    counts = num_tokens_per_expert.to(torch.int64).contiguous()
+    r, d = x.shape
+    e, h_dim, _ = w1.shape
+    u8 = lambda *shape: torch.empty(*shape, dtype=torch.uint8, device=x.device)  # noqa: E731
+    ld = int(lib().moe_mxfp4_scale_ld(h_dim))
+    qh, sh = u8(r, h_dim // 2), u8(r, ld)
+    g8, gs, up8, us = u8(r, h_dim), u8(r, h_dim // MX_BLOCK), u8(r, h_dim), u8(r, h_dim // MX_BLOCK)
+    y = x.new_empty(r, d)
+    with _guard(x):
+        s = stream_of(x)
+        qx, sx = _mxfp4_rows(x, s)
+        packed = []
+        for w in (w1, w2, w3):
+            q, sc = u8(*w.shape[:-1], w.shape[-1] // 2), u8(*w.shape[:-1], w.shape[-1] // MX_BLOCK)
+            call("moe_mxfp4_quant_rows", ptr(w), w.numel() // w.shape[-1], w.shape[-1], 0, w.shape[-1] // MX_BLOCK, ptr(q),
+                 ptr(sc), s)
+            packed += [q, sc]
+        qw1, sw1, qw2, sw2, qw3, sw3 = packed
+        call("moe_mxfp4_gemm_gate_up_keep", ptr(qx), ptr(sx), ptr(qw1), ptr(sw1), ptr(qw3), ptr(sw3), ptr(counts), r, e, d,
+             h_dim, ptr(qh), ptr(sh), ptr(g8), ptr(gs), ptr(up8), ptr(us), s)
+        call("moe_mxfp4_gemm_down", ptr(qh), ptr(sh), ptr(qw2), ptr(sw2), ptr(counts), r, e, d, h_dim, ptr(y), s)
+    return y, qx, sx, qh, sh, qw1, sw1, qw2, sw2, qw3, sw3, g8, gs, up8, us
+
+
+def _scale_ld(cols: int) -> int:  # moe_mxfp4_scale_ld
+    return (cols // 32 + 7) // 8 * 8
+
+
+@grouped_swiglu_mxfp4_train.register_fake
+def _(x, w1, w2, w3, num_tokens_per_expert):
+    r, d = x.shape
+    e, h_dim, _ = w1.shape
+    u8 = lambda *shape: x.new_empty(*shape, dtype=torch.uint8)  # noqa: E731
+    return (x.new_empty(r, d), u8(r, d // 2), u8(r, _scale_ld(d)), u8(r, h_dim // 2), u8(r, _scale_ld(h_dim)),
+            u8(e, h_dim, d // 2), u8(e, h_dim, d // 32), u8(e, d, h_dim // 2), u8(e, d, h_dim // 32),
+            u8(e, h_dim, d // 2), u8(e, h_dim, d // 32), u8(r, h_dim), u8(r, h_dim // 32), u8(r, h_dim),
+            u8(r, h_dim // 32))
+
+
+@torch.library.custom_op("moe_mi355x::grouped_swiglu_mxfp4_train_backward", mutates_args=())
+def grouped_swiglu_mxfp4_train_backward(
+    dy: Tensor, num_tokens_per_expert: Tensor, qx: Tensor, sx: Tensor, qh: Tensor, sh: Tensor, qw1: Tensor, sw1: Tensor,
+    qw2: Tensor, sw2: Tensor, qw3: Tensor, sw3: Tensor, g8: Tensor, gs: Tensor, u8: Tensor, us: Tensor,
+    need_dx: bool = True, need_dw13: bool = True, need_dw2: bool = True,
+) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+    """(dx, dw1, dw2, dw3) of grouped_swiglu_mxfp4_train from what it kept; dx is zero on rows
+    past sum(counts), weights of experts without rows get zeros. What is not needed is empty."""
+    r, d = qx.shape[0], 2 * qx.shape[1]
+    dy = _check_dy("grouped_swiglu_mxfp4_train_backward", dy, r, d, qx)
+    counts = num_tokens_per_expert.to(torch.int64).contiguous()
+    with _guard(dy):
+        s = stream_of(dy)
+        # the values dgu and dx multiply; dW takes only their shapes
+        w2 = _mxfp4_values(qw2, sw2, s) if need_dx or need_dw13 else dy.new_empty(*qw2.shape[:-1], 2 * qw2.shape[-1])
+        w1, w3 = (_mxfp4_values(q, sc, s) if need_dx else dy.new_empty(*q.shape[:-1], 2 * q.shape[-1])
+                  for q, sc in ((qw1, sw1), (qw3, sw3)))
+        h = _mxfp4_values(qh, sh, s) if need_dw2 else dy.new_empty(0)
+        return _narrow_backward(dy, w1, w2, w3, counts, g8, gs, u8, us, lambda: _mxfp4_values(qx, sx, s), h, need_dx,
+                                need_dw13, need_dw2)
+
+
+@grouped_swiglu_mxfp4_train_backward.register_fake
+def _(dy, num_tokens_per_expert, qx, sx, qh, sh, qw1, sw1, qw2, sw2, qw3, sw3, g8, gs, u8, us, need_dx=True,
+      need_dw13=True, need_dw2=True):
+    full = lambda q, need: dy.new_empty(*q.shape[:-1], 2 * q.shape[-1], dtype=torch.bfloat16) if need else dy.new_empty(0, dtype=torch.bfloat16)  # noqa: E501,E731
+    return full(qx, need_dx), full(qw1, need_dw13), full(qw2, need_dw2), full(qw3, need_dw13)
+
+
+def _mxfp4_train_setup(ctx, inputs, output):
+    _y, *kept = output
+    ctx.save_for_backward(inputs[4], *kept)
+    ctx.mark_non_differentiable(*kept)
+    ctx.set_materialize_grads(False)
+
+
+def _mxfp4_train_bwd(ctx, dy, *_unused):
+    if dy is None:
+        return None, None, None, None, None
+    need = ctx.needs_input_grad
+    return _needed(need, grouped_swiglu_mxfp4_train_backward(dy, *ctx.saved_tensors, need[0], need[1] or need[3],
+                                                             need[2]))
+
+
+grouped_swiglu_mxfp4_train.register_autograd(_mxfp4_train_bwd, setup_context=_mxfp4_train_setup)
 
 
 # ---------------------------------------------------------------------------
