@@ -599,8 +599,8 @@ int moe_scatter_rows(const void* src, const int64_t* idx, int64_t n_rows, int32_
  * for a block with an infinity or a NaN, whose values are then all NaN.
  * ------------------------------------------------------------------------- */
 
-/* moe_grouped_gemm_gate_up with g and u, quantized from their fp32 sums, in g8,
- * u8 [R,H] and their scales [R,H/32] instead of in bf16; h is the same. */
+/* h [R,H] = bf16(silu(g) * u) of the fp32 sums g = x.w1^T, u = x.w3^T, and g, u
+ * quantized from them in g8, u8 [R,H] with scales [R,H/32] (g8 NULL: only h). */
 int moe_grouped_gemm_gate_up_keep8(const uint16_t* x, const uint16_t* w1, const uint16_t* w3,
                                    const int64_t* counts, int64_t n_rows, int32_t n_experts, int32_t dim,
                                    int32_t hidden, uint8_t* g8, uint8_t* g8_scale, uint8_t* u8,
@@ -613,6 +613,12 @@ int moe_grouped_gemm_bwd_dgu_keep8(const uint16_t* dy, const uint16_t* w2, const
                                    const uint8_t* g8_scale, const uint8_t* u8, const uint8_t* u8_scale,
                                    const int64_t* counts, int64_t n_rows, int32_t n_experts, int32_t dim,
                                    int32_t hidden, uint16_t* dgu, uint16_t* h, moe_stream_t stream);
+
+/* dx [R,D] = bf16(dg.w1 + du.w3), one fp32 sum (moe_grouped_gemm_bwd_dx rounds the
+ * halves). */
+int moe_grouped_gemm_bwd_dx_once(const uint16_t* dgu, const uint16_t* w1, const uint16_t* w3,
+                                 const int64_t* counts, int64_t n_rows, int32_t n_experts, int32_t dim,
+                                 int32_t hidden, uint16_t* dx, moe_stream_t stream);
 
 /* x [rows, cols] bf16 (cols % 32 == 0) -> q [rows, cols], scale [rows, cols / 32],
  * and back. */

@@ -134,8 +134,7 @@ def experts4(xq, w1q, w2q, w3q, counts, act="silu", limit=7.0, b1=None, b2=None)
 
 def gradients(x, w1, w2, w3, dy, counts, four: bool):
     """[(value, bound)] of y, dx, dw1, dw2, dw3 of the experts that keep g and u in MXFP8, on bf16
-    operands (four False: y in the bf16 experts' roundings, dw with the kept x and h) or on
-    MXFP4 ones."""
+    operands (four False: dw with the kept x and h) or on MXFP4 ones."""
     rows, h_dim = x.shape[0], w1.shape[1]
     xf = q4(x) if four else x.double()
     w1, w2, w3 = ((q4(w) if four else w.double()) for w in (w1, w2, w3))
@@ -159,9 +158,9 @@ def gradients(x, w1, w2, w3, dy, counts, four: bool):
         if four:
             oh = spread(q4, h, activation_off("silu", g, u, og, ou, 0.0))
             h = q4(h)
-        else:  # g, u, silu(g) and h each rounded to bf16
-            oh = activation_off("silu", g, u, og + BF16_HALF * g.abs(), ou + BF16_HALF * u.abs(), 0.0)
-            oh = oh + 2.1 * BF16_HALF * h.abs()
+        else:  # h rounded to bf16
+            oh = activation_off("silu", g, u, og, ou, 0.0)
+            oh = oh + BF16_HALF * (h.abs() + oh)
         put(0, at, h @ w2[e].t(), sum_off(h, w2[e]) + oh @ w2[e].abs().t())
         kg, ku = q8(g), q8(u)
         og, ou = spread(q8, g, og), spread(q8, u, ou)
@@ -176,11 +175,8 @@ def gradients(x, w1, w2, w3, dy, counts, four: bool):
         odg = odh * (ku * slope).abs() + (dh.abs() + odh) * (1.13 * ou + 0.5 * og * (ku.abs() + ou))
         odu, odg = (o + (BF16_HALF + 64 * F32_HALF) * (v.abs() + o) + 64 * F32_HALF * dh.abs() * w
                     for o, v, w in ((odu, du, 0 * ku.abs()), (odg, dg, ku.abs())))
-        half1, half2 = dg @ w1[e], du @ w3[e]
-        o1 = sum_off(dg, w1[e].t()) + odg @ w1[e].abs()
-        o2 = sum_off(du, w3[e].t()) + odu @ w3[e].abs()
-        # each half is rounded to bf16 before the two are added
-        put(1, at, half1 + half2, o1 + o2 + BF16_HALF * (half1.abs() + half2.abs() + o1 + o2))
+        both, w13 = torch.cat([dg, du], 1), torch.cat([w1[e], w3[e]])
+        put(1, at, both @ w13, sum_off(both, w13.t()) + torch.cat([odg, odu], 1) @ w13.abs())
         kx = kept_x[at]
         kh, okh = (h, oh) if four else (kg * s * ku, 1.13 * og * (ku.abs() + ou) + (kg * s).abs() * ou)
         if not four:

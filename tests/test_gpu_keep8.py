@@ -59,14 +59,19 @@ def test_step(dev, four, case):
             assert not any(g[e].any() for g in got[2:])
 
 
-def test_forward_keeps_the_bf16_bits(dev):
-    banner("kept in 8 bits, forward bits")
+def test_forward_alone(dev):
+    """Without a backward to keep for: the same y, nothing kept, and a backward refuses."""
+    banner("kept in 8 bits, forward alone")
     from torchtitan_amd import ops
 
     for counts, d, h in (([5, 0, 300, 40], 320, 192), ([700, 513], 512, 576)):
-        c, x, dy, w1, w2, w3 = _inputs(counts, 0, d, h, 3, dev)
+        c, x, dy, w1, w2, w3 = _inputs(counts, 3, d, h, 3, dev)
         args = [t.to(dev) for t in (x, w1, w2, w3, c)]
-        assert torch.equal(ops.grouped_swiglu_ckpt8(*args)[0], ops.grouped_swiglu(*args)[0])
+        y, *kept = ops.grouped_swiglu_ckpt8(*args, False)
+        assert torch.equal(y, ops.grouped_swiglu_ckpt8(*args)[0]) and not any(t.numel() for t in kept)
+    y = ops.grouped_swiglu_ckpt8(args[0].requires_grad_(True), *args[1:], False)[0]
+    with pytest.raises(RuntimeError, match="nothing was kept"):
+        y.float().sum().backward()
 
 
 def test_kept_values(dev):

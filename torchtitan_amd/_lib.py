@@ -93,6 +93,7 @@ SIGNATURES: dict[str, list] = {
     "moe_mxfp8_gemm_bwd_dw2": [P, P, P, P, P, I64, I64, I32, I32, I32, P, P],
     "moe_grouped_gemm_gate_up_keep8": [P, P, P, P, I64, I32, I32, I32, P, P, P, P, P, P],
     "moe_grouped_gemm_bwd_dgu_keep8": [P, P, P, P, P, P, P, I64, I32, I32, I32, P, P, P],
+    "moe_grouped_gemm_bwd_dx_once": [P, P, P, P, I64, I32, I32, I32, P, P],
     "moe_keep8_rows": [P, I64, I32, P, P, P],
     "moe_restore8_rows": [P, P, I64, I32, P, P],
     "moe_mxfp4_quant_rows": [P, I64, I32, I32, I32, P, P, P],

@@ -116,11 +116,12 @@ struct GemmParams {
 
 // Expert epilogue variants: the SwiGLU of moe.py:53-70 and gpt-oss's biased,
 // clamped SwiGLU with interleaved mlp1 rows (gpt_oss/moe.py:43-52, 92-122), and the SwiGLU
-// whose g and u are kept for the backward in MXFP8 instead of bf16: gate_up writes the same
-// h, bit for bit, and quantizes g and u from the fp32 sums (a rounding to bf16 before it
-// would move 3 % of the e4m3 roundings to a neighbour); dgu reads them back, computes in fp32
-// with one rounding per output, and writes h = silu(g) u of the kept values beside dgu, which
-// dw2 multiplies (keeping h too would be half as many bytes again).
+// whose g and u are kept for the backward in MXFP8 instead of bf16. That one has no reference
+// whose roundings it would follow: the activation and its gradient are taken in fp32 and h, dg
+// and du rounded once each; g and u are quantized from the fp32 sums (a rounding to bf16 before
+// it would move 3 % of the e4m3 roundings to a neighbour); and dgu writes h = silu(g) u of the
+// kept values beside its results, which dw2 multiplies (keeping h too would be half as many
+// bytes again).
 enum ExpertAct : int { kSwiGLU = 0, kOssGLU = 1, kSwiGLUKeep8 = 2 };
 
 // gpt-oss activation on pairs of bf16 values g (glu), u (linear), every op rounded to
@@ -648,7 +649,45 @@ __global__ __launch_bounds__(NW * 64, OCC) void grouped_gemm_kernel(GemmParams p
         bias2[j] = (!TAIL || n < D) ? *(const uint2*)(p.b2 + e64 * D + n) : make_uint2(0, 0);
       }
     }
-    if (MODE == kFwdGateUp) {
+    if constexpr (MODE == kFwdGateUp && ACT == kSwiGLUKeep8) {
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        const int r = row0 + wm * WM + i * 16 + ml;
+        if (r < seg1) {
+#pragma unroll
+          for (int jp = 0; jp < TN / 4; ++jp) {
+            const int hc = nt * (BN / 2) + wn * (WN / 2) + jp * 32 + g8;
+            if (TAIL && hc >= H) continue;
+            float g[2][4], u[2][4];
+            uint2 ph[2];
+#pragma unroll
+            for (int h2 = 0; h2 < 2; ++h2) {
+              float h[4];
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                g[h2][q] = acc[i][4 * jp + 2 * h2][q];
+                u[h2][q] = acc[i][4 * jp + 2 * h2 + 1][q];
+                h[q] = g[h2][q] * mx::sigmoid(g[h2][q]) * u[h2][q];
+              }
+              ph[h2] = pack4(h);
+            }
+            const int64_t off = (int64_t)r * H + hc;
+            *(uint4*)(p.out_h + off) = span64(ph[0], ph[1], lane);
+            if (p.g8) {
+              uint2 qg, qu;
+              const uint32_t eg = mx::block8(g[0], g[1], qg), eu = mx::block8(u[0], u[1], qu);
+              *(uint2*)(p.g8 + off) = qg;
+              *(uint2*)(p.u8 + off) = qu;
+              if (g8 == 0) {
+                const int64_t so = (int64_t)r * (H / 32) + hc / 32;
+                p.g8s[so] = (uint8_t)eg;
+                p.u8s[so] = (uint8_t)eu;
+              }
+            }
+          }
+        }
+      }
+    } else if (MODE == kFwdGateUp) {
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
         const int r = row0 + wm * WM + i * 16 + ml;
@@ -702,33 +741,13 @@ __global__ __launch_bounds__(NW * 64, OCC) void grouped_gemm_kernel(GemmParams p
                         sh = span64(ph[0], ph[1], lane);
             if (TAIL && hc >= H) continue;
             const int64_t off = (int64_t)r * H + hc;
+            *(uint4*)(p.out_g + off) = sg;
+            *(uint4*)(p.out_u + off) = su;
             *(uint4*)(p.out_h + off) = sh;
-            if constexpr (ACT == kSwiGLUKeep8) {
-              float ga[4], gb[4], ua[4], ub[4];
-#pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                ga[q] = acc[i][4 * jp][q];
-                ua[q] = acc[i][4 * jp + 1][q];
-                gb[q] = acc[i][4 * jp + 2][q];
-                ub[q] = acc[i][4 * jp + 3][q];
-              }
-              uint2 qg, qu;
-              const uint32_t eg = mx::block8(ga, gb, qg), eu = mx::block8(ua, ub, qu);
-              *(uint2*)(p.g8 + off) = qg;
-              *(uint2*)(p.u8 + off) = qu;
-              if (g8 == 0) {
-                const int64_t so = (int64_t)r * (H / 32) + hc / 32;
-                p.g8s[so] = (uint8_t)eg;
-                p.u8s[so] = (uint8_t)eu;
-              }
-            } else {
-              *(uint4*)(p.out_g + off) = sg;
-              *(uint4*)(p.out_u + off) = su;
-            }
           }
         };
         if (r < seg1) {
-          if constexpr (ACT != kOssGLU) {
+          if constexpr (ACT == kSwiGLU) {
             // the range of the block's gate values, taken before their rounding to
             // bf16, which keeps them inside it
             float g_min = acc[i][0][0], g_max = acc[i][0][0];
@@ -1189,10 +1208,26 @@ MOE_API int moe_grouped_gemm_gate_up_keep8(const uint16_t* x, const uint16_t* w1
   int st = gemm_params(p, counts, n_rows, n_experts, dim, hidden);
   if (st) return st;
   if (n_rows == 0) return kOk;
-  if (!x || !w1 || !w3 || !g8 || !g8_scale || !u8 || !u8_scale || !h) return kErrInvalidArgument;
+  if (!x || !w1 || !w3 || !h || (g8 && (!g8_scale || !u8 || !u8_scale))) return kErrInvalidArgument;
   p.x = x; p.w1 = w1; p.w3 = w3; p.out_h = h;
   p.g8 = g8; p.g8s = g8_scale; p.u8 = u8; p.u8s = u8_scale;
   launch_mode<kFwdGateUp, kSwiGLUKeep8>(p, n_rows, stream);
+  return launch_status();
+}
+
+// dg.w1 + du.w3 in one fp32 sum, rounded once (moe_grouped_gemm_bwd_dx rounds each half, as
+// autograd adds them): the kernels of the gpt-oss dx, on separate w1 and w3. On rows of bf16
+// dgu that leaves two roundings of the three: 0.0030 -> 0.0024 of dx's size off 64 bits.
+MOE_API int moe_grouped_gemm_bwd_dx_once(const uint16_t* dgu, const uint16_t* w1, const uint16_t* w3,
+                                         const int64_t* counts, int64_t n_rows, int32_t n_experts, int32_t dim,
+                                         int32_t hidden, uint16_t* dx, hipStream_t stream) {
+  GemmParams p;
+  int st = gemm_params(p, counts, n_rows, n_experts, dim, hidden);
+  if (st) return st;
+  if (n_rows == 0) return kOk;
+  if (!dgu || !w1 || !w3 || !dx) return kErrInvalidArgument;
+  p.dgu = dgu; p.w1 = w1; p.w3 = w3; p.out_dx = dx;
+  launch_mode<kBwdDx, kOssGLU>(p, n_rows, stream);
   return launch_status();
 }
 

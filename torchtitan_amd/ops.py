@@ -1198,42 +1198,45 @@ def _zero_rows_past(counts: Tensor, r: int, e: int, t: Tensor, s: int) -> None:
 
 @torch.library.custom_op("moe_mi355x::grouped_swiglu_ckpt8", mutates_args=())
 def grouped_swiglu_ckpt8(
-    x: Tensor, w1: Tensor, w2: Tensor, w3: Tensor, num_tokens_per_expert: Tensor
+    x: Tensor, w1: Tensor, w2: Tensor, w3: Tensor, num_tokens_per_expert: Tensor, for_backward: bool = True
 ) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor]:
-    """grouped_swiglu whose backward works from 8-bit activations: y [R, D], bit for bit
-    grouped_swiglu's on the experts' rows and zero on rows past sum(counts), then what is
-    kept: x [R, D], g and u [R, H] in MXFP8 (e4m3, one e8m0 scale per 32 along the row),
-    each followed by its scales. That is (D + 2H) 33/32 bytes a row instead of 2D + 6H.
-    The gradients are those at the kept values: the activation's at g and u, dw1 and dw3
-    with x, dw2 with h = silu(g) u. An infinity or NaN makes its block of 32 kept values NaN."""
+    """bf16 grouped SwiGLU whose backward works from 8-bit activations. y [R, D] = h w2^T with
+    h = bf16(silu(x w1^T) (x w3^T)) of fp32 sums (grouped_swiglu, which follows the reference's,
+    rounds four times on the way to h), zero on rows past sum(counts). Then what is kept: x
+    [R, D], g and u [R, H] in MXFP8 (e4m3, one e8m0 scale per 32 along the row), each followed
+    by its scales: (D + 2H) 33/32 bytes a row instead of 2D + 6H; empty without `for_backward`.
+    The gradients are those at the kept values: the activation's at g and u, dw1 and dw3 with x,
+    dw2 with h = silu(g) u. An infinity or NaN makes its block of 32 kept values NaN."""
     op = "grouped_swiglu_ckpt8"
     _check_experts(op, x, w1, w2, w3, num_tokens_per_expert, 64)
     x, w1, w2, w3 = (_aligned(t.contiguous()) for t in (x, w1, w2, w3))
     counts = num_tokens_per_expert.to(torch.int64).contiguous()
     r, d = x.shape
     e, h_dim, _ = w1.shape
-    u8 = lambda *shape: torch.empty(*shape, dtype=torch.uint8, device=x.device)  # noqa: E731
-    x8, xs = u8(r, d), u8(r, d // MX_BLOCK)
-    g8, gs, up8, us = u8(r, h_dim), u8(r, h_dim // MX_BLOCK), u8(r, h_dim), u8(r, h_dim // MX_BLOCK)
+    x8, xs, g8, gs, up8, us = _ckpt8_kept(x, h_dim, for_backward)
     h = x.new_empty(r, h_dim)
     y = x.new_empty(r, d)
     with _guard(x):
         s = stream_of(x)
-        call("moe_keep8_rows", ptr(x), r, d, ptr(x8), ptr(xs), s)
-        call("moe_grouped_gemm_gate_up_keep8", ptr(x), ptr(w1), ptr(w3), ptr(counts), r, e, d, h_dim, ptr(g8), ptr(gs),
-             ptr(up8), ptr(us), ptr(h), s)
+        if for_backward:
+            call("moe_keep8_rows", ptr(x), r, d, ptr(x8), ptr(xs), s)
+        call("moe_grouped_gemm_gate_up_keep8", ptr(x), ptr(w1), ptr(w3), ptr(counts), r, e, d, h_dim,
+             *((ptr(g8), ptr(gs), ptr(up8), ptr(us)) if for_backward else (None,) * 4), ptr(h), s)
         call("moe_grouped_gemm_down", ptr(h), ptr(w2), ptr(counts), r, e, d, h_dim, ptr(y), s)
         _zero_rows_past(counts, r, e, y, s)
     return y, x8, xs, g8, gs, up8, us
 
 
+def _ckpt8_kept(x: Tensor, h_dim: int, for_backward: bool) -> list[Tensor]:
+    r, d = x.shape if for_backward else (0, 0)
+    h_dim = h_dim if for_backward else 0
+    return [x.new_empty(r, n, dtype=torch.uint8)
+            for n in (d, d // MX_BLOCK, h_dim, h_dim // MX_BLOCK, h_dim, h_dim // MX_BLOCK)]
+
+
 @grouped_swiglu_ckpt8.register_fake
-def _(x, w1, w2, w3, num_tokens_per_expert):
-    r, d = x.shape
-    h_dim = w1.shape[1]
-    u8 = lambda *shape: x.new_empty(*shape, dtype=torch.uint8)  # noqa: E731
-    return (x.new_empty(r, d), u8(r, d), u8(r, d // 32), u8(r, h_dim), u8(r, h_dim // 32), u8(r, h_dim),
-            u8(r, h_dim // 32))
+def _(x, w1, w2, w3, num_tokens_per_expert, for_backward=True):
+    return (x.new_empty(x.shape), *_ckpt8_kept(x, w1.shape[1], for_backward))
 
 
 def _narrow_backward(dy: Tensor, w1: Tensor, w2: Tensor, w3: Tensor, counts: Tensor, g8: Tensor, gs: Tensor, up8: Tensor,
@@ -1252,7 +1255,7 @@ def _narrow_backward(dy: Tensor, w1: Tensor, w2: Tensor, w3: Tensor, counts: Ten
              d, h_dim, ptr(dgu), ptr(h) if hidden is None else None, s)
     dx = dy.new_empty(r, d) if need_dx else dy.new_empty(0)
     if need_dx:
-        call("moe_grouped_gemm_bwd_dx", ptr(dgu), ptr(w1), ptr(w3), ptr(counts), r, e, d, h_dim, ptr(dx), s)
+        call("moe_grouped_gemm_bwd_dx_once", ptr(dgu), ptr(w1), ptr(w3), ptr(counts), r, e, d, h_dim, ptr(dx), s)
         _zero_rows_past(counts, r, e, dx, s)
     dw1, dw3 = (torch.empty_like(w1) if need_dw13 else dy.new_empty(0) for _ in range(2))
     if need_dw13:
@@ -1300,7 +1303,7 @@ def _(dy, w1, w2, w3, num_tokens_per_expert, x8, xs, g8, gs, u8, us, need_dx=Tru
 
 
 def _ckpt8_setup(ctx, inputs, output):
-    _x, w1, w2, w3, counts = inputs
+    _x, w1, w2, w3, counts, ctx.for_backward = inputs
     _y, *kept = output
     ctx.save_for_backward(w1, w2, w3, counts, *kept)
     ctx.mark_non_differentiable(*kept)
@@ -1308,15 +1311,17 @@ def _ckpt8_setup(ctx, inputs, output):
 
 
 def _needed(need, grads) -> tuple:
-    """(dx, dw1, dw2, dw3, None) with None for inputs that take no gradient."""
-    return tuple(g if n else None for n, g in zip(need[:4], grads)) + (None,)
+    """(dx, dw1, dw2, dw3) with None for inputs that take no gradient."""
+    return tuple(g if n else None for n, g in zip(need[:4], grads))
 
 
 def _ckpt8_bwd(ctx, dy, *_unused):
     if dy is None:
-        return None, None, None, None, None
+        return (None,) * 6
+    if not ctx.for_backward:
+        raise RuntimeError("grouped_swiglu_ckpt8 ran with for_backward=False: nothing was kept for a backward")
     need = ctx.needs_input_grad
-    return _needed(need, grouped_swiglu_ckpt8_backward(dy, *ctx.saved_tensors, need[0], need[1] or need[3], need[2]))
+    return *_needed(need, grouped_swiglu_ckpt8_backward(dy, *ctx.saved_tensors, need[0], need[1] or need[3], need[2])), None, None
 
 
 grouped_swiglu_ckpt8.register_autograd(_ckpt8_bwd, setup_context=_ckpt8_setup)
@@ -1590,8 +1595,8 @@ def _mxfp4_train_bwd(ctx, dy, *_unused):
     if dy is None:
         return None, None, None, None, None
     need = ctx.needs_input_grad
-    return _needed(need, grouped_swiglu_mxfp4_train_backward(dy, *ctx.saved_tensors, need[0], need[1] or need[3],
-                                                             need[2]))
+    return *_needed(need, grouped_swiglu_mxfp4_train_backward(dy, *ctx.saved_tensors, need[0], need[1] or need[3],
+                                                              need[2])), None
 
 
 grouped_swiglu_mxfp4_train.register_autograd(_mxfp4_train_bwd, setup_context=_mxfp4_train_setup)
