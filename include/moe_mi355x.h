@@ -637,21 +637,23 @@ int moe_restore8_rows(const uint8_t* q, const uint8_t* scale, int64_t rows, int3
  * ------------------------------------------------------------------------- */
 
 /* x [rows, cols] (dtype MOE_DTYPE_BF16 or MOE_DTYPE_FP32, cols % 32 == 0) ->
- * q [rows, cols / 2], scale: row r's cols / 32 bytes at scale + r * scale_ld. */
-int moe_mxfp4_quant_rows(const void* x, int64_t rows, int32_t cols, int32_t dtype, int32_t scale_ld,
-                         uint8_t* q, uint8_t* scale, moe_stream_t stream);
+ * q [rows, q_cols / 2], scale [rows, q_cols / 32]; q_cols >= cols, a multiple of 32: zeros
+ * behind the columns. */
+int moe_mxfp4_quant_rows(const void* x, int64_t rows, int32_t cols, int32_t q_cols, int32_t dtype, uint8_t* q,
+                         uint8_t* scale, moe_stream_t stream);
 
-/* The values back: q [rows, cols / 2], row r's scales at scale + r * scale_ld ->
- * x [rows, cols]; values past the dtype's range become infinities. */
-int moe_mxfp4_dequant_rows(const uint8_t* q, const uint8_t* scale, int64_t rows, int32_t cols,
-                           int32_t scale_ld, int32_t dtype, void* x, moe_stream_t stream);
+/* The values of the first cols of q_cols columns: q [rows, q_cols / 2], scale
+ * [rows, q_cols / 32] -> x [rows, cols]; values past the dtype's range become
+ * infinities. */
+int moe_mxfp4_dequant_rows(const uint8_t* q, const uint8_t* scale, int64_t rows, int32_t cols, int32_t q_cols,
+                           int32_t dtype, void* x, moe_stream_t stream);
 
-/* The row stride of the scales that the products' row operands take: cols / 32
- * rounded up to 8 (weights' scales are dense). */
-int moe_mxfp4_scale_ld(int32_t cols);
+/* The columns that the products' row operands have: cols rounded up to 256,
+ * zeros behind (weights are dense). */
+int moe_mxfp4_padded_cols(int32_t cols);
 
 /* Bytes of workspace of moe_mxfp4_swiglu_fwd and moe_mxfp4_oss_fwd. */
-int64_t moe_mxfp4_workspace_bytes(int64_t n_rows, int32_t dim, int32_t hidden);
+int64_t moe_mxfp4_workspace_bytes(int64_t n_rows, int32_t n_experts, int32_t dim, int32_t hidden);
 
 /* The experts' forward on packed weights: x [R,D] bf16 in expert order, counts
  * [E]; qw1, qw3 [E,H,D/2], qw2 [E,D,H/2] with scales [E,H,D/32], [E,D,H/32]:
@@ -672,10 +674,11 @@ int moe_mxfp4_oss_fwd(const uint16_t* x, const uint8_t* qmlp1, const uint8_t* sm
                       float swiglu_limit, uint8_t* workspace, int64_t workspace_bytes, uint16_t* y,
                       moe_stream_t stream);
 
-/* The training step's products, one launch each. gate_up_keep: qx [R,D/2] with
- * scales of stride moe_mxfp4_scale_ld(D) -> qh [R,H/2] with scales of stride
- * moe_mxfp4_scale_ld(H), and g, u in MXFP8 [R,H] with scales [R,H/32]. Rows past
- * sum(counts) are left alone; down zeroes them in y. */
+/* The training step's products, one launch each, for contractions that are
+ * multiples of 64. gate_up_keep: x in MXFP4, rows of moe_mxfp4_padded_cols(D)
+ * columns -> h in MXFP4, rows of moe_mxfp4_padded_cols(H), and g, u in MXFP8 [R,H]
+ * with scales [R,H/32]. Rows past sum(counts) are left alone; down zeroes them in
+ * y. */
 int moe_mxfp4_gemm_gate_up_keep(const uint8_t* qx, const uint8_t* sx, const uint8_t* qw1, const uint8_t* sw1,
                                 const uint8_t* qw3, const uint8_t* sw3, const int64_t* counts, int64_t n_rows,
                                 int32_t n_experts, int32_t dim, int32_t hidden, uint8_t* qh, uint8_t* sh,

@@ -98,8 +98,8 @@ SIGNATURES: dict[str, list] = {
     "moe_restore8_rows": [P, P, I64, I32, P, P],
     "moe_mxfp4_quant_rows": [P, I64, I32, I32, I32, P, P, P],
     "moe_mxfp4_dequant_rows": [P, P, I64, I32, I32, I32, P, P],
-    "moe_mxfp4_scale_ld": [I32],
-    "moe_mxfp4_workspace_bytes": [I64, I32, I32],
+    "moe_mxfp4_padded_cols": [I32],
+    "moe_mxfp4_workspace_bytes": [I64, I32, I32, I32],
     "moe_mxfp4_swiglu_fwd": [P, P, P, P, P, P, P, P, I64, I32, I32, I32, P, I64, P, P],
     "moe_mxfp4_oss_fwd": [P, P, P, P, P, P, P, P, I64, I32, I32, I32, F32, P, I64, P, P],
     "moe_mxfp4_gemm_gate_up_keep": [P, P, P, P, P, P, P, I64, I32, I32, I32, P, P, P, P, P, P, P],

@@ -25,6 +25,10 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kMaxE = 1024;
 
+// The columns of a row operand: whole stages of 256, so that every copy of a stage lies inside
+// its row, and zeros behind the contraction meet whatever is read of a weight row there.
+__host__ __device__ constexpr int padded(int cols) { return (cols + 255) / 256 * 256; }
+
 // ---------------------------------------------------------------------------
 // quantization and its inverse
 // ---------------------------------------------------------------------------
@@ -67,10 +71,10 @@ __device__ __forceinline__ uint32_t quad_block4(const Eight<T>& x, uint32_t& q) 
   return s;
 }
 
-// x as n_chunks chunks of eight elements; chunk c's codes are the word q[c], its block's scale
-// scale[c / 4], or, with rows of cpr chunks whose scales lie s_ld apart (s_ld > 0), in their row.
+// Rows of cpr chunks of eight elements to rows of ocpr >= cpr, zeros behind (ocpr == cpr: one
+// flat run of chunks). Chunk c's codes are the word q[c], its block's scale scale[c / 4].
 template <typename T>
-__global__ __launch_bounds__(256) void quant_kernel(const T* __restrict__ x, int64_t n_chunks, int cpr, int s_ld,
+__global__ __launch_bounds__(256) void quant_kernel(const T* __restrict__ x, int64_t n_chunks, int cpr, int ocpr,
                                                     uint32_t* __restrict__ q, uint8_t* __restrict__ scale) {
   const int64_t S = (int64_t)gridDim.x * 256;
   for (int64_t c0 = (int64_t)blockIdx.x * 256 + threadIdx.x; c0 - threadIdx.x < n_chunks; c0 += 4 * S) {
@@ -78,7 +82,15 @@ __global__ __launch_bounds__(256) void quant_kernel(const T* __restrict__ x, int
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int64_t c = c0 + u * S;
-      if (c < n_chunks) v[u].load(x + 8 * c);
+      int64_t at = c;
+      bool in = c < n_chunks;
+      if (ocpr != cpr) {
+        const int64_t r = c / ocpr;
+        const int k = (int)(c - r * ocpr);
+        at = r * cpr + k;
+        in = in && k < cpr;
+      }
+      if (in) v[u].load(x + 8 * at);
       else v[u].zero();
     }
 #pragma unroll
@@ -88,33 +100,39 @@ __global__ __launch_bounds__(256) void quant_kernel(const T* __restrict__ x, int
       const uint32_t s = quad_block4(v[u], w);
       if (c < n_chunks) {
         q[c] = w;
-        if ((c & 3) == 0) {
-          int64_t at = c >> 2;
-          if (s_ld) {
-            const int64_t r = c / cpr;
-            at = r * s_ld + ((c - r * cpr) >> 2);
-          }
-          scale[at] = (uint8_t)s;
-        }
+        if ((c & 3) == 0) scale[c >> 2] = (uint8_t)s;
       }
     }
   }
 }
 
-// codes back to values: chunk c's eight elements from the word q[c] and its block's scale, which
-// lies as in quant_kernel
+// rows of n scale bytes, each to ld bytes apart with 1.0 behind it
+__global__ __launch_bounds__(256) void pad_scales_kernel(const uint8_t* __restrict__ src, int64_t rows, int n, int ld,
+                                                         uint8_t* __restrict__ dst) {
+  const int64_t total = rows * (ld / 8), S = (int64_t)gridDim.x * 256;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += S) {
+    const int64_t r = i / (ld / 8);
+    const int c = (int)(i - r * (ld / 8)) * 8;
+    uint64_t w = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) w |= (uint64_t)(c + k < n ? src[r * n + c + k] : 0x7f) << (8 * k);
+    *(uint64_t*)(dst + r * ld + c) = w;
+  }
+}
+
+// codes back to values: rows of cpr chunks of eight from rows of icpr >= cpr
 template <typename T>
 __global__ __launch_bounds__(256) void dequant_kernel(const uint32_t* __restrict__ q, const uint8_t* __restrict__ scale,
-                                                      int64_t n_chunks, int cpr, int s_ld, T* __restrict__ x) {
+                                                      int64_t n_chunks, int cpr, int icpr, T* __restrict__ x) {
   const int64_t S = (int64_t)gridDim.x * 256;
   for (int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x; c < n_chunks; c += S) {
-    const uint32_t w = q[c];
-    int64_t at = c >> 2;
-    if (s_ld) {
+    int64_t at = c;
+    if (icpr != cpr) {
       const int64_t r = c / cpr;
-      at = r * s_ld + ((c - r * cpr) >> 2);
+      at = r * icpr + (c - r * cpr);
     }
-    const float s = mx::scale_value(scale[at]);
+    const uint32_t w = q[at];
+    const float s = mx::scale_value(scale[at >> 2]);
     float v[8];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -143,20 +161,19 @@ struct Params {
   int64_t R;              // rows; segments are clamped to them
   int E, K, N;            // contraction, and the output's columns (gate_up: H)
   const uint16_t* x;      // narrow gate_up: the rows in bf16 [R, K]
-  const uint8_t* qp;      // else rows [R, K / 2], their scales [R, p_ld], p_ld a multiple of 8
+  const uint8_t* qp;      // else rows of padded(K) columns in MXFP4, zeros past K, and their scales
   const uint8_t* sp;
-  int p_ld;
   const uint8_t* qa;      // weights: gate rows, or down's
   const uint8_t* sa;
   const uint8_t* qb;      // up rows
   const uint8_t* sb;
+  int w_ld;               // bytes between the scales of two weight rows
   int64_t e_rows;         // row n of expert e is row e * e_rows + n * r_rows of qa and qb
   int r_rows;
   const uint16_t* bias;   // gpt-oss: b1 [E, 2H] (glu 2j, linear 2j + 1), b2 [E, D]
   float limit;
-  uint8_t* qh;            // gate_up: h [R, H / 2], its scales [R, h_ld]
+  uint8_t* qh;            // gate_up: h, rows of padded(H) columns
   uint8_t* sh;
-  int h_ld;
   uint8_t* g8;            // gate_up with KEEP: g and u in MXFP8 [R, H], scales [R, H / 32]
   uint8_t* gs;
   uint8_t* u8;
@@ -176,14 +193,42 @@ __device__ __forceinline__ float activation(int act, float g, float u, float lim
 __device__ __forceinline__ void dma16(const void* g, uint32_t lds) {
   asm volatile("global_load_lds_dwordx4 %0, off" :: "v"(g), "{m0}"(lds) : "memory");
 }
+// The same with lane i's 4 bytes at lds + 4 i; and with its 2 bytes there, zeros above them.
+__device__ __forceinline__ void dma4(const void* g, uint32_t lds) {
+  asm volatile("global_load_lds_dword %0, off" :: "v"(g), "{m0}"(lds) : "memory");
+}
+__device__ __forceinline__ void dma2(const void* g, uint32_t lds) {
+  asm volatile("global_load_lds_ushort %0, off" :: "v"(g), "{m0}"(lds) : "memory");
+}
 __device__ __forceinline__ uint32_t lds_addr(const uint8_t* ptr) { return (uint32_t)(size_t)((LDSP const uint8_t*)ptr); }
 
-// Row-major LDS tile of 128-byte rows (256 k): byte offset of 16-byte chunk c of row r;
-// conflict-free where eight lanes read one chunk of eight rows.
-__device__ __forceinline__ int rm_off(int r, int c) { return r * 128 + ((c ^ ((r >> 1) & 7)) << 4); }
+// The same from a scalar base and a 32-bit offset per lane. (readfirstlane: under pressure the
+// compiler keeps uniform values in vector registers, which the instruction does not take there.
+// s_nop: a scalar register that a vector instruction has just written may be read by a memory
+// instruction five wait states later at the earliest, and the compiler, which keeps to that
+// elsewhere, does not look into the asm.)
+__device__ __forceinline__ uint64_t scalar(const uint8_t* p) {
+  const uint64_t v = (uint64_t)p;
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)v) |
+         ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32);
+}
+__device__ __forceinline__ void dma16(const uint8_t* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" :: "v"(off), "s"(scalar(base)), "{m0}"(lds) : "memory");
+}
+__device__ __forceinline__ void dma4(const uint8_t* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_nop 4\n\tglobal_load_lds_dword %0, %1" :: "v"(off), "s"(scalar(base)), "{m0}"(lds) : "memory");
+}
 
-__device__ const uint4 kZeroRow[8] = {};  // source of rows and k past an edge
-constexpr uint32_t kUnitScales = 0x7f7f7f7fu;
+template <int N, typename F>
+__device__ __forceinline__ void for_each(F f) {  // f(0), ..., f(N - 1) with compile-time indices
+  if constexpr (N > 0) {
+    for_each<N - 1>(f);
+    f(std::integral_constant<int, N - 1>{});
+  }
+}
+constexpr int kTileList = 64;
+
+__device__ const uint4 kZeroRow[8] = {};  // source of columns and k past an edge
 
 // Exclusive prefix sums of up to 1024 non-negative ints, four per thread of the first 256,
 // that stop at `most` (saturating sums are associative, and with most < 2^30 no step passes
@@ -282,9 +327,15 @@ __device__ __forceinline__ void store_hidden(const Params& p, int64_t r, int hc,
   }
   uint32_t q;
   const uint32_t s = mx::block4(ha, hb, q);
+  const int cols = padded(p.N);
   if (valid) {
-    *(uint32_t*)(p.qh + r * (p.N / 2) + hc / 2 + 4 * g4) = q;
-    if (g4 == 0) p.sh[r * p.h_ld + hc / kBlock] = (uint8_t)s;
+    uint32_t* row = (uint32_t*)(p.qh + r * (cols / 2));
+    row[hc / 8 + g4] = q;
+    if (g4 == 0) p.sh[r * (cols / kBlock) + hc / kBlock] = (uint8_t)s;
+    if (hc + kBlock == p.N) {  // the row's padding
+      for (int i = p.N / 8 + g4; i < cols / 8; i += 4) row[i] = 0;
+      for (int i = p.N / kBlock + g4; i < cols / kBlock; i += 4) p.sh[r * (cols / kBlock) + i] = 0;
+    }
   }
   if constexpr (KEEP) {
     uint2 kg, ku;
@@ -300,153 +351,168 @@ __device__ __forceinline__ void store_hidden(const Params& p, int64_t r, int hc,
   }
 }
 
-// Eight scale bytes of which `left` belong to the row (the others: 1.0).
-__device__ __forceinline__ uint2 masked_scales(uint2 v, int left) {
-  if (left >= 8) return v;
-  const uint64_t keep = (1ull << (8 * left)) - 1, unit = 0x7f7f7f7f7f7f7f7full;
-  const uint64_t m = ((((uint64_t)v.y << 32) | v.x) & keep) | (unit & ~keep);
-  return make_uint2((uint32_t)m, (uint32_t)(m >> 32));
-}
-
-// Many rows per expert: 256 x 256 outputs of eight 64 x 128 wave tiles, k in stages of 256 (128
-// bytes a row, as 128 k of 8-bit operands), two stages in LDS, persistent workgroups. The
-// operands reach LDS by direct-to-LDS copies, issued one stage ahead across tile boundaries;
-// the scales (8 bytes a row and stage) through registers, since a row of K / 32 scale bytes has
-// any alignment. MFMA step s of a stage takes chunk 2 q + s of a row in lane row q, so that a
-// lane's two scales are one 16-bit read. gate_up's columns alternate in blocks of 16 between
-// gate and up, so that a lane holds both.
-template <int MODE, int ACT, bool KEEP>
-__global__ __launch_bounds__(512, 1) void wide_kernel(Params p) {
-  constexpr int TM = 4, TN = 8, WGN = 2, BM = 256, BN = 256, CPW = 4;
-  __shared__ __attribute__((aligned(1024))) uint8_t sP[2][BM * 128];
-  __shared__ __attribute__((aligned(1024))) uint8_t sQ[2][BN * 128];
-  __shared__ __attribute__((aligned(16))) uint2 sS[2][BM + BN];
-  __shared__ int s_seg[kMaxE + 1];
-  __shared__ int s_tile[kMaxE + 1];
+// Many rows per expert: tiles of (16 TM WGM) rows x 256 columns by NW waves, k in stages of RB
+// bytes a row (two k an byte), NS stages in LDS, persistent workgroups of eight waves in all
+// per CU. Operands and scales reach LDS by direct-to-LDS copies, NS - 1 stages ahead and across tile
+// boundaries; rows past a segment are not copied, since what they hold stays in output rows
+// that are not stored. PAIR: the weights' scale rows are only 2-byte aligned (w_ld even but not
+// a multiple of 4) and are copied as pairs; odd ones come here padded (pad_scales_kernel). gate_up's columns alternate in blocks of 16
+// between gate and up, so that a lane holds both.
+template <int MODE, int ACT, bool KEEP, int NW, int WGM, int TM, int TN, int NS, int RB, bool PAIR>
+__global__ __launch_bounds__(NW * 64, 2) void wide_kernel(Params p) {
+  constexpr int WGN = NW / WGM, BM = WGM * TM * 16, BN = WGN * TN * 16;
+  constexpr int KH = RB / 64, RPC = 1024 / RB, CPR = RB / 16;  // MFMA steps a stage; rows of a 1 KB copy; chunks of a row
+  constexpr int PW = BM / RPC / NW, SPC = BM * KH / 64, SPW = (SPC + NW - 1) / NW;  // a wave's copies of P, of its scales
+  constexpr int QC = BN / RPC / NW, SQC = BN * KH / 64 / NW * (PAIR ? 2 : 1);  // a wave's copies of Q and of its scales
+  static_assert((RB == 64 || RB == 128) && BN == 256 && NS >= 2 && TN % 4 == 0, "tile");
+  static_assert(PW * RPC * NW == BM && QC * RPC * NW == BN && SQC >= 1 && BM * KH % 64 == 0, "copies");
+  __shared__ __attribute__((aligned(1024))) uint8_t sP[NS][BM * RB];
+  __shared__ __attribute__((aligned(1024))) uint8_t sQ[NS][BN * RB];
+  // scales: row m's RB / 16 at RB / 16 m; PAIR: pair h of row n at 4 (BN h + n)
+  __shared__ __attribute__((aligned(16))) uint8_t sSP[NS][SPC * 256];
+  __shared__ __attribute__((aligned(16))) uint8_t sSQ[NS][SQC * NW * 256];
+  __shared__ int4 s_list[kTileList];  // this workgroup's first tiles: first row, end of the segment, expert, column tile
   __shared__ int s_tmp[8];
+  extern __shared__ __attribute__((aligned(16))) int s_dyn_i[];
+  int* s_seg = s_dyn_i;           // E + 1
+  int* s_tile = s_seg + p.E + 1;  // E + 1
 
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wv / WGN, wn = wv % WGN, ml = lane & 15, g4 = lane >> 4;
   const int E = p.E, K = p.K, N = p.N, KB = K / kBlock, kbytes = K / 2;
   const int NT = MODE == kGateUp ? (N + BN / 2 - 1) / (BN / 2) : (N + BN - 1) / BN;
-  const int nk = (K + 255) / 256;
+  const int nk = (kbytes + RB - 1) / RB;
   segments(p, s_seg, s_tile, s_tmp, [&](int rows) { return (rows + BM - 1) / BM * NT; });
   const int total_tiles = s_tile[E], G = gridDim.x;
   // each XCD works on a contiguous window of tiles
   const int lb = G % 8 == 0 ? (int)(blockIdx.x & 7) * (G >> 3) + (int)(blockIdx.x >> 3) : (int)blockIdx.x;
 
-  struct TileRef { int e, seg0, seg1, mt, nt; };
-  auto decode = [&](int t) {
-    TileRef r;
-    r.e = find(s_tile, E, t);
-    const int local = t - s_tile[r.e];
-    r.seg0 = s_seg[r.e];
-    r.seg1 = s_seg[r.e + 1];
-    const int mtiles = (r.seg1 - r.seg0 + BM - 1) / BM;
-    r.nt = local / mtiles;
-    r.mt = local - r.nt * mtiles;
-    return r;
+  // tile t: a search over the experts and a division, 2000 cycles of dependent LDS reads if a wave
+  // does it between its MFMAs, so the list is made first, a tile a thread
+  auto search = [&](int t) {
+    const int e = find(s_tile, E, t), local = t - s_tile[e], seg0 = s_seg[e], seg1 = s_seg[e + 1];
+    const int mtiles = (seg1 - seg0 + BM - 1) / BM, nt = local / mtiles;
+    return make_int4(seg0 + (local - nt * mtiles) * BM, seg1, e, nt);
   };
-  // row n of the tile's weight columns: its tensor, row number, and whether it is inside
-  auto weight_row = [&](const TileRef& r, int n, bool& up, bool& in) -> int64_t {
-    int col;
-    if (MODE == kGateUp) {
-      const int blk = n >> 4;
-      col = r.nt * (BN / 2) + (blk >> 1) * 16 + (n & 15);
-      up = blk & 1;
-    } else {
-      col = r.nt * BN + n;
-      up = false;
-    }
-    in = col < N;
-    return r.e * p.e_rows + (int64_t)col * p.r_rows;
+  if (tid < kTileList && lb + (int64_t)tid * G < total_tiles) s_list[tid] = search(lb + tid * G);
+  __syncthreads();
+  struct TileRef { int row0, seg1, e, nt; };
+  auto decode = [&](int i) {  // this workgroup's i-th tile
+    int4 v;
+    if (i < kTileList) v = s_list[i];
+    else v = search(lb + i * G);
+    return TileRef{__builtin_amdgcn_readfirstlane(v.x), __builtin_amdgcn_readfirstlane(v.y),
+                   __builtin_amdgcn_readfirstlane(v.z), __builtin_amdgcn_readfirstlane(v.w)};
   };
+  const int my_tiles = lb < total_tiles ? (total_tiles - lb + G - 1) / G : 0;
 
-  // ---- sources of the tile being copied: copy b of this wave fills rows 8 (4 wv + b) .. + 7,
-  // lane i row i / 8, chunk i % 8 with the row's chunk (i % 8) ^ ((row >> 1) & 7) ----
-  const int crow = lane >> 3;
-  const uint8_t* srcP[CPW];
-  const uint8_t* srcQ[CPW];
-  int ch[CPW];
-  bool okP[CPW], okQ[CPW];
-#pragma unroll
-  for (int b = 0; b < CPW; ++b) ch[b] = (lane & 7) ^ ((((wv * CPW + b) * 8 + crow) >> 1) & 7);
-  const uint8_t* srcS = nullptr;  // this thread's row of scales: tid < 256 P row tid, else Q row tid - 256
-  bool okS = false;
+  // ---- copies. One fills RPC rows, lane i row i / CPR, chunk i % CPR with the row's chunk
+  // (i % CPR) ^ ((row >> 1) & (CPR - 1)) (eight lanes that read one chunk of eight rows meet no bank
+  // twice). A source is a base of the tile and stage in scalar registers and a 32-bit offset per
+  // lane. Nothing branches: rows past a segment or the last column repeat the last one inside
+  // (what they give is not stored), chunks past a weight row's end the last one of the row (the
+  // other operand has zeros there), and behind the last stage of a workgroup the last tile's
+  // first is copied once more. ----
+  auto swz = [](int row) { return (row >> 1) & (CPR - 1); };
+  auto q_col = [](int n) { return MODE == kGateUp ? (n >> 5) * 16 + (n & 15) : n; };  // in the tile's columns
+  // word i of the scale copies: of P row i / KH, dword i % KH; of Q the same, PAIR row i % BN, pair
+  // i / BN. Fewer copies than waves: some waves write the same words
+  auto sq_off = [&](int b) {
+    const int i = (wv * SQC + b) * 64 + lane;
+    return PAIR ? i / BN * 2 : i % KH * 4;
+  };
+  const int p_ld = padded(K) / 2, sp_ld = padded(K) / kBlock;
+  const uint8_t *baseP, *baseSP, *baseQ[2];  // of the tile being copied: P, its scales, gate (or down) and up
+  uint32_t offP[PW], offQ[QC], offSP[SPW];
+  const uint8_t* srcSQ[SQC];
   auto setup = [&](const TileRef& r) {
-    const int row0 = r.seg0 + r.mt * BM;
+    int ln = lane;
+    asm volatile("" : "+v"(ln));  // what a tile's offsets come from is made again, not kept in registers
+    const int crow = ln / CPR, cbit = ln % CPR;
+    const int last = r.seg1 - 1 - r.row0, col0 = r.nt * (MODE == kGateUp ? BN / 2 : BN), last_col = N - 1 - col0;
+    baseP = p.qp + (int64_t)r.row0 * p_ld;
+    baseSP = p.sp + (int64_t)r.row0 * sp_ld;
+    const int64_t wr = r.e * p.e_rows + (int64_t)col0 * p.r_rows;
+    baseQ[0] = p.qa + wr * kbytes;
+    if (MODE == kGateUp) baseQ[1] = p.qb + wr * kbytes;
 #pragma unroll
-    for (int b = 0; b < CPW; ++b) {
-      const int m = (wv * CPW + b) * 8 + crow;
-      okP[b] = row0 + m < r.seg1;
-      srcP[b] = p.qp + (int64_t)(row0 + m) * kbytes + ch[b] * 16;
-      bool up;
-      const int64_t wr = weight_row(r, m, up, okQ[b]);
-      srcQ[b] = (up ? p.qb : p.qa) + wr * kbytes + ch[b] * 16;
+    for (int b = 0; b < PW; ++b) {
+      const int m = (wv * PW + b) * RPC + crow;
+      offP[b] = __umul24(min(m, last), p_ld) + (cbit ^ swz(m)) * 16;
     }
-    if (tid < BM) {
-      okS = row0 + tid < r.seg1;
-      srcS = p.sp + (int64_t)(row0 + tid) * p.p_ld;
+#pragma unroll
+    for (int b = 0; b < QC; ++b)
+      offQ[b] = __umul24(min(q_col((wv * QC + b) * RPC + crow), last_col), p.r_rows * kbytes);
+#pragma unroll
+    for (int b = 0; b < SPW; ++b) {
+      const int i = (wv * SPW + b) % SPC * 64 + ln;
+      offSP[b] = __umul24(min(i / KH, last), sp_ld) + i % KH * 4;
+    }
+#pragma unroll
+    for (int b = 0; b < SQC; ++b) {
+      const int i = (wv * SQC + b) * 64 + ln, n = PAIR ? i % BN : i / KH;
+      const uint8_t* base = (MODE == kGateUp && ((n >> 4) & 1) ? p.sb : p.sa) + wr * p.w_ld;
+      srcSQ[b] = base + __umul24(min(q_col(n), last_col), p.r_rows * p.w_ld);
+    }
+  };
+  constexpr int NCOPY = SPW + PW + SQC + QC;
+  auto copy = [&](auto c_c, int kt, int s) {  // copy c of stage kt into buffer s
+    constexpr int c = decltype(c_c)::value;
+    if constexpr (c < SPW) {
+      constexpr int b = c;
+      dma4(baseSP + kt * CPR, offSP[b], lds_addr(&sSP[s][(wv * SPW + b) % SPC * 256]));
+    } else if constexpr (c < SPW + PW) {
+      constexpr int b = c - SPW;
+      dma16(baseP + kt * RB, offP[b], lds_addr(&sP[s][(wv * PW + b) * 1024]));
+    } else if constexpr (c < SPW + PW + SQC) {
+      constexpr int b = c - SPW - PW;
+      const uint32_t lds = lds_addr(&sSQ[s][(wv * SQC + b) * 256]);
+      if constexpr (PAIR) dma2(srcSQ[b] + min(kt * CPR + sq_off(b), p.w_ld - 2), lds);
+      else dma4(srcSQ[b] + min(kt * CPR + sq_off(b), p.w_ld - 4), lds);
     } else {
-      bool up;
-      const int64_t wr = weight_row(r, tid - BM, up, okS);
-      srcS = (up ? p.sb : p.sa) + wr * KB;
+      constexpr int b = c - SPW - PW - SQC;
+      const uint8_t* base = MODE == kGateUp && (((wv * QC + b) * RPC >> 4) & 1) ? baseQ[1] : baseQ[0];
+      const int chunk = min(kt * CPR + (lane % CPR ^ swz((wv * QC + b) * RPC + lane / CPR)), KB - 1);
+      dma16(base, offQ[b] + chunk * 16, lds_addr(&sQ[s][(wv * QC + b) * 1024]));
     }
   };
-  const bool p_side = tid < BM;
-  uint2 scales;  // of the stage in flight
-  auto issue = [&](int kt, int s) {
-#pragma unroll
-    for (int b = 0; b < CPW; ++b) {
-      const bool in = kt * 8 + ch[b] < KB;
-      dma16(okP[b] && in ? (const void*)(srcP[b] + kt * 128) : (const void*)kZeroRow, lds_addr(&sP[s][(wv * CPW + b) * 1024]));
+  int ct = 0, ik = 0, bi = 0, bc = 0;  // copy cursor: tile ct, its stage ik, buffer bi; the buffer bc that is read next
+  auto advance = [&]() {
+    bi = bi + 1 == NS ? 0 : bi + 1;
+    if (++ik == nk) {
+      ik = 0;
+      if (++ct < my_tiles) setup(decode(ct));
     }
+  };
+  if (my_tiles) {
+    setup(decode(0));
 #pragma unroll
-    for (int b = 0; b < CPW; ++b) {
-      const bool in = kt * 8 + ch[b] < KB;
-      dma16(okQ[b] && in ? (const void*)(srcQ[b] + kt * 128) : (const void*)kZeroRow, lds_addr(&sQ[s][(wv * CPW + b) * 1024]));
+    for (int i = 0; i < NS - 1; ++i) {
+      if (i) advance();
+      for_each<NCOPY>([&](auto c) { copy(c, ik, bi); });
     }
-    const int left = KB - kt * 8;  // scale bytes of this stage and after it
-    uint32_t w0 = kUnitScales, w1 = kUnitScales;
-    if (okS) {
-      const uint8_t* src = srcS + kt * 8;
-      if (p_side || KB % 8 == 0) {
-        const uint2 v = masked_scales(*(const uint2*)src, left);  // rows of P's scales are padded to whole words
-        w0 = v.x;
-        w1 = v.y;
-      } else if (KB % 2 == 0) {
-        uint32_t h[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) h[i] = 2 * i < left ? *(const uint16_t*)(src + 2 * i) : 0x7f7fu;
-        w0 = h[0] | (h[1] << 16);
-        w1 = h[2] | (h[3] << 16);
-      } else {
-        uint32_t c[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) c[i] = i < left ? src[i] : 0x7fu;
-        w0 = c[0] | (c[1] << 8) | (c[2] << 16) | (c[3] << 24);
-        w1 = c[4] | (c[5] << 8) | (c[6] << 16) | (c[7] << 24);
-      }
-    }
-    scales = make_uint2(w0, w1);
-  };
-  int ct = lb, ik = 0, gi = 0, gc = 0;  // copy cursor: tile ct, its stage ik; stage gi goes to buffer gi % 2
-  auto seek = [&](int t) {
-    ct = t;
-    ik = 0;
-    if (ct < total_tiles) setup(decode(ct));
-  };
-  auto issue_next = [&]() {
-    issue(ik, gi & 1);
-    ++gi;
-    if (++ik == nk) seek(ct + G);
-  };
-  seek(lb);
-  if (ct < total_tiles) issue_next();
+  }
 
-  for (int t = lb; t < total_tiles; t += G) {
+  for (int t = 0; t < my_tiles; ++t) {
     const TileRef cur = decode(t);
-    const int row0 = cur.seg0 + cur.mt * BM, seg1 = cur.seg1;
+    const int row0 = cur.row0, seg1 = cur.seg1;
+    // every wave issues NCOPY copies a stage, so a stage has landed once those of the NS - 2
+    // stages after it are outstanding (stores of an epilogue only add to the count); the barrier
+    // also retires every read of the buffer that is filled next
+    auto stage_in = [&]() {
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"((NS - 2) * NCOPY) : "memory");
+    };
+    // 16-row blocks of this wave with rows in them; a wave without any only copies
+    const int tmv = min(TM, max(0, (seg1 - (row0 + wm * TM * 16) + 15) >> 4));
+    if (tmv == 0) {
+      for (int kt = 0; kt < nk; ++kt) {
+        advance();
+        stage_in();
+        bc = bc + 1 == NS ? 0 : bc + 1;
+        for_each<NCOPY>([&](auto c) { copy(c, ik, bi); });
+      }
+      continue;
+    }
     f32x4_t acc[TM][TN];
 #pragma unroll
     for (int i = 0; i < TM; ++i)
@@ -454,50 +520,58 @@ __global__ __launch_bounds__(512, 1) void wide_kernel(Params p) {
       for (int j = 0; j < TN; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
     for (int kt = 0; kt < nk; ++kt) {
-      // this stage's copies and scales have landed; its scales go to LDS (the buffer's last
-      // readers are two stages back); the barrier also retires every read of the buffer
-      // that is filled next
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      sS[gc & 1][tid] = scales;
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      if (ct < total_tiles) issue_next();
-      __builtin_amdgcn_sched_barrier(0);
-      const int sl = gc & 1;
-      ++gc;
+      advance();  // ahead of the MFMAs, which the compiler would otherwise sink behind its branches
+      stage_in();
+      const uint8_t *cP = sP[bc], *cQ = sQ[bc], *cSP = sSP[bc], *cSQ = sSQ[bc];
+      bc = bc + 1 == NS ? 0 : bc + 1;
+      // lane row g4 takes a row's chunk KH g4 + step, so that its scales of a stage lie side by side
       int scp[TM], scq[TN];
-      const uint8_t* ss = (const uint8_t*)sS[sl];
-#pragma unroll
-      for (int i = 0; i < TM; ++i) scp[i] = *(const uint16_t*)(ss + (wm * 64 + i * 16 + ml) * 8 + 2 * g4);
-#pragma unroll
-      for (int j = 0; j < TN; ++j) scq[j] = *(const uint16_t*)(ss + (BM + wn * 128 + j * 16 + ml) * 8 + 2 * g4);
-      auto frag = [&](const uint8_t* tile, int row, int s) {
-        const uint4 v = *(const uint4*)(tile + rm_off(row, 2 * g4 + s));
+      v8i_t af[TM], bq[2];
+      auto frag = [&](const uint8_t* tile, int row, int step) {
+        const uint4 v = *(const uint4*)(tile + row * RB + (((KH * g4 + step) ^ swz(row)) << 4));
         return v8i_t{(int)v.x, (int)v.y, (int)v.z, (int)v.w, 0, 0, 0, 0};
       };
+      auto scale_at = [&](const uint8_t* at) { return KH == 2 ? (int)*(const uint16_t*)at : (int)*at; };
+#pragma unroll
+      for (int i = 0; i < TM; ++i) scp[i] = scale_at(cSP + ((wm * TM + i) * 16 + ml) * CPR + KH * g4);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const int n = (wn * TN + j) * 16 + ml;
+        if constexpr (!PAIR) scq[j] = scale_at(cSQ + n * CPR + KH * g4);
+        else if constexpr (KH == 2) scq[j] = *(const int*)(cSQ + (BN * g4 + n) * 4);
+        else scq[j] = cSQ[(BN * (g4 >> 1) + n) * 4 + (g4 & 1)];
+      }
+      // the next stage's copies go between the MFMAs, one behind each of the first blocks of
+      // columns: issued together right behind the barrier they hold every wave up at once (a
+      // copy takes the CU's address path 16 cycles)
       auto step = [&](auto s_c) {
-        constexpr int s = decltype(s_c)::value;
-        v8i_t af[TM], bq[2];
+        constexpr int st = decltype(s_c)::value;
 #pragma unroll
-        for (int i = 0; i < TM; ++i) af[i] = frag(sP[sl], wm * 64 + i * 16 + ml, s);
-        bq[0] = frag(sQ[sl], wn * 128 + ml, s);
-#pragma unroll
-        for (int j = 0; j < TN; ++j) {
-          if (j + 1 < TN) bq[(j + 1) & 1] = frag(sQ[sl], wn * 128 + (j + 1) * 16 + ml, s);
+        for (int i = 0; i < TM; ++i) af[i] = frag(cP, (wm * TM + i) * 16 + ml, st);
+        bq[0] = frag(cQ, wn * TN * 16 + ml, st);
+        for_each<TN>([&](auto j_c) {
+          constexpr int j = decltype(j_c)::value;
+          if constexpr (j + 1 < TN) bq[(j + 1) & 1] = frag(cQ, (wn * TN + j + 1) * 16 + ml, st);
 #pragma unroll
           for (int i = 0; i < TM; ++i)
-            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(bq[j & 1], af[i], acc[i][j], 4, 4, s, scq[j],
-                                                                         s, scp[i]);
-        }
+            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(bq[j & 1], af[i], acc[i][j], 4, 4, st, scq[j],
+                                                                         st, scp[i]);
+          constexpr int slot = st * TN + j, slots = KH * TN;
+          for_each<NCOPY>([&](auto c) {
+            if constexpr (decltype(c)::value * slots / NCOPY == slot) copy(c, ik, bi);
+          });
+          __builtin_amdgcn_sched_barrier(0);
+        });
       };
       step(std::integral_constant<int, 0>{});
-      step(std::integral_constant<int, 1>{});
+      if constexpr (KH == 2) step(std::integral_constant<int, 1>{});
     }
 
     // ---- epilogue: lane holds C[m = .. + ml][n = .. + 4 g4 .. + 3] of each 16-column block ----
     if (MODE == kGateUp) {
 #pragma unroll
       for (int b = 0; b < TN / 4; ++b) {
-        const int hc = cur.nt * (BN / 2) + wn * 64 + b * 32;
+        const int hc = cur.nt * (BN / 2) + wn * (TN * 8) + b * 32;
         if (hc >= N) continue;
         uint4 bias_a{}, bias_b{};
         if constexpr (ACT == kOssGLU) {
@@ -507,7 +581,8 @@ __global__ __launch_bounds__(512, 1) void wide_kernel(Params p) {
         }
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
-          const int r = row0 + wm * 64 + i * 16 + ml;
+          if (i >= tmv) continue;
+          const int r = row0 + (wm * TM + i) * 16 + ml;
           float v[4][4];
 #pragma unroll
           for (int j = 0; j < 4; ++j)
@@ -519,7 +594,7 @@ __global__ __launch_bounds__(512, 1) void wide_kernel(Params p) {
     } else {
 #pragma unroll
       for (int b = 0; b < TN / 2; ++b) {
-        const int n0 = cur.nt * BN + wn * 128 + b * 32;
+        const int n0 = cur.nt * BN + wn * TN * 16 + b * 32;
         if (n0 >= N) continue;
         float ba[4] = {0.f, 0.f, 0.f, 0.f}, bb[4] = {0.f, 0.f, 0.f, 0.f};
         if constexpr (ACT == kOssGLU) {
@@ -529,7 +604,8 @@ __global__ __launch_bounds__(512, 1) void wide_kernel(Params p) {
         }
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
-          const int r = row0 + wm * 64 + i * 16 + ml;
+          if (i >= tmv) continue;
+          const int r = row0 + (wm * TM + i) * 16 + ml;
           float lo[4], hi[4];
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
@@ -542,6 +618,7 @@ __global__ __launch_bounds__(512, 1) void wide_kernel(Params p) {
       }
     }
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the last copies write LDS that is not this workgroup's later
   if (MODE == kDown) zero_rest(p, s_seg[E]);
 }
 
@@ -593,7 +670,7 @@ __global__ __launch_bounds__(512, 2) void narrow_kernel(Params p) {
     const bool up = MODE == kGateUp && nb >= 2, in = col < N;
     const int64_t row = u.e * p.e_rows + (int64_t)col * p.r_rows;
     const uint8_t* wq = (up ? p.qb : p.qa) + row * kbytes;
-    const uint8_t* ws = (up ? p.sb : p.sa) + row * KB;
+    const uint8_t* ws = (up ? p.sb : p.sa) + row * p.w_ld;
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       const int c = 8 * (ks + 2 * (base + i)) + 2 * g4;  // this lane's first chunk of 32 k
@@ -634,12 +711,11 @@ __global__ __launch_bounds__(512, 2) void narrow_kernel(Params p) {
     } else {
       for (int i = tid; i < rows * KB; i += 512) {
         const int r = i / KB, c = i - r * KB;
-        *(uint4*)(sP + r * stride + c * 16) = *(const uint4*)(p.qp + (int64_t)(row0 + r) * kbytes + c * 16);
+        *(uint4*)(sP + r * stride + c * 16) = *(const uint4*)(p.qp + (int64_t)(row0 + r) * (padded(K) / 2) + c * 16);
       }
       for (int i = tid; i < rows * nst; i += 512) {
         const int r = i / nst, st = i - r * nst;
-        *(uint2*)(sc + r * sld + st * 8) =
-            masked_scales(*(const uint2*)(p.sp + (int64_t)(row0 + r) * p.p_ld + st * 8), KB - st * 8);
+        *(uint2*)(sc + r * sld + st * 8) = *(const uint2*)(p.sp + (int64_t)(row0 + r) * (padded(K) / kBlock) + st * 8);
       }
     }
   };
@@ -755,13 +831,25 @@ static int cu_count() {
 
 constexpr int kLdsMost = 144 * 1024;  // dynamic LDS of the narrow kernel (160 KB less its static part)
 
+template <int MODE, int ACT, bool KEEP, int NW, int WGM, int TM, int TN, int NS, int RB>
+static void launch_wide_cfg(const Params& p, hipStream_t stream) {
+  constexpr int BM = WGM * TM * 16;
+  const int64_t nt = MODE == kGateUp ? (p.N + 127) / 128 : (p.N + 255) / 256;
+  int64_t g = (p.R / BM + (p.R < p.E ? p.R : p.E)) * nt;
+  const int64_t most = (int64_t)cu_count() * (8 / NW);
+  if (g > most) g = most;
+  if (g >= 8) g -= g % 8;
+  const unsigned lds = 2 * (p.E + 1) * sizeof(int);
+  if (p.w_ld % 4 == 0)
+    hipLaunchKernelGGL((wide_kernel<MODE, ACT, KEEP, NW, WGM, TM, TN, NS, RB, false>), dim3((unsigned)g), dim3(NW * 64), lds, stream, p);
+  else
+    hipLaunchKernelGGL((wide_kernel<MODE, ACT, KEEP, NW, WGM, TM, TN, NS, RB, true>), dim3((unsigned)g), dim3(NW * 64), lds, stream, p);
+}
 template <int MODE, int ACT, bool KEEP>
 static void launch_wide(const Params& p, hipStream_t stream) {
-  const int64_t nt = MODE == kGateUp ? (p.N + 127) / 128 : (p.N + 255) / 256;
-  int64_t g = (p.R / 256 + p.E) * nt, cus = cu_count();
-  if (g > cus) g = cus;
-  if (g >= 8) g -= g % 8;
-  hipLaunchKernelGGL((wide_kernel<MODE, ACT, KEEP>), dim3((unsigned)g), dim3(512), 0, stream, p);
+  const int64_t used = p.R < p.E ? p.R : p.E;
+  if (p.R <= 64 * used) launch_wide_cfg<MODE, ACT, KEEP, 4, 1, 4, 4, 3, 64>(p, stream);
+  else launch_wide_cfg<MODE, ACT, KEEP, 8, 4, 4, 8, 2, 128>(p, stream);
 }
 template <int MODE, int ACT, int TM>
 static void launch_narrow_tm(const Params& p, hipStream_t stream) {
@@ -795,23 +883,25 @@ static bool takes_narrow(int64_t R, int64_t E, int D, int H) {
 
 static int check_shape(int64_t R, int E, int D, int H) {
   if (R < 0 || E < 1 || E > kMaxE || D < kBlock || H < kBlock) return kErrInvalidArgument;
-  if (D % kBlock || H % kBlock || D > (1 << 24) || H > (1 << 24)) return kErrUnsupportedShape;
+  if (D % kBlock || H % kBlock || D > (1 << 22) || H > (1 << 22)) return kErrUnsupportedShape;
   if (R >= (int64_t)INT32_MAX / 2) return kErrUnsupportedShape;
   // tiles and units are counted in 32 bits
   if ((R / 16 + E) * ((int64_t)(D > H ? D : H) / 32 + 1) >= (int64_t)0x3fffffff) return kErrUnsupportedShape;
   return kOk;
 }
-static int padded_blocks(int cols) { return (cols / kBlock + 7) / 8 * 8; }
-static bool aligned16(const void* a) { return ((uintptr_t)a & 15) == 0; }
 static int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
+static int padded_blocks(int cols) { return padded(cols) / kBlock; }
+static int64_t row_bytes(int64_t rows, int cols) { return up256(rows * (padded(cols) / 2)); }
+static int64_t row_scales(int64_t rows, int cols) { return up256(rows * padded_blocks(cols)); }
+static bool aligned16(const void* a) { return ((uintptr_t)a & 15) == 0; }
 
 template <typename T>
-static void launch_quant(const void* x, int64_t rows, int cols, int s_ld, uint8_t* q, uint8_t* scale, hipStream_t stream) {
-  const int64_t chunks = rows * (cols / 8);
+static void launch_quant(const void* x, int64_t rows, int cols, int out_cols, uint8_t* q, uint8_t* scale, hipStream_t stream) {
+  const int64_t chunks = rows * (out_cols / 8);
   int64_t g = (chunks + 1023) / 1024;
   if (g > 16384) g = 16384;
-  hipLaunchKernelGGL(quant_kernel<T>, dim3((unsigned)g), dim3(256), 0, stream, (const T*)x, chunks, cols / 8,
-                     s_ld == cols / kBlock ? 0 : s_ld, (uint32_t*)q, scale);
+  hipLaunchKernelGGL(quant_kernel<T>, dim3((unsigned)g), dim3(256), 0, stream, (const T*)x, chunks, cols / 8, out_cols / 8,
+                     (uint32_t*)q, scale);
 }
 
 }  // namespace mxfp4
@@ -820,41 +910,53 @@ static void launch_quant(const void* x, int64_t rows, int cols, int s_ld, uint8_
 using namespace moe;
 using namespace moe::mxfp4;
 
-MOE_API int moe_mxfp4_quant_rows(const void* x, int64_t rows, int32_t cols, int32_t dtype, int32_t scale_ld,
-                                 uint8_t* q, uint8_t* scale, hipStream_t stream) {
-  if (rows < 0 || cols < kBlock || cols % kBlock || scale_ld < cols / kBlock || (dtype != 0 && dtype != 1))
+MOE_API int moe_mxfp4_padded_cols(int32_t cols) {
+  return cols < kBlock || cols % kBlock || cols > (1 << 30) ? kErrInvalidArgument : padded(cols);
+}
+
+static int check_rows(const void* x, int64_t rows, int32_t cols, int32_t q_cols, int32_t dtype, const void* q, const void* scale) {
+  if (rows < 0 || cols < kBlock || cols % kBlock || q_cols < cols || q_cols % kBlock || (dtype != 0 && dtype != 1))
     return kErrInvalidArgument;
-  if (rows == 0) return kOk;
-  if (!x || !q || !scale || !aligned16(x) || !aligned16(q)) return kErrInvalidArgument;
-  if (dtype == 0) launch_quant<uint16_t>(x, rows, cols, scale_ld, q, scale, stream);
-  else launch_quant<float>(x, rows, cols, scale_ld, q, scale, stream);
+  if (rows && (!x || !q || !scale || !aligned16(x) || !aligned16(q))) return kErrInvalidArgument;
+  return kOk;
+}
+
+MOE_API int moe_mxfp4_quant_rows(const void* x, int64_t rows, int32_t cols, int32_t q_cols, int32_t dtype, uint8_t* q,
+                                 uint8_t* scale, hipStream_t stream) {
+  const int st = check_rows(x, rows, cols, q_cols, dtype, q, scale);
+  if (st || rows == 0) return st;
+  if (dtype == 0) launch_quant<uint16_t>(x, rows, cols, q_cols, q, scale, stream);
+  else launch_quant<float>(x, rows, cols, q_cols, q, scale, stream);
   return launch_status();
 }
 
-MOE_API int moe_mxfp4_dequant_rows(const uint8_t* q, const uint8_t* scale, int64_t rows, int32_t cols,
-                                   int32_t scale_ld, int32_t dtype, void* x, hipStream_t stream) {
-  if (rows < 0 || cols < kBlock || cols % kBlock || scale_ld < cols / kBlock || (dtype != 0 && dtype != 1))
-    return kErrInvalidArgument;
-  if (rows == 0) return kOk;
-  if (!x || !q || !scale || !aligned16(x) || !aligned16(q)) return kErrInvalidArgument;
+MOE_API int moe_mxfp4_dequant_rows(const uint8_t* q, const uint8_t* scale, int64_t rows, int32_t cols, int32_t q_cols,
+                                   int32_t dtype, void* x, hipStream_t stream) {
+  const int st = check_rows(x, rows, cols, q_cols, dtype, q, scale);
+  if (st || rows == 0) return st;
   const int64_t chunks = rows * (cols / 8);
   int64_t g = (chunks + 255) / 256;
   if (g > 16384) g = 16384;
-  const int s_ld = scale_ld == cols / kBlock ? 0 : scale_ld;
   if (dtype == 0)
-    hipLaunchKernelGGL(dequant_kernel<uint16_t>, dim3((unsigned)g), dim3(256), 0, stream, (const uint32_t*)q, scale, chunks, cols / 8, s_ld, (uint16_t*)x);
+    hipLaunchKernelGGL(dequant_kernel<uint16_t>, dim3((unsigned)g), dim3(256), 0, stream, (const uint32_t*)q, scale, chunks,
+                       cols / 8, q_cols / 8, (uint16_t*)x);
   else
-    hipLaunchKernelGGL(dequant_kernel<float>, dim3((unsigned)g), dim3(256), 0, stream, (const uint32_t*)q, scale, chunks, cols / 8, s_ld, (float*)x);
+    hipLaunchKernelGGL(dequant_kernel<float>, dim3((unsigned)g), dim3(256), 0, stream, (const uint32_t*)q, scale, chunks,
+                       cols / 8, q_cols / 8, (float*)x);
   return launch_status();
 }
 
-MOE_API int moe_mxfp4_scale_ld(int32_t cols) { return cols < kBlock || cols % kBlock ? kErrInvalidArgument : padded_blocks(cols); }
+// bytes of scales of the weights' rows that take a padded copy: odd rows, for the wide kernel
+static int64_t odd_scales(int64_t rows, int cols) { return cols / kBlock % 2 ? up256(rows * padded_blocks(cols)) : 0; }
 
-// workspace of the experts' forward: x in MXFP4 with its scales, h with its scales
-MOE_API int64_t moe_mxfp4_workspace_bytes(int64_t n_rows, int32_t dim, int32_t hidden) {
-  if (n_rows < 0 || dim < kBlock || hidden < kBlock || dim % kBlock || hidden % kBlock) return kErrInvalidArgument;
-  return up256(n_rows * (dim / 2)) + up256(n_rows * padded_blocks(dim)) + up256(n_rows * (hidden / 2)) +
-         up256(n_rows * padded_blocks(hidden));
+// workspace of the experts' forward: x in MXFP4 with its scales, h with its scales, and padded
+// copies of odd scale rows
+MOE_API int64_t moe_mxfp4_workspace_bytes(int64_t n_rows, int32_t n_experts, int32_t dim, int32_t hidden) {
+  if (n_rows < 0 || n_experts < 1 || dim < kBlock || hidden < kBlock || dim % kBlock || hidden % kBlock)
+    return kErrInvalidArgument;
+  const int64_t rows = row_bytes(n_rows, dim) + row_scales(n_rows, dim) + row_bytes(n_rows, hidden) + row_scales(n_rows, hidden);
+  return rows + (takes_narrow(n_rows, n_experts, dim, hidden)
+                     ? 0 : odd_scales(2 * (int64_t)n_experts * hidden, dim) + odd_scales((int64_t)n_experts * dim, hidden));
 }
 
 namespace moe {
@@ -872,30 +974,50 @@ static int experts_fwd(const uint16_t* x, const uint8_t* qw1, const uint8_t* sw1
   for (const void* q : {(const void*)x, (const void*)qw1, (const void*)qw2, (const void*)qw3, (const void*)sw1,
                         (const void*)sw2, (const void*)ws, (const void*)y, (const void*)b1, (const void*)b2})
     if (!aligned16(q)) return kErrInvalidArgument;
-  if (ws_bytes < moe_mxfp4_workspace_bytes(R, D, H)) return kErrWorkspace;
+  if (ws_bytes < moe_mxfp4_workspace_bytes(R, E, D, H)) return kErrWorkspace;
   uint8_t* qx = ws;
-  uint8_t* sx = qx + up256(R * (D / 2));
-  uint8_t* qh = sx + up256(R * padded_blocks(D));
-  uint8_t* sh = qh + up256(R * (H / 2));
-  const bool oss = ACT == kOssGLU;
+  uint8_t* sx = qx + row_bytes(R, D);
+  uint8_t* qh = sx + row_scales(R, D);
+  uint8_t* sh = qh + row_bytes(R, H);
+  uint8_t* pads = sh + row_scales(R, H);
+  const bool oss = ACT == kOssGLU, narrow = takes_narrow(R, E, D, H);
+  // odd scale rows, padded for the wide kernel: the copy, and its row stride
+  auto pad_scales = [&](const uint8_t* src, int64_t rows, int cols, int& ld) {
+    ld = cols / kBlock;
+    if (narrow || ld % 2 == 0) return src;
+    ld = padded_blocks(cols);
+    int64_t g = (rows * (ld / 8) + 255) / 256;
+    if (g > 16384) g = 16384;
+    hipLaunchKernelGGL(pad_scales_kernel, dim3((unsigned)g), dim3(256), 0, stream, src, rows, cols / kBlock, ld, pads);
+    const uint8_t* got = pads;
+    pads += rows * ld;
+    return got;
+  };
   Params p{};
   p.counts = counts; p.R = R; p.E = E; p.K = D; p.N = H;
-  p.x = x; p.qp = qx; p.sp = sx; p.p_ld = padded_blocks(D);
-  p.qa = qw1; p.sa = sw1; p.qb = qw3; p.sb = sw3;
+  p.x = x; p.qp = qx; p.sp = sx;
+  p.qa = qw1; p.qb = qw3;
+  if (oss) {
+    p.sa = pad_scales(sw1, 2 * (int64_t)E * H, D, p.w_ld);
+    p.sb = p.sa + p.w_ld;
+  } else {
+    p.sa = pad_scales(sw1, (int64_t)E * H, D, p.w_ld);
+    p.sb = pad_scales(sw3, (int64_t)E * H, D, p.w_ld);
+  }
+  pads = ws + up256(pads - ws);
   p.e_rows = oss ? 2 * (int64_t)H : H;
   p.r_rows = oss ? 2 : 1;
   p.bias = b1; p.limit = limit;
-  p.qh = qh; p.sh = sh; p.h_ld = padded_blocks(H);
-  const bool narrow = takes_narrow(R, E, D, H);
+  p.qh = qh; p.sh = sh;
   if (narrow) {
     launch_narrow<kGateUp, ACT>(p, stream);
   } else {
-    launch_quant<uint16_t>(x, R, D, p.p_ld, qx, sx, stream);
+    launch_quant<uint16_t>(x, R, D, padded(D), qx, sx, stream);
     launch_wide<kGateUp, ACT, false>(p, stream);
   }
   p.K = H; p.N = D;
-  p.qp = qh; p.sp = sh; p.p_ld = padded_blocks(H);
-  p.qa = qw2; p.sa = sw2; p.e_rows = D; p.r_rows = 1;
+  p.qp = qh; p.sp = sh;
+  p.qa = qw2; p.sa = pad_scales(sw2, (int64_t)E * D, H, p.w_ld); p.e_rows = D; p.r_rows = 1;
   p.bias = b2; p.y = y;
   if (narrow) launch_narrow<kDown, ACT>(p, stream);
   else launch_wide<kDown, ACT, false>(p, stream);
@@ -932,6 +1054,7 @@ MOE_API int moe_mxfp4_gemm_gate_up_keep(const uint8_t* qx, const uint8_t* sx, co
                                         uint8_t* g8, uint8_t* gs, uint8_t* u8, uint8_t* us, hipStream_t stream) {
   const int st = check_shape(n_rows, n_experts, dim, hidden);
   if (st) return st;
+  if (dim / kBlock % 2) return kErrUnsupportedShape;
   if (!counts) return kErrInvalidArgument;
   if (n_rows == 0) return kOk;
   if (!qx || !sx || !qw1 || !sw1 || !qw3 || !sw3 || !qh || !sh || !g8 || !gs || !u8 || !us) return kErrInvalidArgument;
@@ -940,9 +1063,9 @@ MOE_API int moe_mxfp4_gemm_gate_up_keep(const uint8_t* qx, const uint8_t* sx, co
     if (!aligned16(q)) return kErrInvalidArgument;
   Params p{};
   p.counts = counts; p.R = n_rows; p.E = n_experts; p.K = dim; p.N = hidden;
-  p.qp = qx; p.sp = sx; p.p_ld = padded_blocks(dim);
-  p.qa = qw1; p.sa = sw1; p.qb = qw3; p.sb = sw3; p.e_rows = hidden; p.r_rows = 1;
-  p.qh = qh; p.sh = sh; p.h_ld = padded_blocks(hidden);
+  p.qp = qx; p.sp = sx;
+  p.qa = qw1; p.sa = sw1; p.qb = qw3; p.sb = sw3; p.e_rows = hidden; p.r_rows = 1; p.w_ld = dim / kBlock;
+  p.qh = qh; p.sh = sh;
   p.g8 = g8; p.gs = gs; p.u8 = u8; p.us = us;
   launch_wide<kGateUp, kSwiGLU, true>(p, stream);
   return launch_status();
@@ -953,6 +1076,7 @@ MOE_API int moe_mxfp4_gemm_down(const uint8_t* qh, const uint8_t* sh, const uint
                                 uint16_t* y, hipStream_t stream) {
   const int st = check_shape(n_rows, n_experts, dim, hidden);
   if (st) return st;
+  if (hidden / kBlock % 2) return kErrUnsupportedShape;
   if (!counts) return kErrInvalidArgument;
   if (n_rows == 0) return kOk;
   if (!qh || !sh || !qw2 || !sw2 || !y) return kErrInvalidArgument;
@@ -960,8 +1084,8 @@ MOE_API int moe_mxfp4_gemm_down(const uint8_t* qh, const uint8_t* sh, const uint
     if (!aligned16(q)) return kErrInvalidArgument;
   Params p{};
   p.counts = counts; p.R = n_rows; p.E = n_experts; p.K = hidden; p.N = dim;
-  p.qp = qh; p.sp = sh; p.p_ld = padded_blocks(hidden);
-  p.qa = qw2; p.sa = sw2; p.qb = qw2; p.sb = sw2; p.e_rows = dim; p.r_rows = 1;
+  p.qp = qh; p.sp = sh;
+  p.qa = qw2; p.sa = sw2; p.qb = qw2; p.sb = sw2; p.e_rows = dim; p.r_rows = 1; p.w_ld = hidden / kBlock;
   p.y = y;
   launch_wide<kDown, kSwiGLU, false>(p, stream);
   return launch_status();

@@ -1348,8 +1348,7 @@ def mxfp4_quantize(x: Tensor) -> tuple[Tensor, Tensor]:
     q = torch.empty(*x.shape[:-1], cols // 2, dtype=torch.uint8, device=x.device)
     scale = torch.empty(*x.shape[:-1], cols // MX_BLOCK, dtype=torch.uint8, device=x.device)
     with _guard(x):
-        call("moe_mxfp4_quant_rows", ptr(x), x.numel() // cols, cols, code, cols // MX_BLOCK, ptr(q), ptr(scale),
-             stream_of(x))
+        call("moe_mxfp4_quant_rows", ptr(x), x.numel() // cols, cols, cols, code, ptr(q), ptr(scale), stream_of(x))
     return q, scale
 
 
@@ -1376,8 +1375,7 @@ def mxfp4_dequantize(q: Tensor, scale: Tensor, dtype: torch.dtype = torch.bfloat
     q, scale = _aligned(q.contiguous()), scale.contiguous()
     x = torch.empty(*q.shape[:-1], cols, dtype=dtype, device=q.device)
     with _guard(q):
-        call("moe_mxfp4_dequant_rows", ptr(q), ptr(scale), q.numel() // (cols // 2), cols, cols // MX_BLOCK, code, ptr(x),
-             stream_of(q))
+        call("moe_mxfp4_dequant_rows", ptr(q), ptr(scale), q.numel() // (cols // 2), cols, cols, code, ptr(x), stream_of(q))
     return x
 
 
@@ -1402,8 +1400,8 @@ def _check_packed(op: str, name: str, q: Tensor, scale: Tensor, shape: tuple | N
         raise ValueError(f"{op} expects {name} of {list(shape)} values, got {[*q.shape[:-1], 2 * q.shape[-1]]}")
 
 
-def _mxfp4_workspace(r: int, d: int, h_dim: int, device: torch.device) -> Tensor:
-    return torch.empty(max(int(lib().moe_mxfp4_workspace_bytes(r, d, h_dim)), 16), dtype=torch.uint8, device=device)
+def _mxfp4_workspace(r: int, e: int, d: int, h_dim: int, device: torch.device) -> Tensor:
+    return torch.empty(max(int(lib().moe_mxfp4_workspace_bytes(r, e, d, h_dim)), 16), dtype=torch.uint8, device=device)
 
 
 @torch.library.custom_op("moe_mi355x::grouped_swiglu_mxfp4", mutates_args=())
@@ -1424,7 +1422,7 @@ def grouped_swiglu_mxfp4(
     _check_counts(op, num_tokens_per_expert, x, qw1, qw2, qw3)
     x, qw1, sw1, qw2, sw2, qw3, sw3 = (_aligned(t.contiguous()) for t in (x, qw1, sw1, qw2, sw2, qw3, sw3))
     counts = num_tokens_per_expert.to(torch.int64).contiguous()
-    ws = _mxfp4_workspace(r, d, h_dim, x.device)
+    ws = _mxfp4_workspace(r, e, d, h_dim, x.device)
     y = x.new_empty(r, d)
     with _guard(x):
         call("moe_mxfp4_swiglu_fwd", ptr(x), ptr(qw1), ptr(sw1), ptr(qw2), ptr(sw2), ptr(qw3), ptr(sw3), ptr(counts), r, e,
@@ -1470,7 +1468,7 @@ def grouped_swiglu_oss_mxfp4(
     x, qmlp1, smlp1, qmlp2, smlp2 = (_aligned(t.contiguous()) for t in (x, qmlp1, smlp1, qmlp2, smlp2))
     b1, b2 = (_aligned(t.to(torch.bfloat16).contiguous()) for t in (mlp1_bias, mlp2_bias))
     counts = num_tokens_per_expert.to(torch.int64).contiguous()
-    ws = _mxfp4_workspace(r, d, h_dim, x.device)
+    ws = _mxfp4_workspace(r, e, d, h_dim, x.device)
     y = x.new_empty(r, d)
     with _guard(x):
         call("moe_mxfp4_oss_fwd", ptr(x), ptr(qmlp1), ptr(smlp1), ptr(b1), ptr(qmlp2), ptr(smlp2), ptr(b2), ptr(counts), r,
@@ -1483,22 +1481,24 @@ def _(x, qmlp1, smlp1, mlp1_bias, qmlp2, smlp2, mlp2_bias, num_tokens_per_expert
     return x.new_empty(x.shape)
 
 
+def _mxfp4_padded(cols: int) -> int:  # moe_mxfp4_padded_cols
+    return (cols + 255) // 256 * 256
+
+
 def _mxfp4_rows(x: Tensor, s: int) -> tuple[Tensor, Tensor]:
-    """x [R, C] bf16 in MXFP4 as the products take their rows: the scales' row stride is
-    moe_mxfp4_scale_ld(C)."""
+    """x [R, C] bf16 in MXFP4 as the products take their rows: zero columns up to a multiple of 256."""
     r, c = x.shape
-    ld = int(lib().moe_mxfp4_scale_ld(c))
-    q = torch.empty(r, c // 2, dtype=torch.uint8, device=x.device)
-    scale = torch.empty(r, ld, dtype=torch.uint8, device=x.device)
-    call("moe_mxfp4_quant_rows", ptr(x), r, c, 0, ld, ptr(q), ptr(scale), s)
+    pc = _mxfp4_padded(c)
+    q = torch.empty(r, pc // 2, dtype=torch.uint8, device=x.device)
+    scale = torch.empty(r, pc // MX_BLOCK, dtype=torch.uint8, device=x.device)
+    call("moe_mxfp4_quant_rows", ptr(x), r, c, pc, 0, ptr(q), ptr(scale), s)
     return q, scale
 
 
-def _mxfp4_values(q: Tensor, scale: Tensor, s: int) -> Tensor:
-    """The bf16 values of rows [.., C / 2] whose scales have the row stride scale.shape[-1]."""
-    cols = 2 * q.shape[-1]
+def _mxfp4_values(q: Tensor, scale: Tensor, cols: int, s: int) -> Tensor:
+    """The bf16 values of the first `cols` columns of an MXFP4 matrix."""
     x = torch.empty(*q.shape[:-1], cols, dtype=torch.bfloat16, device=q.device)
-    call("moe_mxfp4_dequant_rows", ptr(q), ptr(scale), x.numel() // cols, cols, scale.shape[-1], 0, ptr(x), s)
+    call("moe_mxfp4_dequant_rows", ptr(q), ptr(scale), x.numel() // cols, cols, 2 * q.shape[-1], 0, ptr(x), s)
     return x
 
 
@@ -1520,8 +1520,8 @@ def grouped_swiglu_mxfp4_train(
     r, d = x.shape
     e, h_dim, _ = w1.shape
     u8 = lambda *shape: torch.empty(*shape, dtype=torch.uint8, device=x.device)  # noqa: E731
-    ld = int(lib().moe_mxfp4_scale_ld(h_dim))
-    qh, sh = u8(r, h_dim // 2), u8(r, ld)
+    ph = _mxfp4_padded(h_dim)
+    qh, sh = u8(r, ph // 2), u8(r, ph // MX_BLOCK)
     g8, gs, up8, us = u8(r, h_dim), u8(r, h_dim // MX_BLOCK), u8(r, h_dim), u8(r, h_dim // MX_BLOCK)
     y = x.new_empty(r, d)
     with _guard(x):
@@ -1530,8 +1530,7 @@ def grouped_swiglu_mxfp4_train(
         packed = []
         for w in (w1, w2, w3):
             q, sc = u8(*w.shape[:-1], w.shape[-1] // 2), u8(*w.shape[:-1], w.shape[-1] // MX_BLOCK)
-            call("moe_mxfp4_quant_rows", ptr(w), w.numel() // w.shape[-1], w.shape[-1], 0, w.shape[-1] // MX_BLOCK, ptr(q),
-                 ptr(sc), s)
+            call("moe_mxfp4_quant_rows", ptr(w), w.numel() // w.shape[-1], w.shape[-1], w.shape[-1], 0, ptr(q), ptr(sc), s)
             packed += [q, sc]
         qw1, sw1, qw2, sw2, qw3, sw3 = packed
         call("moe_mxfp4_gemm_gate_up_keep", ptr(qx), ptr(sx), ptr(qw1), ptr(sw1), ptr(qw3), ptr(sw3), ptr(counts), r, e, d,
@@ -1540,16 +1539,13 @@ def grouped_swiglu_mxfp4_train(
     return y, qx, sx, qh, sh, qw1, sw1, qw2, sw2, qw3, sw3, g8, gs, up8, us
 
 
-def _scale_ld(cols: int) -> int:  # moe_mxfp4_scale_ld
-    return (cols // 32 + 7) // 8 * 8
-
-
 @grouped_swiglu_mxfp4_train.register_fake
 def _(x, w1, w2, w3, num_tokens_per_expert):
     r, d = x.shape
     e, h_dim, _ = w1.shape
     u8 = lambda *shape: x.new_empty(*shape, dtype=torch.uint8)  # noqa: E731
-    return (x.new_empty(r, d), u8(r, d // 2), u8(r, _scale_ld(d)), u8(r, h_dim // 2), u8(r, _scale_ld(h_dim)),
+    pd, ph = _mxfp4_padded(d), _mxfp4_padded(h_dim)
+    return (x.new_empty(r, d), u8(r, pd // 2), u8(r, pd // 32), u8(r, ph // 2), u8(r, ph // 32),
             u8(e, h_dim, d // 2), u8(e, h_dim, d // 32), u8(e, d, h_dim // 2), u8(e, d, h_dim // 32),
             u8(e, h_dim, d // 2), u8(e, h_dim, d // 32), u8(r, h_dim), u8(r, h_dim // 32), u8(r, h_dim),
             u8(r, h_dim // 32))
@@ -1563,25 +1559,26 @@ def grouped_swiglu_mxfp4_train_backward(
 ) -> tuple[Tensor, Tensor, Tensor, Tensor]:
     """(dx, dw1, dw2, dw3) of grouped_swiglu_mxfp4_train from what it kept; dx is zero on rows
     past sum(counts), weights of experts without rows get zeros. What is not needed is empty."""
-    r, d = qx.shape[0], 2 * qx.shape[1]
+    r, d, h_dim = qx.shape[0], qw2.shape[1], qw1.shape[1]
     dy = _check_dy("grouped_swiglu_mxfp4_train_backward", dy, r, d, qx)
     counts = num_tokens_per_expert.to(torch.int64).contiguous()
     with _guard(dy):
         s = stream_of(dy)
         # the values dgu and dx multiply; dW takes only their shapes
-        w2 = _mxfp4_values(qw2, sw2, s) if need_dx or need_dw13 else dy.new_empty(*qw2.shape[:-1], 2 * qw2.shape[-1])
-        w1, w3 = (_mxfp4_values(q, sc, s) if need_dx else dy.new_empty(*q.shape[:-1], 2 * q.shape[-1])
+        w2 = _mxfp4_values(qw2, sw2, h_dim, s) if need_dx or need_dw13 else dy.new_empty(*qw2.shape[:-1], h_dim)
+        w1, w3 = (_mxfp4_values(q, sc, d, s) if need_dx else dy.new_empty(*q.shape[:-1], d)
                   for q, sc in ((qw1, sw1), (qw3, sw3)))
-        h = _mxfp4_values(qh, sh, s) if need_dw2 else dy.new_empty(0)
-        return _narrow_backward(dy, w1, w2, w3, counts, g8, gs, u8, us, lambda: _mxfp4_values(qx, sx, s), h, need_dx,
+        h = _mxfp4_values(qh, sh, h_dim, s) if need_dw2 else dy.new_empty(0)
+        return _narrow_backward(dy, w1, w2, w3, counts, g8, gs, u8, us, lambda: _mxfp4_values(qx, sx, d, s), h, need_dx,
                                 need_dw13, need_dw2)
 
 
 @grouped_swiglu_mxfp4_train_backward.register_fake
 def _(dy, num_tokens_per_expert, qx, sx, qh, sh, qw1, sw1, qw2, sw2, qw3, sw3, g8, gs, u8, us, need_dx=True,
       need_dw13=True, need_dw2=True):
-    full = lambda q, need: dy.new_empty(*q.shape[:-1], 2 * q.shape[-1], dtype=torch.bfloat16) if need else dy.new_empty(0, dtype=torch.bfloat16)  # noqa: E501,E731
-    return full(qx, need_dx), full(qw1, need_dw13), full(qw2, need_dw2), full(qw3, need_dw13)
+    r, (e, h_dim, _), d = qx.shape[0], qw1.shape, qw2.shape[1]
+    bf = lambda need, *shape: dy.new_empty(shape if need else (0,), dtype=torch.bfloat16)  # noqa: E731
+    return bf(need_dx, r, d), bf(need_dw13, e, h_dim, d), bf(need_dw2, e, d, h_dim), bf(need_dw13, e, h_dim, d)
 
 
 def _mxfp4_train_setup(ctx, inputs, output):
