@@ -364,11 +364,12 @@ __global__ __launch_bounds__(NW * 64, 2) void wide_kernel(Params p) {
   constexpr int KH = RB / 64, RPC = 1024 / RB, CPR = RB / 16;  // MFMA steps a stage; rows of a 1 KB copy; chunks of a row
   constexpr int PW = BM / RPC / NW, SPC = BM * KH / 64, SPW = (SPC + NW - 1) / NW;  // a wave's copies of P, of its scales
   constexpr int QC = BN / RPC / NW, SQC = BN * KH / 64 / NW * (PAIR ? 2 : 1);  // a wave's copies of Q and of its scales
-  static_assert((RB == 64 || RB == 128) && BN == 256 && NS >= 2 && TN % 4 == 0, "tile");
+  static_assert((RB == 64 || RB == 128) && BN == 256 && NS >= 2 && TN % 4 == 0 && TM % 4 == 0, "tile");
   static_assert(PW * RPC * NW == BM && QC * RPC * NW == BN && SQC >= 1 && BM * KH % 64 == 0, "copies");
   __shared__ __attribute__((aligned(1024))) uint8_t sP[NS][BM * RB];
   __shared__ __attribute__((aligned(1024))) uint8_t sQ[NS][BN * RB];
-  // scales: row m's RB / 16 at RB / 16 m; PAIR: pair h of row n at 4 (BN h + n)
+  // scales: a lane's, for each of its 16-row blocks a word (KH = 2: two of its stage's steps in
+  // half of one; PAIR: in the low half), side by side, so that it reads them four at a time
   __shared__ __attribute__((aligned(16))) uint8_t sSP[NS][SPC * 256];
   __shared__ __attribute__((aligned(16))) uint8_t sSQ[NS][SQC * NW * 256];
   __shared__ int4 s_list[kTileList];  // this workgroup's first tiles: first row, end of the segment, expert, column tile
@@ -415,12 +416,12 @@ __global__ __launch_bounds__(NW * 64, 2) void wide_kernel(Params p) {
   // first is copied once more. ----
   auto swz = [](int row) { return (row >> 1) & (CPR - 1); };
   auto q_col = [](int n) { return MODE == kGateUp ? (n >> 5) * 16 + (n & 15) : n; };  // in the tile's columns
-  // word i of the scale copies: of P row i / KH, dword i % KH; of Q the same, PAIR row i % BN, pair
-  // i / BN. Fewer copies than waves: some waves write the same words
-  auto sq_off = [&](int b) {
-    const int i = (wv * SQC + b) * 64 + lane;
-    return PAIR ? i / BN * 2 : i % KH * 4;
-  };
+  // Word i of the scale copies: for a wave row (of P) or column (of Q), row of a 16-row block
+  // and part of its stage's scales (a dword of four or PAIR two), the T blocks. Fewer copies than
+  // waves: some waves write the same words
+  constexpr int SUB = PAIR ? 2 * KH : KH;
+  auto scale_row = [](int i, int t, int sub) { return (i / (16 * sub * t) * t + i % t) * 16 + i / (t * sub) % 16; };
+  auto sq_off = [&](int b) { return ((wv * SQC + b) * 64 + lane) / TN % SUB * (PAIR ? 2 : 4); };
   const int p_ld = padded(K) / 2, sp_ld = padded(K) / kBlock;
   const uint8_t *baseP, *baseSP, *baseQ[2];  // of the tile being copied: P, its scales, gate (or down) and up
   uint32_t offP[PW], offQ[QC], offSP[SPW];
@@ -446,11 +447,11 @@ __global__ __launch_bounds__(NW * 64, 2) void wide_kernel(Params p) {
 #pragma unroll
     for (int b = 0; b < SPW; ++b) {
       const int i = (wv * SPW + b) % SPC * 64 + ln;
-      offSP[b] = __umul24(min(i / KH, last), sp_ld) + i % KH * 4;
+      offSP[b] = __umul24(min(scale_row(i, TM, KH), last), sp_ld) + i / TM % KH * 4;
     }
 #pragma unroll
     for (int b = 0; b < SQC; ++b) {
-      const int i = (wv * SQC + b) * 64 + ln, n = PAIR ? i % BN : i / KH;
+      const int n = scale_row((wv * SQC + b) * 64 + ln, TN, SUB);
       const uint8_t* base = (MODE == kGateUp && ((n >> 4) & 1) ? p.sb : p.sa) + wr * p.w_ld;
       srcSQ[b] = base + __umul24(min(q_col(n), last_col), p.r_rows * p.w_ld);
     }
@@ -531,15 +532,17 @@ __global__ __launch_bounds__(NW * 64, 2) void wide_kernel(Params p) {
         const uint4 v = *(const uint4*)(tile + row * RB + (((KH * g4 + step) ^ swz(row)) << 4));
         return v8i_t{(int)v.x, (int)v.y, (int)v.z, (int)v.w, 0, 0, 0, 0};
       };
-      auto scale_at = [&](const uint8_t* at) { return KH == 2 ? (int)*(const uint16_t*)at : (int)*at; };
+      const int sh_p = KH == 2 ? 16 * (g4 & 1) : 8 * g4, sh_q = PAIR ? (KH == 2 ? 0 : 8 * (g4 & 1)) : sh_p;
 #pragma unroll
-      for (int i = 0; i < TM; ++i) scp[i] = scale_at(cSP + ((wm * TM + i) * 16 + ml) * CPR + KH * g4);
+      for (int i = 0; i < TM; i += 4) {
+        const uint4 w = *(const uint4*)(cSP + (((wm * 16 + ml) * KH + (KH == 2 ? g4 >> 1 : 0)) * TM + i) * 4);
+        scp[i] = w.x >> sh_p; scp[i + 1] = w.y >> sh_p; scp[i + 2] = w.z >> sh_p; scp[i + 3] = w.w >> sh_p;
+      }
 #pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        const int n = (wn * TN + j) * 16 + ml;
-        if constexpr (!PAIR) scq[j] = scale_at(cSQ + n * CPR + KH * g4);
-        else if constexpr (KH == 2) scq[j] = *(const int*)(cSQ + (BN * g4 + n) * 4);
-        else scq[j] = cSQ[(BN * (g4 >> 1) + n) * 4 + (g4 & 1)];
+      for (int j = 0; j < TN; j += 4) {
+        const int part = PAIR ? (KH == 2 ? g4 : g4 >> 1) : (KH == 2 ? g4 >> 1 : 0);
+        const uint4 w = *(const uint4*)(cSQ + (((wn * 16 + ml) * SUB + part) * TN + j) * 4);
+        scq[j] = w.x >> sh_q; scq[j + 1] = w.y >> sh_q; scq[j + 2] = w.z >> sh_q; scq[j + 3] = w.w >> sh_q;
       }
       // the next stage's copies go between the MFMAs, one behind each of the first blocks of
       // columns: issued together right behind the barrier they hold every wave up at once (a
