@@ -4,7 +4,8 @@ on hand-written gfx950 kernels (``torchtitan_amd.ops``).
 
 Module map (reference file:line -> here):
   _run_experts_for_loop      moe.py:24-50    -> _run_experts_for_loop
-  _run_experts_grouped_mm    moe.py:53-70    -> _run_experts_grouped_mm (ops.grouped_swiglu)
+  _run_experts_grouped_mm    moe.py:53-70    -> _run_experts_grouped_mm (ops.grouped_swiglu), and its
+                                                quantized forms _fp8, _mxfp8, _mxfp4, _ckpt8
   GroupedExperts             moe.py:73-116   -> GroupedExperts
   TokenChoiceTopKRouter      moe.py:119-276  -> TokenChoiceTopKRouter (gate on torch, rest ops.router)
   TokenReorderer             moe.py:281-332  -> TokenReorderer (ops.reorder)
@@ -32,7 +33,9 @@ __all__ = [
     "TokenReorderer",
     "_run_experts_for_loop",
     "_run_experts_grouped_mm",
+    "_run_experts_grouped_mm_ckpt8",
     "_run_experts_grouped_mm_fp8",
+    "_run_experts_grouped_mm_mxfp4",
     "_run_experts_grouped_mm_mxfp8",
 ]
 
@@ -110,6 +113,34 @@ def _run_experts_grouped_mm_mxfp8(
     return y.type_as(x)
 
 
+def _run_experts_grouped_mm_mxfp4(
+    w1: torch.Tensor, w2: torch.Tensor, w3: torch.Tensor, x: torch.Tensor,
+    num_tokens_per_expert: torch.Tensor,
+) -> torch.Tensor:
+    """MXFP4 grouped GEMMs (ops.grouped_swiglu_mxfp4_train): every operand of the forward in
+    4-bit blocks of 32 along its contraction, gradients straight through the quantizations from
+    activations kept in 4 and 8 bits. Without gradients the weights are packed and
+    ops.grouped_swiglu_mxfp4 runs (the same formula; few rows sum in another order)."""
+    args = [t.bfloat16() for t in (x, w1, w2, w3)]
+    if torch.is_grad_enabled() and any(t.requires_grad for t in args):
+        y = ops.grouped_swiglu_mxfp4_train(*args, num_tokens_per_expert)[0]
+    else:
+        packed = [t for w in args[1:] for t in ops.mxfp4_quantize(w)]
+        y = ops.grouped_swiglu_mxfp4(args[0], *packed, num_tokens_per_expert)
+    return y.type_as(x)
+
+
+def _run_experts_grouped_mm_ckpt8(
+    w1: torch.Tensor, w2: torch.Tensor, w3: torch.Tensor, x: torch.Tensor,
+    num_tokens_per_expert: torch.Tensor,
+) -> torch.Tensor:
+    """bf16 grouped GEMMs that keep x, gate and up for the backward in MXFP8
+    (ops.grouped_swiglu_ckpt8)."""
+    args = [t.bfloat16() for t in (x, w1, w2, w3)]
+    for_backward = torch.is_grad_enabled() and any(t.requires_grad for t in args)
+    return ops.grouped_swiglu_ckpt8(*args, num_tokens_per_expert, for_backward)[0].type_as(x)
+
+
 class GroupedExperts(Module):
     @dataclass(kw_only=True, slots=True)
     class Config(Module.Config):
@@ -125,12 +156,19 @@ class GroupedExperts(Module):
         self.w2 = nn.Parameter(torch.empty(config.num_experts, config.dim, config.hidden_dim))
         self.w3 = nn.Parameter(torch.empty(config.num_experts, config.hidden_dim, config.dim))
         self.use_grouped_mm = config.use_grouped_mm
-        # set by quantization.Float8GroupedMMConverter / MXFP8Converter .convert
+        # set by the converters of quantization.py (Float8GroupedMMConverter, MXFP8Converter,
+        # MXFP4Converter, MXFP8ActivationCheckpointConverter)
         self.float8 = False
         self.mxfp8 = False
+        self.mxfp4 = False
+        self.ckpt8 = False
 
     def forward(self, x: torch.Tensor, num_tokens_per_expert: torch.Tensor) -> torch.Tensor:
         w1, w2, w3 = _local(self.w1), _local(self.w2), _local(self.w3)
+        if self.mxfp4:
+            return _run_experts_grouped_mm_mxfp4(w1, w2, w3, x, num_tokens_per_expert)
+        if self.ckpt8:
+            return _run_experts_grouped_mm_ckpt8(w1, w2, w3, x, num_tokens_per_expert)
         if self.mxfp8:
             return _run_experts_grouped_mm_mxfp8(w1, w2, w3, x, num_tokens_per_expert)
         if self.float8:

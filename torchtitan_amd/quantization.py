@@ -10,6 +10,12 @@ MXFP8 (e4m3 elements, one e8m0 scale per 32 along the contraction, RCEIL);
 fp32 accumulation, bf16 outputs. Parameters stay bf16/fp32 master weights and
 the state_dict is unchanged; quantization happens inside each forward and
 backward.
+
+Three more, with the same interface and without a counterpart in the reference:
+``MXFP4Converter`` (training with MXFP4 products, gradients straight through),
+``MXFP8ActivationCheckpointConverter`` (bf16 products, activations kept for the
+backward in MXFP8), and ``MXFP4WeightConverter`` (inference: the experts are
+replaced by ones that hold their weights packed in 4 bits, ``mxfp4.py``).
 """
 
 from __future__ import annotations
@@ -21,9 +27,12 @@ import torch
 from torch import nn
 
 from .configurable import Configurable
+from .gpt_oss import GptOssGroupedExperts
 from .moe import GroupedExperts
+from .mxfp4 import MXFP4GptOssGroupedExperts, MXFP4GroupedExperts
 
-__all__ = ["Float8GroupedMMConverter", "MXFP8Converter", "PAD_MULTIPLE_MAP", "find_pad_multiple"]
+__all__ = ["Float8GroupedMMConverter", "MXFP4Converter", "MXFP4WeightConverter", "MXFP8ActivationCheckpointConverter",
+           "MXFP8Converter", "PAD_MULTIPLE_MAP", "find_pad_multiple"]
 
 logger = logging.getLogger(__name__)
 
@@ -75,13 +84,21 @@ def _split_fqns(fqns: list[str] | str) -> list[str]:
     return [f for f in fqns.split(",") if f] if isinstance(fqns, str) else list(fqns)
 
 
+# how GroupedExperts multiply; the last two take no other beside them
+_RECIPES = ("float8", "mxfp8", "mxfp4", "ckpt8")
+_ALONE = ("mxfp4", "ckpt8")
+
+
 def _mark_experts(model: nn.Module, fqns: list[str], attr: str) -> list[str]:
-    converted = []
-    for name, mod in model.named_modules():
-        if isinstance(mod, GroupedExperts) and any(f in name for f in fqns):
-            setattr(mod, attr, True)
-            converted.append(name)
-    return converted
+    matching = [(name, mod) for name, mod in model.named_modules()
+                if isinstance(mod, GroupedExperts) and any(f in name for f in fqns)]
+    for name, mod in matching:
+        others = [r for r in _RECIPES if r != attr and getattr(mod, r)]
+        if others and (attr in _ALONE or any(r in _ALONE for r in others)):
+            raise ValueError(f"{name} is already converted to {others[0]}: {attr} experts are a recipe of their own")
+    for _name, mod in matching:
+        setattr(mod, attr, True)
+    return [name for name, _mod in matching]
 
 
 class MXFP8Converter(Configurable):
@@ -121,6 +138,72 @@ class MXFP8Converter(Configurable):
 
     def post_optimizer_hook(self, model) -> None:
         pass
+
+
+class _ExpertsConverter(Configurable):
+    """Marks the matching GroupedExperts; needs the hardware's block-scaled formats. The kernels
+    take ragged token groups, so nothing is padded."""
+
+    attr: str
+
+    @dataclass(kw_only=True, slots=True)
+    class Config(Configurable.Config):
+        fqns: list[str] | str = field(default_factory=list)
+
+    def __init__(self, config: Config, *, parallel_dims, model_compile_enabled: bool):
+        if not has_gfx950():
+            raise ValueError(f"{type(self).__name__} is only supported on gfx950 (MI355X)")
+        self.fqns = _split_fqns(config.fqns)
+        self.config = config
+
+    def convert(self, model: nn.Module) -> list[str]:
+        """Switches the matching GroupedExperts; returns their names."""
+        return _mark_experts(model, self.fqns, self.attr)
+
+    def post_optimizer_hook(self, model) -> None:
+        pass
+
+
+class MXFP4Converter(_ExpertsConverter):
+    """MXFP4 grouped GEMMs for the matching experts in training: every operand of the forward
+    products in 4 bits, gradients straight through (ops.grouped_swiglu_mxfp4_train)."""
+
+    attr = "mxfp4"
+
+    @dataclass(kw_only=True, slots=True)
+    class Config(_ExpertsConverter.Config):
+        pass
+
+
+class MXFP8ActivationCheckpointConverter(_ExpertsConverter):
+    """bf16 grouped GEMMs whose x, gate and up are kept for the backward in MXFP8 instead of
+    bf16 (ops.grouped_swiglu_ckpt8): (D + 2H) 33/32 bytes a routed row instead of 2D + 6H."""
+
+    attr = "ckpt8"
+
+    @dataclass(kw_only=True, slots=True)
+    class Config(_ExpertsConverter.Config):
+        pass
+
+
+class MXFP4WeightConverter(_ExpertsConverter):
+    """Inference on weights packed in MXFP4: replaces the matching GroupedExperts and
+    GptOssGroupedExperts by MXFP4GroupedExperts / MXFP4GptOssGroupedExperts, which hold their
+    packed weights in place of the parameters (17/32 of a byte per weight) and take no gradients."""
+
+    @dataclass(kw_only=True, slots=True)
+    class Config(_ExpertsConverter.Config):
+        pass
+
+    def convert(self, model: nn.Module) -> list[str]:
+        packed = {GroupedExperts: MXFP4GroupedExperts, GptOssGroupedExperts: MXFP4GptOssGroupedExperts}
+        converted = []
+        for name, mod in list(model.named_modules()):
+            if name and type(mod) in packed and any(f in name for f in self.fqns):
+                parent, _, child = name.rpartition(".")
+                setattr(model.get_submodule(parent), child, packed[type(mod)].from_experts(mod))
+                converted.append(name)
+        return converted
 
 
 def find_pad_multiple(converters: list) -> int | None:
