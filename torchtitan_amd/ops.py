@@ -1,4 +1,5 @@
-"""torch.library custom ops over the MI355X MoE kernels (namespace ``moe_mi355x``).
+"""torch.library custom ops over the MI355X MoE kernels (namespace ``moe_mi355x``; those on
+block-scaled 4-bit operands and 8-bit kept activations ``moe_mi355x_mx``).
 
 Each op is a thin host wrapper around one C-ABI entry point of
 ``libmoe_mi355x.so``: it allocates outputs and workspaces with torch's caching
@@ -1196,7 +1197,7 @@ def _zero_rows_past(counts: Tensor, r: int, e: int, t: Tensor, s: int) -> None:
     call("moe_zero_rows_past_f32", ptr(counts), r, e, ptr(t), t.shape[1] // 2, None, 0, None, 0, None, 0, s)
 
 
-@torch.library.custom_op("moe_mi355x::grouped_swiglu_ckpt8", mutates_args=())
+@torch.library.custom_op("moe_mi355x_mx::grouped_swiglu_ckpt8", mutates_args=())
 def grouped_swiglu_ckpt8(
     x: Tensor, w1: Tensor, w2: Tensor, w3: Tensor, num_tokens_per_expert: Tensor, for_backward: bool = True
 ) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor]:
@@ -1274,7 +1275,7 @@ def _check_dy(op: str, dy: Tensor, r: int, d: int, like: Tensor) -> Tensor:
     return _aligned(dy.to(torch.bfloat16).contiguous())
 
 
-@torch.library.custom_op("moe_mi355x::grouped_swiglu_ckpt8_backward", mutates_args=())
+@torch.library.custom_op("moe_mi355x_mx::grouped_swiglu_ckpt8_backward", mutates_args=())
 def grouped_swiglu_ckpt8_backward(
     dy: Tensor, w1: Tensor, w2: Tensor, w3: Tensor, num_tokens_per_expert: Tensor, x8: Tensor, xs: Tensor, g8: Tensor,
     gs: Tensor, u8: Tensor, us: Tensor, need_dx: bool = True, need_dw13: bool = True, need_dw2: bool = True,
@@ -1332,7 +1333,7 @@ def _check_mx_matrix(op: str, cols: int) -> None:
         raise ValueError(f"{op} takes rows of whole blocks of {MX_BLOCK} elements, got {cols}")
 
 
-@torch.library.custom_op("moe_mi355x::mxfp4_quantize", mutates_args=())
+@torch.library.custom_op("moe_mi355x_mx::mxfp4_quantize", mutates_args=())
 def mxfp4_quantize(x: Tensor) -> tuple[Tensor, Tensor]:
     """x [.., K] (bf16 or fp32, K a multiple of 32) in MXFP4: (q [.., K / 2] uint8, two e2m1
     codes a byte, the first in the low half; scale [.., K / 32] uint8, e8m0). A block's scale is
@@ -1364,7 +1365,7 @@ def _(x):
     return u8(x.shape[-1] // 2), u8(x.shape[-1] // MX_BLOCK)
 
 
-@torch.library.custom_op("moe_mi355x::mxfp4_dequantize", mutates_args=())
+@torch.library.custom_op("moe_mi355x_mx::mxfp4_dequantize", mutates_args=())
 def mxfp4_dequantize(q: Tensor, scale: Tensor, dtype: torch.dtype = torch.bfloat16) -> Tensor:
     """The values [.., K] of an MXFP4 matrix (q [.., K / 2], scale [.., K / 32] uint8) in bf16 or
     fp32, which hold each of them exactly within their range (past it: infinities)."""
@@ -1404,7 +1405,7 @@ def _mxfp4_workspace(r: int, e: int, d: int, h_dim: int, device: torch.device) -
     return torch.empty(max(int(lib().moe_mxfp4_workspace_bytes(r, e, d, h_dim)), 16), dtype=torch.uint8, device=device)
 
 
-@torch.library.custom_op("moe_mi355x::grouped_swiglu_mxfp4", mutates_args=())
+@torch.library.custom_op("moe_mi355x_mx::grouped_swiglu_mxfp4", mutates_args=())
 def grouped_swiglu_mxfp4(
     x: Tensor, qw1: Tensor, sw1: Tensor, qw2: Tensor, sw2: Tensor, qw3: Tensor, sw3: Tensor,
     num_tokens_per_expert: Tensor,
@@ -1446,7 +1447,7 @@ def _(x, qw1, sw1, qw2, sw2, qw3, sw3, num_tokens_per_expert):
     return x.new_empty(x.shape)
 
 
-@torch.library.custom_op("moe_mi355x::grouped_swiglu_oss_mxfp4", mutates_args=())
+@torch.library.custom_op("moe_mi355x_mx::grouped_swiglu_oss_mxfp4", mutates_args=())
 def grouped_swiglu_oss_mxfp4(
     x: Tensor, qmlp1: Tensor, smlp1: Tensor, mlp1_bias: Tensor, qmlp2: Tensor, smlp2: Tensor, mlp2_bias: Tensor,
     num_tokens_per_expert: Tensor, swiglu_limit: float,
@@ -1502,7 +1503,7 @@ def _mxfp4_values(q: Tensor, scale: Tensor, cols: int, s: int) -> Tensor:
     return x
 
 
-@torch.library.custom_op("moe_mi355x::grouped_swiglu_mxfp4_train", mutates_args=())
+@torch.library.custom_op("moe_mi355x_mx::grouped_swiglu_mxfp4_train", mutates_args=())
 def grouped_swiglu_mxfp4_train(
     x: Tensor, w1: Tensor, w2: Tensor, w3: Tensor, num_tokens_per_expert: Tensor
 ) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor,
@@ -1551,7 +1552,7 @@ def _(x, w1, w2, w3, num_tokens_per_expert):
             u8(r, h_dim // 32))
 
 
-@torch.library.custom_op("moe_mi355x::grouped_swiglu_mxfp4_train_backward", mutates_args=())
+@torch.library.custom_op("moe_mi355x_mx::grouped_swiglu_mxfp4_train_backward", mutates_args=())
 def grouped_swiglu_mxfp4_train_backward(
     dy: Tensor, num_tokens_per_expert: Tensor, qx: Tensor, sx: Tensor, qh: Tensor, sh: Tensor, qw1: Tensor, sw1: Tensor,
     qw2: Tensor, sw2: Tensor, qw3: Tensor, sw3: Tensor, g8: Tensor, gs: Tensor, u8: Tensor, us: Tensor,
