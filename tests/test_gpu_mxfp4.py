@@ -142,6 +142,10 @@ SERVE = [
     ("many rows", [300, 0, 77, 513], 9, 256, 256),
     ("many rows, odd dims", [1000, 130, 0, 300], 3, 416, 352),
     ("one expert", [700], 0, 96, 96),
+    ("few rows, a long contraction", [3, 0, 1], 1, 7168, 64),
+    ("few rows, rows past the LDS", [2, 1], 0, 16384, 32),
+    ("many experts", [0, 2, 0, 0, 17, 1] * 170 + [3, 0, 0, 9], 2, 64, 32),
+    ("many experts, many rows", [0, 40, 0, 0, 300, 1] * 20, 2, 64, 96),
     ("no rows for anyone", [0, 0, 0], 6, 64, 64),
 ]
 

@@ -682,7 +682,7 @@ constexpr int kAhead = 2;
 constexpr int kRows = 16;
 __host__ __device__ constexpr int narrow_stride(int K) { return (K + 255) / 256 * 128 + 16; }  // rows 16 bytes apart mod 128
 __host__ __device__ constexpr int64_t narrow_lds(int K) {  // the rows, their scales, and the waves' sums
-  return (int64_t)kRows * (narrow_stride(K) + (K + 255) / 256 * 8) + 8 * 64 * 16;
+  return (int64_t)kRows * (narrow_stride(K) + (K + 255) / 256 * 8) + 2 * 8 * 64 * 16;
 }
 
 template <int MODE, int ACT>
@@ -695,7 +695,7 @@ __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
   const int E = p.E, K = p.K, N = p.N, KB = K / kBlock, kbytes = K / 2, nst = (K + 255) / 256;
   const int stride = narrow_stride(K), sld = nst * 8;
   uint8_t* sP = s_dyn;
-  f32x4_t* red = (f32x4_t*)(s_dyn + kRows * (stride + sld));  // [2 ks][4 nb][64]
+  f32x4_t* sums = (f32x4_t*)(s_dyn + kRows * (stride + sld));  // two units' [2 ks][4 nb][64]
   uint8_t* sc = s_dyn + kRows * stride;
   const int NCB = MODE == kGateUp ? N / 32 : (N + 63) / 64;
   segments_wave(p, s_seg, s_tile, [&](int rows) { return (rows + kRows - 1) / kRows * NCB; });
@@ -827,16 +827,19 @@ __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
       cur = nxt;
     }
     if (mine == 0 && t + 1 < u1) load(cur, un, 0);
-    __syncthreads();  // the sums of the unit before have been read
+    // one barrier a unit: the waves that read these sums come to the next one before anyone
+    // writes over them; they take turns, so that none is behind the others for good
+    f32x4_t* red = sums + (t & 1) * 8 * 64;
     red[(ks * 4 + nb) * 64 + lane] = acc;
     __syncthreads();
+    const int turn = (wv + t) & 7;
     auto sum = [&](int b, float (&v)[4]) {
       const f32x4_t a = red[b * 64 + lane], c = red[(4 + b) * 64 + lane];
 #pragma unroll
       for (int q = 0; q < 4; ++q) v[q] = a[q] + c[q];
     };
     if (MODE == kGateUp) {
-      if (wv == 0) {
+      if (turn == 0) {
         float ga[4], gb[4], ua[4], ub[4];
         sum(0, ga);
         sum(1, gb);
@@ -851,8 +854,8 @@ __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
         }
         store_hidden<ACT, false>(p, row0 + r, hc, lane, r < rows, ga, gb, ua, ub, bias_a, bias_b);
       }
-    } else if (wv < 2) {
-      const int pr = wv, n0 = u.cb * 64 + pr * 32, r = ml;
+    } else if (turn < 2) {
+      const int pr = turn, n0 = u.cb * 64 + pr * 32, r = ml;
       if (n0 < N) {
         float lo[4], hi[4];
         sum(2 * pr, lo);
