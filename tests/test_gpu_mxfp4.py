@@ -305,7 +305,14 @@ def test_serve_takes_no_gradients(dev):
 
     gen = torch.Generator().manual_seed(8)
     w = [t.to(dev) for t in (*_packed(gen, 2, 32, 64, 0.1), *_packed(gen, 2, 64, 32, 0.1), *_packed(gen, 2, 32, 64, 0.1))]
-    x = torch.randn(4, 64).bfloat16().to(dev).requires_grad_(True)
-    y = ops.grouped_swiglu_mxfp4(x, *w, torch.tensor([2, 2], device=dev))
-    with pytest.raises(RuntimeError):
-        y.float().sum().backward()
+    x, c = torch.randn(4, 64).bfloat16().to(dev).requires_grad_(True), torch.tensor([2, 2], device=dev)
+    with pytest.raises(RuntimeError, match="no gradients"):
+        ops.grouped_swiglu_mxfp4(x, *w, c)
+    with torch.no_grad():
+        assert torch.equal(ops.grouped_swiglu_mxfp4(x, *w, c), ops.grouped_swiglu_mxfp4(x.detach(), *w, c))
+    q, s = ops.mxfp4_quantize(x)  # codes have no gradients to lose
+    assert not q.requires_grad and torch.equal(q, ops.mxfp4_quantize(x.detach())[0])
+    b1, b2 = torch.zeros(2, 64, device=dev, requires_grad=True), torch.zeros(2, 64, device=dev)
+    m1 = [t.to(dev) for t in _packed(gen, 2, 64, 64, 0.1)]
+    with pytest.raises(RuntimeError, match="no gradients"):
+        ops.grouped_swiglu_oss_mxfp4(x.detach(), *m1, b1, *w[2:4], b2, c, 7.0)

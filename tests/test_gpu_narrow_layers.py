@@ -243,6 +243,7 @@ def _op_cases(dev):
     def bf(*shape, grad=False, scale=1.0):
         return (torch.randn(*shape, generator=gen) * scale).bfloat16().to(dev).requires_grad_(grad)
 
+    mx = torch.ops.moe_mi355x_mx
     counts = torch.tensor([30, 0, 20, 14], device=dev)  # every row has an expert: what is kept of others is not defined
     x, w1, w2, w3 = bf(r, d), bf(e, h, d, scale=0.05), bf(e, d, h, scale=0.05), bf(e, h, d, scale=0.05)
     leaves = [t.clone().requires_grad_(True) for t in (x, w1, w2, w3)]
@@ -251,10 +252,10 @@ def _op_cases(dev):
     kept = ops.grouped_swiglu_ckpt8(x, w1, w2, w3, counts)[1:]
     four = ops.grouped_swiglu_mxfp4_train(x, w1, w2, w3, counts)[1:]
     return {
-        "mxfp4_quantize": (ops.mxfp4_quantize, (x,)),
-        "mxfp4_dequantize": (ops.mxfp4_dequantize, (*packed[:2], torch.float32)),
-        "grouped_swiglu_mxfp4": (ops.grouped_swiglu_mxfp4, (x, *packed, counts)),
-        "grouped_swiglu_oss_mxfp4": (ops.grouped_swiglu_oss_mxfp4, (x, *m1, bf(e, 2 * h), *packed[2:4], bf(e, d), counts, 7.0)),
+        "mxfp4_quantize": (mx.mxfp4_quantize, (x,)),
+        "mxfp4_dequantize": (mx.mxfp4_dequantize, (*packed[:2], torch.float32)),
+        "grouped_swiglu_mxfp4": (mx.grouped_swiglu_mxfp4, (x, *packed, counts)),
+        "grouped_swiglu_oss_mxfp4": (mx.grouped_swiglu_oss_mxfp4, (x, *m1, bf(e, 2 * h), *packed[2:4], bf(e, d), counts, 7.0)),
         "grouped_swiglu_ckpt8": (ops.grouped_swiglu_ckpt8, (*leaves, counts)),
         "grouped_swiglu_ckpt8_backward": (ops.grouped_swiglu_ckpt8_backward, (bf(r, d), w1, w2, w3, counts, *kept)),
         "grouped_swiglu_mxfp4_train": (ops.grouped_swiglu_mxfp4_train, (*leaves, counts)),

@@ -14,6 +14,7 @@ when the library is missing.
 
 from __future__ import annotations
 
+import functools
 from contextlib import nullcontext
 
 import torch
@@ -1157,9 +1158,12 @@ grouped_swiglu_mxfp8.register_autograd(_gsmx_bwd, setup_context=_gsmx_setup)
 # bf16 grouped SwiGLU experts whose activations are kept for the backward in
 # MXFP8, and MXFP4 experts (32-element blocks along each contraction)
 # ---------------------------------------------------------------------------
+_HERE = nullcontext()
+
+
 def _guard(t: Tensor):
     """Makes t's device the current one for the launches of an op, where it is not."""
-    return nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+    return _HERE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 def _check_experts(op: str, x: Tensor, w1: Tensor, w2: Tensor, w3: Tensor, counts: Tensor, multiple: int) -> None:
@@ -1328,29 +1332,27 @@ def _ckpt8_bwd(ctx, dy, *_unused):
 grouped_swiglu_ckpt8.register_autograd(_ckpt8_bwd, setup_context=_ckpt8_setup)
 
 
-def _check_mx_matrix(op: str, cols: int) -> None:
-    if cols < MX_BLOCK or cols % MX_BLOCK:
-        raise ValueError(f"{op} takes rows of whole blocks of {MX_BLOCK} elements, got {cols}")
+# The ops without a gradient are defined on the dispatcher directly: a generation step calls
+# them every few microseconds, and without torch.library.custom_op's layers a call takes the host
+# 10 us instead of 13 (mxfp4_quantize) and 23 instead of 25 (grouped_swiglu_mxfp4).
+_MX = torch.library.Library("moe_mi355x_mx", "FRAGMENT")
 
 
-@torch.library.custom_op("moe_mi355x_mx::mxfp4_quantize", mutates_args=())
-def mxfp4_quantize(x: Tensor) -> tuple[Tensor, Tensor]:
-    """x [.., K] (bf16 or fp32, K a multiple of 32) in MXFP4: (q [.., K / 2] uint8, two e2m1
-    codes a byte, the first in the low half; scale [.., K / 32] uint8, e8m0). A block's scale is
-    the least power of two 2^k, k in [-127, 127], with max |x| <= 6 * 2^k; elements are rounded
-    to nearest, ties to the even code. A block with an infinity or a NaN gets the NaN scale 255."""
-    require_gpu(x)
-    code = _mx_dtype("mxfp4_quantize", x.dtype)
-    if x.dim() < 1:
-        raise ValueError("mxfp4_quantize expects rows, got a scalar")
-    cols = x.shape[-1]
-    _check_mx_matrix("mxfp4_quantize", cols)
-    x = _aligned(x.contiguous())
-    q = torch.empty(*x.shape[:-1], cols // 2, dtype=torch.uint8, device=x.device)
-    scale = torch.empty(*x.shape[:-1], cols // MX_BLOCK, dtype=torch.uint8, device=x.device)
-    with _guard(x):
-        call("moe_mxfp4_quant_rows", ptr(x), x.numel() // cols, cols, cols, code, ptr(q), ptr(scale), stream_of(x))
-    return q, scale
+def _mx_op(schema: str):
+    """Defines moe_mi355x_mx::schema with the decorated function as its GPU kernel (and on the CPU,
+    where the kernel's own check refuses)."""
+    def register(fn):
+        name = schema.split("(")[0]
+        _MX.define(schema)
+        _MX.impl(name, fn, "CUDA")
+        _MX.impl(name, fn, "CPU")
+        return getattr(torch.ops.moe_mi355x_mx, name).default
+    return register
+
+
+def _ready(t: Tensor) -> Tensor:
+    """t contiguous and aligned for the kernels."""
+    return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else _aligned(t.contiguous())
 
 
 def _mx_dtype(op: str, dtype: torch.dtype) -> int:
@@ -1359,30 +1361,9 @@ def _mx_dtype(op: str, dtype: torch.dtype) -> int:
     return DTYPE_CODES[dtype]
 
 
-@mxfp4_quantize.register_fake
-def _(x):
-    u8 = lambda n: x.new_empty(*x.shape[:-1], n, dtype=torch.uint8)  # noqa: E731
-    return u8(x.shape[-1] // 2), u8(x.shape[-1] // MX_BLOCK)
-
-
-@torch.library.custom_op("moe_mi355x_mx::mxfp4_dequantize", mutates_args=())
-def mxfp4_dequantize(q: Tensor, scale: Tensor, dtype: torch.dtype = torch.bfloat16) -> Tensor:
-    """The values [.., K] of an MXFP4 matrix (q [.., K / 2], scale [.., K / 32] uint8) in bf16 or
-    fp32, which hold each of them exactly within their range (past it: infinities)."""
-    require_gpu(q, scale)
-    code = _mx_dtype("mxfp4_dequantize", dtype)
-    _check_packed("mxfp4_dequantize", "q", q, scale)
-    cols = 2 * q.shape[-1]
-    q, scale = _aligned(q.contiguous()), scale.contiguous()
-    x = torch.empty(*q.shape[:-1], cols, dtype=dtype, device=q.device)
-    with _guard(q):
-        call("moe_mxfp4_dequant_rows", ptr(q), ptr(scale), q.numel() // (cols // 2), cols, cols, code, ptr(x), stream_of(q))
-    return x
-
-
-@mxfp4_dequantize.register_fake
-def _(q, scale, dtype=torch.bfloat16):
-    return q.new_empty(*q.shape[:-1], 2 * q.shape[-1], dtype=dtype)
+def _check_mx_matrix(op: str, cols: int) -> None:
+    if cols < MX_BLOCK or cols % MX_BLOCK:
+        raise ValueError(f"{op} takes rows of whole blocks of {MX_BLOCK} elements, got {cols}")
 
 
 def _check_packed(op: str, name: str, q: Tensor, scale: Tensor, shape: tuple | None = None) -> None:
@@ -1390,22 +1371,121 @@ def _check_packed(op: str, name: str, q: Tensor, scale: Tensor, shape: tuple | N
     `shape` where one is given."""
     if q.dtype != torch.uint8 or scale.dtype != torch.uint8:
         raise TypeError(f"{op} expects uint8 {name} and scales, got {q.dtype} and {scale.dtype}")
-    if q.dim() < 1 or scale.dim() != q.dim() or scale.shape[:-1] != q.shape[:-1] or q.device != scale.device:
-        raise ValueError(f"{op}: {name} {tuple(q.shape)} on {q.device} and its scales {tuple(scale.shape)} on "
+    qs, ss = q.shape, scale.shape
+    if not qs or len(ss) != len(qs) or ss[:-1] != qs[:-1] or q.device != scale.device:
+        raise ValueError(f"{op}: {name} {tuple(qs)} on {q.device} and its scales {tuple(ss)} on "
                          f"{scale.device} do not belong together")
-    _check_mx_matrix(op, 2 * q.shape[-1])
-    if scale.shape[-1] * 16 != q.shape[-1]:
-        raise ValueError(f"{op}: {name} of {2 * q.shape[-1]} columns takes {q.shape[-1] // 16} scales a row, "
-                         f"got {scale.shape[-1]}")
-    if shape is not None and tuple(q.shape[:-1]) + (2 * q.shape[-1],) != shape:
-        raise ValueError(f"{op} expects {name} of {list(shape)} values, got {[*q.shape[:-1], 2 * q.shape[-1]]}")
+    _check_mx_matrix(op, 2 * qs[-1])
+    if ss[-1] * 16 != qs[-1]:
+        raise ValueError(f"{op}: {name} of {2 * qs[-1]} columns takes {qs[-1] // 16} scales a row, got {ss[-1]}")
+    if shape is not None and (*qs[:-1], 2 * qs[-1]) != shape:
+        raise ValueError(f"{op} expects {name} of {list(shape)} values, got {[*qs[:-1], 2 * qs[-1]]}")
 
 
-def _mxfp4_workspace(r: int, e: int, d: int, h_dim: int, device: torch.device) -> Tensor:
-    return torch.empty(max(int(lib().moe_mxfp4_workspace_bytes(r, e, d, h_dim)), 16), dtype=torch.uint8, device=device)
+@_mx_op("mxfp4_quantize(Tensor x) -> (Tensor, Tensor)")
+def _mxfp4_quantize(x: Tensor) -> tuple[Tensor, Tensor]:
+    require_gpu(x)
+    code = _mx_dtype("mxfp4_quantize", x.dtype)
+    if x.dim() < 1:
+        raise ValueError("mxfp4_quantize expects rows, got a scalar")
+    *lead, cols = x.shape
+    _check_mx_matrix("mxfp4_quantize", cols)
+    x = _ready(x)
+    q = x.new_empty(*lead, cols // 2, dtype=torch.uint8)
+    scale = x.new_empty(*lead, cols // MX_BLOCK, dtype=torch.uint8)
+    with _guard(x):
+        call("moe_mxfp4_quant_rows", ptr(x), x.numel() // cols, cols, cols, code, ptr(q), ptr(scale), stream_of(x))
+    return q, scale
 
 
-@torch.library.custom_op("moe_mi355x_mx::grouped_swiglu_mxfp4", mutates_args=())
+@torch.library.register_fake("moe_mi355x_mx::mxfp4_quantize", lib=_MX)
+def _(x):
+    u8 = lambda n: x.new_empty(*x.shape[:-1], n, dtype=torch.uint8)  # noqa: E731
+    return u8(x.shape[-1] // 2), u8(x.shape[-1] // MX_BLOCK)
+
+
+def mxfp4_quantize(x: Tensor) -> tuple[Tensor, Tensor]:
+    """x [.., K] (bf16 or fp32, K a multiple of 32) in MXFP4: (q [.., K / 2] uint8, two e2m1
+    codes a byte, the first in the low half; scale [.., K / 32] uint8, e8m0). A block's scale is
+    the least power of two 2^k, k in [-127, 127], with max |x| <= 6 * 2^k; elements are rounded
+    to nearest, ties to the even code. A block with an infinity or a NaN gets the NaN scale 255."""
+    return _mxfp4_quantize(x.detach())
+
+
+@_mx_op("mxfp4_dequantize(Tensor q, Tensor scale, ScalarType dtype) -> Tensor")
+def _mxfp4_dequantize(q: Tensor, scale: Tensor, dtype: torch.dtype) -> Tensor:
+    require_gpu(q, scale)
+    code = _mx_dtype("mxfp4_dequantize", dtype)
+    _check_packed("mxfp4_dequantize", "q", q, scale)
+    *lead, half = q.shape
+    q, scale = _ready(q), scale.contiguous()
+    x = q.new_empty(*lead, 2 * half, dtype=dtype)
+    with _guard(q):
+        call("moe_mxfp4_dequant_rows", ptr(q), ptr(scale), q.numel() // half, 2 * half, 2 * half, code, ptr(x), stream_of(q))
+    return x
+
+
+@torch.library.register_fake("moe_mi355x_mx::mxfp4_dequantize", lib=_MX)
+def _(q, scale, dtype):
+    return q.new_empty(*q.shape[:-1], 2 * q.shape[-1], dtype=dtype)
+
+
+def mxfp4_dequantize(q: Tensor, scale: Tensor, dtype: torch.dtype = torch.bfloat16) -> Tensor:
+    """The values [.., K] of an MXFP4 matrix (q [.., K / 2], scale [.., K / 32] uint8) in bf16 or
+    fp32, which hold each of them exactly within their range (past it: infinities)."""
+    return _mxfp4_dequantize(q, scale, dtype)
+
+
+@functools.lru_cache(maxsize=256)
+def _mxfp4_workspace_bytes(r: int, e: int, d: int, h_dim: int) -> int:
+    return max(int(lib().moe_mxfp4_workspace_bytes(r, e, d, h_dim)), 16)
+
+
+def _check_mxfp4_rows(op: str, x: Tensor, qw1: Tensor, counts: Tensor, glu: int = 1) -> tuple[int, int, int, int]:
+    _check_bf16(op, x=x)
+    xs, ws, cs = x.shape, qw1.shape, counts.shape
+    if len(xs) != 2 or len(ws) != 3 or len(cs) != 1 or cs[0] != ws[0] or ws[1] % glu:
+        raise ValueError(f"{op} expects x [R, D], packed weights [E, .., ..] and counts [E], got {tuple(xs)}, "
+                         f"{tuple(ws)}, {tuple(cs)}")
+    r, d = xs
+    e, h_dim = ws[0], ws[1] // glu
+    _check_dims(op, e, d, h_dim, MX_BLOCK)
+    return r, d, e, h_dim
+
+
+def _no_gradients(op: str, *tensors: Tensor) -> None:
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError(f"{op} is for inference and has no gradients: call it under torch.no_grad() or on detached "
+                           "tensors (grouped_swiglu_mxfp4_train trains on bf16 weights)")
+
+
+@_mx_op("grouped_swiglu_mxfp4(Tensor x, Tensor qw1, Tensor sw1, Tensor qw2, Tensor sw2, Tensor qw3, Tensor sw3, "
+        "Tensor num_tokens_per_expert) -> Tensor")
+def _grouped_swiglu_mxfp4(x, qw1, sw1, qw2, sw2, qw3, sw3, num_tokens_per_expert):
+    op = "grouped_swiglu_mxfp4"
+    counts = num_tokens_per_expert
+    require_gpu(x, qw1, sw1, qw2, sw2, qw3, sw3, counts)
+    r, d, e, h_dim = _check_mxfp4_rows(op, x, qw1, counts)
+    _check_packed(op, "w1", qw1, sw1, (e, h_dim, d))
+    _check_packed(op, "w2", qw2, sw2, (e, d, h_dim))
+    _check_packed(op, "w3", qw3, sw3, (e, h_dim, d))
+    _check_counts(op, counts, x, qw1, qw2, qw3)
+    x, qw1, sw1, qw2, sw2, qw3, sw3 = map(_ready, (x, qw1, sw1, qw2, sw2, qw3, sw3))
+    counts = counts.to(torch.int64).contiguous()
+    ws_bytes = _mxfp4_workspace_bytes(r, e, d, h_dim)
+    ws = x.new_empty(ws_bytes, dtype=torch.uint8)
+    y = x.new_empty(r, d)
+    with _guard(x):
+        call("moe_mxfp4_swiglu_fwd", ptr(x), ptr(qw1), ptr(sw1), ptr(qw2), ptr(sw2), ptr(qw3), ptr(sw3), ptr(counts), r, e,
+             d, h_dim, ptr(ws), ws_bytes, ptr(y), stream_of(x))
+    return y
+
+
+@torch.library.register_fake("moe_mi355x_mx::grouped_swiglu_mxfp4", lib=_MX)
+def _(x, qw1, sw1, qw2, sw2, qw3, sw3, num_tokens_per_expert):
+    return x.new_empty(x.shape)
+
+
 def grouped_swiglu_mxfp4(
     x: Tensor, qw1: Tensor, sw1: Tensor, qw2: Tensor, sw2: Tensor, qw3: Tensor, sw3: Tensor,
     num_tokens_per_expert: Tensor,
@@ -1414,50 +1494,17 @@ def grouped_swiglu_mxfp4(
     w2 [E, D, H]): x [R, D] bf16 in expert order is quantized on the way, h = silu(x w1^T)
     (x w3^T) is taken in fp32 and quantized, y = h w2^T [R, D] is rounded to bf16 once. Rows past
     sum(counts) are zero. For inference: no gradients. D and H are multiples of 32."""
-    op = "grouped_swiglu_mxfp4"
-    require_gpu(x, qw1, sw1, qw2, sw2, qw3, sw3, num_tokens_per_expert)
-    r, d, e, h_dim = _check_mxfp4_rows(op, x, qw1, num_tokens_per_expert)
-    _check_packed(op, "w1", qw1, sw1, (e, h_dim, d))
-    _check_packed(op, "w2", qw2, sw2, (e, d, h_dim))
-    _check_packed(op, "w3", qw3, sw3, (e, h_dim, d))
-    _check_counts(op, num_tokens_per_expert, x, qw1, qw2, qw3)
-    x, qw1, sw1, qw2, sw2, qw3, sw3 = (_aligned(t.contiguous()) for t in (x, qw1, sw1, qw2, sw2, qw3, sw3))
-    counts = num_tokens_per_expert.to(torch.int64).contiguous()
-    ws = _mxfp4_workspace(r, e, d, h_dim, x.device)
-    y = x.new_empty(r, d)
-    with _guard(x):
-        call("moe_mxfp4_swiglu_fwd", ptr(x), ptr(qw1), ptr(sw1), ptr(qw2), ptr(sw2), ptr(qw3), ptr(sw3), ptr(counts), r, e,
-             d, h_dim, ptr(ws), ws.numel(), ptr(y), stream_of(x))
-    return y
+    _no_gradients("grouped_swiglu_mxfp4", x)
+    return _grouped_swiglu_mxfp4(x, qw1, sw1, qw2, sw2, qw3, sw3, num_tokens_per_expert)
 
 
-def _check_mxfp4_rows(op: str, x: Tensor, qw1: Tensor, counts: Tensor, glu: int = 1) -> tuple[int, int, int, int]:
-    _check_bf16(op, x=x)
-    if x.dim() != 2 or qw1.dim() != 3 or counts.dim() != 1 or counts.shape[0] != qw1.shape[0] or qw1.shape[1] % glu:
-        raise ValueError(f"{op} expects x [R, D], packed weights [E, .., ..] and counts [E], got {tuple(x.shape)}, "
-                         f"{tuple(qw1.shape)}, {tuple(counts.shape)}")
-    r, d = x.shape
-    e, h_dim = qw1.shape[0], qw1.shape[1] // glu
-    _check_dims(op, e, d, h_dim, MX_BLOCK)
-    return r, d, e, h_dim
-
-
-@grouped_swiglu_mxfp4.register_fake
-def _(x, qw1, sw1, qw2, sw2, qw3, sw3, num_tokens_per_expert):
-    return x.new_empty(x.shape)
-
-
-@torch.library.custom_op("moe_mi355x_mx::grouped_swiglu_oss_mxfp4", mutates_args=())
-def grouped_swiglu_oss_mxfp4(
-    x: Tensor, qmlp1: Tensor, smlp1: Tensor, mlp1_bias: Tensor, qmlp2: Tensor, smlp2: Tensor, mlp2_bias: Tensor,
-    num_tokens_per_expert: Tensor, swiglu_limit: float,
-) -> Tensor:
-    """grouped_swiglu_mxfp4 for gpt-oss's experts (gpt_oss/moe.py:43-122): mlp1 [E, 2H, D] (glu row
-    2j, linear row 2j + 1) and mlp2 [E, D, H] packed in MXFP4, biases [E, 2H] and [E, D] taken in
-    bf16; biases, clamps and activation in fp32 between the products."""
+@_mx_op("grouped_swiglu_oss_mxfp4(Tensor x, Tensor qmlp1, Tensor smlp1, Tensor mlp1_bias, Tensor qmlp2, Tensor smlp2, "
+        "Tensor mlp2_bias, Tensor num_tokens_per_expert, float swiglu_limit) -> Tensor")
+def _grouped_swiglu_oss_mxfp4(x, qmlp1, smlp1, mlp1_bias, qmlp2, smlp2, mlp2_bias, num_tokens_per_expert, swiglu_limit):
     op = "grouped_swiglu_oss_mxfp4"
-    require_gpu(x, qmlp1, smlp1, mlp1_bias, qmlp2, smlp2, mlp2_bias, num_tokens_per_expert)
-    r, d, e, h_dim = _check_mxfp4_rows(op, x, qmlp1, num_tokens_per_expert, 2)
+    counts = num_tokens_per_expert
+    require_gpu(x, qmlp1, smlp1, mlp1_bias, qmlp2, smlp2, mlp2_bias, counts)
+    r, d, e, h_dim = _check_mxfp4_rows(op, x, qmlp1, counts, 2)
     _check_packed(op, "mlp1", qmlp1, smlp1, (e, 2 * h_dim, d))
     _check_packed(op, "mlp2", qmlp2, smlp2, (e, d, h_dim))
     if tuple(mlp1_bias.shape) != (e, 2 * h_dim) or tuple(mlp2_bias.shape) != (e, d):
@@ -1465,21 +1512,34 @@ def grouped_swiglu_oss_mxfp4(
                          f"{tuple(mlp2_bias.shape)}")
     if not swiglu_limit >= 0:
         raise ValueError(f"{op} expects a clamp limit of at least 0, got {swiglu_limit}")
-    _check_counts(op, num_tokens_per_expert, x, qmlp1, mlp1_bias, qmlp2, mlp2_bias)
-    x, qmlp1, smlp1, qmlp2, smlp2 = (_aligned(t.contiguous()) for t in (x, qmlp1, smlp1, qmlp2, smlp2))
-    b1, b2 = (_aligned(t.to(torch.bfloat16).contiguous()) for t in (mlp1_bias, mlp2_bias))
-    counts = num_tokens_per_expert.to(torch.int64).contiguous()
-    ws = _mxfp4_workspace(r, e, d, h_dim, x.device)
+    _check_counts(op, counts, x, qmlp1, mlp1_bias, qmlp2, mlp2_bias)
+    x, qmlp1, smlp1, qmlp2, smlp2 = map(_ready, (x, qmlp1, smlp1, qmlp2, smlp2))
+    b1, b2 = _ready(mlp1_bias.to(torch.bfloat16)), _ready(mlp2_bias.to(torch.bfloat16))
+    counts = counts.to(torch.int64).contiguous()
+    ws_bytes = _mxfp4_workspace_bytes(r, e, d, h_dim)
+    ws = x.new_empty(ws_bytes, dtype=torch.uint8)
     y = x.new_empty(r, d)
     with _guard(x):
         call("moe_mxfp4_oss_fwd", ptr(x), ptr(qmlp1), ptr(smlp1), ptr(b1), ptr(qmlp2), ptr(smlp2), ptr(b2), ptr(counts), r,
-             e, d, h_dim, float(swiglu_limit), ptr(ws), ws.numel(), ptr(y), stream_of(x))
+             e, d, h_dim, float(swiglu_limit), ptr(ws), ws_bytes, ptr(y), stream_of(x))
     return y
 
 
-@grouped_swiglu_oss_mxfp4.register_fake
+@torch.library.register_fake("moe_mi355x_mx::grouped_swiglu_oss_mxfp4", lib=_MX)
 def _(x, qmlp1, smlp1, mlp1_bias, qmlp2, smlp2, mlp2_bias, num_tokens_per_expert, swiglu_limit):
     return x.new_empty(x.shape)
+
+
+def grouped_swiglu_oss_mxfp4(
+    x: Tensor, qmlp1: Tensor, smlp1: Tensor, mlp1_bias: Tensor, qmlp2: Tensor, smlp2: Tensor, mlp2_bias: Tensor,
+    num_tokens_per_expert: Tensor, swiglu_limit: float,
+) -> Tensor:
+    """grouped_swiglu_mxfp4 for gpt-oss's experts (gpt_oss/moe.py:43-122): mlp1 [E, 2H, D] (glu row
+    2j, linear row 2j + 1) and mlp2 [E, D, H] packed in MXFP4, biases [E, 2H] and [E, D] taken in
+    bf16; biases, clamps and activation in fp32 between the products."""
+    _no_gradients("grouped_swiglu_oss_mxfp4", x, mlp1_bias, mlp2_bias)
+    return _grouped_swiglu_oss_mxfp4(x, qmlp1, smlp1, mlp1_bias, qmlp2, smlp2, mlp2_bias, num_tokens_per_expert,
+                                     swiglu_limit)
 
 
 def _mxfp4_padded(cols: int) -> int:  # moe_mxfp4_padded_cols
