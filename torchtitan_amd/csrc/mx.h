@@ -76,6 +76,17 @@ __device__ __forceinline__ void from_e4m3x4(uint32_t w, float s, float (&v)[4]) 
   v[0] = lo[0] * s; v[1] = lo[1] * s; v[2] = hi[0] * s; v[3] = hi[1] * s;
 }
 
+__device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+
+// Lane (row, g) holds words 4 g .. 4 g + 3 of its row and gets words g, 4 + g, 8 + g, 12 + g.
+__device__ __forceinline__ uint4 transpose4(uint4 v) {
+  const auto a = __builtin_amdgcn_permlane32_swap(v.x, v.z, false, false);
+  const auto b = __builtin_amdgcn_permlane32_swap(v.y, v.w, false, false);
+  const auto c = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false);
+  const auto d = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
+  return make_uint4(c[0], c[1], d[0], d[1]);
+}
+
 // One row's block of 32 columns in an accumulator tile: lane (row, g) holds columns 4 g .. of
 // the first 16 (a) and of the second (b). Returns the scale byte (in all four lanes) and in
 // `q` this lane's eight consecutive columns 8 g .. 8 g + 7 of the block, MXFP4 in one word,
