@@ -74,6 +74,31 @@ def test_forward_alone(dev):
         y.float().sum().backward()
 
 
+def test_backwards_of_given_tensors(dev):
+    """The backward operators called directly: kept tensors in any strides, and refusals."""
+    banner("kept in 8 bits, backward operators")
+    from torchtitan_amd import ops
+
+    c, x, dy, w1, w2, w3 = (t.to(dev) for t in _inputs([5, 0, 70], 0, 128, 192, 6, dev))
+    strided = lambda t: t.t().contiguous().t() if t.dim() == 2 else t.transpose(1, 2).contiguous().transpose(1, 2)  # noqa: E731
+    eight = ops.grouped_swiglu_ckpt8(x, w1, w2, w3, c)[1:]
+    four = ops.grouped_swiglu_mxfp4_train(x, w1, w2, w3, c)[1:]
+    for bwd, args, kept in ((ops.grouped_swiglu_ckpt8_backward, (dy, w1, w2, w3, c), eight),
+                            (ops.grouped_swiglu_mxfp4_train_backward, (dy, c), four)):
+        want = bwd(*args, *kept)
+        for a, b in zip(want, bwd(*map(lambda t: strided(t) if t.dim() > 1 else t, args), *map(strided, kept))):
+            assert torch.equal(a, b)
+        for i in range(len(kept)):
+            with pytest.raises(ValueError):
+                bwd(*args, *kept[:i], kept[i][:-1], *kept[i + 1:])
+            with pytest.raises(TypeError):
+                bwd(*args, *kept[:i], kept[i].float(), *kept[i + 1:])
+        with pytest.raises((TypeError, ValueError)):
+            bwd(dy.float(), *args[1:], *kept)
+        with pytest.raises(ValueError):
+            bwd(dy[:, :64], *args[1:], *kept)
+
+
 def test_kept_values(dev):
     """What is kept is MXFP8 of x, and of g and u as 64 bits give them (a step off at a border)."""
     banner("kept in 8 bits, kept values")

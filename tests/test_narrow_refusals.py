@@ -82,6 +82,8 @@ def test_products(lib):
     assert lib.moe_grouped_gemm_gate_up_keep8(null, null, null, at, 0, 2, 64, 64, null, null, null, null, null, null) == 0
     assert lib.moe_grouped_gemm_gate_up_keep8(at, at, at, at, 4, 2, 64, 64, at, null, null, null, at, null) == -1
     assert lib.moe_grouped_gemm_bwd_dgu_keep8(at, at, null, at, at, at, at, 4, 2, 64, 64, at, null, null) == -1
+    for bad in ((at + 8, at, at, at), (at, at + 1, at, at), (at, at, at + 4, at), (at, at, at, at + 1)):  # read in wide pieces
+        assert lib.moe_grouped_gemm_bwd_dgu_keep8(at, at, *bad, at, 4, 2, 64, 64, at, null, null) == -1
     assert lib.moe_grouped_gemm_bwd_dx_once(null, at, at, at, 4, 2, 64, 64, at, null) == -1
 
 
@@ -99,6 +101,21 @@ def test_packed_arguments():
             ops._check_packed("op", "w", a, b)
     with pytest.raises(ValueError, match="expects w"):
         ops._check_packed("op", "w", q, s, (3, 4, 64))
+
+
+def test_kept_arguments(monkeypatch):
+    from torchtitan_amd import ops
+
+    monkeypatch.setattr(ops, "require_gpu", lambda *t: None)
+    dy, q, s = torch.zeros(4, 64), torch.zeros(4, 64, dtype=torch.uint8), torch.zeros(4, 2, dtype=torch.uint8)
+    got = ops._kept("op", dy, g=(q.t().contiguous().t(), s, (4,), 64, 2))
+    assert got[0].is_contiguous() and torch.equal(got[0], q) and torch.equal(got[1], s)
+    for a, b in ((q.view(torch.int8), s), (q, s.float())):
+        with pytest.raises(TypeError, match="uint8 g"):
+            ops._kept("op", dy, g=(a, b, (4,), 64, 2))
+    for a, b in ((q[:3], s), (q, s[:, :1]), (q[:, :32], s), (q, s[:3]), (q[0], s)):
+        with pytest.raises(ValueError, match="expects g"):
+            ops._kept("op", dy, g=(a, b, (4,), 64, 2))
 
 
 def test_expert_arguments(monkeypatch):

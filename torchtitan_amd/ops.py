@@ -1171,13 +1171,14 @@ def _check_experts(op: str, x: Tensor, w1: Tensor, w2: Tensor, w3: Tensor, count
     w2 [E, D, H], counts [E] integers, all on one device."""
     require_gpu(x, w1, w2, w3, counts)
     _check_bf16(op, x=x, w1=w1, w2=w2, w3=w3)
-    if x.dim() != 2 or w1.dim() != 3 or counts.dim() != 1:
-        raise ValueError(f"{op} expects x [R, D], weights [E, .., ..] and counts [E], got {tuple(x.shape)}, "
-                         f"{tuple(w1.shape)}, {tuple(counts.shape)}")
-    e, h, d = w1.shape
-    if x.shape[1] != d or w3.shape != (e, h, d) or w2.shape != (e, d, h) or counts.shape[0] != e:
-        raise ValueError(f"{op}: shapes do not agree: x {tuple(x.shape)}, w1 {tuple(w1.shape)}, w2 {tuple(w2.shape)}, "
-                         f"w3 {tuple(w3.shape)}, counts {tuple(counts.shape)}")
+    xs, ws, cs = x.shape, w1.shape, counts.shape
+    if len(xs) != 2 or len(ws) != 3 or len(cs) != 1:
+        raise ValueError(f"{op} expects x [R, D], weights [E, .., ..] and counts [E], got {tuple(xs)}, {tuple(ws)}, "
+                         f"{tuple(cs)}")
+    e, h, d = ws
+    if xs[1] != d or w3.shape != ws or w2.shape != (e, d, h) or cs[0] != e:
+        raise ValueError(f"{op}: shapes do not agree: x {tuple(xs)}, w1 {tuple(ws)}, w2 {tuple(w2.shape)}, "
+                         f"w3 {tuple(w3.shape)}, counts {tuple(cs)}")
     _check_dims(op, e, d, h, multiple)
     _check_counts(op, counts, x, w1, w2, w3)
 
@@ -1192,7 +1193,8 @@ def _check_dims(op: str, e: int, d: int, h: int, multiple: int) -> None:
 def _check_counts(op: str, counts: Tensor, *others: Tensor) -> None:
     if counts.is_floating_point() or counts.is_complex() or counts.dtype == torch.bool:
         raise TypeError(f"{op} expects integer counts, got {counts.dtype}")
-    if any(t.device != counts.device for t in others):
+    here = counts.device
+    if any([t.device != here for t in others]):
         raise ValueError(f"{op}: tensors on more than one device")
 
 
@@ -1272,11 +1274,18 @@ def _narrow_backward(dy: Tensor, w1: Tensor, w2: Tensor, w3: Tensor, counts: Ten
     return dx, dw1, dw2, dw3
 
 
-def _check_dy(op: str, dy: Tensor, r: int, d: int, like: Tensor) -> Tensor:
-    require_gpu(dy)
-    if tuple(dy.shape) != (r, d) or dy.device != like.device:
-        raise ValueError(f"{op} expects a gradient [{r}, {d}] on {like.device}, got {tuple(dy.shape)} on {dy.device}")
-    return _aligned(dy.to(torch.bfloat16).contiguous())
+def _kept(op: str, like: Tensor, **matrices: tuple) -> list[Tensor]:
+    """Kept matrices given by name as (q, scale, leading sizes, bytes and scales of a row):
+    checked, contiguous and aligned, in that order."""
+    out = []
+    for name, (q, scale, lead, n, m) in matrices.items():
+        if q.dtype is not torch.uint8 or scale.dtype is not torch.uint8:
+            raise TypeError(f"{op} expects uint8 {name} and scales, got {q.dtype} and {scale.dtype}")
+        if q.shape != (*lead, n) or scale.shape != (*lead, m) or not q.device == scale.device == like.device:
+            raise ValueError(f"{op} expects {name} {[*lead, n]} with scales {[*lead, m]} on {like.device}, got "
+                             f"{tuple(q.shape)} on {q.device} with {tuple(scale.shape)} on {scale.device}")
+        out += [_ready(q), _ready(scale)]
+    return out
 
 
 @torch.library.custom_op("moe_mi355x_mx::grouped_swiglu_ckpt8_backward", mutates_args=())
@@ -1286,9 +1295,12 @@ def grouped_swiglu_ckpt8_backward(
 ) -> tuple[Tensor, Tensor, Tensor, Tensor]:
     """(dx, dw1, dw2, dw3) of grouped_swiglu_ckpt8 from what it kept; dx is zero on rows past
     sum(counts), weights of experts without rows get zeros. What is not needed is empty."""
-    r, d = x8.shape
-    dy = _check_dy("grouped_swiglu_ckpt8_backward", dy, r, d, x8)
-    w1, w2, w3 = (_aligned(t.contiguous()) for t in (w1, w2, w3))
+    op = "grouped_swiglu_ckpt8_backward"
+    _check_experts(op, dy, w1, w2, w3, num_tokens_per_expert, 64)
+    r, (_e, h_dim, d) = dy.shape[0], w1.shape
+    x8, xs, g8, gs, u8, us = _kept(op, dy, x=(x8, xs, (r,), d, d // MX_BLOCK), g=(g8, gs, (r,), h_dim, h_dim // MX_BLOCK),
+                                   u=(u8, us, (r,), h_dim, h_dim // MX_BLOCK))
+    dy, w1, w2, w3 = map(_ready, (dy, w1, w2, w3))
     counts = num_tokens_per_expert.to(torch.int64).contiguous()
 
     def rows() -> Tensor:
@@ -1620,9 +1632,18 @@ def grouped_swiglu_mxfp4_train_backward(
 ) -> tuple[Tensor, Tensor, Tensor, Tensor]:
     """(dx, dw1, dw2, dw3) of grouped_swiglu_mxfp4_train from what it kept; dx is zero on rows
     past sum(counts), weights of experts without rows get zeros. What is not needed is empty."""
-    r, d, h_dim = qx.shape[0], qw2.shape[1], qw1.shape[1]
-    dy = _check_dy("grouped_swiglu_mxfp4_train_backward", dy, r, d, qx)
-    counts = num_tokens_per_expert.to(torch.int64).contiguous()
+    op = "grouped_swiglu_mxfp4_train_backward"
+    counts = num_tokens_per_expert
+    require_gpu(dy, counts)
+    r, d, e, h_dim = _check_mxfp4_rows(op, dy, qw1, counts)
+    pd, ph, nd, nh = _mxfp4_padded(d), _mxfp4_padded(h_dim), d // MX_BLOCK, h_dim // MX_BLOCK
+    _check_dims(op, e, d, h_dim, 64)
+    _check_counts(op, counts, dy)
+    qx, sx, qh, sh, qw1, sw1, qw2, sw2, qw3, sw3, g8, gs, u8, us = _kept(
+        op, dy, x=(qx, sx, (r,), pd // 2, pd // MX_BLOCK), h=(qh, sh, (r,), ph // 2, ph // MX_BLOCK),
+        w1=(qw1, sw1, (e, h_dim), d // 2, nd), w2=(qw2, sw2, (e, d), h_dim // 2, nh), w3=(qw3, sw3, (e, h_dim), d // 2, nd),
+        g=(g8, gs, (r,), h_dim, nh), u=(u8, us, (r,), h_dim, nh))
+    dy, counts = _ready(dy), counts.to(torch.int64).contiguous()
     with _guard(dy):
         s = stream_of(dy)
         # the values dgu and dx multiply; dW takes only their shapes
