@@ -146,6 +146,10 @@ SERVE = [
     ("few rows, rows past the LDS", [2, 1], 0, 16384, 32),
     ("many experts", [0, 2, 0, 0, 17, 1] * 170 + [3, 0, 0, 9], 2, 64, 32),
     ("many experts, many rows", [0, 40, 0, 0, 300, 1] * 20, 2, 64, 96),
+    ("many rows, partial stages", [240, 200, 0, 380], 1, 544, 320),
+    ("past the row tile, odd blocks", [270, 300, 765, 3], 0, 320, 416),
+    ("one expert, one stage", [2100], 0, 96, 96),
+    ("small work, many rows", [510, 0, 255], 3, 288, 160),
     ("no rows for anyone", [0, 0, 0], 6, 64, 64),
 ]
 
@@ -183,17 +187,18 @@ def test_serve(dev, act, case):
     assert not got[n:].any()
 
 
-def test_serve_odd_counts(dev):
+@pytest.mark.parametrize("rows", [40, 2000])
+def test_serve_odd_counts(dev, rows):
     """Counts that sum past the rows, negative counts, int32 counts: as the rows there are."""
     banner("mxfp4 experts odd counts")
     from torchtitan_amd import ops
 
     gen = torch.Generator().manual_seed(4)
-    e, d, h, rows = 5, 128, 96, 40
+    e, d, h = 5, 128, 96
     x = torch.randn(rows, d, generator=gen).bfloat16()
     w1, w2, w3 = _packed(gen, e, h, d, 0.1), _packed(gen, e, d, h, 0.1), _packed(gen, e, h, d, 0.1)
     vals = [N.unpack4(*w) for w in (w1, w2, w3)]
-    for counts in ([10, -3, 20, 2 ** 40, 7], [2 ** 62, 2 ** 62, 5, 1, 1], [0, 0, 0, 0, 40]):
+    for counts in ([10, -3, 20, 2 ** 40, 7], [2 ** 62, 2 ** 62, 5, 1, 1], [0, 0, 0, 0, rows]):
         c = torch.tensor(counts)
         got = ops.grouped_swiglu_mxfp4(*(t.to(dev) for t in (x, *w1, *w2, *w3, c)))
         want, tol = N.experts4(N.q4(x), *vals, c)
@@ -206,7 +211,7 @@ def test_serve_odd_counts(dev):
     assert empty.shape == (0, d)
 
 
-@pytest.mark.parametrize("rows", [12, 600])
+@pytest.mark.parametrize("rows", [12, 600, 1800])
 def test_serve_not_finite(dev, rows):
     """A row with an infinity or NaN spoils itself, an expert with a NaN scale its own rows;
     every other row keeps its bits."""
@@ -234,13 +239,14 @@ def test_serve_not_finite(dev, rows):
     assert torch.equal(got[:a], want[:a]) and torch.equal(got[b:], want[b:]) and got[a:b].isnan().all()
 
 
-def test_serve_views_and_alignment(dev):
+@pytest.mark.parametrize("times", [1, 70])
+def test_serve_views_and_alignment(dev, times):
     banner("mxfp4 experts views")
     from torchtitan_amd import ops
 
     gen = torch.Generator().manual_seed(6)
-    e, d, h, rows = 4, 96, 64, 30
-    counts = torch.tensor([8, 2, 0, 20]).to(dev)
+    e, d, h, rows = 4, 96, 64, 30 * times
+    counts = torch.tensor([8, 2, 0, 20]).to(dev) * times
     x = torch.randn(rows, d, generator=gen).bfloat16().to(dev)
     w = [t.to(dev) for t in (*_packed(gen, e, h, d, 0.1), *_packed(gen, e, d, h, 0.1), *_packed(gen, e, h, d, 0.1))]
     want = ops.grouped_swiglu_mxfp4(x, *w, counts)

@@ -71,7 +71,8 @@ def test_products(lib):
     ws = lib.moe_mxfp4_workspace_bytes
     assert ws(0, 2, 64, 64) == 0 and ws(-1, 2, 64, 64) == -1 and ws(4, 2, 48, 64) == -1
     assert ws(2, 4, 64, 64) == 2 * (2 * 128 + 256)
-    assert ws(1000, 4, 96, 64) == 2 * (128000 + 8192) + 4 * 2 * 64 * 8
+    assert ws(1000, 4, 96, 64) == 2 * (128000 + 8192)
+    assert ws(2000, 4, 96, 64) == 2 * (256000 + 16128) + 4 * 2 * 64 * 8
     # the training products take even numbers of blocks
     gate = lambda r, d, h, q=at: lib.moe_mxfp4_gemm_gate_up_keep(q, at, at, at, at, at, at, r, 2, d, h, at, at, at, at, at, at, null)  # noqa: E731
     down = lambda r, d, h, q=at: lib.moe_mxfp4_gemm_down(q, at, at, at, at, r, 2, d, h, at, null)  # noqa: E731

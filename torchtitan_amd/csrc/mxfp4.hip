@@ -672,20 +672,26 @@ __global__ __launch_bounds__(512, 2) void wide_kernel(Params p) {
 
 // Few rows per expert: the weights are read once and decide the time, so every byte goes
 // straight from memory into the MFMAs' registers. A unit is 64 weight rows (gate_up: 32 gate and
-// 32 up rows, one scaling block of h; down: 64 columns) by up to 16 TM rows of one expert;
-// eight waves take four blocks of 16 weight rows by the even and the odd 256-k stages. A wave
-// keeps two groups of kAhead stages in registers, the next group's loads in flight while
-// this group multiplies, through to the following unit. A workgroup's units are consecutive,
-// so the rows, which gate_up quantizes from bf16 on the way into LDS, are prepared once per
-// expert and workgroup.
-constexpr int kAhead = 2;
+// 32 up rows, one scaling block of h; down: 64 columns) by up to 16 rows of one expert; eight
+// waves take four blocks of 16 weight rows by the even and the odd 256-k stages. A wave keeps two
+// stages in registers, in turn, one's loads in flight while the other multiplies, through to the
+// following unit. A workgroup's units are consecutive, so the rows, which gate_up quantizes from
+// bf16 on the way into LDS, are prepared once per expert and workgroup.
+//
+// What bounds it: the weights' bytes. One row on each of 57 experts of 7168 / 2048 takes 248 us, 5.4
+// TB/s; four rows each on 256 of 2304 / 1024 201 us, 4.8 TB/s; eight each on 32 of 2880 / 2880 123
+// us, 3.5 TB/s (rows of 1440 bytes: a stage of 128 straddles two cache lines; 2816 takes 104).
+// One token's 8 experts of 256 take 16 us, of which the 30 MB are 6: two launches that each wait for
+// the counts, then for the weights. A register copy of the stage in flight (the loop not in
+// pairs) waits for its loads: 20 and 139 us. More in flight was slower: groups of two stages
+// 17.5 and 125 us, three or four single ones in turn 17.6 to 19.7 and 126 to 134.
 constexpr int kRows = 16;
 __host__ __device__ constexpr int narrow_stride(int K) { return (K + 255) / 256 * 128 + 16; }  // rows 16 bytes apart mod 128
 __host__ __device__ constexpr int64_t narrow_lds(int K) {  // the rows, their scales, and the waves' sums
   return (int64_t)kRows * (narrow_stride(K) + (K + 255) / 256 * 8) + 2 * 8 * 64 * 16;
 }
 
-template <int MODE, int ACT>
+template <int MODE, int ACT, bool ODD>
 __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
   extern __shared__ __attribute__((aligned(16))) uint8_t s_dyn[];
   __shared__ int s_seg[kMaxE + 1];
@@ -701,9 +707,10 @@ __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
   segments_wave(p, s_seg, s_tile, [&](int rows) { return (rows + kRows - 1) / kRows * NCB; });
   const int64_t total = s_tile[E];
   const int u0 = (int)(total * blockIdx.x / gridDim.x), u1 = (int)(total * (blockIdx.x + 1) / gridDim.x);
-  const int mine = (nst - ks + 1) / 2;  // this wave's stages: ks, ks + 2, ...
+  const int mine = (nst + 1) / 2;  // stages of a half: ks, ks + 2, ...
 
-  struct Group { uint4 w[kAhead][2]; uint32_t s[kAhead]; };
+  using Scale = std::conditional_t<ODD, uint8_t, uint16_t>;
+  struct Stage { uint4 w[2]; Scale s[ODD ? 2 : 1]; };
   struct Unit { int e, rt, cb; };
   auto decode = [&](int u) {
     Unit r;
@@ -713,23 +720,28 @@ __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
     r.cb = local - r.rt * NCB;
     return r;
   };
-  auto load = [&](Group& g, const Unit& u, int base) {
-    const int col = MODE == kGateUp ? u.cb * 32 + (nb & 1) * 16 + ml : u.cb * 64 + nb * 16 + ml;
-    const bool up = MODE == kGateUp && nb >= 2, in = col < N;
+  // Without branches, so that the compiler's waits leave the other stage in flight: chunks past
+  // the row repeat its last ones, against zeros in LDS; columns past N repeat the last block's
+  // (nothing is stored of them); and behind the last unit one piece is loaded again.
+  auto load = [&](Stage& g, const Unit& u, int i, bool on) {
+    const int col = MODE == kGateUp ? u.cb * 32 + (nb & 1) * 16 : min(u.cb * 64 + nb * 16, N - 16);
+    const bool up = MODE == kGateUp && nb >= 2;
     const int64_t row = u.e * p.e_rows + (int64_t)col * p.r_rows;
     const uint8_t* wq = (up ? p.qb : p.qa) + row * kbytes;
     const uint8_t* ws = (up ? p.sb : p.sa) + row * p.w_ld;
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      const int c = 8 * (ks + 2 * (base + i)) + 2 * g4;  // this lane's first chunk of 32 k
-      g.w[i][0] = *(const uint4*)(in && c < KB ? wq + c * 16 : (const uint8_t*)kZeroRow);
-      g.w[i][1] = *(const uint4*)(in && c + 1 < KB ? wq + c * 16 + 16 : (const uint8_t*)kZeroRow);
-      if (KB % 2 == 0) {
-        g.s[i] = in && c < KB ? *(const uint16_t*)(ws + c) : 0x7f7fu;
-      } else {
-        const uint32_t lo = in && c < KB ? ws[c] : 0x7fu, hi = in && c + 1 < KB ? ws[c + 1] : 0x7fu;
-        g.s[i] = lo | (hi << 8);
-      }
+    const uint32_t lq = on ? (uint32_t)(ml * p.r_rows) * (uint32_t)kbytes : 0u, ls = on ? (uint32_t)(ml * p.r_rows * p.w_ld) : 0u;
+    const int c = on ? 8 * (ks + 2 * i) + 2 * g4 : 0;  // this lane's chunks of 32 k: c, c + 1
+    if constexpr (ODD) {
+      const uint32_t c0 = min(c, KB - 1), c1 = min(c + 1, KB - 1);
+      g.w[0] = *(const uint4*)(wq + (lq + c0 * 16));
+      g.w[1] = *(const uint4*)(wq + (lq + c1 * 16));
+      g.s[0] = ws[ls + c0];
+      g.s[1] = ws[ls + c1];
+    } else {
+      const uint32_t c0 = min(c, KB - 2);
+      g.w[0] = *(const uint4*)(wq + (lq + c0 * 16));
+      g.w[1] = *(const uint4*)(wq + (lq + c0 * 16 + 16));
+      g.s[0] = *(const uint16_t*)(ws + (ls + c0));
     }
   };
   struct Rows { Eight<uint16_t> v[4]; };
@@ -759,10 +771,14 @@ __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
           }
         }
       }
-      for (int i = tid; i < rows * (sld - KB); i += 512) sc[i / (sld - KB) * sld + KB + i % (sld - KB)] = 0x7f;
+      for (int i = tid; i < rows * (sld - KB); i += 512) {
+        const int r = i / (sld - KB), c = KB + i % (sld - KB);
+        *(uint4*)(sP + r * stride + c * 16) = make_uint4(0, 0, 0, 0);
+        sc[r * sld + c] = 0x7f;
+      }
     } else {
-      for (int i = tid; i < rows * KB; i += 512) {
-        const int r = i / KB, c = i - r * KB;
+      for (int i = tid; i < rows * sld; i += 512) {
+        const int r = i / sld, c = i - r * sld;
         *(uint4*)(sP + r * stride + c * 16) = *(const uint4*)(p.qp + (int64_t)(row0 + r) * (padded(K) / 2) + c * 16);
       }
       for (int i = tid; i < rows * nst; i += 512) {
@@ -772,7 +788,7 @@ __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
     }
   };
 
-  Group cur, nxt;
+  Stage ga, gb;
   Unit u{};
   Rows x;
   auto unit_rows = [&](const Unit& w, int& rows) {
@@ -787,46 +803,35 @@ __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
       const int row0 = unit_rows(u, rows);
       load_rows(x, row0, rows, tid);
     }
-    load(cur, u, 0);
+    load(ga, u, 0, true);
   }
-  int have_e = -1, have_rt = -1;
-  for (int t = u0; t < u1; ++t) {
-    int rows;
-    const int row0 = unit_rows(u, rows);
-    if (u.e != have_e || u.rt != have_rt) {
-      if (have_e >= 0) {
-        if (MODE == kGateUp) load_rows(x, row0, rows, tid);
-        __syncthreads();  // every wave is done with the rows before
-      }
-      fill(x, row0, rows);
-      __syncthreads();
-      have_e = u.e;
-      have_rt = u.rt;
+  int at = 0, t = u0, row0 = 0, rows = 0;
+  f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+  // unit t's stage `at` from `cur`, with the next one's loads on their way into `nxt`; false
+  // where that one is of other rows, or there is none
+  auto step = [&](Stage& cur, Stage& nxt) __attribute__((always_inline)) {
+    const bool last = at + 1 == mine;
+    const Unit un = last && t + 1 < u1 ? decode(t + 1) : u;
+    load(nxt, un, last ? 0 : at + 1, !last || t + 1 < u1);
+    const int st = ks + 2 * at;
+    if (st < nst) {
+      const uint32_t sw = ODD ? cur.s[0] | (cur.s[ODD] << 8) : cur.s[0];
+      const uint32_t sp = *(const uint16_t*)(sc + ml * sld + st * 8 + 2 * g4);
+      const uint4 a0 = *(const uint4*)(sP + ml * stride + st * 128 + g4 * 32);
+      const uint4 a1 = *(const uint4*)(sP + ml * stride + st * 128 + g4 * 32 + 16);
+      const uint4 b0 = cur.w[0], b1 = cur.w[1];
+      acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+          v8i_t{(int)b0.x, (int)b0.y, (int)b0.z, (int)b0.w, 0, 0, 0, 0},
+          v8i_t{(int)a0.x, (int)a0.y, (int)a0.z, (int)a0.w, 0, 0, 0, 0}, acc, 4, 4, 0, (int)sw, 0, (int)sp);
+      acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+          v8i_t{(int)b1.x, (int)b1.y, (int)b1.z, (int)b1.w, 0, 0, 0, 0},
+          v8i_t{(int)a1.x, (int)a1.y, (int)a1.z, (int)a1.w, 0, 0, 0, 0}, acc, 4, 4, 1, (int)sw, 1, (int)sp);
     }
-    const Unit un = t + 1 < u1 ? decode(t + 1) : u;
-    f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
-    for (int base = 0; base < mine; base += kAhead) {
-      if (base + kAhead < mine) load(nxt, u, base + kAhead);
-      else if (t + 1 < u1) load(nxt, un, 0);
-#pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
-        const int st = ks + 2 * (base + i);
-        if (st < nst) {
-          const uint32_t sp = *(const uint16_t*)(sc + ml * sld + st * 8 + 2 * g4);
-          const uint4 a0 = *(const uint4*)(sP + ml * stride + st * 128 + g4 * 32);
-          const uint4 a1 = *(const uint4*)(sP + ml * stride + st * 128 + g4 * 32 + 16);
-          const uint4 b0 = cur.w[i][0], b1 = cur.w[i][1];
-          acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-              v8i_t{(int)b0.x, (int)b0.y, (int)b0.z, (int)b0.w, 0, 0, 0, 0},
-              v8i_t{(int)a0.x, (int)a0.y, (int)a0.z, (int)a0.w, 0, 0, 0, 0}, acc, 4, 4, 0, (int)cur.s[i], 0, (int)sp);
-          acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-              v8i_t{(int)b1.x, (int)b1.y, (int)b1.z, (int)b1.w, 0, 0, 0, 0},
-              v8i_t{(int)a1.x, (int)a1.y, (int)a1.z, (int)a1.w, 0, 0, 0, 0}, acc, 4, 4, 1, (int)cur.s[i], 1, (int)sp);
-        }
-      }
-      cur = nxt;
+    if (!last) {
+      ++at;
+      return true;
     }
-    if (mine == 0 && t + 1 < u1) load(cur, un, 0);
+    at = 0;
     // one barrier a unit: the waves that read these sums come to the next one before anyone
     // writes over them; they take turns, so that none is behind the others for good
     f32x4_t* red = sums + (t & 1) * 8 * 64;
@@ -840,9 +845,9 @@ __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
     };
     if (MODE == kGateUp) {
       if (turn == 0) {
-        float ga[4], gb[4], ua[4], ub[4];
-        sum(0, ga);
-        sum(1, gb);
+        float ha[4], hb[4], ua[4], ub[4];
+        sum(0, ha);
+        sum(1, hb);
         sum(2, ua);
         sum(3, ub);
         const int hc = u.cb * 32, r = ml;
@@ -852,7 +857,7 @@ __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
           bias_a = *(const uint4*)bp;
           bias_b = *(const uint4*)(bp + 32);
         }
-        store_hidden<ACT, false>(p, row0 + r, hc, lane, r < rows, ga, gb, ua, ub, bias_a, bias_b);
+        store_hidden<ACT, false>(p, row0 + r, hc, lane, r < rows, ha, hb, ua, ub, bias_a, bias_b);
       }
     } else if (turn < 2) {
       const int pr = turn, n0 = u.cb * 64 + pr * 32, r = ml;
@@ -872,7 +877,26 @@ __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
         if (r < rows) *(uint4*)(p.y + (int64_t)(row0 + r) * N + n0 + 8 * g4) = v;
       }
     }
+    acc = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    const bool same = un.e == u.e && un.rt == u.rt;
     u = un;
+    return ++t < u1 && same;
+  };
+  while (t < u1) {
+    row0 = unit_rows(u, rows);
+    if (t > u0) {
+      if (MODE == kGateUp) load_rows(x, row0, rows, tid);
+      __syncthreads();  // every wave is done with the rows before
+    }
+    fill(x, row0, rows);
+    __syncthreads();
+    while (step(ga, gb)) {
+      if (!step(gb, ga)) {
+        gb = ga;
+        break;
+      }
+    }
+    ga = gb;
   }
   if (MODE == kDown) zero_rest(p, s_seg[E]);
 }
@@ -913,16 +937,24 @@ static void launch_narrow(const Params& p, hipStream_t stream) {
   int64_t g = (p.R / kRows + (p.R < p.E ? p.R : p.E)) * ncb;
   const int64_t most = (int64_t)cu_count() * 2;
   if (g > most) g = most;
-  if (narrow_lds(p.K) > 64 * 1024)
-    (void)hipFuncSetAttribute((const void*)narrow_kernel<MODE, ACT>, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsMost);
-  hipLaunchKernelGGL((narrow_kernel<MODE, ACT>), dim3((unsigned)g), dim3(512), (unsigned)narrow_lds(p.K), stream, p);
+  auto launch = [&](auto kernel) {
+    if (narrow_lds(p.K) > 64 * 1024)
+      (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsMost);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)g), dim3(512), (unsigned)narrow_lds(p.K), stream, p);
+  };
+  if (p.K / kBlock % 2) launch(narrow_kernel<MODE, ACT, true>);
+  else launch(narrow_kernel<MODE, ACT, false>);
 }
 
-// Up to eight rows per expert that can have one take the narrow kernel (us, narrow / wide: one
-// token top 8 on 256 experts of 2304 / 1024 20 / 35; 128 tokens, 4 rows each, 223 / 219; gpt-oss's
-// 32 experts with 8 rows each 140 / 152, with 32 each 165 / 161), where its rows fit into LDS.
+// The narrow kernel takes up to eight rows per expert that can have one, and small work, where the
+// wide kernel's tiles leave most of the chip idle, where its rows fit into LDS (us, narrow / wide
+// with its quantization; rows per expert): 256 experts of 2304 / 1024 one token 17 / 35, 4 rows 205 /
+// 221, 8 rows 229 / 228, 16 rows 295 / 239; 32 of gpt-oss's 2880 / 2880 8 rows 123 / 152, 16 rows 156 /
+// 155; 32 of 7168 / 2048 16 rows 238 / 198. Small: 8 experts of 2048 / 1408 16 rows 22 / 32, 32 rows 34 /
+// 34; 4 of 2880 / 2880 32 rows 33 / 67; 16 of 320 / 704 19 rows 17 / 25; one of 512 / 512 128 rows 13 / 23.
 static bool takes_narrow(int64_t R, int64_t E, int D, int H) {
-  return R <= 8 * (R < E ? R : E) && narrow_lds(D) <= kLdsMost && narrow_lds(H) <= kLdsMost;
+  const int64_t cols = 2 * (int64_t)H > D ? 2 * (int64_t)H : D;
+  return (R <= 8 * (R < E ? R : E) || R * ((cols + 255) / 256) <= 1536) && narrow_lds(D) <= kLdsMost && narrow_lds(H) <= kLdsMost;
 }
 
 static int check_shape(int64_t R, int E, int D, int H) {
