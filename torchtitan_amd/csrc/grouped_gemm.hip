@@ -650,6 +650,8 @@ __global__ __launch_bounds__(NW * 64, OCC) void grouped_gemm_kernel(GemmParams p
       }
     }
     if constexpr (MODE == kFwdGateUp && ACT == kSwiGLUKeep8) {
+      // h in 16-byte pieces, g and u in 8-byte ones of 32 columns a row: 1.37 ms at 2304 / 1024 /
+      // 256 / 131072, as the bf16 epilogue (16-byte pieces of g and u too: the same)
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
         const int r = row0 + wm * WM + i * 16 + ml;
