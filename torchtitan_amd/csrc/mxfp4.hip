@@ -681,26 +681,30 @@ __global__ __launch_bounds__(512, 2) void wide_kernel(Params p) {
 // waves take four blocks of 16 weight rows by the even and the odd 256-k stages. A wave keeps two
 // stages in registers, in turn, one's loads in flight while the other multiplies, through to the
 // following unit. A workgroup's units are consecutive, so the rows, which gate_up quantizes from
-// bf16 on the way into LDS, are prepared once per expert and workgroup.
+// bf16 on the way into LDS, are prepared once per expert and workgroup. The weights' scales come
+// through LDS, a unit ahead: 64 rows of them are one or two runs of memory, of which each thread
+// brings two bytes a stage.
 //
-// What bounds it: the weights' bytes. One row on each of 57 experts of 7168 / 2048 takes 248 us, 5.4
-// TB/s; four rows each on 256 of 2304 / 1024 201 us, 4.8 TB/s; eight each on 32 of 2880 / 2880 123
-// us, 3.5 TB/s (rows of 1440 bytes: a stage of 128 straddles two cache lines; 2816 takes 104).
-// One token's 8 experts of 256 take 16 us, of which the 30 MB are 6: two launches that each wait for
-// the counts, then for the weights. A register copy of the stage in flight (the loop not in
-// pairs) waits for its loads: 20 and 139 us. More in flight was slower: groups of two stages
-// 17.5 and 125 us, three or four single ones in turn 17.6 to 19.7 and 126 to 134.
+// What bounds it: the weights' bytes. One row on each of 57 experts of 7168 / 2048 takes 236 us, 5.6
+// TB/s; four rows each on 256 of 2304 / 1024 189 us, 5.1 TB/s; eight each on 32 of gpt-oss's 2880 / 2880
+// 102 us, 4.2 TB/s (rows of 1440 bytes: a stage of 128 straddles two cache lines). One token's 8
+// experts of 256 take 17 us, of which the 30 MB are 6: two launches that each wait for the counts,
+// then for the weights.
+// Measured otherwise: scales loaded where they are multiplied, two bytes a lane from 16 rows, 248, 203
+// and 123 us (a load costs by the cache lines it touches, and these were as many as the weights');
+// a register copy of the stage in flight (the loop not in pairs) waits for its loads: 220 and 139
+// us. More in flight was slower: groups of two stages 206 and 125 us, three or four single ones in
+// turn 199 to 219 and 126 to 134; loads past the caches 223 and 160.
 constexpr int kRows = 16;
 __host__ __device__ constexpr int narrow_stride(int K) { return (K + 255) / 256 * 128 + 16; }  // rows 16 bytes apart mod 128
-__host__ __device__ constexpr int64_t narrow_lds(int K) {  // the rows, their scales, and the waves' sums
-  return (int64_t)kRows * (narrow_stride(K) + (K + 255) / 256 * 8) + 2 * 8 * 64 * 16;
+__host__ __device__ constexpr int64_t narrow_lds(int K, int E) {  // rows and their scales, sums, the weights' scales, segments
+  return (int64_t)kRows * (narrow_stride(K) + (K + 255) / 256 * 8) + 2 * 8 * 64 * 16 + 2 * 64 * (K / kBlock) +
+         2 * (E + 1) * (int)sizeof(int);
 }
 
 template <int MODE, int ACT, bool ODD>
 __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
   extern __shared__ __attribute__((aligned(16))) uint8_t s_dyn[];
-  __shared__ int s_seg[kMaxE + 1];
-  __shared__ int s_tile[kMaxE + 1];
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int nb = wv & 3, ks = wv >> 2, ml = lane & 15, g4 = lane >> 4;
   const int E = p.E, K = p.K, N = p.N, KB = K / kBlock, kbytes = K / 2, nst = (K + 255) / 256;
@@ -708,14 +712,16 @@ __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
   uint8_t* sP = s_dyn;
   f32x4_t* sums = (f32x4_t*)(s_dyn + kRows * (stride + sld));  // two units' [2 ks][4 nb][64]
   uint8_t* sc = s_dyn + kRows * stride;
+  uint8_t* sW = (uint8_t*)(sums + 2 * 8 * 64);  // two units' weight scales, 64 rows of KB
+  int* s_seg = (int*)(sW + 2 * 64 * KB);
+  int* s_tile = s_seg + E + 1;
   const int NCB = MODE == kGateUp ? N / 32 : (N + 63) / 64;
   segments_wave(p, s_seg, s_tile, [&](int rows) { return (rows + kRows - 1) / kRows * NCB; });
   const int64_t total = s_tile[E];
   const int u0 = (int)(total * blockIdx.x / gridDim.x), u1 = (int)(total * (blockIdx.x + 1) / gridDim.x);
   const int mine = (nst + 1) / 2;  // stages of a half: ks, ks + 2, ...
 
-  using Scale = std::conditional_t<ODD, uint8_t, uint16_t>;
-  struct Stage { uint4 w[2]; Scale s[ODD ? 2 : 1]; };
+  struct Stage { uint4 w[2]; uint16_t s; };  // s: a pair of the next unit's scales
   struct Unit { int e, rt, cb; };
   auto decode = [&](int u) {
     Unit r;
@@ -725,29 +731,38 @@ __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
     r.cb = local - r.rt * NCB;
     return r;
   };
-  // Without branches, so that the compiler's waits leave the other stage in flight: chunks past
-  // the row repeat its last ones, against zeros in LDS; columns past N repeat the last block's
-  // (nothing is stored of them); and behind the last unit one piece is loaded again.
-  auto load = [&](Stage& g, const Unit& u, int i, bool on) {
+  // The 64 weight rows' scales of a unit, in the order of their addresses (gate_up of separate
+  // weights: 32 gate rows, then 32 up rows): bytes o .. of them, o at most n from the end.
+  auto scales = [&](const Unit& u, int o, int n) {
+    if (MODE == kGateUp && ACT == kSwiGLU) {
+      const int64_t row = u.e * p.e_rows + u.cb * 32;
+      o = min(o, 64 * KB - n);
+      return o < 32 * KB ? p.sa + row * KB + o : p.sb + row * KB + (o - 32 * KB);
+    }
+    const int64_t row = u.e * p.e_rows + u.cb * 64;
+    return p.sa + row * KB + min(o, (MODE == kGateUp ? 64 : min(64, N - u.cb * 64)) * KB - n);
+  };
+  const int srow = MODE == kDown ? nb * 16 + ml : ACT == kSwiGLU ? (nb & 1) * 16 + ml + (nb >= 2 ? 32 : 0)
+                                                                : 2 * ((nb & 1) * 16 + ml) + (nb >= 2 ? 1 : 0);
+  // Stage i of unit u, and the thread's pair of the scales of unit `then` behind it. Without
+  // branches, so that the compiler's waits leave the other stage in flight: chunks past the row
+  // repeat its last ones, against zeros in LDS; columns past N repeat the last block's (nothing
+  // is stored of them); and behind the last unit one piece is loaded again.
+  auto load = [&](Stage& g, const Unit& u, const Unit& then, int i, bool on) {
     const int col = MODE == kGateUp ? u.cb * 32 + (nb & 1) * 16 : min(u.cb * 64 + nb * 16, N - 16);
     const bool up = MODE == kGateUp && nb >= 2;
-    const int64_t row = u.e * p.e_rows + (int64_t)col * p.r_rows;
-    const uint8_t* wq = (up ? p.qb : p.qa) + row * kbytes;
-    const uint8_t* ws = (up ? p.sb : p.sa) + row * p.w_ld;
-    const uint32_t lq = on ? (uint32_t)(ml * p.r_rows) * (uint32_t)kbytes : 0u, ls = on ? (uint32_t)(ml * p.r_rows * p.w_ld) : 0u;
+    const uint8_t* wq = (up ? p.qb : p.qa) + (u.e * p.e_rows + (int64_t)col * p.r_rows) * kbytes;
+    const uint32_t lq = on ? (uint32_t)(ml * p.r_rows) * (uint32_t)kbytes : 0u;
     const int c = on ? 8 * (ks + 2 * i) + 2 * g4 : 0;  // this lane's chunks of 32 k: c, c + 1
     if constexpr (ODD) {
-      const uint32_t c0 = min(c, KB - 1), c1 = min(c + 1, KB - 1);
-      g.w[0] = *(const uint4*)(wq + (lq + c0 * 16));
-      g.w[1] = *(const uint4*)(wq + (lq + c1 * 16));
-      g.s[0] = ws[ls + c0];
-      g.s[1] = ws[ls + c1];
+      g.w[0] = *(const uint4*)(wq + (lq + (uint32_t)min(c, KB - 1) * 16));
+      g.w[1] = *(const uint4*)(wq + (lq + (uint32_t)min(c + 1, KB - 1) * 16));
     } else {
-      const uint32_t c0 = min(c, KB - 2);
-      g.w[0] = *(const uint4*)(wq + (lq + c0 * 16));
-      g.w[1] = *(const uint4*)(wq + (lq + c0 * 16 + 16));
-      g.s[0] = *(const uint16_t*)(ws + (ls + c0));
+      const uint32_t at = lq + (uint32_t)min(c, KB - 2) * 16;
+      g.w[0] = *(const uint4*)(wq + at);
+      g.w[1] = *(const uint4*)(wq + (at + 16));
     }
+    g.s = *(const uint16_t*)scales(then, 2 * (i * 512 + tid), 2);
   };
   struct Rows { Eight<uint16_t> v[4]; };
   auto load_rows = [&](Rows& x, int row0, int rows, int c0) {
@@ -794,7 +809,7 @@ __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
   };
 
   Stage ga, gb;
-  Unit u{};
+  Unit u{}, un{};
   Rows x;
   auto unit_rows = [&](const Unit& w, int& rows) {
     const int row0 = s_seg[w.e] + w.rt * kRows;
@@ -808,7 +823,12 @@ __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
       const int row0 = unit_rows(u, rows);
       load_rows(x, row0, rows, tid);
     }
-    load(ga, u, 0, true);
+    un = u0 + 1 < u1 ? decode(u0 + 1) : u;
+    uint8_t* own = sW + (u0 & 1) * 64 * KB;
+    const uint4 first = *(const uint4*)scales(u, tid * 16, 16);
+    load(ga, u, un, 0, true);
+    *(uint4*)(own + min(tid * 16, 64 * KB - 16)) = first;
+    for (int o = (tid + 512) * 16; o < 64 * KB; o += 512 * 16) *(uint4*)(own + o) = *(const uint4*)scales(u, o, 16);
   }
   int at = 0, t = u0, row0 = 0, rows = 0;
   f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
@@ -816,11 +836,14 @@ __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
   // where that one is of other rows, or there is none
   auto step = [&](Stage& cur, Stage& nxt) __attribute__((always_inline)) {
     const bool last = at + 1 == mine;
-    const Unit un = last && t + 1 < u1 ? decode(t + 1) : u;
-    load(nxt, un, last ? 0 : at + 1, !last || t + 1 < u1);
+    const Unit to = last ? un : u, then = last && t + 2 < u1 ? decode(t + 2) : un;
+    load(nxt, to, then, last ? 0 : at + 1, !last || t + 1 < u1);
     const int st = ks + 2 * at;
+    *(uint16_t*)(sW + ((t + 1) & 1) * 64 * KB + min(2 * (at * 512 + tid), 64 * KB - 2)) = cur.s;
     if (st < nst) {
-      const uint32_t sw = ODD ? cur.s[0] | (cur.s[ODD] << 8) : cur.s[0];
+      const uint8_t* ws = sW + (t & 1) * 64 * KB + srow * KB;
+      const int c = 8 * st + 2 * g4;
+      const uint32_t sw = ODD ? ws[min(c, KB - 1)] | (ws[min(c + 1, KB - 1)] << 8) : *(const uint16_t*)(ws + min(c, KB - 2));
       const uint32_t sp = *(const uint16_t*)(sc + ml * sld + st * 8 + 2 * g4);
       const uint4 a0 = *(const uint4*)(sP + ml * stride + st * 128 + g4 * 32);
       const uint4 a1 = *(const uint4*)(sP + ml * stride + st * 128 + g4 * 32 + 16);
@@ -883,8 +906,9 @@ __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
       }
     }
     acc = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    const bool same = un.e == u.e && un.rt == u.rt;
-    u = un;
+    const bool same = to.e == u.e && to.rt == u.rt;
+    u = to;
+    un = then;
     return ++t < u1 && same;
   };
   while (t < u1) {
@@ -921,7 +945,7 @@ static int cu_count() {
   return g_cus[dev];
 }
 
-constexpr int kLdsMost = 144 * 1024;  // dynamic LDS of the narrow kernel (160 KB less its static part)
+constexpr int kLdsMost = 156 * 1024;  // dynamic LDS of the narrow kernel
 
 template <int MODE, int ACT, bool KEEP>
 static void launch_wide(const Params& p, hipStream_t stream) {
@@ -942,24 +966,27 @@ static void launch_narrow(const Params& p, hipStream_t stream) {
   int64_t g = (p.R / kRows + (p.R < p.E ? p.R : p.E)) * ncb;
   const int64_t most = (int64_t)cu_count() * 2;
   if (g > most) g = most;
+  const int64_t lds = narrow_lds(p.K, p.E);
   auto launch = [&](auto kernel) {
-    if (narrow_lds(p.K) > 64 * 1024)
+    if (lds > 64 * 1024)
       (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsMost);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)g), dim3(512), (unsigned)narrow_lds(p.K), stream, p);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)g), dim3(512), (unsigned)lds, stream, p);
   };
   if (p.K / kBlock % 2) launch(narrow_kernel<MODE, ACT, true>);
   else launch(narrow_kernel<MODE, ACT, false>);
 }
 
-// The narrow kernel takes up to eight rows per expert that can have one, and small work, where the
+// The narrow kernel takes up to twelve rows per expert that can have one, and small work, where the
 // wide kernel's tiles leave most of the chip idle, where its rows fit into LDS (us, narrow / wide
-// with its quantization; rows per expert): 256 experts of 2304 / 1024 one token 17 / 35, 4 rows 205 /
-// 221, 8 rows 229 / 228, 16 rows 295 / 239; 32 of gpt-oss's 2880 / 2880 8 rows 123 / 152, 16 rows 156 /
-// 155; 32 of 7168 / 2048 16 rows 238 / 198. Small: 8 experts of 2048 / 1408 16 rows 22 / 32, 32 rows 34 /
-// 34; 4 of 2880 / 2880 32 rows 33 / 67; 16 of 320 / 704 19 rows 17 / 25; one of 512 / 512 128 rows 13 / 23.
+// with its quantization; rows per expert): 256 experts of 2304 / 1024 one token 18 / 31, 4 rows 189 /
+// 220, 8 rows 208 / 227, 16 rows 274 / 239; 32 of gpt-oss's 2880 / 2880 8 rows 102 / 152, 16 rows 130 /
+// 156, 24 rows 155 / 158; 32 of 7168 / 2048 8 rows 161 / 190, 12 rows 192 / 194, 16 rows 215 / 197. Small:
+// 8 experts of 2048 / 1408 16 rows 22 / 32, 32 rows 34 / 34; 4 of 2880 / 2880 32 rows 33 / 67; 16 of 320 /
+// 704 19 rows 17 / 24; one of 512 / 512 128 rows 12 / 22.
 static bool takes_narrow(int64_t R, int64_t E, int D, int H) {
   const int64_t cols = 2 * (int64_t)H > D ? 2 * (int64_t)H : D;
-  return (R <= 8 * (R < E ? R : E) || R * ((cols + 255) / 256) <= 1536) && narrow_lds(D) <= kLdsMost && narrow_lds(H) <= kLdsMost;
+  return (R <= 12 * (R < E ? R : E) || R * ((cols + 255) / 256) <= 1536) && narrow_lds(D, E) <= kLdsMost &&
+         narrow_lds(H, E) <= kLdsMost;
 }
 
 static int check_shape(int64_t R, int E, int D, int H) {
