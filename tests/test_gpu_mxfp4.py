@@ -143,6 +143,8 @@ SERVE = [
     ("many rows, odd dims", [1000, 130, 0, 300], 3, 416, 352),
     ("one expert", [700], 0, 96, 96),
     ("few rows, a long contraction", [3, 0, 1], 1, 7168, 64),
+    ("two blocks of rows", [20, 33, 16, 0, 17, 32], 3, 2880, 96),
+    ("17 rows, a long contraction", [17, 2, 0], 1, 4640, 4640),
     ("few rows, rows past the LDS", [2, 1], 0, 16384, 32),
     ("many experts", [0, 2, 0, 0, 17, 1] * 170 + [3, 0, 0, 9], 2, 64, 32),
     ("many experts, many rows", [0, 40, 0, 0, 300, 1] * 20, 2, 64, 96),

@@ -11,6 +11,7 @@
 //
 // v_mfma_scale_f32_16x16x128_f8f6f4 on e2m1 operands: lane (row, q), q = lane / 16, holds 32
 // consecutive k of its row, which is one scaling block, and passes that block's scale.
+#include <algorithm>
 #include <type_traits>
 
 #include "mx.h"
@@ -677,7 +678,7 @@ __global__ __launch_bounds__(512, 2) void wide_kernel(Params p) {
 
 // Few rows per expert: the weights are read once and decide the time, so every byte goes
 // straight from memory into the MFMAs' registers. A unit is 64 weight rows (gate_up: 32 gate and
-// 32 up rows, one scaling block of h; down: 64 columns) by up to 16 rows of one expert; eight
+// 32 up rows, one scaling block of h; down: 64 columns) by up to 16 TM rows of one expert; eight
 // waves take four blocks of 16 weight rows by the even and the odd 256-k stages. A wave keeps two
 // stages in registers, in turn, one's loads in flight while the other multiplies, through to the
 // following unit. A workgroup's units are consecutive, so the rows, which gate_up quantizes from
@@ -687,7 +688,7 @@ __global__ __launch_bounds__(512, 2) void wide_kernel(Params p) {
 //
 // What bounds it: the weights' bytes. One row on each of 57 experts of 7168 / 2048 takes 236 us, 5.6
 // TB/s; four rows each on 256 of 2304 / 1024 189 us, 5.1 TB/s; eight each on 32 of gpt-oss's 2880 / 2880
-// 102 us, 4.2 TB/s (rows of 1440 bytes: a stage of 128 straddles two cache lines). One token's 8
+// 101 us, 4.2 TB/s (rows of 1440 bytes: a stage of 128 straddles two cache lines). One token's 8
 // experts of 256 take 17 us, of which the 30 MB are 6: two launches that each wait for the counts,
 // then for the weights.
 // Measured otherwise: scales loaded where they are multiplied, two bytes a lane from 16 rows, 248, 203
@@ -695,22 +696,22 @@ __global__ __launch_bounds__(512, 2) void wide_kernel(Params p) {
 // a register copy of the stage in flight (the loop not in pairs) waits for its loads: 220 and 139
 // us. More in flight was slower: groups of two stages 206 and 125 us, three or four single ones in
 // turn 199 to 219 and 126 to 134; loads past the caches 223 and 160.
-constexpr int kRows = 16;
 __host__ __device__ constexpr int narrow_stride(int K) { return (K + 255) / 256 * 128 + 16; }  // rows 16 bytes apart mod 128
-__host__ __device__ constexpr int64_t narrow_lds(int K, int E) {  // rows and their scales, sums, the weights' scales, segments
-  return (int64_t)kRows * (narrow_stride(K) + (K + 255) / 256 * 8) + 2 * 8 * 64 * 16 + 2 * 64 * (K / kBlock) +
+__host__ __device__ constexpr int64_t narrow_lds(int K, int E, int TM) {  // rows and their scales, sums, the weights' scales, segments
+  return 16 * (int64_t)TM * (narrow_stride(K) + (K + 255) / 256 * 8) + 2 * 8 * 64 * 16 + 2 * 64 * (K / kBlock) +
          2 * (E + 1) * (int)sizeof(int);
 }
 
-template <int MODE, int ACT, bool ODD>
+template <int MODE, int ACT, bool ODD, int TM>
 __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
   extern __shared__ __attribute__((aligned(16))) uint8_t s_dyn[];
+  constexpr int kRows = 16 * TM;
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int nb = wv & 3, ks = wv >> 2, ml = lane & 15, g4 = lane >> 4;
   const int E = p.E, K = p.K, N = p.N, KB = K / kBlock, kbytes = K / 2, nst = (K + 255) / 256;
   const int stride = narrow_stride(K), sld = nst * 8;
   uint8_t* sP = s_dyn;
-  f32x4_t* sums = (f32x4_t*)(s_dyn + kRows * (stride + sld));  // two units' [2 ks][4 nb][64]
+  f32x4_t* sums = (f32x4_t*)(s_dyn + kRows * (stride + sld));  // [2 units or row blocks][2 ks][4 nb][64]
   uint8_t* sc = s_dyn + kRows * stride;
   uint8_t* sW = (uint8_t*)(sums + 2 * 8 * 64);  // two units' weight scales, 64 rows of KB
   int* s_seg = (int*)(sW + 2 * 64 * KB);
@@ -831,7 +832,7 @@ __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
     for (int o = (tid + 512) * 16; o < 64 * KB; o += 512 * 16) *(uint4*)(own + o) = *(const uint4*)scales(u, o, 16);
   }
   int at = 0, t = u0, row0 = 0, rows = 0;
-  f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+  f32x4_t acc[TM] = {};
   // unit t's stage `at` from `cur`, with the next one's loads on their way into `nxt`; false
   // where that one is of other rows, or there is none
   auto step = [&](Stage& cur, Stage& nxt) __attribute__((always_inline)) {
@@ -844,16 +845,21 @@ __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
       const uint8_t* ws = sW + (t & 1) * 64 * KB + srow * KB;
       const int c = 8 * st + 2 * g4;
       const uint32_t sw = ODD ? ws[min(c, KB - 1)] | (ws[min(c + 1, KB - 1)] << 8) : *(const uint16_t*)(ws + min(c, KB - 2));
-      const uint32_t sp = *(const uint16_t*)(sc + ml * sld + st * 8 + 2 * g4);
-      const uint4 a0 = *(const uint4*)(sP + ml * stride + st * 128 + g4 * 32);
-      const uint4 a1 = *(const uint4*)(sP + ml * stride + st * 128 + g4 * 32 + 16);
       const uint4 b0 = cur.w[0], b1 = cur.w[1];
-      acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-          v8i_t{(int)b0.x, (int)b0.y, (int)b0.z, (int)b0.w, 0, 0, 0, 0},
-          v8i_t{(int)a0.x, (int)a0.y, (int)a0.z, (int)a0.w, 0, 0, 0, 0}, acc, 4, 4, 0, (int)sw, 0, (int)sp);
-      acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-          v8i_t{(int)b1.x, (int)b1.y, (int)b1.z, (int)b1.w, 0, 0, 0, 0},
-          v8i_t{(int)a1.x, (int)a1.y, (int)a1.z, (int)a1.w, 0, 0, 0, 0}, acc, 4, 4, 1, (int)sw, 1, (int)sp);
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        if (i > 0 && rows <= 16 * i) continue;
+        const int r = 16 * i + ml;
+        const uint32_t sp = *(const uint16_t*)(sc + r * sld + st * 8 + 2 * g4);
+        const uint4 a0 = *(const uint4*)(sP + r * stride + st * 128 + g4 * 32);
+        const uint4 a1 = *(const uint4*)(sP + r * stride + st * 128 + g4 * 32 + 16);
+        acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+            v8i_t{(int)b0.x, (int)b0.y, (int)b0.z, (int)b0.w, 0, 0, 0, 0},
+            v8i_t{(int)a0.x, (int)a0.y, (int)a0.z, (int)a0.w, 0, 0, 0, 0}, acc[i], 4, 4, 0, (int)sw, 0, (int)sp);
+        acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+            v8i_t{(int)b1.x, (int)b1.y, (int)b1.z, (int)b1.w, 0, 0, 0, 0},
+            v8i_t{(int)a1.x, (int)a1.y, (int)a1.z, (int)a1.w, 0, 0, 0, 0}, acc[i], 4, 4, 1, (int)sw, 1, (int)sp);
+      }
     }
     if (!last) {
       ++at;
@@ -862,23 +868,26 @@ __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
     at = 0;
     // one barrier a unit: the waves that read these sums come to the next one before anyone
     // writes over them; they take turns, so that none is behind the others for good
-    f32x4_t* red = sums + (t & 1) * 8 * 64;
-    red[(ks * 4 + nb) * 64 + lane] = acc;
+    // (with two blocks of rows in the two buffers: with a barrier for that)
+    f32x4_t* red = sums + (TM == 1 ? t & 1 : 0) * 8 * 64;
+    if (TM > 1) __syncthreads();
+#pragma unroll
+    for (int i = 0; i < TM; ++i) red[((i * 2 + ks) * 4 + nb) * 64 + lane] = acc[i];
     __syncthreads();
-    const int turn = (wv + t) & 7;
+    const int turn = (wv + t) & 7, blk = MODE == kGateUp ? turn : turn >> 1;  // this wave's block of rows
     auto sum = [&](int b, float (&v)[4]) {
-      const f32x4_t a = red[b * 64 + lane], c = red[(4 + b) * 64 + lane];
+      const f32x4_t a = red[(blk * 8 + b) * 64 + lane], c = red[(blk * 8 + 4 + b) * 64 + lane];
 #pragma unroll
       for (int q = 0; q < 4; ++q) v[q] = a[q] + c[q];
     };
     if (MODE == kGateUp) {
-      if (turn == 0) {
+      if (blk < TM && 16 * blk < rows) {
         float ha[4], hb[4], ua[4], ub[4];
         sum(0, ha);
         sum(1, hb);
         sum(2, ua);
         sum(3, ub);
-        const int hc = u.cb * 32, r = ml;
+        const int hc = u.cb * 32, r = 16 * blk + ml;
         uint4 bias_a{}, bias_b{};
         if constexpr (ACT == kOssGLU) {
           const uint16_t* bp = p.bias + (int64_t)u.e * 2 * N + 2 * (hc + 4 * g4);
@@ -887,8 +896,8 @@ __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
         }
         store_hidden<ACT, false>(p, row0 + r, hc, lane, r < rows, ha, hb, ua, ub, bias_a, bias_b);
       }
-    } else if (turn < 2) {
-      const int pr = turn, n0 = u.cb * 64 + pr * 32, r = ml;
+    } else if (blk < TM && 16 * blk < rows) {
+      const int pr = turn & 1, n0 = u.cb * 64 + pr * 32, r = 16 * blk + ml;
       if (n0 < N) {
         float lo[4], hi[4];
         sum(2 * pr, lo);
@@ -905,7 +914,8 @@ __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
         if (r < rows) *(uint4*)(p.y + (int64_t)(row0 + r) * N + n0 + 8 * g4) = v;
       }
     }
-    acc = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < TM; ++i) acc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     const bool same = to.e == u.e && to.rt == u.rt;
     u = to;
     un = then;
@@ -960,33 +970,45 @@ static void launch_wide(const Params& p, hipStream_t stream) {
   else
     hipLaunchKernelGGL((wide_kernel<MODE, ACT, KEEP, true>), dim3((unsigned)g), dim3(512), lds, stream, p);
 }
+// Blocks of 16 rows in a unit of the narrow kernel on a contraction of K: two where two workgroups
+// share a CU's LDS still, else one, where that fits; 0: neither does. With up to eight rows per
+// expert one and two take the same time (189 / 189 us at 4 of 256 experts of 2304 / 1024, 210 / 200 at 8);
+// with more, one reads the weights more often (16 rows 275 / 219, gpt-oss 129 / 111), and two without
+// the second workgroup lose what they win (192 us instead of 161 at 8 rows of 32 of 7168 / 2048).
+static int narrow_blocks(int K, int64_t E) {
+  return narrow_lds(K, (int)E, 2) <= 80 * 1024 ? 2 : narrow_lds(K, (int)E, 1) <= kLdsMost ? 1 : 0;
+}
+
 template <int MODE, int ACT>
 static void launch_narrow(const Params& p, hipStream_t stream) {
+  const int tm = narrow_blocks(p.K, p.E);
   const int64_t ncb = MODE == kGateUp ? p.N / 32 : (p.N + 63) / 64;
-  int64_t g = (p.R / kRows + (p.R < p.E ? p.R : p.E)) * ncb;
+  int64_t g = (p.R / (16 * tm) + (p.R < p.E ? p.R : p.E)) * ncb;
   const int64_t most = (int64_t)cu_count() * 2;
   if (g > most) g = most;
-  const int64_t lds = narrow_lds(p.K, p.E);
+  const int64_t lds = narrow_lds(p.K, p.E, tm);
   auto launch = [&](auto kernel) {
     if (lds > 64 * 1024)
       (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsMost);
     hipLaunchKernelGGL(kernel, dim3((unsigned)g), dim3(512), (unsigned)lds, stream, p);
   };
-  if (p.K / kBlock % 2) launch(narrow_kernel<MODE, ACT, true>);
-  else launch(narrow_kernel<MODE, ACT, false>);
+  const bool odd = p.K / kBlock % 2;
+  if (tm == 1) odd ? launch(narrow_kernel<MODE, ACT, true, 1>) : launch(narrow_kernel<MODE, ACT, false, 1>);
+  else odd ? launch(narrow_kernel<MODE, ACT, true, 2>) : launch(narrow_kernel<MODE, ACT, false, 2>);
 }
 
-// The narrow kernel takes up to twelve rows per expert that can have one, and small work, where the
-// wide kernel's tiles leave most of the chip idle, where its rows fit into LDS (us, narrow / wide
-// with its quantization; rows per expert): 256 experts of 2304 / 1024 one token 18 / 31, 4 rows 189 /
-// 220, 8 rows 208 / 227, 16 rows 274 / 239; 32 of gpt-oss's 2880 / 2880 8 rows 102 / 152, 16 rows 130 /
-// 156, 24 rows 155 / 158; 32 of 7168 / 2048 8 rows 161 / 190, 12 rows 192 / 194, 16 rows 215 / 197. Small:
-// 8 experts of 2048 / 1408 16 rows 22 / 32, 32 rows 34 / 34; 4 of 2880 / 2880 32 rows 33 / 67; 16 of 320 /
-// 704 19 rows 17 / 24; one of 512 / 512 128 rows 12 / 22.
+// The narrow kernel takes up to 20 rows per expert that can have one (12 with units of one block),
+// and small work, where the wide kernel's tiles leave most of the chip idle, where its rows fit
+// into LDS (us, narrow / wide with its quantization; rows per expert): 256 experts of 2304 / 1024 one
+// token 18 / 30, 4 rows 189 / 220, 16 rows 219 / 238, 24 rows 247 / 247, 31 rows 292 / 268; 32 of
+// gpt-oss's 2880 / 2880 8 rows 101 / 152, 16 rows 111 / 156, 24 rows 132 / 159, 50 rows 176 / 168; 32 of 7168 /
+// 2048 8 rows 161 / 191, 12 rows 192 / 194, 16 rows 218 / 198; 16 of 2304 / 1024 16 rows 29 / 32, 24 rows 39 /
+// 33. Small: 8 experts of 2048 / 1408 16 rows 22 / 32; 16 of 320 / 704 19 rows 16 / 24; one of 512 / 512 128
+// rows 13 / 22.
 static bool takes_narrow(int64_t R, int64_t E, int D, int H) {
+  const int tm = std::min(narrow_blocks(D, E), narrow_blocks(H, E));
   const int64_t cols = 2 * (int64_t)H > D ? 2 * (int64_t)H : D;
-  return (R <= 12 * (R < E ? R : E) || R * ((cols + 255) / 256) <= 1536) && narrow_lds(D, E) <= kLdsMost &&
-         narrow_lds(H, E) <= kLdsMost;
+  return tm && (R <= (tm == 2 ? 20 : 12) * (R < E ? R : E) || R * ((cols + 255) / 256) <= 1536);
 }
 
 static int check_shape(int64_t R, int E, int D, int H) {
@@ -1088,7 +1110,8 @@ static int experts_fwd(const uint16_t* x, const uint8_t* qw1, const uint8_t* sw1
   uint8_t* qh = sx + row_scales(R, D);
   uint8_t* sh = qh + row_bytes(R, H);
   uint8_t* pads = sh + row_scales(R, H);
-  const bool oss = ACT == kOssGLU, narrow = takes_narrow(R, E, D, H);
+  const bool oss = ACT == kOssGLU;
+  const bool narrow = takes_narrow(R, E, D, H);
   // odd scale rows, padded for the wide kernel: the copy, and its row stride
   auto pad_scales = [&](const uint8_t* src, int64_t rows, int cols, int& ld) {
     ld = cols / kBlock;
