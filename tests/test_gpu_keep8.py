@@ -67,36 +67,44 @@ def test_forward_alone(dev):
     for counts, d, h in (([5, 0, 300, 40], 320, 192), ([700, 513], 512, 576)):
         c, x, dy, w1, w2, w3 = _inputs(counts, 3, d, h, 3, dev)
         args = [t.to(dev) for t in (x, w1, w2, w3, c)]
-        y, *kept = ops.grouped_swiglu_ckpt8(*args, False)
-        assert torch.equal(y, ops.grouped_swiglu_ckpt8(*args)[0]) and not any(t.numel() for t in kept)
+        y, kept = ops.grouped_swiglu_ckpt8(*args, False)
+        assert torch.equal(y, ops.grouped_swiglu_ckpt8(*args)[0]) and kept.numel() == 0
     y = ops.grouped_swiglu_ckpt8(args[0].requires_grad_(True), *args[1:], False)[0]
     with pytest.raises(RuntimeError, match="nothing was kept"):
         y.float().sum().backward()
 
 
 def test_backwards_of_given_tensors(dev):
-    """The backward operators called directly: kept tensors in any strides, and refusals."""
+    """The backward operators called directly: tensors in any strides, and refusals."""
     banner("kept in 8 bits, backward operators")
     from torchtitan_amd import ops
 
     c, x, dy, w1, w2, w3 = (t.to(dev) for t in _inputs([5, 0, 70], 0, 128, 192, 6, dev))
-    strided = lambda t: t.t().contiguous().t() if t.dim() == 2 else t.transpose(1, 2).contiguous().transpose(1, 2)  # noqa: E731
-    eight = ops.grouped_swiglu_ckpt8(x, w1, w2, w3, c)[1:]
-    four = ops.grouped_swiglu_mxfp4_train(x, w1, w2, w3, c)[1:]
-    for bwd, args, kept in ((ops.grouped_swiglu_ckpt8_backward, (dy, w1, w2, w3, c), eight),
-                            (ops.grouped_swiglu_mxfp4_train_backward, (dy, c), four)):
-        want = bwd(*args, *kept)
-        for a, b in zip(want, bwd(*map(lambda t: strided(t) if t.dim() > 1 else t, args), *map(strided, kept))):
+
+    def strided(t):
+        wide = t.new_zeros(*t.shape[:-1], 2 * t.shape[-1])
+        wide[..., 1::2] = t
+        return wide[..., 1::2]
+
+    eight = ops.grouped_swiglu_ckpt8(x, w1, w2, w3, c)[1]
+    four = ops.grouped_swiglu_mxfp4_train(x, w1, w2, w3, c)[1]
+    for bwd, args, kept, rest in ((ops.grouped_swiglu_ckpt8_backward, (dy, w1, w2, w3, c), eight, ()),
+                                  (ops.grouped_swiglu_mxfp4_train_backward, (dy, c), four, (192,))):
+        want = bwd(*args, kept, *rest)
+        for a, b in zip(want, bwd(*map(strided, args), strided(kept), *rest)):
             assert torch.equal(a, b)
-        for i in range(len(kept)):
-            with pytest.raises(ValueError):
-                bwd(*args, *kept[:i], kept[i][:-1], *kept[i + 1:])
-            with pytest.raises(TypeError):
-                bwd(*args, *kept[:i], kept[i].float(), *kept[i + 1:])
-        with pytest.raises((TypeError, ValueError)):
-            bwd(dy.float(), *args[1:], *kept)
+        for bad in (kept[:-1], kept.view(2, -1), kept[:0], kept.cpu()):
+            with pytest.raises((ValueError, RuntimeError)):
+                bwd(*args, bad, *rest)
+        with pytest.raises(TypeError):
+            bwd(*args, kept.view(torch.int8), *rest)
+        with pytest.raises(TypeError):
+            bwd(dy.float(), *args[1:], kept, *rest)
         with pytest.raises(ValueError):
-            bwd(dy[:, :64], *args[1:], *kept)
+            bwd(dy[:, :64], *args[1:], kept, *rest)
+    for h in (128, 96, 256):
+        with pytest.raises(ValueError):
+            ops.grouped_swiglu_mxfp4_train_backward(dy, c, four, h)
 
 
 def test_kept_values(dev):
@@ -107,7 +115,10 @@ def test_kept_values(dev):
     c, x, dy, w1, w2, w3 = _inputs([9, 0, 70], 0, 128, 96 * 2, 4, dev)
     x[3, 40], x[20, 5] = float("inf"), float("nan")
     x[5, :32], x[6, 32:64] = 0.0, 2.0 ** -130
-    _y, x8, xs, g8, gs, u8, us = (t.cpu() for t in ops.grouped_swiglu_ckpt8(*(t.to(dev) for t in (x, w1, w2, w3, c))))
+    kept = ops.grouped_swiglu_ckpt8(*(t.to(dev) for t in (x, w1, w2, w3, c)))[1].cpu()
+    offsets, size = ops._ckpt8_layout(79, 128, 192)
+    assert kept.numel() == size
+    x8, xs, g8, gs, u8, us = (kept[at:at + 79 * n].view(79, n) for at, n in zip(offsets, (128, 4, 192, 6, 192, 6)))
 
     def value(q, s):
         sc = torch.where(s == 255, torch.nan, torch.exp2(s.double() - 127))

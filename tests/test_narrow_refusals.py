@@ -104,19 +104,23 @@ def test_packed_arguments():
         ops._check_packed("op", "w", q, s, (3, 4, 64))
 
 
-def test_kept_arguments(monkeypatch):
+def test_kept_arguments():
     from torchtitan_amd import ops
 
-    monkeypatch.setattr(ops, "require_gpu", lambda *t: None)
-    dy, q, s = torch.zeros(4, 64), torch.zeros(4, 64, dtype=torch.uint8), torch.zeros(4, 2, dtype=torch.uint8)
-    got = ops._kept("op", dy, g=(q.t().contiguous().t(), s, (4,), 64, 2))
-    assert got[0].is_contiguous() and torch.equal(got[0], q) and torch.equal(got[1], s)
-    for a, b in ((q.view(torch.int8), s), (q, s.float())):
-        with pytest.raises(TypeError, match="uint8 g"):
-            ops._kept("op", dy, g=(a, b, (4,), 64, 2))
-    for a, b in ((q[:3], s), (q, s[:, :1]), (q[:, :32], s), (q, s[:3]), (q[0], s)):
-        with pytest.raises(ValueError, match="expects g"):
-            ops._kept("op", dy, g=(a, b, (4,), 64, 2))
+    assert ops._carve((1, 256, 257, 0, 5)) == ((0, 256, 512, 1024, 1024), 1280)
+    offsets, size = ops._ckpt8_layout(3, 64, 128)
+    assert offsets == (0, 256, 512, 1024, 1280, 1792) and size == 2048
+    offsets, size = ops._mxfp4_train_layout(3, 2, 64, 128)  # w of 16384 elements, rows of 256 columns, g and u of 128
+    assert offsets == (0, 8192, 8704, 16896, 17408, 25600, 26112, 26624, 26880, 27392, 27648, 28160, 28416, 28928)
+    assert size == 29184
+    dy, kept = torch.zeros(3, 64), torch.zeros(2048, dtype=torch.uint8)
+    wide = torch.zeros(4096, dtype=torch.uint8)[::2]
+    assert ops._check_kept("op", kept, 2048, dy) is kept and ops._check_kept("op", wide, 2048, dy).is_contiguous()
+    with pytest.raises(TypeError, match="uint8"):
+        ops._check_kept("op", kept.view(torch.int8), 2048, dy)
+    for bad in (kept[1:], kept.view(2, -1)):
+        with pytest.raises(ValueError, match="2048 bytes"):
+            ops._check_kept("op", bad, 2048, dy)
 
 
 def test_expert_arguments(monkeypatch):

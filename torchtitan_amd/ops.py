@@ -1203,127 +1203,145 @@ def _zero_rows_past(counts: Tensor, r: int, e: int, t: Tensor, s: int) -> None:
     call("moe_zero_rows_past_f32", ptr(counts), r, e, ptr(t), t.shape[1] // 2, None, 0, None, 0, None, 0, s)
 
 
+def _carve(sizes) -> tuple[tuple[int, ...], int]:
+    """Offsets of regions of these many bytes in one allocation, each on a 256-byte boundary (the
+    kernels' wide loads; whole cache lines), and its size. One kept tensor and one workspace in
+    place of 6 to 14 take an eighth to a quarter off a small step's host time (145 -> 125 us of
+    grouped_swiglu_ckpt8's forward and backward, 200 -> 147 of grouped_swiglu_mxfp4_train's)."""
+    offsets, at = [], 0
+    for n in sizes:
+        offsets.append(at)
+        at += (n + 255) // 256 * 256
+    return tuple(offsets), at
+
+
+@functools.lru_cache(maxsize=256)
+def _ckpt8_layout(r: int, d: int, h: int) -> tuple[tuple[int, ...], int]:
+    """grouped_swiglu_ckpt8's kept tensor: x [r, d], g and u [r, h] in MXFP8, each with its scales."""
+    return _carve(n for c in (d, h, h) for n in (r * c, r * c // MX_BLOCK))
+
+
+def _at(t: Tensor, offsets) -> list[int]:
+    base = t.data_ptr()
+    return [base + o for o in offsets]
+
+
+def _check_kept(op: str, kept: Tensor, size: int, like: Tensor) -> Tensor:
+    if kept.dtype is not torch.uint8:
+        raise TypeError(f"{op} expects the forward's kept uint8 tensor, got {kept.dtype}")
+    if kept.shape != (size,) or kept.device != like.device:
+        raise ValueError(f"{op} expects the forward's kept tensor of {size} bytes on {like.device}, got "
+                         f"{tuple(kept.shape)} on {kept.device}")
+    return _ready(kept)
+
+
 @torch.library.custom_op("moe_mi355x_mx::grouped_swiglu_ckpt8", mutates_args=())
 def grouped_swiglu_ckpt8(
     x: Tensor, w1: Tensor, w2: Tensor, w3: Tensor, num_tokens_per_expert: Tensor, for_backward: bool = True
-) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor]:
+) -> tuple[Tensor, Tensor]:
     """bf16 grouped SwiGLU whose backward works from 8-bit activations. y [R, D] = h w2^T with
     h = bf16(silu(x w1^T) (x w3^T)) of fp32 sums (grouped_swiglu, which follows the reference's,
-    rounds four times on the way to h), zero on rows past sum(counts). Then what is kept: x
-    [R, D], g and u [R, H] in MXFP8 (e4m3, one e8m0 scale per 32 along the row), each followed
-    by its scales: (D + 2H) 33/32 bytes a row instead of 2D + 6H; empty without `for_backward`.
-    The gradients are those at the kept values: the activation's at g and u, dw1 and dw3 with x,
-    dw2 with h = silu(g) u. An infinity or NaN makes its block of 32 kept values NaN."""
+    rounds four times on the way to h), zero on rows past sum(counts). Then what is kept, as one
+    tensor of bytes: x [R, D], g and u [R, H] in MXFP8 (e4m3, one e8m0 scale per 32 along the
+    row), each followed by its scales: (D + 2H) 33/32 bytes a row instead of 2D + 6H; empty
+    without `for_backward`. The gradients are those at the kept values: the activation's at g and
+    u, dw1 and dw3 with x, dw2 with h = silu(g) u. An infinity or NaN makes its block of 32 kept
+    values NaN."""
     op = "grouped_swiglu_ckpt8"
     _check_experts(op, x, w1, w2, w3, num_tokens_per_expert, 64)
-    x, w1, w2, w3 = (_aligned(t.contiguous()) for t in (x, w1, w2, w3))
+    x, w1, w2, w3 = map(_ready, (x, w1, w2, w3))
     counts = num_tokens_per_expert.to(torch.int64).contiguous()
     r, d = x.shape
     e, h_dim, _ = w1.shape
-    x8, xs, g8, gs, up8, us = _ckpt8_kept(x, h_dim, for_backward)
+    offsets, size = _ckpt8_layout(r, d, h_dim)
+    kept = x.new_empty(size if for_backward else 0, dtype=torch.uint8)
+    x8, xs, g8, gs, up8, us = _at(kept, offsets) if for_backward else (None,) * 6
     h = x.new_empty(r, h_dim)
     y = x.new_empty(r, d)
     with _guard(x):
         s = stream_of(x)
         if for_backward:
-            call("moe_keep8_rows", ptr(x), r, d, ptr(x8), ptr(xs), s)
-        call("moe_grouped_gemm_gate_up_keep8", ptr(x), ptr(w1), ptr(w3), ptr(counts), r, e, d, h_dim,
-             *((ptr(g8), ptr(gs), ptr(up8), ptr(us)) if for_backward else (None,) * 4), ptr(h), s)
+            call("moe_keep8_rows", ptr(x), r, d, x8, xs, s)
+        call("moe_grouped_gemm_gate_up_keep8", ptr(x), ptr(w1), ptr(w3), ptr(counts), r, e, d, h_dim, g8, gs, up8, us,
+             ptr(h), s)
         call("moe_grouped_gemm_down", ptr(h), ptr(w2), ptr(counts), r, e, d, h_dim, ptr(y), s)
         _zero_rows_past(counts, r, e, y, s)
-    return y, x8, xs, g8, gs, up8, us
-
-
-def _ckpt8_kept(x: Tensor, h_dim: int, for_backward: bool) -> list[Tensor]:
-    r, d = x.shape if for_backward else (0, 0)
-    h_dim = h_dim if for_backward else 0
-    return [x.new_empty(r, n, dtype=torch.uint8)
-            for n in (d, d // MX_BLOCK, h_dim, h_dim // MX_BLOCK, h_dim, h_dim // MX_BLOCK)]
+    return y, kept
 
 
 @grouped_swiglu_ckpt8.register_fake
 def _(x, w1, w2, w3, num_tokens_per_expert, for_backward=True):
-    return (x.new_empty(x.shape), *_ckpt8_kept(x, w1.shape[1], for_backward))
+    size = _ckpt8_layout.__wrapped__(x.shape[0], x.shape[1], w1.shape[1])[1] if for_backward else 0
+    return x.new_empty(x.shape), x.new_empty(size, dtype=torch.uint8)
 
 
-def _narrow_backward(dy: Tensor, w1: Tensor, w2: Tensor, w3: Tensor, counts: Tensor, g8: Tensor, gs: Tensor, up8: Tensor,
-                     us: Tensor, rows, hidden: Tensor | None, need_dx: bool, need_dw13: bool,
+def _narrow_backward(dy: Tensor, e: int, h_dim: int, w1: int, w2: int, w3: int, counts: Tensor, g8: int, gs: int, up8: int,
+                     us: int, dgu: int, rows, h: int | None, hidden_kept: bool, need_dx: bool, need_dw13: bool,
                      need_dw2: bool) -> tuple[Tensor, Tensor, Tensor, Tensor]:
-    """dx, dw1, dw2, dw3 of experts with bf16 weight values and g, u kept in MXFP8; rows()
-    gives the forward's x in bf16, `hidden` its h (None: silu(g) u of the kept values).
-    What is not needed comes back empty."""
+    """dx, dw1, dw2, dw3 of experts with bf16 weight values and g, u kept in MXFP8, all given by
+    address: dgu [R, 2H] is workspace, h [R, H] the forward's (hidden_kept) or where silu(g) u of
+    the kept values goes; rows() gives the forward's x. What is not needed comes back empty."""
     r, d = dy.shape
-    e, h_dim, _ = w1.shape
     s = stream_of(dy)
-    dgu = dy.new_empty(r, 2 * h_dim)
-    h = dy.new_empty(r, h_dim) if hidden is None and need_dw2 else hidden
-    if need_dx or need_dw13 or hidden is None:
-        call("moe_grouped_gemm_bwd_dgu_keep8", ptr(dy), ptr(w2), ptr(g8), ptr(gs), ptr(up8), ptr(us), ptr(counts), r, e,
-             d, h_dim, ptr(dgu), ptr(h) if hidden is None else None, s)
+    if need_dx or need_dw13 or not hidden_kept:
+        call("moe_grouped_gemm_bwd_dgu_keep8", ptr(dy), w2, g8, gs, up8, us, ptr(counts), r, e, d, h_dim, dgu,
+             None if hidden_kept else h, s)
     dx = dy.new_empty(r, d) if need_dx else dy.new_empty(0)
     if need_dx:
-        call("moe_grouped_gemm_bwd_dx_once", ptr(dgu), ptr(w1), ptr(w3), ptr(counts), r, e, d, h_dim, ptr(dx), s)
+        call("moe_grouped_gemm_bwd_dx_once", dgu, w1, w3, ptr(counts), r, e, d, h_dim, ptr(dx), s)
         _zero_rows_past(counts, r, e, dx, s)
-    dw1, dw3 = (torch.empty_like(w1) if need_dw13 else dy.new_empty(0) for _ in range(2))
+    dw1, dw3 = (dy.new_empty((e, h_dim, d) if need_dw13 else 0) for _ in range(2))
     if need_dw13:
-        x = rows()
-        call("moe_grouped_gemm_bwd_dw13", ptr(dgu), ptr(x), ptr(counts), r, e, d, h_dim, ptr(dw1), ptr(dw3), s)
-    dw2 = torch.empty_like(w2) if need_dw2 else dy.new_empty(0)
+        call("moe_grouped_gemm_bwd_dw13", dgu, rows(), ptr(counts), r, e, d, h_dim, ptr(dw1), ptr(dw3), s)
+    dw2 = dy.new_empty((e, d, h_dim) if need_dw2 else 0)
     if need_dw2:
-        call("moe_grouped_gemm_bwd_dw2", ptr(dy), ptr(h), ptr(counts), r, e, d, h_dim, ptr(dw2), s)
+        call("moe_grouped_gemm_bwd_dw2", ptr(dy), h, ptr(counts), r, e, d, h_dim, ptr(dw2), s)
     return dx, dw1, dw2, dw3
 
 
-def _kept(op: str, like: Tensor, **matrices: tuple) -> list[Tensor]:
-    """Kept matrices given by name as (q, scale, leading sizes, bytes and scales of a row):
-    checked, contiguous and aligned, in that order."""
-    out = []
-    for name, (q, scale, lead, n, m) in matrices.items():
-        if q.dtype is not torch.uint8 or scale.dtype is not torch.uint8:
-            raise TypeError(f"{op} expects uint8 {name} and scales, got {q.dtype} and {scale.dtype}")
-        if q.shape != (*lead, n) or scale.shape != (*lead, m) or not q.device == scale.device == like.device:
-            raise ValueError(f"{op} expects {name} {[*lead, n]} with scales {[*lead, m]} on {like.device}, got "
-                             f"{tuple(q.shape)} on {q.device} with {tuple(scale.shape)} on {scale.device}")
-        out += [_ready(q), _ready(scale)]
-    return out
+def _narrow_backward_fake(dy, e, h_dim, need_dx, need_dw13, need_dw2):
+    r, d = dy.shape
+    bf = lambda need, *shape: dy.new_empty(shape if need else (0,), dtype=torch.bfloat16)  # noqa: E731
+    return bf(need_dx, r, d), bf(need_dw13, e, h_dim, d), bf(need_dw2, e, d, h_dim), bf(need_dw13, e, h_dim, d)
 
 
 @torch.library.custom_op("moe_mi355x_mx::grouped_swiglu_ckpt8_backward", mutates_args=())
 def grouped_swiglu_ckpt8_backward(
-    dy: Tensor, w1: Tensor, w2: Tensor, w3: Tensor, num_tokens_per_expert: Tensor, x8: Tensor, xs: Tensor, g8: Tensor,
-    gs: Tensor, u8: Tensor, us: Tensor, need_dx: bool = True, need_dw13: bool = True, need_dw2: bool = True,
+    dy: Tensor, w1: Tensor, w2: Tensor, w3: Tensor, num_tokens_per_expert: Tensor, kept: Tensor, need_dx: bool = True,
+    need_dw13: bool = True, need_dw2: bool = True,
 ) -> tuple[Tensor, Tensor, Tensor, Tensor]:
     """(dx, dw1, dw2, dw3) of grouped_swiglu_ckpt8 from what it kept; dx is zero on rows past
     sum(counts), weights of experts without rows get zeros. What is not needed is empty."""
     op = "grouped_swiglu_ckpt8_backward"
     _check_experts(op, dy, w1, w2, w3, num_tokens_per_expert, 64)
-    r, (_e, h_dim, d) = dy.shape[0], w1.shape
-    x8, xs, g8, gs, u8, us = _kept(op, dy, x=(x8, xs, (r,), d, d // MX_BLOCK), g=(g8, gs, (r,), h_dim, h_dim // MX_BLOCK),
-                                   u=(u8, us, (r,), h_dim, h_dim // MX_BLOCK))
+    r, (e, h_dim, d) = dy.shape[0], w1.shape
+    offsets, size = _ckpt8_layout(r, d, h_dim)
+    kept = _check_kept(op, kept, size, dy)
     dy, w1, w2, w3 = map(_ready, (dy, w1, w2, w3))
     counts = num_tokens_per_expert.to(torch.int64).contiguous()
+    x8, xs, g8, gs, up8, us = _at(kept, offsets)
+    parts, size = _carve((4 * r * h_dim, 2 * r * h_dim if need_dw2 else 0, 2 * r * d if need_dw13 else 0))
+    ws = dy.new_empty(size, dtype=torch.uint8)
+    dgu, h, x = _at(ws, parts)
 
-    def rows() -> Tensor:
-        x = dy.new_empty(r, d)
-        call("moe_restore8_rows", ptr(x8), ptr(xs), r, d, ptr(x), stream_of(dy))
+    def rows() -> int:
+        call("moe_restore8_rows", x8, xs, r, d, x, stream_of(dy))
         return x
 
     with _guard(dy):
-        return _narrow_backward(dy, w1, w2, w3, counts, g8, gs, u8, us, rows, None, need_dx, need_dw13, need_dw2)
+        return _narrow_backward(dy, e, h_dim, ptr(w1), ptr(w2), ptr(w3), counts, g8, gs, up8, us, dgu, rows,
+                                h if need_dw2 else None, False, need_dx, need_dw13, need_dw2)
 
 
 @grouped_swiglu_ckpt8_backward.register_fake
-def _(dy, w1, w2, w3, num_tokens_per_expert, x8, xs, g8, gs, u8, us, need_dx=True, need_dw13=True, need_dw2=True):
-    empty = lambda: w1.new_empty(0)  # noqa: E731
-    return (w1.new_empty(x8.shape) if need_dx else empty(), torch.empty_like(w1) if need_dw13 else empty(),
-            torch.empty_like(w2) if need_dw2 else empty(), torch.empty_like(w3) if need_dw13 else empty())
+def _(dy, w1, w2, w3, num_tokens_per_expert, kept, need_dx=True, need_dw13=True, need_dw2=True):
+    return _narrow_backward_fake(dy, w1.shape[0], w1.shape[1], need_dx, need_dw13, need_dw2)
 
 
 def _ckpt8_setup(ctx, inputs, output):
     _x, w1, w2, w3, counts, ctx.for_backward = inputs
-    _y, *kept = output
-    ctx.save_for_backward(w1, w2, w3, counts, *kept)
-    ctx.mark_non_differentiable(*kept)
+    ctx.save_for_backward(w1, w2, w3, counts, output[1])
+    ctx.mark_non_differentiable(output[1])
     ctx.set_materialize_grads(False)
 
 
@@ -1558,115 +1576,104 @@ def _mxfp4_padded(cols: int) -> int:  # moe_mxfp4_padded_cols
     return (cols + 255) // 256 * 256
 
 
-def _mxfp4_rows(x: Tensor, s: int) -> tuple[Tensor, Tensor]:
-    """x [R, C] bf16 in MXFP4 as the products take their rows: zero columns up to a multiple of 256."""
-    r, c = x.shape
-    pc = _mxfp4_padded(c)
-    q = torch.empty(r, pc // 2, dtype=torch.uint8, device=x.device)
-    scale = torch.empty(r, pc // MX_BLOCK, dtype=torch.uint8, device=x.device)
-    call("moe_mxfp4_quant_rows", ptr(x), r, c, pc, 0, ptr(q), ptr(scale), s)
-    return q, scale
-
-
-def _mxfp4_values(q: Tensor, scale: Tensor, cols: int, s: int) -> Tensor:
-    """The bf16 values of the first `cols` columns of an MXFP4 matrix."""
-    x = torch.empty(*q.shape[:-1], cols, dtype=torch.bfloat16, device=q.device)
-    call("moe_mxfp4_dequant_rows", ptr(q), ptr(scale), x.numel() // cols, cols, 2 * q.shape[-1], 0, ptr(x), s)
-    return x
+@functools.lru_cache(maxsize=256)
+def _mxfp4_train_layout(r: int, e: int, d: int, h: int) -> tuple[tuple[int, ...], int]:
+    """grouped_swiglu_mxfp4_train's kept tensor: w1, w2, w3, x and h in MXFP4 (the rows of x and h
+    padded to 256 columns, zeros behind), g and u in MXFP8, each with its scales."""
+    w = e * d * h
+    four = [n for c in (w, w, w, r * _mxfp4_padded(d), r * _mxfp4_padded(h)) for n in (c // 2, c // MX_BLOCK)]
+    return _carve(four + [n for c in (r * h, r * h) for n in (c, c // MX_BLOCK)])
 
 
 @torch.library.custom_op("moe_mi355x_mx::grouped_swiglu_mxfp4_train", mutates_args=())
 def grouped_swiglu_mxfp4_train(
     x: Tensor, w1: Tensor, w2: Tensor, w3: Tensor, num_tokens_per_expert: Tensor
-) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor,
-           Tensor, Tensor]:
+) -> tuple[Tensor, Tensor]:
     """The SwiGLU experts in MXFP4 from bf16 weights, with gradients: y [R, D] is
     grouped_swiglu_mxfp4's on the packed weights. The backward passes the quantizations
     straight through: it takes the products' gradients at their quantized operands (in bf16,
     which holds them exactly) and the activation's at g and u kept in MXFP8. Returns y, then
-    what is kept: x and h, w1, w2, w3 in MXFP4 and g, u in MXFP8, each with its scales. D and
-    H are multiples of 64."""
+    what is kept, as one tensor of bytes: w1, w2, w3, x and h in MXFP4 and g, u in MXFP8, each
+    with its scales. D and H are multiples of 64."""
     op = "grouped_swiglu_mxfp4_train"
     _check_experts(op, x, w1, w2, w3, num_tokens_per_expert, 64)
-    x, w1, w2, w3 = (_aligned(t.contiguous()) for t in (x, w1, w2, w3))
+    x, w1, w2, w3 = map(_ready, (x, w1, w2, w3))
     counts = num_tokens_per_expert.to(torch.int64).contiguous()
     r, d = x.shape
     e, h_dim, _ = w1.shape
-    u8 = lambda *shape: torch.empty(*shape, dtype=torch.uint8, device=x.device)  # noqa: E731
-    ph = _mxfp4_padded(h_dim)
-    qh, sh = u8(r, ph // 2), u8(r, ph // MX_BLOCK)
-    g8, gs, up8, us = u8(r, h_dim), u8(r, h_dim // MX_BLOCK), u8(r, h_dim), u8(r, h_dim // MX_BLOCK)
+    offsets, size = _mxfp4_train_layout(r, e, d, h_dim)
+    kept = x.new_empty(size, dtype=torch.uint8)
+    qw1, sw1, qw2, sw2, qw3, sw3, qx, sx, qh, sh, g8, gs, up8, us = _at(kept, offsets)
     y = x.new_empty(r, d)
     with _guard(x):
         s = stream_of(x)
-        qx, sx = _mxfp4_rows(x, s)
-        packed = []
-        for w in (w1, w2, w3):
-            q, sc = u8(*w.shape[:-1], w.shape[-1] // 2), u8(*w.shape[:-1], w.shape[-1] // MX_BLOCK)
-            call("moe_mxfp4_quant_rows", ptr(w), w.numel() // w.shape[-1], w.shape[-1], w.shape[-1], 0, ptr(q), ptr(sc), s)
-            packed += [q, sc]
-        qw1, sw1, qw2, sw2, qw3, sw3 = packed
-        call("moe_mxfp4_gemm_gate_up_keep", ptr(qx), ptr(sx), ptr(qw1), ptr(sw1), ptr(qw3), ptr(sw3), ptr(counts), r, e, d,
-             h_dim, ptr(qh), ptr(sh), ptr(g8), ptr(gs), ptr(up8), ptr(us), s)
-        call("moe_mxfp4_gemm_down", ptr(qh), ptr(sh), ptr(qw2), ptr(sw2), ptr(counts), r, e, d, h_dim, ptr(y), s)
-    return y, qx, sx, qh, sh, qw1, sw1, qw2, sw2, qw3, sw3, g8, gs, up8, us
+        call("moe_mxfp4_quant_rows", ptr(x), r, d, _mxfp4_padded(d), 0, qx, sx, s)
+        for w, q, sc, rows, cols in ((w1, qw1, sw1, e * h_dim, d), (w2, qw2, sw2, e * d, h_dim), (w3, qw3, sw3, e * h_dim, d)):
+            call("moe_mxfp4_quant_rows", ptr(w), rows, cols, cols, 0, q, sc, s)
+        call("moe_mxfp4_gemm_gate_up_keep", qx, sx, qw1, sw1, qw3, sw3, ptr(counts), r, e, d, h_dim, qh, sh, g8, gs, up8, us,
+             s)
+        call("moe_mxfp4_gemm_down", qh, sh, qw2, sw2, ptr(counts), r, e, d, h_dim, ptr(y), s)
+    return y, kept
 
 
 @grouped_swiglu_mxfp4_train.register_fake
 def _(x, w1, w2, w3, num_tokens_per_expert):
-    r, d = x.shape
-    e, h_dim, _ = w1.shape
-    u8 = lambda *shape: x.new_empty(*shape, dtype=torch.uint8)  # noqa: E731
-    pd, ph = _mxfp4_padded(d), _mxfp4_padded(h_dim)
-    return (x.new_empty(r, d), u8(r, pd // 2), u8(r, pd // 32), u8(r, ph // 2), u8(r, ph // 32),
-            u8(e, h_dim, d // 2), u8(e, h_dim, d // 32), u8(e, d, h_dim // 2), u8(e, d, h_dim // 32),
-            u8(e, h_dim, d // 2), u8(e, h_dim, d // 32), u8(r, h_dim), u8(r, h_dim // 32), u8(r, h_dim),
-            u8(r, h_dim // 32))
+    e, h_dim, d = w1.shape
+    size = _mxfp4_train_layout.__wrapped__(x.shape[0], e, d, h_dim)[1]
+    return x.new_empty(x.shape), x.new_empty(size, dtype=torch.uint8)
 
 
 @torch.library.custom_op("moe_mi355x_mx::grouped_swiglu_mxfp4_train_backward", mutates_args=())
 def grouped_swiglu_mxfp4_train_backward(
-    dy: Tensor, num_tokens_per_expert: Tensor, qx: Tensor, sx: Tensor, qh: Tensor, sh: Tensor, qw1: Tensor, sw1: Tensor,
-    qw2: Tensor, sw2: Tensor, qw3: Tensor, sw3: Tensor, g8: Tensor, gs: Tensor, u8: Tensor, us: Tensor,
-    need_dx: bool = True, need_dw13: bool = True, need_dw2: bool = True,
+    dy: Tensor, num_tokens_per_expert: Tensor, kept: Tensor, hidden_dim: int, need_dx: bool = True, need_dw13: bool = True,
+    need_dw2: bool = True,
 ) -> tuple[Tensor, Tensor, Tensor, Tensor]:
     """(dx, dw1, dw2, dw3) of grouped_swiglu_mxfp4_train from what it kept; dx is zero on rows
     past sum(counts), weights of experts without rows get zeros. What is not needed is empty."""
     op = "grouped_swiglu_mxfp4_train_backward"
-    counts = num_tokens_per_expert
+    counts, h_dim = num_tokens_per_expert, hidden_dim
     require_gpu(dy, counts)
-    r, d, e, h_dim = _check_mxfp4_rows(op, dy, qw1, counts)
-    pd, ph, nd, nh = _mxfp4_padded(d), _mxfp4_padded(h_dim), d // MX_BLOCK, h_dim // MX_BLOCK
+    _check_bf16(op, dy=dy)
+    if dy.dim() != 2 or counts.dim() != 1:
+        raise ValueError(f"{op} expects dy [R, D] and counts [E], got {tuple(dy.shape)}, {tuple(counts.shape)}")
+    (r, d), e = dy.shape, counts.shape[0]
     _check_dims(op, e, d, h_dim, 64)
     _check_counts(op, counts, dy)
-    qx, sx, qh, sh, qw1, sw1, qw2, sw2, qw3, sw3, g8, gs, u8, us = _kept(
-        op, dy, x=(qx, sx, (r,), pd // 2, pd // MX_BLOCK), h=(qh, sh, (r,), ph // 2, ph // MX_BLOCK),
-        w1=(qw1, sw1, (e, h_dim), d // 2, nd), w2=(qw2, sw2, (e, d), h_dim // 2, nh), w3=(qw3, sw3, (e, h_dim), d // 2, nd),
-        g=(g8, gs, (r,), h_dim, nh), u=(u8, us, (r,), h_dim, nh))
+    offsets, size = _mxfp4_train_layout(r, e, d, h_dim)
+    kept = _check_kept(op, kept, size, dy)
     dy, counts = _ready(dy), counts.to(torch.int64).contiguous()
+    qw1, sw1, qw2, sw2, qw3, sw3, qx, sx, qh, sh, g8, gs, up8, us = _at(kept, offsets)
+    need_dgu, n_w = need_dx or need_dw13, 2 * e * d * h_dim
+    parts, size = _carve((n_w if need_dx else 0, n_w if need_dgu else 0, n_w if need_dx else 0,
+                          4 * r * h_dim if need_dgu else 0, 2 * r * h_dim if need_dw2 else 0, 2 * r * d if need_dw13 else 0))
+    ws = dy.new_empty(size, dtype=torch.uint8)
+    w1, w2, w3, dgu, h, x = _at(ws, parts)
+
+    def values(q: int, scale: int, rows: int, cols: int, q_cols: int, out: int) -> int:
+        call("moe_mxfp4_dequant_rows", q, scale, rows, cols, q_cols, 0, out, stream_of(dy))
+        return out
+
     with _guard(dy):
-        s = stream_of(dy)
-        # the values dgu and dx multiply; dW takes only their shapes
-        w2 = _mxfp4_values(qw2, sw2, h_dim, s) if need_dx or need_dw13 else dy.new_empty(*qw2.shape[:-1], h_dim)
-        w1, w3 = (_mxfp4_values(q, sc, d, s) if need_dx else dy.new_empty(*q.shape[:-1], d)
-                  for q, sc in ((qw1, sw1), (qw3, sw3)))
-        h = _mxfp4_values(qh, sh, h_dim, s) if need_dw2 else dy.new_empty(0)
-        return _narrow_backward(dy, w1, w2, w3, counts, g8, gs, u8, us, lambda: _mxfp4_values(qx, sx, d, s), h, need_dx,
-                                need_dw13, need_dw2)
+        if need_dgu:
+            values(qw2, sw2, e * d, h_dim, h_dim, w2)
+        if need_dx:
+            values(qw1, sw1, e * h_dim, d, d, w1)
+            values(qw3, sw3, e * h_dim, d, d, w3)
+        if need_dw2:
+            values(qh, sh, r, h_dim, _mxfp4_padded(h_dim), h)
+        return _narrow_backward(dy, e, h_dim, w1, w2, w3, counts, g8, gs, up8, us, dgu,
+                                lambda: values(qx, sx, r, d, _mxfp4_padded(d), x), h, True, need_dx, need_dw13, need_dw2)
 
 
 @grouped_swiglu_mxfp4_train_backward.register_fake
-def _(dy, num_tokens_per_expert, qx, sx, qh, sh, qw1, sw1, qw2, sw2, qw3, sw3, g8, gs, u8, us, need_dx=True,
-      need_dw13=True, need_dw2=True):
-    r, (e, h_dim, _), d = qx.shape[0], qw1.shape, qw2.shape[1]
-    bf = lambda need, *shape: dy.new_empty(shape if need else (0,), dtype=torch.bfloat16)  # noqa: E731
-    return bf(need_dx, r, d), bf(need_dw13, e, h_dim, d), bf(need_dw2, e, d, h_dim), bf(need_dw13, e, h_dim, d)
+def _(dy, num_tokens_per_expert, kept, hidden_dim, need_dx=True, need_dw13=True, need_dw2=True):
+    return _narrow_backward_fake(dy, num_tokens_per_expert.shape[0], hidden_dim, need_dx, need_dw13, need_dw2)
 
 
 def _mxfp4_train_setup(ctx, inputs, output):
-    _y, *kept = output
-    ctx.save_for_backward(inputs[4], *kept)
-    ctx.mark_non_differentiable(*kept)
+    ctx.save_for_backward(inputs[4], output[1])
+    ctx.mark_non_differentiable(output[1])
+    ctx.hidden_dim = inputs[1].shape[1]
     ctx.set_materialize_grads(False)
 
 
@@ -1674,8 +1681,8 @@ def _mxfp4_train_bwd(ctx, dy, *_unused):
     if dy is None:
         return None, None, None, None, None
     need = ctx.needs_input_grad
-    return *_needed(need, grouped_swiglu_mxfp4_train_backward(dy, *ctx.saved_tensors, need[0], need[1] or need[3],
-                                                              need[2])), None
+    return *_needed(need, grouped_swiglu_mxfp4_train_backward(dy, *ctx.saved_tensors, ctx.hidden_dim, need[0],
+                                                              need[1] or need[3], need[2])), None
 
 
 grouped_swiglu_mxfp4_train.register_autograd(_mxfp4_train_bwd, setup_context=_mxfp4_train_setup)
