@@ -234,8 +234,6 @@ __device__ __forceinline__ void for_each(F f) {  // f(0), ..., f(N - 1) with com
 }
 constexpr int kTileList = 64;
 
-__device__ const uint4 kZeroRow[8] = {};  // source of columns and k past an edge
-
 // Exclusive prefix sums of up to 1024 non-negative ints, four per thread of the first 256,
 // that stop at `most` (saturating sums are associative, and with most < 2^30 no step passes
 // 2^31 whatever the values). Returns the total. Called by every thread; tmp: one int per wave.
