@@ -973,9 +973,11 @@ struct Params {
 
 #define LDSP __attribute__((address_space(3)))
 // One wave-wide direct-to-LDS copy: lane i's 16 bytes at g land at LDS byte
-// address lds + 16 i; issued as inline asm and waited for with vmcnt.
+// address lds + 16 i; issued as inline asm and waited for with vmcnt. s_nop: a copy may read m0 one
+// wait state after a scalar instruction wrote it at the earliest, which the compiler keeps to for its
+// own instructions only.
 __device__ __forceinline__ void dma16(const void* g, uint32_t lds) {
-  asm volatile("global_load_lds_dwordx4 %0, off" :: "v"(g), "{m0}"(lds) : "memory");
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(g), "{m0}"(lds) : "memory");
 }
 __device__ __forceinline__ uint32_t lds_addr(const uint8_t* ptr) { return (uint32_t)(size_t)((LDSP const uint8_t*)ptr); }
 
@@ -985,7 +987,7 @@ __device__ __forceinline__ int rm_off(int r, int c) { return r * 128 + ((c ^ ((r
 
 // One wave-wide 4-byte direct-to-LDS copy: lane i's dword lands at lds + 4 i.
 __device__ __forceinline__ void dma4(const void* g, uint32_t lds) {
-  asm volatile("global_load_lds_dword %0, off" :: "v"(g), "{m0}"(lds) : "memory");
+  asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" :: "v"(g), "{m0}"(lds) : "memory");
 }
 
 __device__ const uint4 kZeroRow[64] = {};  // source of zero rows and k past a segment

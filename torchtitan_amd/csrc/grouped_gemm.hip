@@ -178,9 +178,11 @@ typedef short v8s_t __attribute__((ext_vector_type(8)));
 
 // One wave-wide direct-to-LDS copy: lane i's 16 bytes at g land at LDS byte
 // address lds + 16 i. Issued as inline asm so the compiler neither waits on it
-// before unrelated LDS reads nor reorders it; the kernel waits with vmcnt.
+// before unrelated LDS reads nor reorders it; the kernel waits with vmcnt. s_nop: a copy may
+// read m0 one wait state after a scalar instruction wrote it at the earliest, which the compiler
+// keeps to for its own instructions only.
 __device__ __forceinline__ void dma16(const void* g, uint32_t lds) {
-  asm volatile("global_load_lds_dwordx4 %0, off" :: "v"(g), "{m0}"(lds) : "memory");
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(g), "{m0}"(lds) : "memory");
 }
 template <typename T>
 __device__ __forceinline__ uint32_t lds_addr(T* ptr) { return (uint32_t)(size_t)((LDSP T*)ptr); }

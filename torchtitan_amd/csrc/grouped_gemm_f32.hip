@@ -74,11 +74,13 @@ __device__ const float4 kZeroChunk[4] = {};  // source of the k-rows past a segm
 typedef f32x4_t f32x4_u __attribute__((aligned(4)));
 
 // lane i's 16 bytes at g land at LDS byte address lds + 16 i: a direct-to-LDS copy, or,
-// where an operand is not 16-byte aligned, through registers
+// where an operand is not 16-byte aligned, through registers (s_nop: a copy may read m0 one wait
+// state after a scalar instruction wrote it at the earliest, and the compiler, which keeps to
+// that elsewhere, does not look into the asm)
 template <bool ALIGNED>
 __device__ __forceinline__ void copy16(const float* g, uint32_t lds) {
   if constexpr (ALIGNED)
-    asm volatile("global_load_lds_dwordx4 %0, off" :: "v"(g), "{m0}"(lds) : "memory");
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(g), "{m0}"(lds) : "memory");
   else
     *(LDSP f32x4_t*)(size_t)(lds + 16 * (threadIdx.x & 63)) = *(const f32x4_u*)g;
 }

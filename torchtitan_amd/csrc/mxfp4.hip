@@ -195,16 +195,18 @@ __device__ __forceinline__ float activation(int act, float g, float u, float lim
 
 #define LDSP __attribute__((address_space(3)))
 // One wave-wide direct-to-LDS copy: lane i's 16 bytes at g land at LDS byte address
-// lds + 16 i; waited for with vmcnt.
+// lds + 16 i; waited for with vmcnt. s_nop: a copy may read m0 one wait state after a scalar
+// instruction wrote it at the earliest, and the compiler, which keeps to that elsewhere, does
+// not look into the asm.
 __device__ __forceinline__ void dma16(const void* g, uint32_t lds) {
-  asm volatile("global_load_lds_dwordx4 %0, off" :: "v"(g), "{m0}"(lds) : "memory");
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(g), "{m0}"(lds) : "memory");
 }
 // The same with lane i's 4 bytes at lds + 4 i; and with its 2 bytes there, zeros above them.
 __device__ __forceinline__ void dma4(const void* g, uint32_t lds) {
-  asm volatile("global_load_lds_dword %0, off" :: "v"(g), "{m0}"(lds) : "memory");
+  asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" :: "v"(g), "{m0}"(lds) : "memory");
 }
 __device__ __forceinline__ void dma2(const void* g, uint32_t lds) {
-  asm volatile("global_load_lds_ushort %0, off" :: "v"(g), "{m0}"(lds) : "memory");
+  asm volatile("s_nop 0\n\tglobal_load_lds_ushort %0, off" :: "v"(g), "{m0}"(lds) : "memory");
 }
 __device__ __forceinline__ uint32_t lds_addr(const uint8_t* ptr) { return (uint32_t)(size_t)((LDSP const uint8_t*)ptr); }
 
