@@ -19,6 +19,7 @@ from contextlib import nullcontext
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from ._lib import call, lib, ptr, require_gpu, stream_of
 
@@ -1166,6 +1167,11 @@ def _guard(t: Tensor):
     return _HERE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
+def _has_tangent(t: Tensor) -> bool:
+    """Whether t carries a derivative of forward mode (a dual tensor, torch.func.jvp's input)."""
+    return forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None
+
+
 def _check_experts(op: str, x: Tensor, w1: Tensor, w2: Tensor, w3: Tensor, counts: Tensor, multiple: int) -> None:
     """The arguments of experts with separate bf16 weights: x [R, D], w1 and w3 [E, H, D],
     w2 [E, D, H], counts [E] integers, all on one device."""
@@ -1181,6 +1187,8 @@ def _check_experts(op: str, x: Tensor, w1: Tensor, w2: Tensor, w3: Tensor, count
                          f"w3 {tuple(w3.shape)}, counts {tuple(cs)}")
     _check_dims(op, e, d, h, multiple)
     _check_counts(op, counts, x, w1, w2, w3)
+    if any([_has_tangent(t) for t in (x, w1, w2, w3)]):
+        raise RuntimeError(f"{op} has no derivatives in forward mode")
 
 
 def _check_dims(op: str, e: int, d: int, h: int, multiple: int) -> None:
@@ -1368,15 +1376,30 @@ grouped_swiglu_ckpt8.register_autograd(_ckpt8_bwd, setup_context=_ckpt8_setup)
 _MX = torch.library.Library("moe_mi355x_mx", "FRAGMENT")
 
 
-def _mx_op(schema: str):
-    """Defines moe_mi355x_mx::schema with the decorated function as its GPU kernel (and on the CPU,
-    where the kernel's own check refuses)."""
+# The kernels of the experts' inference, which drop gradients: behind the ops of the same names in
+# moe_mi355x_mx and this module, which refuse them.
+_MX_BARE = torch.library.Library("moe_mi355x_mx_bare", "FRAGMENT")
+
+
+def _mx_op(schema: str, lib: torch.library.Library = _MX):
+    """Defines the op of this schema in lib with the decorated function as its GPU kernel (and on the
+    CPU, where the kernel's own check refuses)."""
     def register(fn):
         name = schema.split("(")[0]
-        _MX.define(schema)
-        _MX.impl(name, fn, "CUDA")
-        _MX.impl(name, fn, "CPU")
-        return getattr(torch.ops.moe_mi355x_mx, name).default
+        lib.define(schema)
+        lib.impl(name, fn, "CUDA")
+        lib.impl(name, fn, "CPU")
+        return getattr(getattr(torch.ops, lib.ns), name).default
+    return register
+
+
+def _inference_op(bare):
+    """Defines moe_mi355x_mx's op of the bare one's name and schema as the decorated function, above
+    autograd and torch.func's transforms, where it sees what it has to refuse."""
+    def register(fn):
+        _MX.define(str(bare._schema).split("::")[1])
+        _MX.impl(fn.__name__, fn, "CompositeImplicitAutograd")
+        return fn
     return register
 
 
@@ -1484,13 +1507,14 @@ def _check_mxfp4_rows(op: str, x: Tensor, qw1: Tensor, counts: Tensor, glu: int 
 
 
 def _no_gradients(op: str, *tensors: Tensor) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+    grad = torch.is_grad_enabled()
+    if any([(grad and t.requires_grad) or _has_tangent(t) for t in tensors]):
         raise RuntimeError(f"{op} is for inference and has no gradients: call it under torch.no_grad() or on detached "
                            "tensors (grouped_swiglu_mxfp4_train trains on bf16 weights)")
 
 
 @_mx_op("grouped_swiglu_mxfp4(Tensor x, Tensor qw1, Tensor sw1, Tensor qw2, Tensor sw2, Tensor qw3, Tensor sw3, "
-        "Tensor num_tokens_per_expert) -> Tensor")
+        "Tensor num_tokens_per_expert) -> Tensor", _MX_BARE)
 def _grouped_swiglu_mxfp4(x, qw1, sw1, qw2, sw2, qw3, sw3, num_tokens_per_expert):
     op = "grouped_swiglu_mxfp4"
     counts = num_tokens_per_expert
@@ -1511,11 +1535,12 @@ def _grouped_swiglu_mxfp4(x, qw1, sw1, qw2, sw2, qw3, sw3, num_tokens_per_expert
     return y
 
 
-@torch.library.register_fake("moe_mi355x_mx::grouped_swiglu_mxfp4", lib=_MX)
+@torch.library.register_fake("moe_mi355x_mx_bare::grouped_swiglu_mxfp4", lib=_MX_BARE)
 def _(x, qw1, sw1, qw2, sw2, qw3, sw3, num_tokens_per_expert):
     return x.new_empty(x.shape)
 
 
+@_inference_op(_grouped_swiglu_mxfp4)
 def grouped_swiglu_mxfp4(
     x: Tensor, qw1: Tensor, sw1: Tensor, qw2: Tensor, sw2: Tensor, qw3: Tensor, sw3: Tensor,
     num_tokens_per_expert: Tensor,
@@ -1529,7 +1554,7 @@ def grouped_swiglu_mxfp4(
 
 
 @_mx_op("grouped_swiglu_oss_mxfp4(Tensor x, Tensor qmlp1, Tensor smlp1, Tensor mlp1_bias, Tensor qmlp2, Tensor smlp2, "
-        "Tensor mlp2_bias, Tensor num_tokens_per_expert, float swiglu_limit) -> Tensor")
+        "Tensor mlp2_bias, Tensor num_tokens_per_expert, float swiglu_limit) -> Tensor", _MX_BARE)
 def _grouped_swiglu_oss_mxfp4(x, qmlp1, smlp1, mlp1_bias, qmlp2, smlp2, mlp2_bias, num_tokens_per_expert, swiglu_limit):
     op = "grouped_swiglu_oss_mxfp4"
     counts = num_tokens_per_expert
@@ -1555,11 +1580,12 @@ def _grouped_swiglu_oss_mxfp4(x, qmlp1, smlp1, mlp1_bias, qmlp2, smlp2, mlp2_bia
     return y
 
 
-@torch.library.register_fake("moe_mi355x_mx::grouped_swiglu_oss_mxfp4", lib=_MX)
+@torch.library.register_fake("moe_mi355x_mx_bare::grouped_swiglu_oss_mxfp4", lib=_MX_BARE)
 def _(x, qmlp1, smlp1, mlp1_bias, qmlp2, smlp2, mlp2_bias, num_tokens_per_expert, swiglu_limit):
     return x.new_empty(x.shape)
 
 
+@_inference_op(_grouped_swiglu_oss_mxfp4)
 def grouped_swiglu_oss_mxfp4(
     x: Tensor, qmlp1: Tensor, smlp1: Tensor, mlp1_bias: Tensor, qmlp2: Tensor, smlp2: Tensor, mlp2_bias: Tensor,
     num_tokens_per_expert: Tensor, swiglu_limit: float,
