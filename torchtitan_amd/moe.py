@@ -149,6 +149,11 @@ class GroupedExperts(Module):
         num_experts: int
         use_grouped_mm: bool = True
 
+    # set by MXFP4Converter and MXFP8ActivationCheckpointConverter (of the class, so that whole modules
+    # saved before these recipes run as they did)
+    mxfp4 = False
+    ckpt8 = False
+
     def __init__(self, config: Config):
         super().__init__()
         self.num_experts = config.num_experts
@@ -156,12 +161,9 @@ class GroupedExperts(Module):
         self.w2 = nn.Parameter(torch.empty(config.num_experts, config.dim, config.hidden_dim))
         self.w3 = nn.Parameter(torch.empty(config.num_experts, config.hidden_dim, config.dim))
         self.use_grouped_mm = config.use_grouped_mm
-        # set by the converters of quantization.py (Float8GroupedMMConverter, MXFP8Converter,
-        # MXFP4Converter, MXFP8ActivationCheckpointConverter)
+        # set by the converters of quantization.py (Float8GroupedMMConverter, MXFP8Converter)
         self.float8 = False
         self.mxfp8 = False
-        self.mxfp4 = False
-        self.ckpt8 = False
 
     def forward(self, x: torch.Tensor, num_tokens_per_expert: torch.Tensor) -> torch.Tensor:
         w1, w2, w3 = _local(self.w1), _local(self.w2), _local(self.w3)
