@@ -32,3 +32,42 @@ def test_modules_of_before(monkeypatch):
         model = torch.nn.ModuleDict({"experts": m})
         assert Q._mark_experts(model, ["experts"], attr) == ["experts"]
         assert m(torch.zeros(4, 64), torch.tensor([2, 2])) == attr
+
+
+@pytest.fixture
+def converter(monkeypatch):
+    """The converters by name, built as on the hardware; the packing on the CPU."""
+    from tests import narrow_util as N
+    from torchtitan_amd import ops
+    from torchtitan_amd import quantization as Q
+
+    monkeypatch.setattr(Q, "has_gfx950", lambda: True)
+    monkeypatch.setattr(ops, "mxfp4_quantize", N.pack4)
+
+    def build(name, *fqns):
+        conv = getattr(Q, name).Config(fqns=list(fqns))
+        return conv.build(parallel_dims=DIMS, model_compile_enabled=False)
+    return build
+
+
+def test_shared_experts_are_packed_under_each_name(converter):
+    """Experts that two layers share: one packed module in both places, under whichever name asked for."""
+    from torchtitan_amd.mxfp4 import MXFP4GroupedExperts
+
+    for fqns in (("a", "b"), ("b",)):
+        m = _experts()
+        torch.nn.init.normal_(m.w1), torch.nn.init.normal_(m.w2), torch.nn.init.normal_(m.w3)
+        model = torch.nn.ModuleDict({n: torch.nn.ModuleDict({"experts": m}) for n in "ab"})
+        assert converter("MXFP4WeightConverter", *fqns).convert(model) == [f"{n}.experts" for n in fqns]
+        assert type(model["b"]["experts"]) is MXFP4GroupedExperts
+        assert (model["a"]["experts"] is model["b"]["experts"]) == (len(fqns) == 2)
+        assert len(list(model["a"].parameters())) == (0 if len(fqns) == 2 else 3)
+
+
+def test_shared_experts_are_marked_once():
+    from torchtitan_amd import quantization as Q
+
+    for fqns, names in ((["a", "b"], ["a.experts"]), (["b"], ["b.experts"])):
+        m = _experts()
+        model = torch.nn.ModuleDict({n: torch.nn.ModuleDict({"experts": m}) for n in "ab"})
+        assert Q._mark_experts(model, fqns, "ckpt8") == names and m.ckpt8

@@ -90,15 +90,17 @@ _ALONE = ("mxfp4", "ckpt8")
 
 
 def _mark_experts(model: nn.Module, fqns: list[str], attr: str) -> list[str]:
-    matching = [(name, mod) for name, mod in model.named_modules()
-                if isinstance(mod, GroupedExperts) and any(f in name for f in fqns)]
-    for name, mod in matching:
+    matching = {}  # a module that several names share: under the first that matches
+    for name, mod in model.named_modules(remove_duplicate=False):
+        if isinstance(mod, GroupedExperts) and any(f in name for f in fqns):
+            matching.setdefault(mod, name)
+    for mod, name in matching.items():
         others = [r for r in _RECIPES if r != attr and getattr(mod, r)]
         if others and (attr in _ALONE or any(r in _ALONE for r in others)):
             raise ValueError(f"{name} is already converted to {others[0]}: {attr} experts are a recipe of their own")
-    for _name, mod in matching:
+    for mod in matching:
         setattr(mod, attr, True)
-    return [name for name, _mod in matching]
+    return list(matching.values())
 
 
 class MXFP8Converter(Configurable):
@@ -198,10 +200,13 @@ class MXFP4WeightConverter(_ExpertsConverter):
     def convert(self, model: nn.Module) -> list[str]:
         packed = {GroupedExperts: MXFP4GroupedExperts, GptOssGroupedExperts: MXFP4GptOssGroupedExperts}
         converted = []
-        for name, mod in list(model.named_modules()):
+        made = {}  # of a module that several names share, one
+        for name, mod in list(model.named_modules(remove_duplicate=False)):
             if name and type(mod) in packed and any(f in name for f in self.fqns):
+                if mod not in made:
+                    made[mod] = packed[type(mod)].from_experts(mod)
                 parent, _, child = name.rpartition(".")
-                setattr(model.get_submodule(parent), child, packed[type(mod)].from_experts(mod))
+                setattr(model.get_submodule(parent), child, made[mod])
                 converted.append(name)
         return converted
 
