@@ -71,3 +71,48 @@ def test_shared_experts_are_marked_once():
         m = _experts()
         model = torch.nn.ModuleDict({n: torch.nn.ModuleDict({"experts": m}) for n in "ab"})
         assert Q._mark_experts(model, fqns, "ckpt8") == names and m.ckpt8
+
+
+def _gptoss():
+    from torchtitan_amd.gpt_oss import GptOssGroupedExperts
+
+    return GptOssGroupedExperts.Config(dim=64, hidden_dim=64, num_experts=2).build()
+
+
+def _packed():
+    from torchtitan_amd.mxfp4 import MXFP4GroupedExperts
+
+    return MXFP4GroupedExperts.Config(dim=64, hidden_dim=64, num_experts=2).build()
+
+
+@pytest.mark.parametrize("name", ["MXFP4Converter", "MXFP8ActivationCheckpointConverter"])
+@pytest.mark.parametrize("make", [_gptoss, _packed])
+def test_experts_without_a_training_form_are_refused(converter, name, make):
+    """gpt-oss's experts and packed ones have no such recipe: a match raises, and marks no others."""
+    model = torch.nn.ModuleDict({"experts": _experts(), "later": torch.nn.ModuleDict({"experts": make()})})
+    with pytest.raises(ValueError, match="later.experts"):
+        converter(name, "experts").convert(model)
+    assert not model["experts"].mxfp4 and not model["experts"].ckpt8
+    model = torch.nn.ModuleDict({"experts": _experts(), "rest": make()})  # not matched: not refused
+    assert converter(name, "experts").convert(model) == ["experts"]
+
+
+def test_experts_that_cannot_be_packed_are_refused(converter):
+    """A subclass may compute something else, a hook sees calls of the module it is on: neither goes
+    with the module that is replaced."""
+    from torchtitan_amd import GroupedExperts
+
+    class Scaled(GroupedExperts):
+        def forward(self, x, num_tokens_per_expert):
+            return 2 * super().forward(x, num_tokens_per_expert)
+
+    hooked = _experts()
+    hooked.register_forward_pre_hook(lambda mod, args: None)
+    for bad in (Scaled(GroupedExperts.Config(dim=64, hidden_dim=64, num_experts=2)), hooked):
+        model = torch.nn.ModuleDict({"a": torch.nn.ModuleDict({"experts": _experts()}),
+                                     "b": torch.nn.ModuleDict({"experts": bad})})
+        with pytest.raises(ValueError, match="b.experts"):
+            converter("MXFP4WeightConverter", "experts").convert(model)
+        assert type(model["a"]["experts"]) is GroupedExperts  # nothing is replaced half way
+    model = torch.nn.ModuleDict({"a": _packed()})
+    assert converter("MXFP4WeightConverter", "a").convert(model) == []  # packed already

@@ -142,6 +142,9 @@ class MXFP8Converter(Configurable):
         pass
 
 
+_PACKED = {GroupedExperts: MXFP4GroupedExperts, GptOssGroupedExperts: MXFP4GptOssGroupedExperts}
+
+
 class _ExpertsConverter(Configurable):
     """Marks the matching GroupedExperts; needs the hardware's block-scaled formats. The kernels
     take ragged token groups, so nothing is padded."""
@@ -158,8 +161,15 @@ class _ExpertsConverter(Configurable):
         self.fqns = _split_fqns(config.fqns)
         self.config = config
 
+    def _matches(self, name: str) -> bool:
+        return bool(name) and any(f in name for f in self.fqns)
+
     def convert(self, model: nn.Module) -> list[str]:
-        """Switches the matching GroupedExperts; returns their names."""
+        """Switches the matching GroupedExperts; returns their names. Matching experts of other
+        classes, which have no such recipe, are refused."""
+        for name, mod in model.named_modules(remove_duplicate=False):
+            if self._matches(name) and isinstance(mod, (GptOssGroupedExperts, *_PACKED.values())):
+                raise ValueError(f"{name}: {type(mod).__name__} cannot be converted to {self.attr}")
         return _mark_experts(model, self.fqns, self.attr)
 
     def post_optimizer_hook(self, model) -> None:
@@ -198,17 +208,22 @@ class MXFP4WeightConverter(_ExpertsConverter):
         pass
 
     def convert(self, model: nn.Module) -> list[str]:
-        packed = {GroupedExperts: MXFP4GroupedExperts, GptOssGroupedExperts: MXFP4GptOssGroupedExperts}
-        converted = []
+        """Replaces the matching experts; returns their names. Subclasses, which may compute something
+        else, and modules with hooks, which would not see the calls any more, are refused."""
+        matching = [(name, mod) for name, mod in model.named_modules(remove_duplicate=False)
+                    if self._matches(name) and isinstance(mod, tuple(_PACKED))]
+        for name, mod in matching:
+            if type(mod) not in _PACKED:
+                raise ValueError(f"{name}: the subclass {type(mod).__name__} has no packed form")
+            if mod._forward_hooks or mod._forward_pre_hooks or mod._backward_hooks or mod._backward_pre_hooks:
+                raise ValueError(f"{name} has hooks, which its packed form would not run: register them after packing")
         made = {}  # of a module that several names share, one
-        for name, mod in list(model.named_modules(remove_duplicate=False)):
-            if name and type(mod) in packed and any(f in name for f in self.fqns):
-                if mod not in made:
-                    made[mod] = packed[type(mod)].from_experts(mod)
-                parent, _, child = name.rpartition(".")
-                setattr(model.get_submodule(parent), child, made[mod])
-                converted.append(name)
-        return converted
+        for name, mod in matching:
+            if mod not in made:
+                made[mod] = _PACKED[type(mod)].from_experts(mod)
+            parent, _, child = name.rpartition(".")
+            setattr(model.get_submodule(parent), child, made[mod])
+        return [name for name, _mod in matching]
 
 
 def find_pad_multiple(converters: list) -> int | None:
