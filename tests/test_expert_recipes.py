@@ -116,3 +116,24 @@ def test_experts_that_cannot_be_packed_are_refused(converter):
         assert type(model["a"]["experts"]) is GroupedExperts  # nothing is replaced half way
     model = torch.nn.ModuleDict({"a": _packed()})
     assert converter("MXFP4WeightConverter", "a").convert(model) == []  # packed already
+
+
+def test_a_checkpoint_goes_in_whole():
+    """load_hf of a checkpoint with something missing or of another shape leaves every weight as it was."""
+    from torchtitan_amd.mxfp4 import MXFP4GptOssGroupedExperts
+
+    m = MXFP4GptOssGroupedExperts.Config(dim=64, hidden_dim=64, num_experts=2).build()
+    at = "model.layers.0.mlp.experts."
+    hf = {}
+    for key, rows in (("gate_up_proj", 128), ("down_proj", 64)):
+        hf |= {f"{at}{key}_blocks": torch.zeros(2, rows, 2, 16, dtype=torch.uint8),
+               f"{at}{key}_scales": torch.zeros(2, rows, 2, dtype=torch.uint8), f"{at}{key}_bias": torch.zeros(2, rows)}
+    m.load_hf(hf, 0)
+    other = {k: v + 1 for k, v in hf.items()}
+    for key in other:
+        for bad in ({k: v for k, v in other.items() if k != key}, {**other, key: other[key][:1]}):
+            with pytest.raises((KeyError, ValueError)):
+                m.load_hf(bad, 0)
+            assert not any(t.any() for t in m.state_dict().values()), key
+    m.load_hf(other, 0)
+    assert all((t == 1).all() for t in m.state_dict().values())

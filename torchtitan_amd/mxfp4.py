@@ -49,14 +49,6 @@ class _Packed(Module):
         """The values of a packed weight."""
         return ops.mxfp4_dequantize(*self.packed(name), dtype)
 
-    def _take_blocks(self, name: str, blocks: torch.Tensor, scales: torch.Tensor) -> None:
-        """A packed weight as checkpoints hold it: blocks [.., K / 32, 16], scales [.., K / 32]."""
-        for kind, t in (("_blocks", blocks.flatten(-2)), ("_scales", scales)):
-            own = getattr(self, name + kind)
-            if t.dtype != torch.uint8 or t.shape != own.shape:
-                raise ValueError(f"{name}{kind}: expected uint8 {list(own.shape)}, got {t.dtype} {list(t.shape)}")
-            setattr(self, name + kind, t.to(own.device).contiguous())
-
     @classmethod
     def _like(cls, experts: Module, config: Module.Config) -> "_Packed":
         """An instance of this config with experts' weights packed."""
@@ -120,14 +112,22 @@ class MXFP4GptOssGroupedExperts(_Packed):
 
     def load_hf(self, hf: dict[str, torch.Tensor], layer: int) -> None:
         """Takes layer `layer`'s experts from a gpt-oss checkpoint as it is, its weights packed
-        (model.layers.L.mlp.experts.{gate_up,down}_proj_{blocks,scales,bias})."""
+        (model.layers.L.mlp.experts.{gate_up,down}_proj_{blocks,scales,bias}): blocks [.., K / 32, 16],
+        scales [.., K / 32]. All of it or, where something is missing or does not fit, nothing."""
+        taken = {}
         for name, key in (("mlp1", "gate_up_proj"), ("mlp2", "down_proj")):
             at = f"model.layers.{layer}.mlp.experts.{key}_"
-            self._take_blocks(name + "_weight", hf[at + "blocks"], hf[at + "scales"])
-            own = getattr(self, name + "_bias")
-            if hf[at + "bias"].shape != own.shape:
-                raise ValueError(f"{at}bias: expected {list(own.shape)}, got {list(hf[at + 'bias'].shape)}")
-            setattr(self, name + "_bias", hf[at + "bias"].to(own.device, torch.bfloat16).contiguous())
+            for own, t in ((f"{name}_weight_blocks", hf[at + "blocks"].flatten(-2)),
+                           (f"{name}_weight_scales", hf[at + "scales"]),
+                           (f"{name}_bias", hf[at + "bias"])):
+                like = getattr(self, own)
+                if t.shape != like.shape or (like.dtype == torch.uint8 and t.dtype != torch.uint8):
+                    raise ValueError(f"{at[:-1]} for {own}: expected {like.dtype} {list(like.shape)}, got {t.dtype} "
+                                     f"{list(t.shape)}")
+                taken[own] = t
+        for own, t in taken.items():
+            like = getattr(self, own)
+            setattr(self, own, t.to(like.device, torch.uint8 if like.dtype == torch.uint8 else torch.bfloat16).contiguous())
 
     def forward(self, x: torch.Tensor, num_tokens_per_expert: torch.Tensor) -> torch.Tensor:
         y = ops.grouped_swiglu_oss_mxfp4(x.bfloat16(), *self.packed("mlp1_weight"), self.mlp1_bias,
