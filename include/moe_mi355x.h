@@ -600,7 +600,8 @@ int moe_scatter_rows(const void* src, const int64_t* idx, int64_t n_rows, int32_
  * ------------------------------------------------------------------------- */
 
 /* h [R,H] = bf16(silu(g) * u) of the fp32 sums g = x.w1^T, u = x.w3^T, and g, u
- * quantized from them in g8, u8 [R,H] with scales [R,H/32] (g8 NULL: only h). */
+ * quantized from them in g8, u8 [R,H], 8-byte aligned, with scales [R,H/32] (g8
+ * NULL: only h). */
 int moe_grouped_gemm_gate_up_keep8(const uint16_t* x, const uint16_t* w1, const uint16_t* w3,
                                    const int64_t* counts, int64_t n_rows, int32_t n_experts, int32_t dim,
                                    int32_t hidden, uint8_t* g8, uint8_t* g8_scale, uint8_t* u8,

@@ -1229,6 +1229,7 @@ MOE_API int moe_grouped_gemm_gate_up_keep8(const uint16_t* x, const uint16_t* w1
   if (st) return st;
   if (n_rows == 0) return kOk;
   if (!x || !w1 || !w3 || !h || (g8 && (!g8_scale || !u8 || !u8_scale))) return kErrInvalidArgument;
+  if (g8 && ((uintptr_t)g8 | (uintptr_t)u8) & 7) return kErrInvalidArgument;
   p.x = x; p.w1 = w1; p.w3 = w3; p.out_h = h;
   p.g8 = g8; p.g8s = g8_scale; p.u8 = u8; p.u8s = u8_scale;
   launch_mode<kFwdGateUp, kSwiGLUKeep8>(p, n_rows, stream);
