@@ -272,14 +272,11 @@ __global__ __launch_bounds__(NW * 64, OCC) void grouped_gemm_kernel(GemmParams p
       cnt[i] = c < 0 ? 0 : (c > p.R ? (int)p.R : (int)c);
     }
     {
+      // cut where they run past R, by sums that stop there: 1024 counts of R wrap 32 bits
       int pre[4];
-      block_exclusive_scan4(cnt, pre, s_tmp);
+      saturating_scan4(cnt, pre, s_tmp, (int)p.R);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int64_t lo = pre[i] < p.R ? pre[i] : p.R;
-        const int64_t hi = (int64_t)pre[i] + cnt[i] < p.R ? (int64_t)pre[i] + cnt[i] : p.R;
-        cnt[i] = (int)(hi - lo);
-      }
+      for (int i = 0; i < 4; ++i) cnt[i] = min(cnt[i], (int)p.R - pre[i]);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {

@@ -236,37 +236,6 @@ __device__ __forceinline__ void for_each(F f) {  // f(0), ..., f(N - 1) with com
 }
 constexpr int kTileList = 64;
 
-// Exclusive prefix sums of up to 1024 non-negative ints, four per thread of the first 256,
-// that stop at `most` (saturating sums are associative, and with most < 2^30 no step passes
-// 2^31 whatever the values). Returns the total. Called by every thread; tmp: one int per wave.
-__device__ __forceinline__ int saturating_scan4(const int (&v)[4], int (&out)[4], int* tmp, int most) {
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, nw = blockDim.x >> 6;
-  auto add = [&](int a, int b) { return min(a + b, most); };
-  const int local = add(add(min(v[0], most), min(v[1], most)), add(min(v[2], most), min(v[3], most)));
-  int incl = local;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int o = __shfl_up(incl, off);
-    if (lane >= off) incl = add(incl, o);
-  }
-  if (lane == 63) tmp[wv] = incl;
-  __syncthreads();
-  int run = 0, total = 0;
-  for (int w = 0; w < nw; ++w) {
-    if (w < wv) run = add(run, tmp[w]);
-    total = add(total, tmp[w]);
-  }
-  __syncthreads();
-  const int before = __shfl_up(incl, 1);
-  if (lane) run = add(run, before);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    out[i] = run;
-    run = add(run, min(v[i], most));
-  }
-  return total;
-}
-
 // Expert e's rows [seg[e], seg[e + 1]), clamped to R, and the exclusive sums of
 // tiles_of(rows) in `tile`, both of E + 1 ints in LDS. Called by every thread of a workgroup of
 // at least 256; negative counts count as none.
