@@ -1,6 +1,7 @@
 // Rows kept in MXFP8 between a forward and its backward (gfx950): e4m3 elements, one e8m0 scale
 // per 32 along the row (mx.h). Streaming kernels, bound by HBM: 3.03 bytes per element each way.
-// 131072 rows of 2304 are kept in 167 us (5.5 TB/s) and restored in 144 us (6.4 TB/s).
+// In a training step 131072 rows of 2304 are kept in 175 us (5.2 TB/s) and restored in 152 us
+// (6.0 TB/s).
 #include "mx.h"
 
 namespace moe {

@@ -29,8 +29,9 @@ __device__ __forceinline__ uint32_t scale_byte(uint32_t amax_bits) {
 __device__ __forceinline__ uint32_t scale_byte4(uint32_t amax_bits) { return scale_byte<0x400000u, 2>(amax_bits); }
 __device__ __forceinline__ uint32_t scale_byte8(uint32_t amax_bits) { return scale_byte<0x600000u, 8>(amax_bits); }
 
-// 2^-k, the elements' multiplier (exact: k <= 126 for finite blocks); 0 for a NaN block,
-// whose elements do not matter, so that none of them becomes a NaN or infinity on the way
+// 2^-k, the elements' multiplier (exact: k <= 126 for finite blocks); 0 for a NaN block, whose
+// scale byte makes all of its values NaN: its codes, conversions of zeros and NaN then, are not
+// defined
 __device__ __forceinline__ float multiplier(uint32_t byte) {
   return byte == 255u ? 0.f : __uint_as_float((254u - byte) << 23);
 }

@@ -74,8 +74,9 @@ __device__ __forceinline__ uint32_t quad_block4(const Eight<T>& x, uint32_t& q) 
 
 // Rows of cpr chunks of eight elements to rows of ocpr >= cpr, zeros behind (ocpr == cpr: one
 // flat run of chunks). Chunk c's codes are the word q[c], its block's scale scale[c / 4]. One
-// pass, bound by HBM (2.53 bytes an element from bf16): 65536 x 2304 in 82 us, 4.7 TB/s, 131072
-// rows 155 us, 5.0 TB/s. Eight elements a lane are one 16-byte load and two lane exchanges a block;
+// pass, bound by HBM (2.53 bytes an element from bf16): 65536 x 2304 in 75 us, 5.1 TB/s (fp32 136
+// us, 5.0), 94 behind a kernel that leaves its own 300 MB in the caches; 131072 rows before the
+// products 166 us. Eight elements a lane are one 16-byte load and two lane exchanges a block;
 // four loads are in flight before the first is used.
 template <typename T>
 __global__ __launch_bounds__(256) void quant_kernel(const T* __restrict__ x, int64_t n_chunks, int cpr, int ocpr,
@@ -126,7 +127,8 @@ __global__ __launch_bounds__(256) void pad_scales_kernel(const uint8_t* __restri
 
 // codes back to values: rows of cpr chunks of eight from rows of icpr >= cpr. A product of a
 // code and a power of two is exact in bf16 too (two bits of mantissa). Bound by HBM, mostly its
-// writes: 65536 x 2304 to bf16 in 62 us, 6.2 TB/s with the codes partly in the cache still.
+// writes: 65536 x 2304 to bf16 in 64 us, 6.0 TB/s, with the codes partly in the cache still, 73
+// without, 5.2 TB/s; to fp32 182 us, 3.8 TB/s.
 template <typename T>
 __global__ __launch_bounds__(256) void dequant_kernel(const uint32_t* __restrict__ q, const uint8_t* __restrict__ scale,
                                                       int64_t n_chunks, int cpr, int icpr, T* __restrict__ x) {
@@ -194,27 +196,24 @@ __device__ __forceinline__ float activation(int act, float g, float u, float lim
 }
 
 #define LDSP __attribute__((address_space(3)))
-// One wave-wide direct-to-LDS copy: lane i's 16 bytes at g land at LDS byte address
-// lds + 16 i; waited for with vmcnt. s_nop: a copy may read m0 one wait state after a scalar
-// instruction wrote it at the earliest, and the compiler, which keeps to that elsewhere, does
-// not look into the asm.
-__device__ __forceinline__ void dma16(const void* g, uint32_t lds) {
-  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(g), "{m0}"(lds) : "memory");
-}
-// The same with lane i's 4 bytes at lds + 4 i; and with its 2 bytes there, zeros above them.
+// One wave-wide direct-to-LDS copy: lane i's 4 bytes at g land at LDS byte address lds + 4 i;
+// waited for with vmcnt. s_nop: a copy may read m0 one wait state after a scalar instruction
+// wrote it at the earliest, and the compiler, which keeps to that elsewhere, does not look into
+// the asm.
 __device__ __forceinline__ void dma4(const void* g, uint32_t lds) {
   asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" :: "v"(g), "{m0}"(lds) : "memory");
 }
+// The same with lane i's 2 bytes there, zeros above them.
 __device__ __forceinline__ void dma2(const void* g, uint32_t lds) {
   asm volatile("s_nop 0\n\tglobal_load_lds_ushort %0, off" :: "v"(g), "{m0}"(lds) : "memory");
 }
 __device__ __forceinline__ uint32_t lds_addr(const uint8_t* ptr) { return (uint32_t)(size_t)((LDSP const uint8_t*)ptr); }
 
-// The same from a scalar base and a 32-bit offset per lane. (readfirstlane: under pressure the
-// compiler keeps uniform values in vector registers, which the instruction does not take there.
-// s_nop: a scalar register that a vector instruction has just written may be read by a memory
-// instruction five wait states later at the earliest, and the compiler, which keeps to that
-// elsewhere, does not look into the asm.)
+// Copies from a scalar base and a 32-bit offset per lane, 16 bytes a lane at lds + 16 i or 4 at
+// lds + 4 i. (readfirstlane: under pressure the compiler keeps uniform values in vector registers,
+// which the instruction does not take there. s_nop: a scalar register that a vector instruction
+// has just written may be read by a memory instruction five wait states later at the earliest;
+// m0's one lies within them.)
 __device__ __forceinline__ uint64_t scalar(const uint8_t* p) {
   const uint64_t v = (uint64_t)p;
   return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)v) |
@@ -389,8 +388,8 @@ __device__ __forceinline__ void store_hidden(const Params& p, int64_t r, int hc,
 // (pad_scales_kernel). gate_up's columns alternate in blocks of 16 between gate and up, so that a
 // lane holds both.
 //
-// What bounds it (131072 rows on 256 experts of 2304 / 1024: gate_up 435 us = 2.8 PFLOP/s, down
-// 300): of a tile's 43000 cycles the MFMAs take 18400 and the LDS reads beside them as many, the
+// What bounds it (131072 rows on 256 experts of 2304 / 1024, call upon call: gate_up 435 us = 2.8
+// PFLOP/s, down 302; 547 and 347 in the first calls after a pause): of a tile's 43000 cycles the MFMAs take 18400 and the LDS reads beside them as many, the
 // epilogue 7500 (an exponential and a reciprocal, at a quarter of the rate, per element). Measured
 // and slower: four waves of 128 x 128 with the fragments a step ahead in registers (569 us: one
 // wave per SIMD leaves the epilogue alone on it), two workgroups of 128 x 256 per CU on 64-byte
@@ -973,7 +972,8 @@ static void launch_narrow(const Params& p, hipStream_t stream) {
 // gpt-oss's 2880 / 2880 8 rows 101 / 152, 16 rows 111 / 156, 24 rows 132 / 159, 50 rows 176 / 168; 32 of 7168 /
 // 2048 8 rows 161 / 191, 12 rows 192 / 194, 16 rows 218 / 198; 16 of 2304 / 1024 16 rows 29 / 32, 24 rows 39 /
 // 33. Small: 8 experts of 2048 / 1408 16 rows 22 / 32; 16 of 320 / 704 19 rows 16 / 24; one of 512 / 512 128
-// rows 13 / 22.
+// rows 13 / 22. One bound in rows fits 256 experts and misses on few wide ones: gpt-oss's cross near
+// 45 rows, and between 21 and there take the wide kernel, 159 us where the narrow one took 132.
 static bool takes_narrow(int64_t R, int64_t E, int D, int H) {
   const int tm = std::min(narrow_blocks(D, E), narrow_blocks(H, E));
   const int64_t cols = 2 * (int64_t)H > D ? 2 * (int64_t)H : D;

@@ -1253,7 +1253,8 @@ def grouped_swiglu_ckpt8(
     tensor of bytes: x [R, D], g and u [R, H] in MXFP8 (e4m3, one e8m0 scale per 32 along the
     row), each followed by its scales: (D + 2H) 33/32 bytes a row instead of 2D + 6H; empty
     without `for_backward`. The gradients are those at the kept values: the activation's at g and
-    u, dw1 and dw3 with x, dw2 with h = silu(g) u. An infinity or NaN makes its block of 32 kept
+    u, dw1 and dw3 with x, dw2 with h = silu(g) u; dg, du and that h are taken in fp32 and rounded
+    to bf16 once for the products that follow. An infinity or NaN makes its block of 32 kept
     values NaN."""
     op = "grouped_swiglu_ckpt8"
     _check_experts(op, x, w1, w2, w3, num_tokens_per_expert, 64)
@@ -1618,8 +1619,8 @@ def grouped_swiglu_mxfp4_train(
     """The SwiGLU experts in MXFP4 from bf16 weights, with gradients: y [R, D] is
     grouped_swiglu_mxfp4's on the packed weights. The backward passes the quantizations
     straight through: it takes the products' gradients at their quantized operands (in bf16,
-    which holds them exactly) and the activation's at g and u kept in MXFP8. Returns y, then
-    what is kept, as one tensor of bytes: w1, w2, w3, x and h in MXFP4 and g, u in MXFP8, each
+    which holds them exactly) and the activation's at g and u kept in MXFP8, in fp32, with dg and du
+    rounded to bf16 once for the products that follow. Returns y, then what is kept, as one tensor of bytes: w1, w2, w3, x and h in MXFP4 and g, u in MXFP8, each
     with its scales. D and H are multiples of 64."""
     op = "grouped_swiglu_mxfp4_train"
     _check_experts(op, x, w1, w2, w3, num_tokens_per_expert, 64)
