@@ -23,7 +23,7 @@ for q s. A product of a row and a weight row (out channel) n is
     y_n = s s_n (q . q_n) + b_n
 
 with a sum of integers, and the activation between two products, silu(g) u or gpt-oss's, is
-quantized from 32 bits.
+quantized from 32 bits; the layers that have one take and return bf16.
 
 Sizes are those of the layers that this repository's benchmark and tests name (dims
 256/512, 2304/1024, 7168/2048, 2880/2880) and generic ones between them.
@@ -90,11 +90,11 @@ def draw(rng) -> dict:
         return dict(kind=kind, rows=_log_int(rng, 1, 16384), dim=dim, out=_log_int(rng, 100, 7000),
                     bias=rng.random() < 0.4, dtype=dtype)
     if kind == "ffn":
-        return dict(kind=kind, rows=_log_int(rng, 1, 16384), dim=dim, hidden=16 * _log_int(rng, 16, 128), dtype=dtype)
+        return dict(kind=kind, rows=_log_int(rng, 1, 16384), dim=dim, hidden=16 * _log_int(rng, 16, 128), dtype="bf16")
     dim = 16 * _log_int(rng, 16, 180)
     top_k = rng.choice([1, 2, 4, 6, 8])
     tail = dict(tokens=_log_int(rng, 1, 65536 // top_k), top_k=top_k, dim=dim, skew=rng.choice([0.0, 0.3, 0.7, 1.0]),
-                spare=rng.choice([0, 0, _log_int(rng, 1, 300)]), dtype=dtype)
+                spare=rng.choice([0, 0, _log_int(rng, 1, 300)]), dtype="bf16" if kind == "experts" else dtype)
     if kind == "grouped":
         return dict(kind=kind, out=_log_int(rng, 100, 2880), experts=rng.choice([8, 32, 48, 64, 128]),
                     bias=rng.random() < 0.4, **tail)
