@@ -93,13 +93,13 @@ def draw(rng) -> dict:
         return dict(kind=kind, rows=_log_int(rng, 1, 16384), dim=dim, hidden=16 * _log_int(rng, 16, 128), dtype="bf16")
     dim = 16 * _log_int(rng, 16, 180)
     top_k = rng.choice([1, 2, 4, 6, 8])
-    tail = dict(tokens=_log_int(rng, 1, 65536 // top_k), top_k=top_k, dim=dim, skew=rng.choice([0.0, 0.3, 0.7, 1.0]),
+    tail = dict(tokens=_log_int(rng, 1, 49152 // top_k), top_k=top_k, dim=dim, skew=rng.choice([0.0, 0.3, 0.7, 1.0]),
                 spare=rng.choice([0, 0, _log_int(rng, 1, 300)]), dtype="bf16" if kind == "experts" else dtype)
     if kind == "grouped":
         return dict(kind=kind, out=_log_int(rng, 100, 2880), experts=rng.choice([8, 32, 48, 64, 128]),
                     bias=rng.random() < 0.4, **tail)
     act = rng.choice(["silu", "silu", "oss"])
-    return dict(kind=kind, act=act, hidden=16 * _log_int(rng, 16, 180),
+    return dict(kind=kind, act=act, hidden=16 * _log_int(rng, 16, 128),
                 experts=rng.choice([8, 32, 48, 64, 128]) if act == "silu" else 32, **tail)
 
 
