@@ -688,6 +688,56 @@ int moe_mxfp4_gemm_down(const uint8_t* qh, const uint8_t* sh, const uint8_t* qw2
                         const int64_t* counts, int64_t n_rows, int32_t n_experts, int32_t dim, int32_t hidden,
                         uint16_t* y, moe_stream_t stream);
 
+/* ---------------------------------------------------------------------------
+ * 8-bit integers, for inference: rows (of activations: tokens; of weights: output
+ * channels) in int8 codes with one fp32 scale each. With a = max(max |v|,
+ * 127 * 2^-126) and the fp32 quotients r = 127 / a, s = a / 127 a row's codes are
+ * v * r rounded once to the nearest integer, ties to even, and stand for code * s; a
+ * row with an infinity or a NaN gets the scale NaN and zero codes. Products sum codes
+ * in 32-bit integers (exactly) and scale the sums in fp32. Contractions are multiples
+ * of 16 up to 131072, experts 1 to 1024; x, codes of weights, workspace and outputs
+ * 16-byte aligned.
+ * ------------------------------------------------------------------------- */
+
+/* x [rows, cols] (dtype MOE_DTYPE_BF16 or MOE_DTYPE_FP32), rows ld >= cols elements
+ * apart -> q [rows, cols], scale [rows], and back (x [rows, cols] in dtype). Any cols
+ * and alignment; 16-byte aligned rows of a multiple of 8 columns are read in wide
+ * pieces. */
+int moe_int8_quant_rows(const void* x, int64_t ld, int64_t rows, int32_t cols, int32_t dtype, int8_t* q, float* scale,
+                        moe_stream_t stream);
+int moe_int8_dequant_rows(const int8_t* q, const float* scale, int64_t rows, int32_t cols, int32_t dtype, void* x,
+                          moe_stream_t stream);
+
+/* Bytes of workspace of moe_int8_linear (0: none is taken). */
+int64_t moe_int8_linear_workspace_bytes(int64_t n_rows, int32_t n_experts, int32_t in_features);
+
+/* y [R, out_features] = x.w^T + bias in x's dtype: x [R, in_features] (bf16 or fp32) is
+ * quantized on the way; w = qw [E, out, in] with sw [E, out]; bias [E, out] in bias_dtype or
+ * NULL. Rows are sorted by expert, counts [E]; rows past sum(counts) are zero. counts NULL:
+ * one expert (n_experts == 1) with all rows. */
+int moe_int8_linear(const void* x, int32_t dtype, const int8_t* qw, const float* sw, const void* bias,
+                    int32_t bias_dtype, const int64_t* counts, int64_t n_rows, int32_t n_experts, int32_t in_features,
+                    int32_t out_features, uint8_t* workspace, int64_t workspace_bytes, void* y, moe_stream_t stream);
+
+/* Bytes of workspace of moe_int8_swiglu and moe_int8_oss. */
+int64_t moe_int8_layer_workspace_bytes(int64_t n_rows, int32_t n_experts, int32_t dim, int32_t hidden);
+
+/* x [R,D] bf16, counts as above: h = silu(x.w1^T) * (x.w3^T) in fp32, quantized,
+ * y = bf16(h.w2^T) [R,D]; qw1, qw3 [E,H,D], qw2 [E,D,H] with scales [E,H] and [E,D]. */
+int moe_int8_swiglu(const uint16_t* x, const int8_t* qw1, const float* sw1, const int8_t* qw2, const float* sw2,
+                    const int8_t* qw3, const float* sw3, const int64_t* counts, int64_t n_rows, int32_t n_experts,
+                    int32_t dim, int32_t hidden, uint8_t* workspace, int64_t workspace_bytes, uint16_t* y,
+                    moe_stream_t stream);
+
+/* The same with gpt-oss's experts (gpt_oss/moe.py:43-122): qmlp1 [E,2H,D] (glu row 2j,
+ * linear row 2j + 1), biases [E,2H] and [E,D] in bias_dtype, all in fp32 between the
+ * products: g = min(glu + b, L), u = clamp(linear + b, -L, L),
+ * h = g * sigmoid(1.702 g) * (u + 1), quantized, y = bf16(h.mlp2^T + b2). */
+int moe_int8_oss(const uint16_t* x, const int8_t* qmlp1, const float* smlp1, const void* mlp1_bias, const int8_t* qmlp2,
+                 const float* smlp2, const void* mlp2_bias, int32_t bias_dtype, const int64_t* counts, int64_t n_rows,
+                 int32_t n_experts, int32_t dim, int32_t hidden, float swiglu_limit, uint8_t* workspace,
+                 int64_t workspace_bytes, uint16_t* y, moe_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -109,9 +109,17 @@ SIGNATURES: dict[str, list] = {
     "moe_ep_permute_pad_indices": [P, I32, I32, I32, I64, P, P, P, P],
     "moe_gather_rows": [P, I64, P, I64, I32, I32, P, P],
     "moe_scatter_rows": [P, P, I64, I32, I32, P, I64, P],
+    "moe_int8_quant_rows": [P, I64, I64, I32, I32, P, P, P],
+    "moe_int8_dequant_rows": [P, P, I64, I32, I32, P, P],
+    "moe_int8_linear_workspace_bytes": [I64, I32, I32],
+    "moe_int8_linear": [P, I32, P, P, P, I32, P, I64, I32, I32, I32, P, I64, P, P],
+    "moe_int8_layer_workspace_bytes": [I64, I32, I32, I32],
+    "moe_int8_swiglu": [P, P, P, P, P, P, P, P, I64, I32, I32, I32, P, I64, P, P],
+    "moe_int8_oss": [P, P, P, P, P, P, P, I32, P, I64, I32, I32, I32, F32, P, I64, P, P],
 }
 _RESTYPES = {"moe_reorder_workspace_bytes": ctypes.c_int64, "moe_fp8_padded_rows": ctypes.c_int64,
-             "moe_mxfp8_padded_rows": ctypes.c_int64, "moe_mxfp4_workspace_bytes": ctypes.c_int64}
+             "moe_mxfp8_padded_rows": ctypes.c_int64, "moe_mxfp4_workspace_bytes": ctypes.c_int64,
+             "moe_int8_linear_workspace_bytes": ctypes.c_int64, "moe_int8_layer_workspace_bytes": ctypes.c_int64}
 
 _ERRORS = {
     -1: "invalid argument",

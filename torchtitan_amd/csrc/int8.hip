@@ -1,0 +1,946 @@
+// 8-bit integers on MI355X (gfx950): rows to codes with a scale each, and products of such rows
+// with packed weights, dense or grouped by expert, alone or as the SwiGLU layers.
+//
+// For a row v with a = max(max |v|, 127 * 2^-126), the fp32 numbers r = 127 / a and s = a / 127
+// (so that neither leaves the normal range), the codes are q = v r rounded once to the nearest
+// integer, ties to even, |q| <= 127, and stand for q s. A row with an infinity or a NaN has the
+// scale NaN and zero codes. For the rows of expert e (sorted by expert, counts [E] on the device;
+// a dense product has one expert with all rows) and weight rows n, quantized the same way:
+//
+//   linear    y_n = s s_n (q . q_n) + b_n, written in bf16 or fp32:      rows x N, k = K
+//   gate_up   g, u as y of w1 and w3, h = act(g, u), written in fp32:    rows x 2H, k = D
+//
+// with act(g, u) = silu(g) u, or gpt-oss's on interleaved rows with biases:
+//   g' = min(g + b, L), u' = clamp(u + b, -L, L), g' sigmoid(1.702 g') (u' + 1).
+//
+// v_mfma_i32_16x16x64_i8: lane (row, q), q = lane / 16, holds 16 consecutive k of its row; the sums
+// are exact (K <= 131072: 2^17 * 127 * 128 < 2^31).
+#include <algorithm>
+
+#include "grouped.h"
+#include "mx.h"
+
+namespace moe {
+namespace int8 {
+
+using namespace grouped;
+
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
+
+constexpr int kMaxK = 131072;
+constexpr float kLeast = 127.0f * 0x1p-126f;
+
+// The columns of a row operand: whole stages of 128, so that every copy of a stage lies inside
+// its row, and zeros behind the contraction meet whatever is read of a weight row there.
+__host__ __device__ constexpr int padded(int cols) { return (cols + 127) / 128 * 128; }
+
+// ---------------------------------------------------------------------------
+// quantization and its inverse
+// ---------------------------------------------------------------------------
+
+// Eight elements of a bf16 or fp32 row.
+template <typename T> struct Eight;
+template <> struct Eight<uint16_t> {
+  uint4 v;
+  __device__ __forceinline__ void load(const uint16_t* p) { v = *(const uint4*)p; }
+  __device__ __forceinline__ void zero() { v = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ void get(float (&a)[8]) const { Chunk<uint16_t>::unpack(v, a); }
+};
+template <> struct Eight<float> {
+  float4 lo, hi;
+  __device__ __forceinline__ void load(const float* p) { lo = *(const float4*)p; hi = *(const float4*)(p + 4); }
+  __device__ __forceinline__ void zero() { lo = hi = make_float4(0.f, 0.f, 0.f, 0.f); }
+  __device__ __forceinline__ void get(float (&a)[8]) const {
+    a[0] = lo.x; a[1] = lo.y; a[2] = lo.z; a[3] = lo.w;
+    a[4] = hi.x; a[5] = hi.y; a[6] = hi.z; a[7] = hi.w;
+  }
+};
+template <typename T>
+__device__ __forceinline__ uint32_t amax8(const Eight<T>& e) {
+  float a[8];
+  e.get(a);
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, mx::abs_bits(a[i]));
+  return m;
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, off));
+  return v;
+}
+
+// A row's multiplier and scale from the bits of its max |v| taken over integers (bits of |v| order
+// as the values do, with infinities and NaN on top). r = 0 stands for a row without a scale.
+struct RowScale { float r, s; };
+__device__ __forceinline__ RowScale row_scale(uint32_t amax_bits) {
+  if (amax_bits >= 0x7f800000u) return {0.f, __uint_as_float(0x7fc00000u)};
+  const float a = fmaxf(__uint_as_float(amax_bits), kLeast);
+  return {127.0f / a, a / 127.0f};
+}
+// v r rounded once: the fused sum with 1.5 * 2^23, whose unit in the last place is 1, has the code
+// in its low byte (two's complement; the constant is even, so ties go to even codes).
+__device__ __forceinline__ uint32_t code(float v, float r) { return __float_as_uint(fmaf(v, r, 12582912.0f)); }
+__device__ __forceinline__ uint32_t codes4(const float* v, float r) {
+  const uint32_t lo = __builtin_amdgcn_perm(code(v[1], r), code(v[0], r), 0x0c0c0400u);
+  const uint32_t hi = __builtin_amdgcn_perm(code(v[3], r), code(v[2], r), 0x04000c0cu);
+  return lo | hi;
+}
+template <typename T>
+__device__ __forceinline__ uint2 codes8(const Eight<T>& e, float r) {
+  float v[8];
+  e.get(v);
+  return r == 0.f ? make_uint2(0, 0) : make_uint2(codes4(v, r), codes4(v + 4, r));
+}
+
+// Rows of cols elements, ld apart, to rows of q_cols >= cols codes, zeros behind. W waves a row,
+// up to 8 chunks of eight elements a lane in registers between the maximum and the codes; longer
+// rows are read again.
+template <typename T, int W>
+__global__ __launch_bounds__(256) void quant_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int cols,
+                                                    int q_cols, int8_t* __restrict__ q, float* __restrict__ scale) {
+  constexpr int C = 8;
+  __shared__ uint32_t s_max[4];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, sub = W == 1 ? 0 : wv;
+  const int64_t row = W == 1 ? (int64_t)workgroup() * 4 + wv : (int64_t)workgroup();
+  if (row >= rows) return;  // (W == 4: of the whole workgroup)
+  const T* xr = x + row * ld;
+  const int cpr = cols / 8, c0 = sub * 64 + lane;
+  Eight<T> v[C];
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < C; ++i) {
+    const int c = c0 + i * 64 * W;
+    if (c < cpr) v[i].load(xr + 8 * (int64_t)c);
+    else v[i].zero();
+  }
+#pragma unroll
+  for (int i = 0; i < C; ++i) m = max(m, amax8(v[i]));
+  for (int c = c0 + C * 64 * W; c < cpr; c += 64 * W) {
+    Eight<T> e;
+    e.load(xr + 8 * (int64_t)c);
+    m = max(m, amax8(e));
+  }
+  m = wave_max(m);
+  if (W > 1) {
+    if (lane == 0) s_max[wv] = m;
+    __syncthreads();
+    m = max(max(s_max[0], s_max[1]), max(s_max[2], s_max[3]));
+  }
+  const RowScale rs = row_scale(m);
+  int8_t* qr = q + row * (int64_t)q_cols;
+#pragma unroll
+  for (int i = 0; i < C; ++i) {
+    const int c = c0 + i * 64 * W;
+    if (c < cpr) *(uint2*)(qr + 8 * (int64_t)c) = codes8(v[i], rs.r);
+  }
+  for (int c = c0 + C * 64 * W; c < cpr; c += 64 * W) {
+    Eight<T> e;
+    e.load(xr + 8 * (int64_t)c);
+    *(uint2*)(qr + 8 * (int64_t)c) = codes8(e, rs.r);
+  }
+  for (int c = cpr + c0; c < q_cols / 8; c += 64 * W) *(uint2*)(qr + 8 * (int64_t)c) = make_uint2(0, 0);
+  if (lane == 0 && sub == 0) scale[row] = rs.s;
+}
+
+__device__ __forceinline__ float element(const uint16_t* p) { return bf2f(*p); }
+__device__ __forceinline__ float element(const float* p) { return *p; }
+
+// Rows whose pieces of eight are not aligned: an element at a time, a wave a row.
+template <typename T>
+__global__ __launch_bounds__(256) void quant_any_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int cols,
+                                                        int8_t* __restrict__ q, float* __restrict__ scale) {
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)workgroup() * 4 + (threadIdx.x >> 6);
+  if (row >= rows) return;
+  const T* xr = x + row * ld;
+  uint32_t m = 0;
+  for (int c = lane; c < cols; c += 64) m = max(m, mx::abs_bits(element(xr + c)));
+  const RowScale rs = row_scale(wave_max(m));
+  int8_t* qr = q + row * (int64_t)cols;
+  for (int c = lane; c < cols; c += 64) qr[c] = rs.r == 0.f ? (int8_t)0 : (int8_t)code(element(xr + c), rs.r);
+  if (lane == 0) scale[row] = rs.s;
+}
+
+__device__ __forceinline__ void put(uint16_t* p, float v) { *p = (uint16_t)f2bf(v); }
+__device__ __forceinline__ void put(float* p, float v) { *p = v; }
+
+// Codes back to values: a wave a row, in pieces of eight where they are aligned.
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void dequant_kernel(const int8_t* __restrict__ q, const float* __restrict__ scale,
+                                                      int64_t rows, int cols, T* __restrict__ x) {
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)workgroup() * 4 + (threadIdx.x >> 6);
+  if (row >= rows) return;
+  const float s = scale[row];
+  const int8_t* qr = q + row * (int64_t)cols;
+  T* xr = x + row * (int64_t)cols;
+  if constexpr (VEC) {
+    for (int c = lane; c < cols / 8; c += 64) {
+      const uint2 w = *(const uint2*)(qr + 8 * (int64_t)c);
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] = (float)(int8_t)(w.x >> (8 * i)) * s;
+        v[4 + i] = (float)(int8_t)(w.y >> (8 * i)) * s;
+      }
+      if constexpr (sizeof(T) == 2) {
+        *(uint4*)(xr + 8 * (int64_t)c) = Chunk<uint16_t>::pack(v);
+      } else {
+        *(float4*)(xr + 8 * (int64_t)c) = make_float4(v[0], v[1], v[2], v[3]);
+        *(float4*)(xr + 8 * (int64_t)c + 4) = make_float4(v[4], v[5], v[6], v[7]);
+      }
+    }
+  } else {
+    for (int c = lane; c < cols; c += 64) put(xr + c, (float)qr[c] * s);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// products
+// ---------------------------------------------------------------------------
+enum Mode : int { kGateUp = 0, kLinear = 1 };
+enum Act : int { kSwiGLU = 0, kOssGLU = 1 };
+constexpr float kOssAlpha = 1.702f;
+
+struct Params {
+  const int64_t* counts;  // [E]; null: one expert with all rows
+  int64_t R;              // rows; segments are clamped to them
+  int E, K, N;            // contraction, and the output's columns (gate_up: H)
+  const void* x;          // narrow: the rows [R, K] in bf16 or (x_f32) fp32
+  int x_f32;
+  const int8_t* q;        // wide: rows of padded(K) codes, zeros past K, and their scales
+  const float* s;
+  const int8_t* wa;       // weights: gate rows, or linear's
+  const float* sa;
+  const int8_t* wb;       // up rows
+  const float* sb;
+  int64_t e_rows;         // row n of expert e is row e * e_rows + n * r_rows of wa and wb
+  int r_rows;
+  const void* bias;       // in bf16 or (bias_f32) fp32: linear [E, N] or null, gpt-oss's b1 [E, 2H] (glu 2j, linear 2j + 1)
+  int bias_f32;
+  float limit;
+  float* h;               // gate_up: [R, N]
+  void* y;                // linear: [R, N] in bf16 or (y_f32) fp32; rows past the last expert's are zeroed
+  int y_f32;
+};
+
+__device__ __forceinline__ int64_t count_of(const Params& p, int e) { return p.counts ? p.counts[e] : p.R; }
+
+// sigmoid(z) = 1 / (1 + 2^t), t = -z log2 e, on the hardware's exponential and reciprocal (each
+// within a unit of the last place). t's rounding, which 2^t would magnify by |t|, is made good: the
+// result feeds a rounding to codes, which moves with every unit here.
+__device__ __forceinline__ float sigmoid(float z) {
+  constexpr float kL = -1.44269504088896341f, kLow = -1.44269504088896341 - (double)-1.44269504088896341f;
+  const float t = z * kL, lo = fmaf(z, kL, -t) + z * kLow;
+  const float e = __builtin_amdgcn_exp2f(t);
+  return __builtin_amdgcn_rcpf(1.0f + (e < 1e30f ? fmaf(e * 0.693147180559945309f, lo, e) : e));
+}
+__device__ __forceinline__ float activation(int act, float g, float u, float limit) {
+  if (act == kSwiGLU) return g * sigmoid(g) * u;
+  const float a = g > limit ? limit : g, b = u < -limit ? -limit : (u > limit ? limit : u);  // NaN passes
+  return a * sigmoid(kOssAlpha * a) * (b + 1.0f);
+}
+
+__device__ __forceinline__ float bias_at(const Params& p, int64_t i) {
+  return p.bias_f32 ? ((const float*)p.bias)[i] : bf2f(((const uint16_t*)p.bias)[i]);
+}
+// scales of weight rows n .. n + 3 of expert e, linear's biases (the last row's past the end)
+__device__ __forceinline__ void col_scales(const float* s, const Params& p, int e, int n, float (&v)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = s[e * p.e_rows + (int64_t)min(n + i, p.N - 1) * p.r_rows];
+}
+__device__ __forceinline__ void col_bias(const Params& p, int e, int n, float (&v)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = p.bias ? bias_at(p, (int64_t)e * p.N + min(n + i, p.N - 1)) : 0.f;
+}
+// gpt-oss's biases of columns n .. n + 3: glu and linear
+__device__ __forceinline__ void glu_bias(const Params& p, int e, int n, float (&a)[4], float (&b)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t at = ((int64_t)e * p.N + min(n + i, p.N - 1)) * 2;
+    a[i] = bias_at(p, at);
+    b[i] = bias_at(p, at + 1);
+  }
+}
+
+// columns n .. n + 3 of row r of y
+__device__ __forceinline__ void store4(const Params& p, int64_t r, int n, const float (&v)[4]) {
+  if (p.y_f32) {
+    float* y = (float*)p.y + r * p.N + n;
+    if (p.N % 4 == 0) {
+      if (n < p.N) *(float4*)y = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) if (n + i < p.N) y[i] = v[i];
+    }
+  } else {
+    uint16_t* y = (uint16_t*)p.y + r * p.N + n;
+    if (p.N % 4 == 0) {
+      if (n < p.N) *(uint2*)y = pack4(v);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) if (n + i < p.N) y[i] = (uint16_t)f2bf(v[i]);
+    }
+  }
+}
+// rows [from, R) of y zeroed by all workgroups together
+__device__ __forceinline__ void zero_rest(const Params& p, int from) {
+  const int64_t S = (int64_t)gridDim.x * blockDim.x, i0 = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  const int es = p.y_f32 ? 4 : 2;
+  const int64_t at = (int64_t)from * p.N * es, n = (p.R - from) * p.N * es;
+  uint8_t* y = (uint8_t*)p.y + at;
+  if (at % 16 == 0 && n % 16 == 0)
+    for (int64_t i = i0; i < n / 16; i += S) ((uint4*)y)[i] = make_uint4(0, 0, 0, 0);
+  else
+    for (int64_t i = i0; i < n / 2; i += S) ((uint16_t*)y)[i] = 0;
+}
+
+// Many rows per expert: tiles of BM rows x BN columns by WM x WN waves of 16 TM x 16 TN, k in stages
+// of 128 (a cache line), two stages in LDS, persistent workgroups. Operands reach LDS by
+// direct-to-LDS copies, a stage ahead and across tile boundaries. gate_up's columns alternate in
+// blocks of 16 between gate and up, so that a lane holds both.
+template <int MODE, int ACT, int WM, int WN, int TM, int TN>
+__global__ __launch_bounds__(64 * WM * WN, 2) void wide_kernel(Params p) {
+  constexpr int NW = WM * WN, BM = 16 * WM * TM, BN = 16 * WN * TN;
+  constexpr int RB = 128, RPC = 8, CPR = 8;                // bytes of a stage's row; rows of a 1 KB copy; chunks of a row
+  constexpr int PW = BM / RPC / NW, QC = BN / RPC / NW;    // a wave's copies a stage: of P, of Q
+  constexpr int NCOPY = PW + QC, GM = 8;
+  static_assert(PW * RPC * NW == BM && QC * RPC * NW == BN && TN % 2 == 0 && 64 * NW >= 256, "whole copies");
+  __shared__ __attribute__((aligned(1024))) uint8_t sP[2][BM * RB];
+  __shared__ __attribute__((aligned(1024))) uint8_t sQ[2][BN * RB];
+  __shared__ int4 s_list[kTileList];  // this workgroup's first tiles: first row, end of the segment, expert, column tile
+  __shared__ int s_tmp[NW];
+  extern __shared__ __attribute__((aligned(16))) int s_dyn_i[];
+  int* s_seg = s_dyn_i;           // E + 1
+  int* s_tile = s_seg + p.E + 1;  // E + 1
+
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wv / WN, wn = wv % WN, ml = lane & 15, g4 = lane >> 4;
+  const int E = p.E, K = p.K, N = p.N, KC = K / 16;
+  const int NT = MODE == kGateUp ? (N + BN / 2 - 1) / (BN / 2) : (N + BN - 1) / BN;
+  const int nk = (K + RB - 1) / RB;
+  segments(p, s_seg, s_tile, s_tmp, [&](int rows) { return (rows + BM - 1) / BM * NT; });
+  const int total_tiles = s_tile[E], G = gridDim.x;
+  // each XCD works on a contiguous window of tiles
+  const int lb = G % 8 == 0 ? (int)(blockIdx.x & 7) * (G >> 3) + (int)(blockIdx.x >> 3) : (int)blockIdx.x;
+
+  // An expert's tiles run over its rows first, in groups of GM row tiles, so that the tiles that an
+  // XCD works on at a time share rows and columns.
+  auto search = [&](int t) {
+    const int e = find(s_tile, E, t), local = t - s_tile[e], seg0 = s_seg[e], seg1 = s_seg[e + 1];
+    const int mtiles = (seg1 - seg0 + BM - 1) / BM, grp = local / (GM * NT), gm = min(GM, mtiles - grp * GM);
+    const int in = local - grp * GM * NT, nt = in / gm;
+    return make_int4(seg0 + (grp * GM + in - nt * gm) * BM, seg1, e, nt);
+  };
+  if (tid < kTileList && lb + (int64_t)tid * G < total_tiles) s_list[tid] = search(lb + tid * G);
+  __syncthreads();
+  struct TileRef { int row0, seg1, e, nt; };
+  auto decode = [&](int i) {  // this workgroup's i-th tile
+    int4 v;
+    if (i < kTileList) v = s_list[i];
+    else v = search(lb + i * G);
+    return TileRef{__builtin_amdgcn_readfirstlane(v.x), __builtin_amdgcn_readfirstlane(v.y),
+                   __builtin_amdgcn_readfirstlane(v.z), __builtin_amdgcn_readfirstlane(v.w)};
+  };
+  const int my_tiles = lb < total_tiles ? (total_tiles - lb + G - 1) / G : 0;
+
+  // ---- copies. One fills RPC rows, lane i row i / 8, chunk i % 8 with the row's chunk
+  // (i % 8) ^ ((row >> 1) & 7) (eight lanes that read one chunk of eight rows meet no bank
+  // twice). Rows past a segment or the last column repeat the last one inside (what they give is
+  // not stored), chunks past a weight row's end the last one of the row (the other operand has
+  // zeros there), and behind the last stage of a workgroup the last tile's first is copied once
+  // more. ----
+  auto swz = [](int row) { return (row >> 1) & 7; };
+  auto q_col = [](int n) { return MODE == kGateUp ? (n >> 5) * 16 + (n & 15) : n; };  // in the tile's columns
+  const int p_ld = padded(K);
+  const uint8_t *baseP, *baseQ[2];  // of the tile being copied: P, gate (or linear) and up
+  uint32_t offP[PW], offQ[QC];
+  auto setup = [&](const TileRef& r) {
+    int ln = lane;
+    asm volatile("" : "+v"(ln));  // what a tile's offsets come from is made again, not kept in registers
+    const int crow = ln / CPR, cbit = ln % CPR;
+    const int last = r.seg1 - 1 - r.row0, col0 = r.nt * (MODE == kGateUp ? BN / 2 : BN), last_col = N - 1 - col0;
+    baseP = (const uint8_t*)p.q + (int64_t)r.row0 * p_ld;
+    const int64_t wr = r.e * p.e_rows + (int64_t)col0 * p.r_rows;
+    baseQ[0] = (const uint8_t*)p.wa + wr * K;
+    if (MODE == kGateUp) baseQ[1] = (const uint8_t*)p.wb + wr * K;
+#pragma unroll
+    for (int b = 0; b < PW; ++b) {
+      const int m = (wv * PW + b) * RPC + crow;
+      offP[b] = __umul24(min(m, last), p_ld) + (cbit ^ swz(m)) * 16;
+    }
+#pragma unroll
+    for (int b = 0; b < QC; ++b)
+      offQ[b] = __umul24(min(q_col((wv * QC + b) * RPC + crow), last_col), p.r_rows * K);
+  };
+  auto copy = [&](auto c_c, int kt, int s) {  // copy c of stage kt into buffer s
+    constexpr int c = decltype(c_c)::value;
+    if constexpr (c < PW) {
+      dma16(baseP + kt * RB, offP[c], lds_addr(&sP[s][(wv * PW + c) * 1024]));
+    } else {
+      constexpr int b = c - PW;
+      const uint8_t* base = MODE == kGateUp && (((wv * QC + b) * RPC >> 4) & 1) ? baseQ[1] : baseQ[0];
+      const int chunk = min(kt * CPR + (lane % CPR ^ swz((wv * QC + b) * RPC + lane / CPR)), KC - 1);
+      dma16(base, offQ[b] + chunk * 16, lds_addr(&sQ[s][(wv * QC + b) * 1024]));
+    }
+  };
+  int ct = 0, ik = 0, bi = 0, bc = 0;  // copy cursor: tile ct, its stage ik, buffer bi; the buffer bc that is read next
+  auto advance = [&]() {
+    bi ^= 1;
+    if (++ik == nk) {
+      ik = 0;
+      if (++ct < my_tiles) setup(decode(ct));
+    }
+  };
+  if (my_tiles) {
+    setup(decode(0));
+    for_each<NCOPY>([&](auto c) { copy(c, 0, 0); });
+  }
+
+  for (int t = 0; t < my_tiles; ++t) {
+    const TileRef cur = decode(t);
+    const int row0 = cur.row0, seg1 = cur.seg1;
+    // the stage that is read next has landed (its copies are the last there are; an epilogue's
+    // stores are waited for too), and every read of the buffer that is filled next is done
+    auto stage_in = [&]() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+    // 16-row blocks of this wave with rows in them; a wave without any only copies
+    const int tmv = min(TM, max(0, (seg1 - (row0 + wm * TM * 16) + 15) >> 4));
+    if (tmv == 0) {
+      for (int kt = 0; kt < nk; ++kt) {
+        advance();
+        stage_in();
+        bc ^= 1;
+        for_each<NCOPY>([&](auto c) { copy(c, ik, bi); });
+      }
+      continue;
+    }
+    i32x4_t acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) acc[i][j] = i32x4_t{0, 0, 0, 0};
+
+    for (int kt = 0; kt < nk; ++kt) {
+      advance();  // ahead of the MFMAs, which the compiler would otherwise sink behind its branches
+      stage_in();
+      const uint8_t *cP = sP[bc], *cQ = sQ[bc];
+      bc ^= 1;
+      auto frag = [&](const uint8_t* tile, int row, int step) {
+        return *(const i32x4_t*)(tile + row * RB + (((2 * g4 + step) ^ swz(row)) << 4));
+      };
+      i32x4_t af[TM], bq[2];
+      // the next stage's copies go between the MFMAs
+      auto step = [&](auto s_c) {
+        constexpr int st = decltype(s_c)::value;
+#pragma unroll
+        for (int i = 0; i < TM; ++i) af[i] = frag(cP, (wm * TM + i) * 16 + ml, st);
+        bq[0] = frag(cQ, wn * TN * 16 + ml, st);
+        for_each<TN>([&](auto j_c) {
+          constexpr int j = decltype(j_c)::value;
+          if constexpr (j + 1 < TN) bq[(j + 1) & 1] = frag(cQ, (wn * TN + j + 1) * 16 + ml, st);
+#pragma unroll
+          for (int i = 0; i < TM; ++i)
+            acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bq[j & 1], af[i], acc[i][j], 0, 0, 0);
+          constexpr int slot = st * TN + j, slots = 2 * TN;
+          for_each<NCOPY>([&](auto c) {
+            if constexpr (decltype(c)::value * slots / NCOPY == slot) copy(c, ik, bi);
+          });
+          __builtin_amdgcn_sched_barrier(0);
+        });
+      };
+      step(std::integral_constant<int, 0>{});
+      step(std::integral_constant<int, 1>{});
+    }
+
+    // ---- epilogue: lane holds C[m = .. + ml][n = .. + 4 g4 .. + 3] of each 16-column block ----
+    float rs[TM];
+#pragma unroll
+    for (int i = 0; i < TM; ++i) rs[i] = p.s[min(row0 + (wm * TM + i) * 16 + ml, seg1 - 1)];
+#pragma unroll
+    for (int b = 0; b < TN / 2; ++b) {
+      float ca[4], cb[4], ba[4], bb[4];
+      if (MODE == kGateUp) {
+        const int hc = cur.nt * (BN / 2) + wn * (TN * 8) + b * 16 + 4 * g4;
+        if (hc - 4 * g4 >= N) continue;
+        col_scales(p.sa, p, cur.e, hc, ca);
+        col_scales(p.sb, p, cur.e, hc, cb);
+        if constexpr (ACT == kOssGLU) glu_bias(p, cur.e, hc, ba, bb);
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+          if (i >= tmv) continue;
+          const int r = row0 + (wm * TM + i) * 16 + ml;
+          float v[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            float g = (float)acc[i][2 * b][k] * rs[i] * ca[k], u = (float)acc[i][2 * b + 1][k] * rs[i] * cb[k];
+            if constexpr (ACT == kOssGLU) { g += ba[k]; u += bb[k]; }
+            v[k] = activation(ACT, g, u, p.limit);
+          }
+          if (r < seg1) *(float4*)(p.h + (int64_t)r * N + hc) = make_float4(v[0], v[1], v[2], v[3]);
+        }
+      } else {
+        const int n0 = cur.nt * BN + wn * TN * 16 + b * 32;
+        if (n0 >= N) continue;
+        col_scales(p.sa, p, cur.e, n0 + 4 * g4, ca);
+        col_scales(p.sa, p, cur.e, n0 + 16 + 4 * g4, cb);
+        col_bias(p, cur.e, n0 + 4 * g4, ba);
+        col_bias(p, cur.e, n0 + 16 + 4 * g4, bb);
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+          if (i >= tmv) continue;
+          const int r = row0 + (wm * TM + i) * 16 + ml;
+          float lo[4], hi[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            lo[k] = (float)acc[i][2 * b][k] * rs[i] * ca[k] + ba[k];
+            hi[k] = (float)acc[i][2 * b + 1][k] * rs[i] * cb[k] + bb[k];
+          }
+          if (p.y_f32 || N % 8) {
+            if (r < seg1) {
+              store4(p, r, n0 + 4 * g4, lo);
+              store4(p, r, n0 + 16 + 4 * g4, hi);
+            }
+          } else {
+            const uint4 v = span64(pack4(lo), pack4(hi), lane);
+            if (r < seg1 && n0 + 8 * g4 < N) *(uint4*)((uint16_t*)p.y + (int64_t)r * N + n0 + 8 * g4) = v;
+          }
+        }
+      }
+    }
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the last copies write LDS that is not this workgroup's later
+  if (MODE == kLinear) zero_rest(p, s_seg[E]);
+}
+
+// Few rows per expert: the weights are read once and decide the time, so every byte goes straight
+// from memory into the MFMAs' registers. A unit is NB blocks of 16 weight rows (gate_up: 8 gate and
+// 8 up rows each) by up to 16 TM rows of one expert; of eight waves, NB take a block each, and 8 / NB
+// of them share its k, stages of 128 in turn. A wave keeps DEPTH stages in registers, one being
+// multiplied, the rest on their way, through to the following units. A workgroup's units are
+// consecutive, so the rows, which are quantized on the way into LDS, are prepared once per expert
+// and workgroup.
+__host__ __device__ constexpr int narrow_stride(int K) { return padded(K) + 16; }  // rows 16 bytes apart mod 128
+__host__ __device__ constexpr int64_t narrow_lds(int K, int E, int TM) {  // rows, two units' sums, row scales and maxima, segments
+  return 16 * (int64_t)TM * narrow_stride(K) + 2 * 8 * TM * 64 * 16 + 16 * TM * 4 + 8 * 4 + 2 * (E + 1) * (int)sizeof(int);
+}
+
+template <int MODE, int ACT, int NB, int TM>
+__global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t s_dyn[];
+  constexpr int kRows = 16 * TM, KS = 8 / NB, DEPTH = 2, CPU = MODE == kGateUp ? 8 : 16;  // CPU: columns of a block
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int nb = wv % NB, ks = wv / NB, ml = lane & 15, g4 = lane >> 4;
+  const int E = p.E, K = p.K, N = p.N, KC = K / 16, nst = (K + 127) / 128;
+  const int stride = narrow_stride(K);
+  uint8_t* sP = s_dyn;
+  i32x4_t* sums = (i32x4_t*)(s_dyn + kRows * stride);  // [2 units][KS][NB][TM][64]
+  float* s_scale = (float*)(sums + 2 * 8 * TM * 64);    // [kRows]
+  uint32_t* s_max = (uint32_t*)(s_scale + kRows);       // [8]
+  int* s_seg = (int*)(s_max + 8);
+  int* s_tile = s_seg + E + 1;
+  const int nblk = (N + CPU - 1) / CPU, NCB = (nblk + NB - 1) / NB;
+  segments_wave(p, s_seg, s_tile, [&](int rows) { return (rows + kRows - 1) / kRows * NCB; });
+  const int64_t total = s_tile[E];
+  const int u0 = (int)(total * blockIdx.x / gridDim.x), u1 = (int)(total * (blockIdx.x + 1) / gridDim.x);
+  const int mine = (nst + KS - 1) / KS;  // stages of a share of k: ks, ks + KS, ...
+
+  struct Unit { int e, rt, cb; };
+  auto decode = [&](int u) {
+    Unit r;
+    r.e = __builtin_amdgcn_readfirstlane(find_wave(s_tile, E, u));
+    const int local = __builtin_amdgcn_readfirstlane(u - s_tile[r.e]);
+    r.rt = local / NCB;
+    r.cb = local - r.rt * NCB;
+    return r;
+  };
+  struct Stage { i32x4_t w[2]; };
+  // this lane's weight row of a unit (blocks past the last one repeat it, rows past N the last row)
+  auto weight_row = [&](const Unit& u) {
+    const int blk = min(u.cb * NB + nb, nblk - 1);
+    if (MODE == kGateUp)
+      return (ml < 8 ? p.wa : p.wb) + (u.e * p.e_rows + (int64_t)(blk * 8 + (ml & 7)) * p.r_rows) * K;
+    return p.wa + (u.e * p.e_rows + min(blk * 16 + ml, N - 1)) * (int64_t)K;
+  };
+  // chunks past a row's end repeat its last one, against zeros in LDS
+  auto load = [&](Stage& g, const int8_t* row, int i) {
+    const int c = 8 * (ks + KS * i) + 2 * g4;
+    g.w[0] = *(const i32x4_t*)(row + min(c, KC - 1) * 16);
+    g.w[1] = *(const i32x4_t*)(row + min(c + 1, KC - 1) * 16);
+  };
+
+  // Rows row0 .. of x into LDS as codes: a wave a row, or with few rows 2, 4 or 8 waves.
+  auto fill = [&](auto* x, int row0, int rows) {
+    using T = std::remove_const_t<std::remove_pointer_t<decltype(x)>>;
+    const int lw = rows == 1 ? 3 : rows == 2 ? 2 : rows <= 4 ? 1 : 0, W = 1 << lw, sub = wv & (W - 1);
+    const int cpr = K / 8;
+    for (int r = wv >> lw; r < kRows; r += 8 >> lw) {  // (one pass where W > 1)
+      const bool on = r < rows;
+      const T* xr = x + (int64_t)(row0 + r) * K;
+      Eight<T> v[4];
+      uint32_t m = 0;
+      if (on) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int c = sub * 64 + lane + k * 64 * W;
+          if (c < cpr) v[k].load(xr + 8 * (int64_t)c);
+          else v[k].zero();
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) m = max(m, amax8(v[k]));
+        for (int c = sub * 64 + lane + 4 * 64 * W; c < cpr; c += 64 * W) {
+          Eight<T> e;
+          e.load(xr + 8 * (int64_t)c);
+          m = max(m, amax8(e));
+        }
+        m = wave_max(m);
+      }
+      if (lw) {
+        if (lane == 0) s_max[wv] = m;
+        __syncthreads();
+        for (int k = 0; k < W; ++k) m = max(m, s_max[(wv & ~(W - 1)) + k]);
+      }
+      if (on) {
+        const RowScale rs = row_scale(m);
+        uint8_t* row = sP + r * stride;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int c = sub * 64 + lane + k * 64 * W;
+          if (c < cpr) *(uint2*)(row + 8 * c) = codes8(v[k], rs.r);
+        }
+        for (int c = sub * 64 + lane + 4 * 64 * W; c < cpr; c += 64 * W) {
+          Eight<T> e;
+          e.load(xr + 8 * (int64_t)c);
+          *(uint2*)(row + 8 * c) = codes8(e, rs.r);
+        }
+        if (sub == 0) {
+          for (int c = cpr + lane; c < nst * 16; c += 64) *(uint2*)(row + 8 * c) = make_uint2(0, 0);
+          if (lane == 0) s_scale[r] = rs.s;
+        }
+      }
+      if (lw) break;
+    }
+  };
+
+  if (u0 < u1) {
+    Stage ring[DEPTH];
+    int lt = u0, li = 0;  // load cursor
+    const int8_t* lrow = weight_row(decode(u0));
+    auto load_next = [&](Stage& g) {
+      load(g, lrow, li);
+      if (++li == mine) {
+        li = 0;
+        if (lt + 1 < u1) lrow = weight_row(decode(++lt));
+      }
+    };
+    for_each<DEPTH - 1>([&](auto k) { load_next(ring[decltype(k)::value]); });
+    int t = u0, at = 0, rows = 0, row0 = 0;
+    Unit u{-1, -1, 0};
+    i32x4_t acc[TM];
+#pragma unroll
+    for (int i = 0; i < TM; ++i) acc[i] = i32x4_t{0, 0, 0, 0};
+    auto enter = [&]() {  // unit t
+      const Unit n = decode(t);
+      const bool same = n.e == u.e && n.rt == u.rt;
+      u = n;
+      if (same) return;
+      row0 = s_seg[u.e] + u.rt * kRows;
+      rows = min(kRows, s_seg[u.e + 1] - row0);
+      __syncthreads();  // every wave is done with the rows before
+      if (p.x_f32) fill((const float*)p.x, row0, rows);
+      else fill((const uint16_t*)p.x, row0, rows);
+      __syncthreads();
+    };
+    enter();
+    auto step = [&](Stage& cur, Stage& free) __attribute__((always_inline)) {
+      load_next(free);
+      const int st = ks + KS * at;
+      if (st < nst) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+          if (i > 0 && rows <= 16 * i) continue;
+          const uint8_t* a = sP + (16 * i + ml) * stride + st * 128 + g4 * 32;
+          acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(cur.w[0], *(const i32x4_t*)a, acc[i], 0, 0, 0);
+          acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(cur.w[1], *(const i32x4_t*)(a + 16), acc[i], 0, 0, 0);
+        }
+      }
+      if (++at < mine) return true;
+      at = 0;
+      // one barrier a unit: the waves that read these sums come to the next one before anyone
+      // writes over them
+      i32x4_t* red = sums + (t & 1) * 8 * TM * 64;
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        red[((ks * NB + nb) * TM + i) * 64 + lane] = acc[i];
+        acc[i] = i32x4_t{0, 0, 0, 0};
+      }
+      __syncthreads();
+      auto sum = [&](int b, int i, int l) {
+        i32x4_t v = red[(b * TM + i) * 64 + l];
+#pragma unroll
+        for (int k = 1; k < KS; ++k) {
+          const i32x4_t o = red[((k * NB + b) * TM + i) * 64 + l];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) v[q] += o[q];
+        }
+        return v;
+      };
+      if (MODE == kGateUp) {
+        if (tid < NB * TM * 32) {
+          const int b = tid / (TM * 32), i = tid / 32 % TM, l = tid & 31, r = 16 * i + (l & 15);
+          const int hc = (u.cb * NB + b) * 8 + 4 * (l >> 4);
+          if (r < rows && hc < N) {
+            const i32x4_t sg = sum(b, i, l), su = sum(b, i, l + 32);
+            float ca[4], cb[4], ba[4], bb[4], v[4];
+            col_scales(p.sa, p, u.e, hc, ca);
+            col_scales(p.sb, p, u.e, hc, cb);
+            if constexpr (ACT == kOssGLU) glu_bias(p, u.e, hc, ba, bb);
+            const float s = s_scale[r];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              float gv = (float)sg[q] * s * ca[q], uv = (float)su[q] * s * cb[q];
+              if constexpr (ACT == kOssGLU) { gv += ba[q]; uv += bb[q]; }
+              v[q] = activation(ACT, gv, uv, p.limit);
+            }
+            *(float4*)(p.h + (int64_t)(row0 + r) * N + hc) = make_float4(v[0], v[1], v[2], v[3]);
+          }
+        }
+      } else if (tid < NB * TM * 64) {
+        const int b = tid / (TM * 64), i = tid / 64 % TM, l = tid & 63, r = 16 * i + (l & 15);
+        const int n = (u.cb * NB + b) * 16 + 4 * (l >> 4);
+        if (r < rows && n < N) {
+          const i32x4_t sv = sum(b, i, l);
+          float c[4], bias[4], v[4];
+          col_scales(p.sa, p, u.e, n, c);
+          col_bias(p, u.e, n, bias);
+          const float s = s_scale[r];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) v[q] = (float)sv[q] * s * c[q] + bias[q];
+          store4(p, row0 + r, n, v);
+        }
+      }
+      if (++t >= u1) return false;
+      enter();
+      return true;
+    };
+    while (step(ring[0], ring[1]) && step(ring[1], ring[0])) {}
+  }
+  if (MODE == kLinear) zero_rest(p, s_seg[E]);
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+constexpr int kLdsMost = 156 * 1024;  // dynamic LDS of the narrow kernel
+
+static bool aligned16(const void* a) { return ((uintptr_t)a & 15) == 0; }
+static int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
+
+template <int MODE, int ACT, int WM, int WN, int TM, int TN>
+static void launch_tiles(const Params& p, hipStream_t stream) {
+  constexpr int BM = 16 * WM * TM, BN = 16 * WN * TN;
+  const int64_t nt = MODE == kGateUp ? (p.N + BN / 2 - 1) / (BN / 2) : (p.N + BN - 1) / BN;
+  int64_t g = (p.R / BM + (p.R < p.E ? p.R : p.E)) * nt;
+  const int64_t most = (int64_t)cu_count() * (8 / (WM * WN));
+  if (g > most) g = most;
+  if (g >= 8) g -= g % 8;
+  hipLaunchKernelGGL((wide_kernel<MODE, ACT, WM, WN, TM, TN>), dim3((unsigned)g), dim3(64 * WM * WN),
+                     2 * (p.E + 1) * sizeof(int), stream, p);
+}
+template <int MODE, int ACT>
+static void launch_wide(const Params& p, hipStream_t stream) {
+  launch_tiles<MODE, ACT, 4, 2, 4, 8>(p, stream);
+}
+
+static int narrow_blocks(int K, int E) {
+  return narrow_lds(K, E, 2) <= 80 * 1024 ? 2 : narrow_lds(K, E, 1) <= kLdsMost ? 1 : 0;
+}
+template <int MODE, int ACT>
+static void launch_narrow(const Params& p, hipStream_t stream) {
+  const int tm = narrow_blocks(p.K, p.E);
+  const int64_t nblk = MODE == kGateUp ? p.N / 8 : (p.N + 15) / 16;
+  const int64_t ncb = (nblk + 3) / 4;
+  int64_t g = (p.R / (16 * tm) + (p.R < p.E ? p.R : p.E)) * ncb;
+  const int64_t most = (int64_t)cu_count() * 2;
+  if (g > most) g = most;
+  const int64_t lds = narrow_lds(p.K, p.E, tm);
+  auto launch = [&](auto kernel) {
+    if (lds > 64 * 1024)
+      (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsMost);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)g), dim3(512), (unsigned)lds, stream, p);
+  };
+  if (tm == 1) launch(narrow_kernel<MODE, ACT, 4, 1>);
+  else launch(narrow_kernel<MODE, ACT, 4, 2>);
+}
+
+// Whether a product of contraction K goes to the narrow kernel.
+static bool takes_narrow(int64_t R, int64_t E, int K) {
+  return narrow_blocks(K, (int)E) && R <= 16 * (R < E ? R : E);
+}
+
+static int check_shape(int64_t R, int E, int K, int N) {
+  if (R < 0 || E < 1 || E > kMaxE || K < 16 || N < 1) return kErrInvalidArgument;
+  if (K % 16 || K > kMaxK || N > (1 << 22)) return kErrUnsupportedShape;
+  if (R >= (int64_t)INT32_MAX / 2) return kErrUnsupportedShape;
+  // tiles and units are counted in 32 bits
+  if ((R / 16 + E) * ((int64_t)N / 8 + 1) >= (int64_t)0x3fffffff) return kErrUnsupportedShape;
+  return kOk;
+}
+
+// rows without codes behind theirs where q_cols is cols; x 16-byte aligned rows or not
+template <typename T>
+static void launch_quant(const T* x, int64_t ld, int64_t rows, int cols, int q_cols, int8_t* q, float* scale,
+                         hipStream_t stream) {
+  const bool vec = cols % 8 == 0 && aligned16(x) && ld * (int64_t)sizeof(T) % 16 == 0 && ((uintptr_t)q & 7) == 0;
+  const int64_t four = (rows + 3) / 4;
+  if (!vec) hipLaunchKernelGGL(quant_any_kernel<T>, sliced(four), dim3(256), 0, stream, x, ld, rows, cols, q, scale);
+  else if (cols <= 4096)
+    hipLaunchKernelGGL((quant_kernel<T, 1>), sliced(four), dim3(256), 0, stream, x, ld, rows, cols, q_cols, q, scale);
+  else
+    hipLaunchKernelGGL((quant_kernel<T, 4>), sliced(rows), dim3(256), 0, stream, x, ld, rows, cols, q_cols, q, scale);
+}
+
+// The rows of a wide product in codes: [R, padded(K)] and [R] scales.
+static int64_t row_bytes(int64_t R, int K) { return up256(R * padded(K)) + up256(R * 4); }
+struct Rows { int8_t* q; float* s; };
+static Rows rows_at(uint8_t* ws, int64_t R, int K) { return {(int8_t*)ws, (float*)(ws + up256(R * padded(K)))}; }
+
+// y = x w^T + b from rows in bf16 or fp32: at x in the workspace or the caller's.
+static void product(Params& p, uint8_t* ws, hipStream_t stream) {
+  if (takes_narrow(p.R, p.E, p.K)) return launch_narrow<kLinear, kSwiGLU>(p, stream);
+  const Rows rows = rows_at(ws, p.R, p.K);
+  if (p.x_f32) launch_quant((const float*)p.x, p.K, p.R, p.K, padded(p.K), rows.q, rows.s, stream);
+  else launch_quant((const uint16_t*)p.x, p.K, p.R, p.K, padded(p.K), rows.q, rows.s, stream);
+  p.q = rows.q;
+  p.s = rows.s;
+  launch_wide<kLinear, kSwiGLU>(p, stream);
+}
+
+template <int ACT>
+static int layer(const uint16_t* x, const int8_t* qw1, const float* sw1, const int8_t* qw2, const float* sw2,
+                 const int8_t* qw3, const float* sw3, const void* b1, const void* b2, int bias_f32, float limit,
+                 const int64_t* counts, int64_t R, int E, int D, int H, uint8_t* ws, int64_t ws_bytes, uint16_t* y,
+                 hipStream_t stream) {
+  if (H > (1 << 21)) return kErrUnsupportedShape;
+  for (const int st : {check_shape(R, E, D, 2 * H), check_shape(R, E, H, D)})
+    if (st) return st;
+  if (!counts && E != 1) return kErrInvalidArgument;
+  if (R == 0) return kOk;
+  if (!x || !qw1 || !sw1 || !qw2 || !sw2 || !qw3 || !sw3 || !ws || !y) return kErrInvalidArgument;
+  for (const void* q : {(const void*)x, (const void*)qw1, (const void*)qw2, (const void*)qw3, (const void*)ws, (const void*)y})
+    if (!aligned16(q)) return kErrInvalidArgument;
+  if (ws_bytes < moe_int8_layer_workspace_bytes(R, E, D, H)) return kErrWorkspace;
+  float* h = (float*)ws;
+  uint8_t* rows_ws = ws + up256(R * 4 * (int64_t)H);  // x's rows, then h's
+  Params p{};
+  p.counts = counts; p.R = R; p.E = E; p.K = D; p.N = H;
+  p.x = x;
+  p.wa = qw1; p.sa = sw1; p.wb = qw3; p.sb = sw3;
+  p.e_rows = ACT == kOssGLU ? 2 * (int64_t)H : H;
+  p.r_rows = ACT == kOssGLU ? 2 : 1;
+  p.bias = b1; p.bias_f32 = bias_f32; p.limit = limit;
+  p.h = h;
+  if (takes_narrow(R, E, D)) {
+    launch_narrow<kGateUp, ACT>(p, stream);
+  } else {
+    const Rows rows = rows_at(rows_ws, R, D);
+    launch_quant(x, D, R, D, padded(D), rows.q, rows.s, stream);
+    p.q = rows.q; p.s = rows.s;
+    launch_wide<kGateUp, ACT>(p, stream);
+  }
+  p.K = H; p.N = D;
+  p.x = h; p.x_f32 = 1;
+  p.wa = qw2; p.sa = sw2; p.e_rows = D; p.r_rows = 1;
+  p.bias = b2; p.y = y;
+  product(p, rows_ws, stream);
+  return launch_status();
+}
+
+}  // namespace int8
+}  // namespace moe
+
+using namespace moe;
+using namespace moe::int8;
+
+MOE_API int moe_int8_quant_rows(const void* x, int64_t ld, int64_t rows, int32_t cols, int32_t dtype, int8_t* q,
+                                float* scale, hipStream_t stream) {
+  if (rows < 0 || cols < 1 || ld < cols || (dtype != 0 && dtype != 1)) return kErrInvalidArgument;
+  if (rows >= kMaxGrid) return kErrUnsupportedShape;
+  if (rows == 0) return kOk;
+  if (!x || !q || !scale) return kErrInvalidArgument;
+  if (dtype == 0) launch_quant((const uint16_t*)x, ld, rows, cols, cols, q, scale, stream);
+  else launch_quant((const float*)x, ld, rows, cols, cols, q, scale, stream);
+  return launch_status();
+}
+
+MOE_API int moe_int8_dequant_rows(const int8_t* q, const float* scale, int64_t rows, int32_t cols, int32_t dtype, void* x,
+                                  hipStream_t stream) {
+  if (rows < 0 || cols < 1 || (dtype != 0 && dtype != 1)) return kErrInvalidArgument;
+  if (rows >= kMaxGrid) return kErrUnsupportedShape;
+  if (rows == 0) return kOk;
+  if (!q || !scale || !x) return kErrInvalidArgument;
+  const bool vec = cols % 8 == 0 && aligned16(x) && ((uintptr_t)q & 7) == 0;
+  const dim3 grid = sliced((rows + 3) / 4);
+  auto launch = [&](auto kernel, auto* out) {
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, q, scale, rows, cols, out);
+  };
+  if (dtype == 0) vec ? launch(dequant_kernel<uint16_t, true>, (uint16_t*)x) : launch(dequant_kernel<uint16_t, false>, (uint16_t*)x);
+  else vec ? launch(dequant_kernel<float, true>, (float*)x) : launch(dequant_kernel<float, false>, (float*)x);
+  return launch_status();
+}
+
+MOE_API int64_t moe_int8_linear_workspace_bytes(int64_t n_rows, int32_t n_experts, int32_t in_features) {
+  if (n_rows < 0 || n_experts < 1 || in_features < 16 || in_features % 16) return kErrInvalidArgument;
+  return takes_narrow(n_rows, n_experts, in_features) ? 0 : row_bytes(n_rows, in_features);
+}
+
+MOE_API int moe_int8_linear(const void* x, int32_t dtype, const int8_t* qw, const float* sw, const void* bias,
+                            int32_t bias_dtype, const int64_t* counts, int64_t n_rows, int32_t n_experts,
+                            int32_t in_features, int32_t out_features, uint8_t* workspace, int64_t workspace_bytes, void* y,
+                            hipStream_t stream) {
+  const int st = check_shape(n_rows, n_experts, in_features, out_features);
+  if (st) return st;
+  if ((dtype != 0 && dtype != 1) || (bias_dtype != 0 && bias_dtype != 1) || (!counts && n_experts != 1))
+    return kErrInvalidArgument;
+  if (n_rows == 0) return kOk;
+  if (!x || !qw || !sw || !y) return kErrInvalidArgument;
+  for (const void* q : {x, (const void*)qw, (const void*)workspace, (const void*)y})
+    if (!aligned16(q)) return kErrInvalidArgument;
+  const int64_t need = moe_int8_linear_workspace_bytes(n_rows, n_experts, in_features);
+  if (need && !workspace) return kErrInvalidArgument;
+  if (workspace_bytes < need) return kErrWorkspace;
+  Params p{};
+  p.counts = counts; p.R = n_rows; p.E = n_experts; p.K = in_features; p.N = out_features;
+  p.x = x; p.x_f32 = dtype;
+  p.wa = qw; p.sa = sw; p.e_rows = out_features; p.r_rows = 1;
+  p.bias = bias; p.bias_f32 = bias_dtype;
+  p.y = y; p.y_f32 = dtype;
+  product(p, workspace, stream);
+  return launch_status();
+}
+
+MOE_API int64_t moe_int8_layer_workspace_bytes(int64_t n_rows, int32_t n_experts, int32_t dim, int32_t hidden) {
+  if (n_rows < 0 || n_experts < 1 || dim < 16 || hidden < 16 || dim % 16 || hidden % 16) return kErrInvalidArgument;
+  return up256(n_rows * 4 * (int64_t)hidden) + std::max(row_bytes(n_rows, dim), row_bytes(n_rows, hidden));
+}
+
+MOE_API int moe_int8_swiglu(const uint16_t* x, const int8_t* qw1, const float* sw1, const int8_t* qw2, const float* sw2,
+                            const int8_t* qw3, const float* sw3, const int64_t* counts, int64_t n_rows, int32_t n_experts,
+                            int32_t dim, int32_t hidden, uint8_t* workspace, int64_t workspace_bytes, uint16_t* y,
+                            hipStream_t stream) {
+  return layer<kSwiGLU>(x, qw1, sw1, qw2, sw2, qw3, sw3, nullptr, nullptr, 0, 0.f, counts, n_rows, n_experts, dim, hidden,
+                        workspace, workspace_bytes, y, stream);
+}
+
+MOE_API int moe_int8_oss(const uint16_t* x, const int8_t* qmlp1, const float* smlp1, const void* mlp1_bias,
+                         const int8_t* qmlp2, const float* smlp2, const void* mlp2_bias, int32_t bias_dtype,
+                         const int64_t* counts, int64_t n_rows, int32_t n_experts, int32_t dim, int32_t hidden,
+                         float swiglu_limit, uint8_t* workspace, int64_t workspace_bytes, uint16_t* y,
+                         hipStream_t stream) {
+  if (bias_dtype != 0 && bias_dtype != 1) return kErrInvalidArgument;
+  if (n_rows > 0 && (!qmlp1 || !smlp1 || !mlp1_bias || !mlp2_bias)) return kErrInvalidArgument;
+  if (dim < 16 || dim % 16) return dim < 16 ? kErrInvalidArgument : kErrUnsupportedShape;
+  return layer<kOssGLU>(x, qmlp1, smlp1, qmlp2, smlp2, qmlp1 ? qmlp1 + dim : nullptr, smlp1 ? smlp1 + 1 : nullptr,
+                        mlp1_bias, mlp2_bias, bias_dtype, swiglu_limit, counts, n_rows, n_experts, dim, hidden, workspace,
+                        workspace_bytes, y, stream);
+}

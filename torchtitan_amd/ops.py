@@ -1,5 +1,6 @@
 """torch.library custom ops over the MI355X MoE kernels (namespace ``moe_mi355x``; those on
-block-scaled 4-bit operands and 8-bit kept activations ``moe_mi355x_mx``).
+block-scaled 4-bit operands and 8-bit kept activations ``moe_mi355x_mx``, those on 8-bit integers
+``moe_mi355x_int8``).
 
 Each op is a thin host wrapper around one C-ABI entry point of
 ``libmoe_mi355x.so``: it allocates outputs and workspaces with torch's caching
@@ -1394,12 +1395,12 @@ def _mx_op(schema: str, lib: torch.library.Library = _MX):
     return register
 
 
-def _inference_op(bare):
-    """Defines moe_mi355x_mx's op of the bare one's name and schema as the decorated function, above
+def _inference_op(bare, lib: torch.library.Library = _MX):
+    """Defines lib's op of the bare one's name and schema as the decorated function, above
     autograd and torch.func's transforms, where it sees what it has to refuse."""
     def register(fn):
-        _MX.define(str(bare._schema).split("::")[1])
-        _MX.impl(fn.__name__, fn, "CompositeImplicitAutograd")
+        lib.define(str(bare._schema).split("::")[1])
+        lib.impl(fn.__name__, fn, "CompositeImplicitAutograd")
         return fn
     return register
 
@@ -1507,11 +1508,11 @@ def _check_mxfp4_rows(op: str, x: Tensor, qw1: Tensor, counts: Tensor, glu: int 
     return r, d, e, h_dim
 
 
-def _no_gradients(op: str, *tensors: Tensor) -> None:
+def _no_gradients(op: str, *tensors: Tensor | None, instead: str = "grouped_swiglu_mxfp4_train trains on bf16 weights") -> None:
     grad = torch.is_grad_enabled()
-    if any([(grad and t.requires_grad) or _has_tangent(t) for t in tensors]):
+    if any([t is not None and ((grad and t.requires_grad) or _has_tangent(t)) for t in tensors]):
         raise RuntimeError(f"{op} is for inference and has no gradients: call it under torch.no_grad() or on detached "
-                           "tensors (grouped_swiglu_mxfp4_train trains on bf16 weights)")
+                           f"tensors ({instead})")
 
 
 @_mx_op("grouped_swiglu_mxfp4(Tensor x, Tensor qw1, Tensor sw1, Tensor qw2, Tensor sw2, Tensor qw3, Tensor sw3, "
@@ -1713,6 +1714,315 @@ def _mxfp4_train_bwd(ctx, dy, *_unused):
 
 
 grouped_swiglu_mxfp4_train.register_autograd(_mxfp4_train_bwd, setup_context=_mxfp4_train_setup)
+
+
+# ---------------------------------------------------------------------------
+# 8-bit integers with a scale per row (token or output channel), for inference
+# ---------------------------------------------------------------------------
+_I8 = torch.library.Library("moe_mi355x_int8", "FRAGMENT")
+_I8_BARE = torch.library.Library("moe_mi355x_int8_bare", "FRAGMENT")  # (as _MX_BARE)
+INT8_MULTIPLE = 16  # of the products' contractions: weight rows are read in 16-byte pieces
+INT8_MAX_K = 131072  # past it a sum of code products can leave 32 bits
+
+
+def _check_int8(op: str, name: str, q: Tensor, scale: Tensor, shape: tuple | None = None) -> None:
+    """A matrix in codes: q [.., K] int8 and scale [..] fp32 on one device, of `shape` where one is given."""
+    if q.dtype != torch.int8 or scale.dtype != torch.float32:
+        raise TypeError(f"{op} expects int8 {name} and float32 scales, got {q.dtype} and {scale.dtype}")
+    qs, ss = q.shape, scale.shape
+    if not qs or ss != qs[:-1] or q.device != scale.device:
+        raise ValueError(f"{op}: {name} {tuple(qs)} on {q.device} and its scales {tuple(ss)} on {scale.device} do not "
+                         "belong together")
+    if shape is not None and qs != shape:
+        raise ValueError(f"{op} expects {name} of {list(shape)}, got {list(qs)}")
+
+
+def _check_int8_bias(op: str, bias: Tensor | None, shape: tuple, like: Tensor) -> int:
+    """The bias's dtype code."""
+    if bias is None:
+        return 0
+    if bias.dtype not in DTYPE_CODES:
+        raise TypeError(f"{op} takes biases in bfloat16 and float32, got {bias.dtype}")
+    if bias.shape != shape or bias.device != like.device:
+        raise ValueError(f"{op} expects a bias of {list(shape)} on {like.device}, got {list(bias.shape)} on {bias.device}")
+    return DTYPE_CODES[bias.dtype]
+
+
+def _check_int8_dims(op: str, e: int, *contractions: int) -> None:
+    if e < 1 or e > MAX_GEMM_EXPERTS:
+        raise ValueError(f"{op} takes 1 to {MAX_GEMM_EXPERTS} experts, got {e}")
+    for k in contractions:
+        if k < INT8_MULTIPLE or k % INT8_MULTIPLE or k > INT8_MAX_K:
+            raise ValueError(f"{op} takes contractions that are multiples of {INT8_MULTIPLE} up to {INT8_MAX_K}, got {k}")
+
+
+def _int8_code(op: str, dtype: torch.dtype) -> int:
+    if dtype not in DTYPE_CODES:
+        raise TypeError(f"{op} supports bfloat16 and float32, got {dtype}")
+    return DTYPE_CODES[dtype]
+
+
+def _no_int8_gradients(op: str, *tensors: Tensor | None) -> None:
+    _no_gradients(op, *tensors, instead="codes are not differentiable: train on the bf16 weights")
+
+
+@_mx_op("int8_quantize(Tensor x) -> (Tensor, Tensor)", _I8)
+def _int8_quantize(x: Tensor) -> tuple[Tensor, Tensor]:
+    require_gpu(x)
+    code = _int8_code("int8_quantize", x.dtype)
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"int8_quantize expects rows of at least one column, got {tuple(x.shape)}")
+    *lead, cols = x.shape
+    ld = cols
+    if x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= cols:
+        ld = x.stride(0)  # a slice of wider rows is read where it is
+    else:
+        x = x.contiguous()
+    q = x.new_empty(x.shape, dtype=torch.int8)
+    scale = x.new_empty(lead, dtype=torch.float32)
+    with _guard(x):
+        call("moe_int8_quant_rows", ptr(x), ld, scale.numel(), cols, code, ptr(q), ptr(scale), stream_of(x))
+    return q, scale
+
+
+@torch.library.register_fake("moe_mi355x_int8::int8_quantize", lib=_I8)
+def _(x):
+    return x.new_empty(x.shape, dtype=torch.int8), x.new_empty(x.shape[:-1], dtype=torch.float32)
+
+
+def int8_quantize(x: Tensor) -> tuple[Tensor, Tensor]:
+    """x [.., K] (bf16 or fp32) in 8-bit integers with a scale for each row: (q [.., K] int8,
+    scale [..] fp32). With a = max(max |x|, 127 * 2^-126) of a row and the fp32 quotients
+    r = 127 / a, scale = a / 127, its codes are x r rounded once to the nearest integer, ties to
+    even (|q| <= 127), and stand for q scale. A row with an infinity or a NaN has the scale NaN
+    and zero codes. Rows of weights [.., N, K] are output channels, rows of activations tokens."""
+    return _int8_quantize(x.detach())
+
+
+@_mx_op("int8_dequantize(Tensor q, Tensor scale, ScalarType dtype) -> Tensor", _I8)
+def _int8_dequantize(q: Tensor, scale: Tensor, dtype: torch.dtype) -> Tensor:
+    require_gpu(q, scale)
+    code = _int8_code("int8_dequantize", dtype)
+    _check_int8("int8_dequantize", "q", q, scale)
+    if q.shape[-1] < 1:
+        raise ValueError(f"int8_dequantize expects rows of at least one column, got {tuple(q.shape)}")
+    q, scale = q.contiguous(), scale.contiguous()
+    x = q.new_empty(q.shape, dtype=dtype)
+    with _guard(q):
+        call("moe_int8_dequant_rows", ptr(q), ptr(scale), scale.numel(), q.shape[-1], code, ptr(x), stream_of(q))
+    return x
+
+
+@torch.library.register_fake("moe_mi355x_int8::int8_dequantize", lib=_I8)
+def _(q, scale, dtype):
+    return q.new_empty(q.shape, dtype=dtype)
+
+
+def int8_dequantize(q: Tensor, scale: Tensor, dtype: torch.dtype = torch.bfloat16) -> Tensor:
+    """The values q scale [.., K] of a matrix in codes (int8_quantize), taken in fp32, in bf16 or
+    fp32."""
+    return _int8_dequantize(q, scale.detach(), dtype)
+
+
+@functools.lru_cache(maxsize=256)
+def _int8_workspace_bytes(r: int, e: int, k: int, hidden: int | None) -> int:
+    if hidden is None:
+        return int(lib().moe_int8_linear_workspace_bytes(r, e, k))
+    return int(lib().moe_int8_layer_workspace_bytes(r, e, k, hidden))
+
+
+def _int8_product(op: str, x: Tensor, qw: Tensor, sw: Tensor, counts: Tensor | None, bias: Tensor | None, rows: int) -> Tensor:
+    """x [.., K] of `rows` rows by qw [(E,) N, K]."""
+    code = _int8_code(op, x.dtype)
+    e, (n, k) = 1 if counts is None else qw.shape[0], qw.shape[-2:]
+    _check_int8_dims(op, e, k)
+    if n < 1:
+        raise ValueError(f"{op} expects at least one output channel, got {tuple(qw.shape)}")
+    bias_code = _check_int8_bias(op, bias, qw.shape[:-1], x)
+    x, qw, sw = _ready(x), _ready(qw), sw.contiguous()
+    if bias is not None:
+        bias = bias.contiguous()
+    ws_bytes = _int8_workspace_bytes(rows, e, k, None)
+    ws = x.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
+    y = x.new_empty(*x.shape[:-1], n)
+    with _guard(x):
+        call("moe_int8_linear", ptr(x), code, ptr(qw), ptr(sw), ptr(bias), bias_code, ptr(counts), rows, e, k, n, ptr(ws),
+             ws_bytes, ptr(y), stream_of(x))
+    return y
+
+
+@_mx_op("linear_int8(Tensor x, Tensor qw, Tensor sw, Tensor? bias=None) -> Tensor", _I8_BARE)
+def _linear_int8(x, qw, sw, bias=None):
+    op = "linear_int8"
+    require_gpu(x, qw, sw, bias)
+    _check_int8(op, "qw", qw, sw)
+    if qw.dim() != 2 or x.dim() < 1 or x.shape[-1] != qw.shape[1] or x.device != qw.device:
+        raise ValueError(f"{op} expects x [.., K] and qw [N, K] on one device, got {tuple(x.shape)} on {x.device} and "
+                         f"{tuple(qw.shape)} on {qw.device}")
+    return _int8_product(op, x, qw, sw, None, bias, x.shape[:-1].numel())
+
+
+@torch.library.register_fake("moe_mi355x_int8_bare::linear_int8", lib=_I8_BARE)
+def _(x, qw, sw, bias=None):
+    return x.new_empty(*x.shape[:-1], qw.shape[0])
+
+
+@_inference_op(_linear_int8, _I8)
+def linear_int8(x: Tensor, qw: Tensor, sw: Tensor, bias: Tensor | None = None) -> Tensor:
+    """x w^T + bias in x's dtype (bf16 or fp32), for x [.., K] and a weight in codes, qw [N, K]
+    int8 with sw [N] (int8_quantize). x's rows are quantized on the way; the sums of code products
+    are exact, their scales and the bias (bf16 or fp32) are applied in fp32 and the result is
+    rounded once. For inference: no gradients. K is a multiple of 16."""
+    _no_int8_gradients("linear_int8", x, sw, bias)
+    return _linear_int8(x, qw, sw, bias)
+
+
+def _int8_counts(op: str, x: Tensor, qw: Tensor, counts: Tensor) -> Tensor:
+    """The counts of grouped rows as the kernels read them."""
+    if x.dim() != 2 or qw.dim() != 3 or counts.dim() != 1 or counts.shape[0] != qw.shape[0] or x.shape[1] != qw.shape[2]:
+        raise ValueError(f"{op} expects x [R, K], weights [E, .., K] and counts [E], got {tuple(x.shape)}, "
+                         f"{tuple(qw.shape)}, {tuple(counts.shape)}")
+    _check_counts(op, counts, x, qw)
+    return counts.to(torch.int64).contiguous()
+
+
+@_mx_op("grouped_linear_int8(Tensor x, Tensor qw, Tensor sw, Tensor num_tokens_per_expert, Tensor? bias=None) -> Tensor",
+        _I8_BARE)
+def _grouped_linear_int8(x, qw, sw, num_tokens_per_expert, bias=None):
+    op = "grouped_linear_int8"
+    require_gpu(x, qw, sw, num_tokens_per_expert, bias)
+    _check_int8(op, "qw", qw, sw)
+    counts = _int8_counts(op, x, qw, num_tokens_per_expert)
+    return _int8_product(op, x, qw, sw, counts, bias, x.shape[0])
+
+
+@torch.library.register_fake("moe_mi355x_int8_bare::grouped_linear_int8", lib=_I8_BARE)
+def _(x, qw, sw, num_tokens_per_expert, bias=None):
+    return x.new_empty(x.shape[0], qw.shape[1])
+
+
+@_inference_op(_grouped_linear_int8, _I8)
+def grouped_linear_int8(x: Tensor, qw: Tensor, sw: Tensor, num_tokens_per_expert: Tensor, bias: Tensor | None = None) -> Tensor:
+    """linear_int8 with a weight (and bias) per expert: x [R, K] in expert order, qw [E, N, K], sw and
+    bias [E, N], counts [E] -> [R, N]. Rows past sum(counts) are zero."""
+    _no_int8_gradients("grouped_linear_int8", x, sw, bias)
+    return _grouped_linear_int8(x, qw, sw, num_tokens_per_expert, bias)
+
+
+def _int8_swiglu(op: str, x, qw1, sw1, qw2, sw2, qw3, sw3, counts, rows) -> Tensor:
+    _check_bf16(op, x=x)
+    lead, (h, d) = qw1.shape[:-2], qw1.shape[-2:]
+    _check_int8(op, "w1", qw1, sw1, (*lead, h, d))
+    _check_int8(op, "w2", qw2, sw2, (*lead, d, h))
+    _check_int8(op, "w3", qw3, sw3, (*lead, h, d))
+    if any(t.device != x.device for t in (qw1, qw2, qw3)):
+        raise ValueError(f"{op}: tensors on more than one device")
+    e = lead[0] if lead else 1
+    _check_int8_dims(op, e, d, h)
+    x, qw1, qw2, qw3 = map(_ready, (x, qw1, qw2, qw3))
+    sw1, sw2, sw3 = sw1.contiguous(), sw2.contiguous(), sw3.contiguous()
+    ws_bytes = _int8_workspace_bytes(rows, e, d, h)
+    ws = x.new_empty(ws_bytes, dtype=torch.uint8)
+    y = x.new_empty(x.shape)
+    with _guard(x):
+        call("moe_int8_swiglu", ptr(x), ptr(qw1), ptr(sw1), ptr(qw2), ptr(sw2), ptr(qw3), ptr(sw3), ptr(counts), rows, e, d, h,
+             ptr(ws), ws_bytes, ptr(y), stream_of(x))
+    return y
+
+
+@_mx_op("swiglu_ffn_int8(Tensor x, Tensor qw1, Tensor sw1, Tensor qw2, Tensor sw2, Tensor qw3, Tensor sw3) -> Tensor", _I8_BARE)
+def _swiglu_ffn_int8(x, qw1, sw1, qw2, sw2, qw3, sw3):
+    op = "swiglu_ffn_int8"
+    require_gpu(x, qw1, sw1, qw2, sw2, qw3, sw3)
+    if qw1.dim() != 2 or x.dim() < 1 or x.shape[-1] != qw1.shape[1]:
+        raise ValueError(f"{op} expects x [.., D] and weights [H, D] and [D, H], got {tuple(x.shape)} and {tuple(qw1.shape)}")
+    return _int8_swiglu(op, x, qw1, sw1, qw2, sw2, qw3, sw3, None, x.shape[:-1].numel())
+
+
+@torch.library.register_fake("moe_mi355x_int8_bare::swiglu_ffn_int8", lib=_I8_BARE)
+def _(x, qw1, sw1, qw2, sw2, qw3, sw3):
+    return x.new_empty(x.shape)
+
+
+@_inference_op(_swiglu_ffn_int8, _I8)
+def swiglu_ffn_int8(x: Tensor, qw1: Tensor, sw1: Tensor, qw2: Tensor, sw2: Tensor, qw3: Tensor, sw3: Tensor) -> Tensor:
+    """The SwiGLU feed-forward on weights in codes: x [.., D] bf16, w1 and w3 [H, D], w2 [D, H]
+    (int8_quantize). h = silu(x w1^T) (x w3^T) is taken in fp32 and quantized like x, h w2^T is
+    rounded to bf16 once. For inference: no gradients. D and H are multiples of 16."""
+    _no_int8_gradients("swiglu_ffn_int8", x, sw1, sw2, sw3)
+    return _swiglu_ffn_int8(x, qw1, sw1, qw2, sw2, qw3, sw3)
+
+
+@_mx_op("grouped_swiglu_int8(Tensor x, Tensor qw1, Tensor sw1, Tensor qw2, Tensor sw2, Tensor qw3, Tensor sw3, "
+        "Tensor num_tokens_per_expert) -> Tensor", _I8_BARE)
+def _grouped_swiglu_int8(x, qw1, sw1, qw2, sw2, qw3, sw3, num_tokens_per_expert):
+    op = "grouped_swiglu_int8"
+    require_gpu(x, qw1, sw1, qw2, sw2, qw3, sw3, num_tokens_per_expert)
+    counts = _int8_counts(op, x, qw1, num_tokens_per_expert)
+    return _int8_swiglu(op, x, qw1, sw1, qw2, sw2, qw3, sw3, counts, x.shape[0])
+
+
+@torch.library.register_fake("moe_mi355x_int8_bare::grouped_swiglu_int8", lib=_I8_BARE)
+def _(x, qw1, sw1, qw2, sw2, qw3, sw3, num_tokens_per_expert):
+    return x.new_empty(x.shape)
+
+
+@_inference_op(_grouped_swiglu_int8, _I8)
+def grouped_swiglu_int8(
+    x: Tensor, qw1: Tensor, sw1: Tensor, qw2: Tensor, sw2: Tensor, qw3: Tensor, sw3: Tensor,
+    num_tokens_per_expert: Tensor,
+) -> Tensor:
+    """swiglu_ffn_int8 with weights per expert, w1 and w3 [E, H, D], w2 [E, D, H]: x [R, D] bf16 in
+    expert order, counts [E]. Rows past sum(counts) are zero."""
+    _no_int8_gradients("grouped_swiglu_int8", x, sw1, sw2, sw3)
+    return _grouped_swiglu_int8(x, qw1, sw1, qw2, sw2, qw3, sw3, num_tokens_per_expert)
+
+
+@_mx_op("grouped_swiglu_oss_int8(Tensor x, Tensor qmlp1, Tensor smlp1, Tensor mlp1_bias, Tensor qmlp2, Tensor smlp2, "
+        "Tensor mlp2_bias, Tensor num_tokens_per_expert, float swiglu_limit) -> Tensor", _I8_BARE)
+def _grouped_swiglu_oss_int8(x, qmlp1, smlp1, mlp1_bias, qmlp2, smlp2, mlp2_bias, num_tokens_per_expert, swiglu_limit):
+    op = "grouped_swiglu_oss_int8"
+    require_gpu(x, qmlp1, smlp1, mlp1_bias, qmlp2, smlp2, mlp2_bias, num_tokens_per_expert)
+    _check_bf16(op, x=x)
+    counts = _int8_counts(op, x, qmlp1, num_tokens_per_expert)
+    (r, d), (e, h2, _) = x.shape, qmlp1.shape
+    h = h2 // 2
+    _check_int8(op, "mlp1", qmlp1, smlp1, (e, 2 * h, d))
+    _check_int8(op, "mlp2", qmlp2, smlp2, (e, d, h))
+    if qmlp2.device != x.device:
+        raise ValueError(f"{op}: tensors on more than one device")
+    _check_int8_dims(op, e, d, h)
+    code = _check_int8_bias(op, mlp1_bias, (e, 2 * h), x)
+    if _check_int8_bias(op, mlp2_bias, (e, d), x) != code:
+        raise TypeError(f"{op} takes both biases in one dtype, got {mlp1_bias.dtype} and {mlp2_bias.dtype}")
+    if not swiglu_limit >= 0:
+        raise ValueError(f"{op} expects a clamp limit of at least 0, got {swiglu_limit}")
+    x, qmlp1, qmlp2 = map(_ready, (x, qmlp1, qmlp2))
+    smlp1, smlp2, b1, b2 = (t.contiguous() for t in (smlp1, smlp2, mlp1_bias, mlp2_bias))
+    ws_bytes = _int8_workspace_bytes(r, e, d, h)
+    ws = x.new_empty(ws_bytes, dtype=torch.uint8)
+    y = x.new_empty(r, d)
+    with _guard(x):
+        call("moe_int8_oss", ptr(x), ptr(qmlp1), ptr(smlp1), ptr(b1), ptr(qmlp2), ptr(smlp2), ptr(b2), code, ptr(counts), r, e, d,
+             h, float(swiglu_limit), ptr(ws), ws_bytes, ptr(y), stream_of(x))
+    return y
+
+
+@torch.library.register_fake("moe_mi355x_int8_bare::grouped_swiglu_oss_int8", lib=_I8_BARE)
+def _(x, qmlp1, smlp1, mlp1_bias, qmlp2, smlp2, mlp2_bias, num_tokens_per_expert, swiglu_limit):
+    return x.new_empty(x.shape)
+
+
+@_inference_op(_grouped_swiglu_oss_int8, _I8)
+def grouped_swiglu_oss_int8(
+    x: Tensor, qmlp1: Tensor, smlp1: Tensor, mlp1_bias: Tensor, qmlp2: Tensor, smlp2: Tensor, mlp2_bias: Tensor,
+    num_tokens_per_expert: Tensor, swiglu_limit: float,
+) -> Tensor:
+    """grouped_swiglu_int8 for gpt-oss's experts (gpt_oss/moe.py:43-122): mlp1 [E, 2H, D] (glu row 2j,
+    linear row 2j + 1) and mlp2 [E, D, H] in codes, biases [E, 2H] and [E, D], both in bf16 or both
+    in fp32; biases, clamps and activation in fp32 between the products."""
+    _no_int8_gradients("grouped_swiglu_oss_int8", x, smlp1, mlp1_bias, smlp2, mlp2_bias)
+    return _grouped_swiglu_oss_int8(x, qmlp1, smlp1, mlp1_bias, qmlp2, smlp2, mlp2_bias, num_tokens_per_expert, swiglu_limit)
 
 
 # ---------------------------------------------------------------------------
