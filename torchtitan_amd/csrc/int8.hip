@@ -516,19 +516,20 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wide_kernel(Params p) {
 // Few rows per expert: the weights are read once and decide the time, so every byte goes straight
 // from memory into the MFMAs' registers. A unit is NB blocks of 16 weight rows (gate_up: 8 gate and
 // 8 up rows each) by up to 16 TM rows of one expert; of eight waves, NB take a block each, and 8 / NB
-// of them share its k, stages of 128 in turn. A wave keeps DEPTH stages in registers, one being
-// multiplied, the rest on their way, through to the following units. A workgroup's units are
-// consecutive, so the rows, which are quantized on the way into LDS, are prepared once per expert
-// and workgroup.
+// of them share its k, stages of 128 in turn. A wave multiplies a group of DEPTH stages while the
+// next one is on its way, through to the following unit. A workgroup's units are consecutive, so
+// the rows, which are quantized on the way into LDS, are prepared once per expert and workgroup.
+// The columns' scales and biases are asked for ahead of the unit's first stages: loads come back in
+// order, so that one asked for where it is used would wait for the stages behind it.
 __host__ __device__ constexpr int narrow_stride(int K) { return padded(K) + 16; }  // rows 16 bytes apart mod 128
 __host__ __device__ constexpr int64_t narrow_lds(int K, int E, int TM) {  // rows, two units' sums, row scales and maxima, segments
   return 16 * (int64_t)TM * narrow_stride(K) + 2 * 8 * TM * 64 * 16 + 16 * TM * 4 + 8 * 4 + 2 * (E + 1) * (int)sizeof(int);
 }
 
-template <int MODE, int ACT, int NB, int TM>
+template <int MODE, int ACT, int NB, int TM, int DEPTH>
 __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
   extern __shared__ __attribute__((aligned(16))) uint8_t s_dyn[];
-  constexpr int kRows = 16 * TM, KS = 8 / NB, DEPTH = 2, CPU = MODE == kGateUp ? 8 : 16;  // CPU: columns of a block
+  constexpr int kRows = 16 * TM, KS = 8 / NB, COLS = MODE == kGateUp ? 8 : 16;  // COLS: columns of a block
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int nb = wv % NB, ks = wv / NB, ml = lane & 15, g4 = lane >> 4;
   const int E = p.E, K = p.K, N = p.N, KC = K / 16, nst = (K + 127) / 128;
@@ -539,11 +540,11 @@ __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
   uint32_t* s_max = (uint32_t*)(s_scale + kRows);       // [8]
   int* s_seg = (int*)(s_max + 8);
   int* s_tile = s_seg + E + 1;
-  const int nblk = (N + CPU - 1) / CPU, NCB = (nblk + NB - 1) / NB;
+  const int nblk = (N + COLS - 1) / COLS, NCB = (nblk + NB - 1) / NB;
   segments_wave(p, s_seg, s_tile, [&](int rows) { return (rows + kRows - 1) / kRows * NCB; });
   const int64_t total = s_tile[E];
   const int u0 = (int)(total * blockIdx.x / gridDim.x), u1 = (int)(total * (blockIdx.x + 1) / gridDim.x);
-  const int mine = (nst + KS - 1) / KS;  // stages of a share of k: ks, ks + KS, ...
+  const int groups = (nst + KS * DEPTH - 1) / (KS * DEPTH);  // of a wave's stages ks, ks + KS, ...
 
   struct Unit { int e, rt, cb; };
   auto decode = [&](int u) {
@@ -554,7 +555,6 @@ __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
     r.cb = local - r.rt * NCB;
     return r;
   };
-  struct Stage { i32x4_t w[2]; };
   // this lane's weight row of a unit (blocks past the last one repeat it, rows past N the last row)
   auto weight_row = [&](const Unit& u) {
     const int blk = min(u.cb * NB + nb, nblk - 1);
@@ -562,11 +562,28 @@ __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
       return (ml < 8 ? p.wa : p.wb) + (u.e * p.e_rows + (int64_t)(blk * 8 + (ml & 7)) * p.r_rows) * K;
     return p.wa + (u.e * p.e_rows + min(blk * 16 + ml, N - 1)) * (int64_t)K;
   };
+  struct Group { i32x4_t w[DEPTH][2]; };
   // chunks past a row's end repeat its last one, against zeros in LDS
-  auto load = [&](Stage& g, const int8_t* row, int i) {
-    const int c = 8 * (ks + KS * i) + 2 * g4;
-    g.w[0] = *(const i32x4_t*)(row + min(c, KC - 1) * 16);
-    g.w[1] = *(const i32x4_t*)(row + min(c + 1, KC - 1) * 16);
+  auto load = [&](Group& g, const int8_t* row, int i) {
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) {
+      const int c = 8 * (ks + KS * (i * DEPTH + d)) + 2 * g4;
+      g.w[d][0] = *(const i32x4_t*)(row + min(c, KC - 1) * 16);
+      g.w[d][1] = *(const i32x4_t*)(row + min(c + 1, KC - 1) * 16);
+    }
+  };
+  // A thread's part of a unit's results: columns 4 fc .. of block fb, row fr.
+  constexpr int kQuads = MODE == kGateUp ? 2 : 4;
+  const int fl = tid % (16 * kQuads), fi = tid / (16 * kQuads) % TM, fb = tid / (16 * kQuads * TM);
+  const int fc = fl >> 4, fr = 16 * fi + (fl & 15);
+  struct Cols { float a[4], b[4], ba[4], bb[4]; };  // scales (of gate and up) and biases
+  auto first_col = [&](const Unit& u) { return (u.cb * NB + fb) * COLS + 4 * fc; };
+  auto load_cols = [&](Cols& c, const Unit& u) {
+    const int n = min(first_col(u), N - 1);
+    col_scales(p.sa, p, u.e, n, c.a);
+    if (MODE == kGateUp) col_scales(p.sb, p, u.e, n, c.b);
+    if (MODE == kGateUp && ACT == kOssGLU) glu_bias(p, u.e, n, c.ba, c.bb);
+    if (MODE == kLinear) col_bias(p, u.e, n, c.ba);
   };
 
   // Rows row0 .. of x into LDS as codes: a wave a row, or with few rows 2, 4 or 8 waves.
@@ -622,108 +639,108 @@ __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
     }
   };
 
+  Group ga, gb;
+  Cols cols{};
+  Unit u{};
+  const int8_t* wrow = nullptr;
   if (u0 < u1) {
-    Stage ring[DEPTH];
-    int lt = u0, li = 0;  // load cursor
-    const int8_t* lrow = weight_row(decode(u0));
-    auto load_next = [&](Stage& g) {
-      load(g, lrow, li);
-      if (++li == mine) {
-        li = 0;
-        if (lt + 1 < u1) lrow = weight_row(decode(++lt));
-      }
-    };
-    for_each<DEPTH - 1>([&](auto k) { load_next(ring[decltype(k)::value]); });
-    int t = u0, at = 0, rows = 0, row0 = 0;
-    Unit u{-1, -1, 0};
-    i32x4_t acc[TM];
+    u = decode(u0);
+    wrow = weight_row(u);
+    load_cols(cols, u);
+    load(ga, wrow, 0);
+  }
+  int at = 0, t = u0, row0 = 0, rows = 0;
+  i32x4_t acc[TM];
 #pragma unroll
-    for (int i = 0; i < TM; ++i) acc[i] = i32x4_t{0, 0, 0, 0};
-    auto enter = [&]() {  // unit t
-      const Unit n = decode(t);
-      const bool same = n.e == u.e && n.rt == u.rt;
-      u = n;
-      if (same) return;
-      row0 = s_seg[u.e] + u.rt * kRows;
-      rows = min(kRows, s_seg[u.e + 1] - row0);
-      __syncthreads();  // every wave is done with the rows before
-      if (p.x_f32) fill((const float*)p.x, row0, rows);
-      else fill((const uint16_t*)p.x, row0, rows);
-      __syncthreads();
-    };
-    enter();
-    auto step = [&](Stage& cur, Stage& free) __attribute__((always_inline)) {
-      load_next(free);
-      const int st = ks + KS * at;
+  for (int i = 0; i < TM; ++i) acc[i] = i32x4_t{0, 0, 0, 0};
+  // group `at` of unit t from `cur`, with the next one's loads on their way into `nxt`; false where
+  // that one is of other rows, or there is none
+  auto step = [&](Group& cur, Group& nxt) __attribute__((always_inline)) {
+    const bool last = at + 1 == groups;
+    Unit to = u;
+    Cols next{};
+    if (last) {
+      if (t + 1 < u1) to = decode(t + 1);
+      wrow = weight_row(to);
+      load_cols(next, to);
+    }
+    load(nxt, wrow, last ? 0 : at + 1);
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) {
+      const int st = ks + KS * (at * DEPTH + d);
       if (st < nst) {
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
           if (i > 0 && rows <= 16 * i) continue;
           const uint8_t* a = sP + (16 * i + ml) * stride + st * 128 + g4 * 32;
-          acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(cur.w[0], *(const i32x4_t*)a, acc[i], 0, 0, 0);
-          acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(cur.w[1], *(const i32x4_t*)(a + 16), acc[i], 0, 0, 0);
+          acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(cur.w[d][0], *(const i32x4_t*)a, acc[i], 0, 0, 0);
+          acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(cur.w[d][1], *(const i32x4_t*)(a + 16), acc[i], 0, 0, 0);
         }
       }
-      if (++at < mine) return true;
-      at = 0;
-      // one barrier a unit: the waves that read these sums come to the next one before anyone
-      // writes over them
-      i32x4_t* red = sums + (t & 1) * 8 * TM * 64;
+    }
+    if (!last) {
+      ++at;
+      return true;
+    }
+    at = 0;
+    // one barrier a unit: the waves that read these sums come to the next one before anyone
+    // writes over them
+    i32x4_t* red = sums + (t & 1) * 8 * TM * 64;
 #pragma unroll
-      for (int i = 0; i < TM; ++i) {
-        red[((ks * NB + nb) * TM + i) * 64 + lane] = acc[i];
-        acc[i] = i32x4_t{0, 0, 0, 0};
-      }
-      __syncthreads();
-      auto sum = [&](int b, int i, int l) {
-        i32x4_t v = red[(b * TM + i) * 64 + l];
+    for (int i = 0; i < TM; ++i) {
+      red[((ks * NB + nb) * TM + i) * 64 + lane] = acc[i];
+      acc[i] = i32x4_t{0, 0, 0, 0};
+    }
+    __syncthreads();
+    const int n = first_col(u);
+    if (fb < NB && fr < rows && n < N) {
+      auto sum = [&](int l) {
+        i32x4_t v = red[(fb * TM + fi) * 64 + l];
 #pragma unroll
         for (int k = 1; k < KS; ++k) {
-          const i32x4_t o = red[((k * NB + b) * TM + i) * 64 + l];
+          const i32x4_t o = red[((k * NB + fb) * TM + fi) * 64 + l];
 #pragma unroll
           for (int q = 0; q < 4; ++q) v[q] += o[q];
         }
         return v;
       };
+      const float s = s_scale[fr];
+      float v[4];
+      const i32x4_t sg = sum(fl);
       if (MODE == kGateUp) {
-        if (tid < NB * TM * 32) {
-          const int b = tid / (TM * 32), i = tid / 32 % TM, l = tid & 31, r = 16 * i + (l & 15);
-          const int hc = (u.cb * NB + b) * 8 + 4 * (l >> 4);
-          if (r < rows && hc < N) {
-            const i32x4_t sg = sum(b, i, l), su = sum(b, i, l + 32);
-            float ca[4], cb[4], ba[4], bb[4], v[4];
-            col_scales(p.sa, p, u.e, hc, ca);
-            col_scales(p.sb, p, u.e, hc, cb);
-            if constexpr (ACT == kOssGLU) glu_bias(p, u.e, hc, ba, bb);
-            const float s = s_scale[r];
+        const i32x4_t su = sum(fl + 32);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              float gv = (float)sg[q] * s * ca[q], uv = (float)su[q] * s * cb[q];
-              if constexpr (ACT == kOssGLU) { gv += ba[q]; uv += bb[q]; }
-              v[q] = activation(ACT, gv, uv, p.limit);
-            }
-            *(float4*)(p.h + (int64_t)(row0 + r) * N + hc) = make_float4(v[0], v[1], v[2], v[3]);
-          }
+        for (int q = 0; q < 4; ++q) {
+          float gv = (float)sg[q] * s * cols.a[q], uv = (float)su[q] * s * cols.b[q];
+          if constexpr (ACT == kOssGLU) { gv += cols.ba[q]; uv += cols.bb[q]; }
+          v[q] = activation(ACT, gv, uv, p.limit);
         }
-      } else if (tid < NB * TM * 64) {
-        const int b = tid / (TM * 64), i = tid / 64 % TM, l = tid & 63, r = 16 * i + (l & 15);
-        const int n = (u.cb * NB + b) * 16 + 4 * (l >> 4);
-        if (r < rows && n < N) {
-          const i32x4_t sv = sum(b, i, l);
-          float c[4], bias[4], v[4];
-          col_scales(p.sa, p, u.e, n, c);
-          col_bias(p, u.e, n, bias);
-          const float s = s_scale[r];
+        *(float4*)(p.h + (int64_t)(row0 + fr) * N + n) = make_float4(v[0], v[1], v[2], v[3]);
+      } else {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) v[q] = (float)sv[q] * s * c[q] + bias[q];
-          store4(p, row0 + r, n, v);
-        }
+        for (int q = 0; q < 4; ++q) v[q] = (float)sg[q] * s * cols.a[q] + cols.ba[q];
+        store4(p, row0 + fr, n, v);
       }
-      if (++t >= u1) return false;
-      enter();
-      return true;
-    };
-    while (step(ring[0], ring[1]) && step(ring[1], ring[0])) {}
+    }
+    const bool same = to.e == u.e && to.rt == u.rt;
+    u = to;
+    cols = next;
+    return ++t < u1 && same;
+  };
+  while (t < u1) {
+    row0 = s_seg[u.e] + u.rt * kRows;
+    rows = min(kRows, s_seg[u.e + 1] - row0);
+    if (t > u0) __syncthreads();  // every wave is done with the rows before
+    if (p.x_f32) fill((const float*)p.x, row0, rows);
+    else fill((const uint16_t*)p.x, row0, rows);
+    __syncthreads();
+    while (step(ga, gb)) {
+      if (!step(gb, ga)) {
+        gb = ga;
+        break;
+      }
+    }
+    ga = gb;
   }
   if (MODE == kLinear) zero_rest(p, s_seg[E]);
 }
@@ -758,19 +775,18 @@ static int narrow_blocks(int K, int E) {
 template <int MODE, int ACT>
 static void launch_narrow(const Params& p, hipStream_t stream) {
   const int tm = narrow_blocks(p.K, p.E);
-  const int64_t nblk = MODE == kGateUp ? p.N / 8 : (p.N + 15) / 16;
-  const int64_t ncb = (nblk + 3) / 4;
-  int64_t g = (p.R / (16 * tm) + (p.R < p.E ? p.R : p.E)) * ncb;
-  const int64_t most = (int64_t)cu_count() * 2;
-  if (g > most) g = most;
-  const int64_t lds = narrow_lds(p.K, p.E, tm);
-  auto launch = [&](auto kernel) {
+  const int64_t nblk = MODE == kGateUp ? p.N / 8 : (p.N + 15) / 16, tiles = p.R / (16 * tm) + (p.R < p.E ? p.R : p.E);
+  const int64_t lds = narrow_lds(p.K, p.E, tm), most = (int64_t)cu_count() * 2;
+  auto launch = [&](auto kernel, int nb) {
+    const int64_t units = tiles * ((nblk + nb - 1) / nb);
     if (lds > 64 * 1024)
       (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsMost);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)g), dim3(512), (unsigned)lds, stream, p);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)std::min(units, most)), dim3(512), (unsigned)lds, stream, p);
   };
-  if (tm == 1) launch(narrow_kernel<MODE, ACT, 4, 1>);
-  else launch(narrow_kernel<MODE, ACT, 4, 2>);
+  if (tm == 1 && tiles * nblk < 4 * most) launch(narrow_kernel<MODE, ACT, 1, 1, 4>, 1);
+  else if (tiles * nblk < 4 * most) launch(narrow_kernel<MODE, ACT, 1, 2, 4>, 1);
+  else if (tm == 1) launch(narrow_kernel<MODE, ACT, 4, 1, 2>, 4);
+  else launch(narrow_kernel<MODE, ACT, 4, 2, 2>, 4);
 }
 
 // Whether a product of contraction K goes to the narrow kernel.
