@@ -80,33 +80,45 @@ __device__ __forceinline__ void segments(const P& p, int* seg, int* tile, int* t
   if (tid == 0) { seg[p.E] = rows; tile[p.E] = tiles; }
   __syncthreads();
 }
+// Inclusive sums over the wave's lanes that stop at `most`, of non-negative ints: four steps in
+// rows of 16 lanes, then the last lanes of the rows before. Cross-lane operands of vector
+// instructions: a step costs a few cycles where one through LDS costs a hundred.
+__device__ __forceinline__ int wave_scan(int v, int most) {
+  v = min(v, most);
+  v = min(v + __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false), most);  // row_shr 1, 2, 4, 8
+  v = min(v + __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false), most);
+  v = min(v + __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false), most);
+  v = min(v + __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false), most);
+  v = min(v + __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false), most);  // lane 15 of the row before
+  return min(v + __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false), most);  // lane 31
+}
+// the sums over the lanes below
+__device__ __forceinline__ int wave_scan_below(int v, int most) {
+  return __builtin_amdgcn_update_dpp(0, wave_scan(v, most), 0x138, 0xf, 0xf, false);  // wave_shr 1
+}
+
 // The same by the first wave alone (lane l the experts l n .. l n + n - 1, n = ceil(E / 64)), where a
 // launch is so short that the barriers of the scans above are a third of it. One barrier.
 template <typename P, typename F>
 __device__ __forceinline__ void segments_wave(const P& p, int* seg, int* tile, F tiles_of) {
   if (threadIdx.x < 64) {
     const int lane = threadIdx.x, R = (int)p.R, n = (p.E + 63) / 64;
+    int64_t raw[kMaxE / 64];
     int cnt[kMaxE / 64];
+#pragma unroll
+    for (int i = 0; i < kMaxE / 64; ++i) {  // all of them on their way before the first is used
+      if (i >= n) break;
+      const int e = lane * n + i;
+      raw[i] = e < p.E ? count_of(p, e) : 0;
+    }
     int rows = 0;
 #pragma unroll
     for (int i = 0; i < kMaxE / 64; ++i) {
       if (i >= n) break;
-      const int e = lane * n + i;
-      const int64_t c = e < p.E ? count_of(p, e) : 0;
-      cnt[i] = c < 0 ? 0 : (c > p.R ? R : (int)c);
+      cnt[i] = raw[i] < 0 ? 0 : (raw[i] > p.R ? R : (int)raw[i]);
       rows = min(rows + cnt[i], R);
     }
-    auto before = [&](int v, int most) {  // saturating sum over the lanes below
-      int incl = v;
-#pragma unroll
-      for (int off = 1; off < 64; off <<= 1) {
-        const int o = __shfl_up(incl, off);
-        if (lane >= off) incl = min(incl + o, most);
-      }
-      const int ex = __shfl_up(incl, 1);
-      return lane ? ex : 0;
-    };
-    int at = before(rows, R), tiles = 0;
+    int at = wave_scan_below(rows, R), tiles = 0;
     const int at0 = at;
 #pragma unroll
     for (int i = 0; i < kMaxE / 64; ++i) {
@@ -115,7 +127,7 @@ __device__ __forceinline__ void segments_wave(const P& p, int* seg, int* tile, F
       at += cnt[i];
       tiles += tiles_of(cnt[i]);
     }
-    int run = at0, tl = before(tiles, 0x3fffffff);
+    int run = at0, tl = wave_scan_below(tiles, 0x3fffffff);
 #pragma unroll
     for (int i = 0; i < kMaxE / 64; ++i) {
       if (i >= n) break;

@@ -64,10 +64,13 @@ __device__ __forceinline__ uint32_t amax8(const Eight<T>& e) {
   for (int i = 0; i < 8; ++i) m = max(m, mx::abs_bits(a[i]));
   return m;
 }
+// the maximum over the wave's lanes: turns within rows of 16, then two lane swaps
 __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, off));
-  return v;
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xf, 0xf, false));  // row_ror 8, 4, 2, 1
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x124, 0xf, 0xf, false));
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x122, 0xf, 0xf, false));
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x121, 0xf, 0xf, false));
+  return mx::row_max(v);
 }
 
 // A row's multiplier and scale from the bits of its max |v| taken over integers (bits of |v| order
@@ -526,7 +529,7 @@ __host__ __device__ constexpr int64_t narrow_lds(int K, int E, int TM) {  // row
   return 16 * (int64_t)TM * narrow_stride(K) + 2 * 8 * TM * 64 * 16 + 16 * TM * 4 + 8 * 4 + 2 * (E + 1) * (int)sizeof(int);
 }
 
-template <int MODE, int ACT, int NB, int TM, int DEPTH>
+template <int MODE, int ACT, typename T, int NB, int TM, int DEPTH>
 __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
   extern __shared__ __attribute__((aligned(16))) uint8_t s_dyn[];
   constexpr int kRows = 16 * TM, KS = 8 / NB, COLS = MODE == kGateUp ? 8 : 16;  // COLS: columns of a block
@@ -541,18 +544,29 @@ __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
   int* s_seg = (int*)(s_max + 8);
   int* s_tile = s_seg + E + 1;
   const int nblk = (N + COLS - 1) / COLS, NCB = (nblk + NB - 1) / NB;
-  segments_wave(p, s_seg, s_tile, [&](int rows) { return (rows + kRows - 1) / kRows * NCB; });
+  auto tiles_of = [&](int rows) { return (rows + kRows - 1) / kRows * NCB; };
+  if (!p.counts) {  // (every thread writes the same)
+    s_seg[0] = s_tile[0] = 0;
+    s_seg[1] = (int)p.R;
+    s_tile[1] = tiles_of((int)p.R);
+  } else {
+    segments_wave(p, s_seg, s_tile, tiles_of);
+  }
   const int64_t total = s_tile[E];
   const int u0 = (int)(total * blockIdx.x / gridDim.x), u1 = (int)(total * (blockIdx.x + 1) / gridDim.x);
   const int groups = (nst + KS * DEPTH - 1) / (KS * DEPTH);  // of a wave's stages ks, ks + KS, ...
 
   struct Unit { int e, rt, cb; };
   auto decode = [&](int u) {
-    Unit r;
-    r.e = __builtin_amdgcn_readfirstlane(find_wave(s_tile, E, u));
-    const int local = __builtin_amdgcn_readfirstlane(u - s_tile[r.e]);
-    r.rt = local / NCB;
-    r.cb = local - r.rt * NCB;
+    Unit r{0, 0, u};
+    if (p.counts) {
+      r.e = __builtin_amdgcn_readfirstlane(find_wave(s_tile, E, u));
+      r.cb = __builtin_amdgcn_readfirstlane(u - s_tile[r.e]);
+    }
+    if (r.cb >= NCB) {
+      r.rt = r.cb / NCB;
+      r.cb -= r.rt * NCB;
+    }
     return r;
   };
   // this lane's weight row of a unit (blocks past the last one repeat it, rows past N the last row)
@@ -586,32 +600,36 @@ __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
     if (MODE == kLinear) col_bias(p, u.e, n, c.ba);
   };
 
-  // Rows row0 .. of x into LDS as codes: a wave a row, or with few rows 2, 4 or 8 waves.
-  auto fill = [&](auto* x, int row0, int rows) {
-    using T = std::remove_const_t<std::remove_pointer_t<decltype(x)>>;
-    const int lw = rows == 1 ? 3 : rows == 2 ? 2 : rows <= 4 ? 1 : 0, W = 1 << lw, sub = wv & (W - 1);
-    const int cpr = K / 8;
+  // Rows row0 .. of x into LDS as codes: a wave a row, or with few rows 2, 4 or 8 waves. A lane's first
+  // four chunks are asked for ahead of the unit's weights, behind which they would come back.
+  const int cpr = K / 8;
+  auto waves_log = [](int rows) { return rows == 1 ? 3 : rows == 2 ? 2 : rows <= 4 ? 1 : 0; };
+  auto load_row = [&](Eight<T> (&v)[4], int row0, int rows, int r, int lw) {
+    const T* xr = (const T*)p.x + (int64_t)(row0 + r) * K;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int c = (wv & ((1 << lw) - 1)) * 64 + lane + (k << (6 + lw));
+      if (r < rows && c < cpr) v[k].load(xr + 8 * (int64_t)c);
+      else v[k].zero();
+    }
+  };
+  auto fill = [&](Eight<T> (&v)[4], int row0, int rows) {
+    const int lw = waves_log(rows), W = 1 << lw, sub = wv & (W - 1);
     for (int r = wv >> lw; r < kRows; r += 8 >> lw) {  // (one pass where W > 1)
       const bool on = r < rows;
-      const T* xr = x + (int64_t)(row0 + r) * K;
-      Eight<T> v[4];
+      const T* xr = (const T*)p.x + (int64_t)(row0 + r) * K;
       uint32_t m = 0;
+      if (r >= 8) load_row(v, row0, rows, r, 0);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) m = max(m, amax8(v[k]));
       if (on) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int c = sub * 64 + lane + k * 64 * W;
-          if (c < cpr) v[k].load(xr + 8 * (int64_t)c);
-          else v[k].zero();
-        }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) m = max(m, amax8(v[k]));
         for (int c = sub * 64 + lane + 4 * 64 * W; c < cpr; c += 64 * W) {
           Eight<T> e;
           e.load(xr + 8 * (int64_t)c);
           m = max(m, amax8(e));
         }
-        m = wave_max(m);
       }
+      m = wave_max(m);
       if (lw) {
         if (lane == 0) s_max[wv] = m;
         __syncthreads();
@@ -638,18 +656,26 @@ __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
       if (lw) break;
     }
   };
+  auto unit_rows = [&](const Unit& w, int& rows) {
+    const int row0 = s_seg[w.e] + w.rt * kRows;
+    rows = min(kRows, s_seg[w.e + 1] - row0);
+    return row0;
+  };
 
   Group ga, gb;
   Cols cols{};
   Unit u{};
   const int8_t* wrow = nullptr;
+  Eight<T> x[4];
+  int at = 0, t = u0, row0 = 0, rows = 0;
   if (u0 < u1) {
     u = decode(u0);
+    row0 = unit_rows(u, rows);
+    load_row(x, row0, rows, wv >> waves_log(rows), waves_log(rows));
     wrow = weight_row(u);
     load_cols(cols, u);
     load(ga, wrow, 0);
   }
-  int at = 0, t = u0, row0 = 0, rows = 0;
   i32x4_t acc[TM];
 #pragma unroll
   for (int i = 0; i < TM; ++i) acc[i] = i32x4_t{0, 0, 0, 0};
@@ -728,11 +754,12 @@ __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
     return ++t < u1 && same;
   };
   while (t < u1) {
-    row0 = s_seg[u.e] + u.rt * kRows;
-    rows = min(kRows, s_seg[u.e + 1] - row0);
-    if (t > u0) __syncthreads();  // every wave is done with the rows before
-    if (p.x_f32) fill((const float*)p.x, row0, rows);
-    else fill((const uint16_t*)p.x, row0, rows);
+    if (t > u0) {
+      row0 = unit_rows(u, rows);
+      load_row(x, row0, rows, wv >> waves_log(rows), waves_log(rows));
+      __syncthreads();  // every wave is done with the rows before
+    }
+    fill(x, row0, rows);
     __syncthreads();
     while (step(ga, gb)) {
       if (!step(gb, ga)) {
@@ -772,8 +799,8 @@ static void launch_wide(const Params& p, hipStream_t stream) {
 static int narrow_blocks(int K, int E) {
   return narrow_lds(K, E, 2) <= 80 * 1024 ? 2 : narrow_lds(K, E, 1) <= kLdsMost ? 1 : 0;
 }
-template <int MODE, int ACT>
-static void launch_narrow(const Params& p, hipStream_t stream) {
+template <int MODE, int ACT, typename T>
+static void launch_narrow_of(const Params& p, hipStream_t stream) {
   const int tm = narrow_blocks(p.K, p.E);
   const int64_t nblk = MODE == kGateUp ? p.N / 8 : (p.N + 15) / 16, tiles = p.R / (16 * tm) + (p.R < p.E ? p.R : p.E);
   const int64_t lds = narrow_lds(p.K, p.E, tm), most = (int64_t)cu_count() * 2;
@@ -783,10 +810,15 @@ static void launch_narrow(const Params& p, hipStream_t stream) {
       (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsMost);
     hipLaunchKernelGGL(kernel, dim3((unsigned)std::min(units, most)), dim3(512), (unsigned)lds, stream, p);
   };
-  if (tm == 1 && tiles * nblk < 4 * most) launch(narrow_kernel<MODE, ACT, 1, 1, 4>, 1);
-  else if (tiles * nblk < 4 * most) launch(narrow_kernel<MODE, ACT, 1, 2, 4>, 1);
-  else if (tm == 1) launch(narrow_kernel<MODE, ACT, 4, 1, 2>, 4);
-  else launch(narrow_kernel<MODE, ACT, 4, 2, 2>, 4);
+  if (tm == 1 && tiles * nblk < 4 * most) launch(narrow_kernel<MODE, ACT, T, 1, 1, 1>, 1);
+  else if (tiles * nblk < 4 * most) launch(narrow_kernel<MODE, ACT, T, 1, 2, 1>, 1);
+  else if (tm == 1) launch(narrow_kernel<MODE, ACT, T, 4, 1, 1>, 4);
+  else launch(narrow_kernel<MODE, ACT, T, 4, 2, 1>, 4);
+}
+template <int MODE, int ACT>
+static void launch_narrow(const Params& p, hipStream_t stream) {
+  if (MODE == kLinear && p.x_f32) launch_narrow_of<kLinear, kSwiGLU, float>(p, stream);
+  else launch_narrow_of<MODE, ACT, uint16_t>(p, stream);
 }
 
 // Whether a product of contraction K goes to the narrow kernel.
