@@ -245,25 +245,30 @@ __device__ __forceinline__ float activation(int act, float g, float u, float lim
   return a * sigmoid(kOssAlpha * a) * (b + 1.0f);
 }
 
-__device__ __forceinline__ float bias_at(const Params& p, int64_t i) {
-  return p.bias_f32 ? ((const float*)p.bias)[i] : bf2f(((const uint16_t*)p.bias)[i]);
-}
-// scales of weight rows n .. n + 3 of expert e, linear's biases (the last row's past the end)
+// scales of weight rows n .. n + 3 of expert e (uniform), linear's biases, gpt-oss's of gate and up
+// (the last row's past the end)
 __device__ __forceinline__ void col_scales(const float* s, const Params& p, int e, int n, float (&v)[4]) {
+  const float* se = s + e * p.e_rows;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = s[e * p.e_rows + (int64_t)min(n + i, p.N - 1) * p.r_rows];
+  for (int i = 0; i < 4; ++i) v[i] = se[(uint32_t)(min(n + i, p.N - 1) * p.r_rows)];
+}
+__device__ __forceinline__ float bias_at(const Params& p, int64_t row0, uint32_t i) {
+  return p.bias_f32 ? ((const float*)p.bias + row0)[i] : bf2f(((const uint16_t*)p.bias + row0)[i]);
 }
 __device__ __forceinline__ void col_bias(const Params& p, int e, int n, float (&v)[4]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = p.bias ? bias_at(p, (int64_t)e * p.N + min(n + i, p.N - 1)) : 0.f;
+  for (int i = 0; i < 4; ++i) v[i] = 0.f;
+  if (p.bias) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = bias_at(p, e * (int64_t)p.N, (uint32_t)min(n + i, p.N - 1));
+  }
 }
-// gpt-oss's biases of columns n .. n + 3: glu and linear
 __device__ __forceinline__ void glu_bias(const Params& p, int e, int n, float (&a)[4], float (&b)[4]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int64_t at = ((int64_t)e * p.N + min(n + i, p.N - 1)) * 2;
-    a[i] = bias_at(p, at);
-    b[i] = bias_at(p, at + 1);
+    const uint32_t at = 2u * (uint32_t)min(n + i, p.N - 1);
+    a[i] = bias_at(p, 2 * e * (int64_t)p.N, at);
+    b[i] = bias_at(p, 2 * e * (int64_t)p.N, at + 1);
   }
 }
 
@@ -299,20 +304,23 @@ __device__ __forceinline__ void zero_rest(const Params& p, int from) {
     for (int64_t i = i0; i < n / 2; i += S) ((uint16_t*)y)[i] = 0;
 }
 
-// Many rows per expert: tiles of BM rows x BN columns by WM x WN waves of 16 TM x 16 TN, k in stages
-// of 128 (a cache line), two stages in LDS, persistent workgroups. Operands reach LDS by
-// direct-to-LDS copies, a stage ahead and across tile boundaries. gate_up's columns alternate in
-// blocks of 16 between gate and up, so that a lane holds both.
-template <int MODE, int ACT, int WM, int WN, int TM, int TN>
+// Many rows per expert: tiles of up to BM rows x BN columns by WM x WN waves of 16 TM x 16 TN, k in
+// stages of 128 (a cache line), S stages in LDS, persistent workgroups. Operands reach LDS by
+// direct-to-LDS copies, S - 1 stages ahead and across tile boundaries. gate_up's columns alternate
+// in blocks of 16 between gate and up, so that a lane holds both. An expert's rows are shared
+// evenly by its tiles, a tile's by its waves, in blocks of 16, and a wave's stages are compiled for
+// each number of blocks.
+template <int MODE, int ACT, int WM, int WN, int TM, int TN, int S>
 __global__ __launch_bounds__(64 * WM * WN, 2) void wide_kernel(Params p) {
   constexpr int NW = WM * WN, BM = 16 * WM * TM, BN = 16 * WN * TN;
   constexpr int RB = 128, RPC = 8, CPR = 8;                // bytes of a stage's row; rows of a 1 KB copy; chunks of a row
   constexpr int PW = BM / RPC / NW, QC = BN / RPC / NW;    // a wave's copies a stage: of P, of Q
   constexpr int NCOPY = PW + QC, GM = 8;
   static_assert(PW * RPC * NW == BM && QC * RPC * NW == BN && TN % 2 == 0 && 64 * NW >= 256, "whole copies");
-  __shared__ __attribute__((aligned(1024))) uint8_t sP[2][BM * RB];
-  __shared__ __attribute__((aligned(1024))) uint8_t sQ[2][BN * RB];
-  __shared__ int4 s_list[kTileList];  // this workgroup's first tiles: first row, end of the segment, expert, column tile
+  static_assert(NCOPY * (S - 2) < 64, "vmcnt");
+  __shared__ __attribute__((aligned(1024))) uint8_t sP[S][BM * RB];
+  __shared__ __attribute__((aligned(1024))) uint8_t sQ[S][BN * RB];
+  __shared__ int4 s_list[kTileList];  // this workgroup's first tiles: first row, end of its rows, expert, column tile
   __shared__ int s_tmp[NW];
   extern __shared__ __attribute__((aligned(16))) int s_dyn_i[];
   int* s_seg = s_dyn_i;           // E + 1
@@ -332,13 +340,15 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wide_kernel(Params p) {
   // XCD works on at a time share rows and columns.
   auto search = [&](int t) {
     const int e = find(s_tile, E, t), local = t - s_tile[e], seg0 = s_seg[e], seg1 = s_seg[e + 1];
-    const int mtiles = (seg1 - seg0 + BM - 1) / BM, grp = local / (GM * NT), gm = min(GM, mtiles - grp * GM);
-    const int in = local - grp * GM * NT, nt = in / gm;
-    return make_int4(seg0 + (grp * GM + in - nt * gm) * BM, seg1, e, nt);
+    const int blocks = (seg1 - seg0 + 15) >> 4, mtiles = (seg1 - seg0 + BM - 1) / BM;
+    const int grp = local / (GM * NT), gm = min(GM, mtiles - grp * GM), in = local - grp * GM * NT, nt = in / gm;
+    const int mt = grp * GM + in - nt * gm, per = blocks / mtiles, more = blocks - per * mtiles;
+    const int first = mt * per + min(mt, more), end = first + per + (mt < more ? 1 : 0);
+    return make_int4(seg0 + 16 * first, min(seg1, seg0 + 16 * end), e, nt);
   };
   if (tid < kTileList && lb + (int64_t)tid * G < total_tiles) s_list[tid] = search(lb + tid * G);
   __syncthreads();
-  struct TileRef { int row0, seg1, e, nt; };
+  struct TileRef { int row0, end, e, nt; };
   auto decode = [&](int i) {  // this workgroup's i-th tile
     int4 v;
     if (i < kTileList) v = s_list[i];
@@ -350,9 +360,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wide_kernel(Params p) {
 
   // ---- copies. One fills RPC rows, lane i row i / 8, chunk i % 8 with the row's chunk
   // (i % 8) ^ ((row >> 1) & 7) (eight lanes that read one chunk of eight rows meet no bank
-  // twice). Rows past a segment or the last column repeat the last one inside (what they give is
+  // twice). Rows past the tile's or the last column repeat the last one inside (what they give is
   // not stored), chunks past a weight row's end the last one of the row (the other operand has
-  // zeros there), and behind the last stage of a workgroup the last tile's first is copied once
+  // zeros there), and behind the last stage of a workgroup the last tile's first are copied once
   // more. ----
   auto swz = [](int row) { return (row >> 1) & 7; };
   auto q_col = [](int n) { return MODE == kGateUp ? (n >> 5) * 16 + (n & 15) : n; };  // in the tile's columns
@@ -363,7 +373,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wide_kernel(Params p) {
     int ln = lane;
     asm volatile("" : "+v"(ln));  // what a tile's offsets come from is made again, not kept in registers
     const int crow = ln / CPR, cbit = ln % CPR;
-    const int last = r.seg1 - 1 - r.row0, col0 = r.nt * (MODE == kGateUp ? BN / 2 : BN), last_col = N - 1 - col0;
+    const int last = r.end - 1 - r.row0, col0 = r.nt * (MODE == kGateUp ? BN / 2 : BN), last_col = N - 1 - col0;
     baseP = (const uint8_t*)p.q + (int64_t)r.row0 * p_ld;
     const int64_t wr = r.e * p.e_rows + (int64_t)col0 * p.r_rows;
     baseQ[0] = (const uint8_t*)p.wa + wr * K;
@@ -380,17 +390,17 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wide_kernel(Params p) {
   auto copy = [&](auto c_c, int kt, int s) {  // copy c of stage kt into buffer s
     constexpr int c = decltype(c_c)::value;
     if constexpr (c < PW) {
-      dma16(baseP + kt * RB, offP[c], lds_addr(&sP[s][(wv * PW + c) * 1024]));
+      dma16(baseP + kt * RB, offP[c], lds_addr(sP[0] + s * (BM * RB) + (wv * PW + c) * 1024));
     } else {
       constexpr int b = c - PW;
       const uint8_t* base = MODE == kGateUp && (((wv * QC + b) * RPC >> 4) & 1) ? baseQ[1] : baseQ[0];
       const int chunk = min(kt * CPR + (lane % CPR ^ swz((wv * QC + b) * RPC + lane / CPR)), KC - 1);
-      dma16(base, offQ[b] + chunk * 16, lds_addr(&sQ[s][(wv * QC + b) * 1024]));
+      dma16(base, offQ[b] + chunk * 16, lds_addr(sQ[0] + s * (BN * RB) + (wv * QC + b) * 1024));
     }
   };
   int ct = 0, ik = 0, bi = 0, bc = 0;  // copy cursor: tile ct, its stage ik, buffer bi; the buffer bc that is read next
   auto advance = [&]() {
-    bi ^= 1;
+    bi = bi + 1 == S ? 0 : bi + 1;
     if (++ik == nk) {
       ik = 0;
       if (++ct < my_tiles) setup(decode(ct));
@@ -399,67 +409,83 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wide_kernel(Params p) {
   if (my_tiles) {
     setup(decode(0));
     for_each<NCOPY>([&](auto c) { copy(c, 0, 0); });
+#pragma unroll
+    for (int s = 1; s < S - 1; ++s) {
+      advance();
+      for_each<NCOPY>([&](auto c) { copy(c, ik, s); });
+    }
   }
+  // The stage that is read next has landed (behind its copies only those of the S - 2 stages after
+  // it need still be on their way; an epilogue's loads and stores make the wait longer, not
+  // shorter), and every read of the buffer that is filled next is done.
+  auto stage_in = [&]() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(NCOPY * (S - 2)) : "memory");
+  };
+  i32x4_t acc[TM][TN];
+  int wave_row = 0;
+  // a tile's stages by a wave with MB blocks of rows
+  auto stages = [&](auto mb_c) {
+    constexpr int MB = decltype(mb_c)::value;
+    for (int kt = 0; kt < nk; ++kt) {
+      advance();  // ahead of the MFMAs, which the compiler would otherwise sink behind its branches
+      stage_in();
+      const uint8_t *cP = sP[0] + bc * (BM * RB), *cQ = sQ[0] + bc * (BN * RB);
+      bc = bc + 1 == S ? 0 : bc + 1;
+      if constexpr (MB == 0) {
+        for_each<NCOPY>([&](auto c) { copy(c, ik, bi); });
+      } else {
+        auto frag = [&](const uint8_t* tile, int row, int step) {
+          return *(const i32x4_t*)(tile + row * RB + (((2 * g4 + step) ^ swz(row)) << 4));
+        };
+        i32x4_t af[MB], bq[2];
+        // the next stage's copies go between the MFMAs
+        auto step = [&](auto s_c) {
+          constexpr int st = decltype(s_c)::value;
+#pragma unroll
+          for (int i = 0; i < MB; ++i) af[i] = frag(cP, (wave_row + i) * 16 + ml, st);
+          bq[0] = frag(cQ, wn * TN * 16 + ml, st);
+          for_each<TN>([&](auto j_c) {
+            constexpr int j = decltype(j_c)::value;
+            if constexpr (j + 1 < TN) bq[(j + 1) & 1] = frag(cQ, (wn * TN + j + 1) * 16 + ml, st);
+#pragma unroll
+            for (int i = 0; i < MB; ++i)
+              acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bq[j & 1], af[i], acc[i][j], 0, 0, 0);
+            constexpr int slot = st * TN + j, slots = 2 * TN;
+            for_each<NCOPY>([&](auto c) {
+              if constexpr (decltype(c)::value * slots / NCOPY == slot) copy(c, ik, bi);
+            });
+            __builtin_amdgcn_sched_barrier(0);
+          });
+        };
+        step(std::integral_constant<int, 0>{});
+        step(std::integral_constant<int, 1>{});
+      }
+    }
+  };
 
   for (int t = 0; t < my_tiles; ++t) {
     const TileRef cur = decode(t);
-    const int row0 = cur.row0, seg1 = cur.seg1;
-    // the stage that is read next has landed (its copies are the last there are; an epilogue's
-    // stores are waited for too), and every read of the buffer that is filled next is done
-    auto stage_in = [&]() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
-    // 16-row blocks of this wave with rows in them; a wave without any only copies
-    const int tmv = min(TM, max(0, (seg1 - (row0 + wm * TM * 16) + 15) >> 4));
-    if (tmv == 0) {
-      for (int kt = 0; kt < nk; ++kt) {
-        advance();
-        stage_in();
-        bc ^= 1;
-        for_each<NCOPY>([&](auto c) { copy(c, ik, bi); });
-      }
-      continue;
-    }
-    i32x4_t acc[TM][TN];
+    const int row0 = cur.row0, end = cur.end;
+    const int blocks = (end - row0 + 15) >> 4, each = (blocks + WM - 1) / WM;
+    wave_row = wm * each;  // this wave's first block, and their number
+    const int tmv = max(0, min(each, blocks - wave_row));
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
       for (int j = 0; j < TN; ++j) acc[i][j] = i32x4_t{0, 0, 0, 0};
-
-    for (int kt = 0; kt < nk; ++kt) {
-      advance();  // ahead of the MFMAs, which the compiler would otherwise sink behind its branches
-      stage_in();
-      const uint8_t *cP = sP[bc], *cQ = sQ[bc];
-      bc ^= 1;
-      auto frag = [&](const uint8_t* tile, int row, int step) {
-        return *(const i32x4_t*)(tile + row * RB + (((2 * g4 + step) ^ swz(row)) << 4));
-      };
-      i32x4_t af[TM], bq[2];
-      // the next stage's copies go between the MFMAs
-      auto step = [&](auto s_c) {
-        constexpr int st = decltype(s_c)::value;
-#pragma unroll
-        for (int i = 0; i < TM; ++i) af[i] = frag(cP, (wm * TM + i) * 16 + ml, st);
-        bq[0] = frag(cQ, wn * TN * 16 + ml, st);
-        for_each<TN>([&](auto j_c) {
-          constexpr int j = decltype(j_c)::value;
-          if constexpr (j + 1 < TN) bq[(j + 1) & 1] = frag(cQ, (wn * TN + j + 1) * 16 + ml, st);
-#pragma unroll
-          for (int i = 0; i < TM; ++i)
-            acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bq[j & 1], af[i], acc[i][j], 0, 0, 0);
-          constexpr int slot = st * TN + j, slots = 2 * TN;
-          for_each<NCOPY>([&](auto c) {
-            if constexpr (decltype(c)::value * slots / NCOPY == slot) copy(c, ik, bi);
-          });
-          __builtin_amdgcn_sched_barrier(0);
-        });
-      };
-      step(std::integral_constant<int, 0>{});
-      step(std::integral_constant<int, 1>{});
-    }
+    bool done = false;
+    for_each<TM + 1>([&](auto mb) {
+      if (!done && tmv == decltype(mb)::value) {
+        stages(mb);
+        done = true;
+      }
+    });
+    if (tmv == 0) continue;
 
     // ---- epilogue: lane holds C[m = .. + ml][n = .. + 4 g4 .. + 3] of each 16-column block ----
     float rs[TM];
 #pragma unroll
-    for (int i = 0; i < TM; ++i) rs[i] = p.s[min(row0 + (wm * TM + i) * 16 + ml, seg1 - 1)];
+    for (int i = 0; i < TM; ++i) rs[i] = p.s[min(row0 + (wave_row + i) * 16 + ml, end - 1)];
 #pragma unroll
     for (int b = 0; b < TN / 2; ++b) {
       float ca[4], cb[4], ba[4], bb[4];
@@ -472,7 +498,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wide_kernel(Params p) {
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
           if (i >= tmv) continue;
-          const int r = row0 + (wm * TM + i) * 16 + ml;
+          const int r = row0 + (wave_row + i) * 16 + ml;
           float v[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
@@ -480,7 +506,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wide_kernel(Params p) {
             if constexpr (ACT == kOssGLU) { g += ba[k]; u += bb[k]; }
             v[k] = activation(ACT, g, u, p.limit);
           }
-          if (r < seg1) *(float4*)(p.h + (int64_t)r * N + hc) = make_float4(v[0], v[1], v[2], v[3]);
+          if (r < end) *(float4*)(p.h + (int64_t)r * N + hc) = make_float4(v[0], v[1], v[2], v[3]);
         }
       } else {
         const int n0 = cur.nt * BN + wn * TN * 16 + b * 32;
@@ -492,7 +518,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wide_kernel(Params p) {
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
           if (i >= tmv) continue;
-          const int r = row0 + (wm * TM + i) * 16 + ml;
+          const int r = row0 + (wave_row + i) * 16 + ml;
           float lo[4], hi[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
@@ -500,13 +526,13 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wide_kernel(Params p) {
             hi[k] = (float)acc[i][2 * b + 1][k] * rs[i] * cb[k] + bb[k];
           }
           if (p.y_f32 || N % 8) {
-            if (r < seg1) {
+            if (r < end) {
               store4(p, r, n0 + 4 * g4, lo);
               store4(p, r, n0 + 16 + 4 * g4, hi);
             }
           } else {
             const uint4 v = span64(pack4(lo), pack4(hi), lane);
-            if (r < seg1 && n0 + 8 * g4 < N) *(uint4*)((uint16_t*)p.y + (int64_t)r * N + n0 + 8 * g4) = v;
+            if (r < end && n0 + 8 * g4 < N) *(uint4*)((uint16_t*)p.y + (int64_t)r * N + n0 + 8 * g4) = v;
           }
         }
       }
@@ -552,8 +578,9 @@ __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
   } else {
     segments_wave(p, s_seg, s_tile, tiles_of);
   }
-  const int64_t total = s_tile[E];
-  const int u0 = (int)(total * blockIdx.x / gridDim.x), u1 = (int)(total * (blockIdx.x + 1) / gridDim.x);
+  // consecutive units, of which the first workgroups have one more
+  const uint32_t total = (uint32_t)__builtin_amdgcn_readfirstlane(s_tile[E]), per = total / gridDim.x, more = total - per * gridDim.x;
+  const int u0 = (int)(blockIdx.x * per + min(blockIdx.x, more)), u1 = u0 + (int)per + (blockIdx.x < more ? 1 : 0);
   const int groups = (nst + KS * DEPTH - 1) / (KS * DEPTH);  // of a wave's stages ks, ks + KS, ...
 
   struct Unit { int e, rt, cb; };
@@ -570,20 +597,20 @@ __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
     return r;
   };
   // this lane's weight row of a unit (blocks past the last one repeat it, rows past N the last row)
+  const int8_t* lane_row = MODE == kGateUp ? (ml < 8 ? p.wa : p.wb) + (uint32_t)((ml & 7) * p.r_rows * K) : p.wa;
   auto weight_row = [&](const Unit& u) {
-    const int blk = min(u.cb * NB + nb, nblk - 1);
-    if (MODE == kGateUp)
-      return (ml < 8 ? p.wa : p.wb) + (u.e * p.e_rows + (int64_t)(blk * 8 + (ml & 7)) * p.r_rows) * K;
-    return p.wa + (u.e * p.e_rows + min(blk * 16 + ml, N - 1)) * (int64_t)K;
+    const int first = min(u.cb * NB + nb, nblk - 1) * COLS;
+    const int8_t* row = lane_row + (u.e * p.e_rows + (int64_t)first * p.r_rows) * K;
+    return MODE == kGateUp ? row : row + (uint32_t)(min(ml, N - 1 - first) * K);
   };
   struct Group { i32x4_t w[DEPTH][2]; };
   // chunks past a row's end repeat its last one, against zeros in LDS
   auto load = [&](Group& g, const int8_t* row, int i) {
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d) {
-      const int c = 8 * (ks + KS * (i * DEPTH + d)) + 2 * g4;
-      g.w[d][0] = *(const i32x4_t*)(row + min(c, KC - 1) * 16);
-      g.w[d][1] = *(const i32x4_t*)(row + min(c + 1, KC - 1) * 16);
+      const int c = 8 * (ks + KS * (i * DEPTH + d)) + g4;
+      g.w[d][0] = *(const i32x4_t*)(row + (uint32_t)(min(c, KC - 1) * 16));
+      g.w[d][1] = *(const i32x4_t*)(row + (uint32_t)(min(c + 4, KC - 1) * 16));
     }
   };
   // A thread's part of a unit's results: columns 4 fc .. of block fb, row fr.
@@ -679,18 +706,7 @@ __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
   i32x4_t acc[TM];
 #pragma unroll
   for (int i = 0; i < TM; ++i) acc[i] = i32x4_t{0, 0, 0, 0};
-  // group `at` of unit t from `cur`, with the next one's loads on their way into `nxt`; false where
-  // that one is of other rows, or there is none
-  auto step = [&](Group& cur, Group& nxt) __attribute__((always_inline)) {
-    const bool last = at + 1 == groups;
-    Unit to = u;
-    Cols next{};
-    if (last) {
-      if (t + 1 < u1) to = decode(t + 1);
-      wrow = weight_row(to);
-      load_cols(next, to);
-    }
-    load(nxt, wrow, last ? 0 : at + 1);
+  auto multiply = [&](const Group& g) {
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d) {
       const int st = ks + KS * (at * DEPTH + d);
@@ -698,11 +714,29 @@ __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
           if (i > 0 && rows <= 16 * i) continue;
-          const uint8_t* a = sP + (16 * i + ml) * stride + st * 128 + g4 * 32;
-          acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(cur.w[d][0], *(const i32x4_t*)a, acc[i], 0, 0, 0);
-          acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(cur.w[d][1], *(const i32x4_t*)(a + 16), acc[i], 0, 0, 0);
+          const uint8_t* a = sP + (16 * i + ml) * stride + st * 128 + g4 * 16;
+          acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(g.w[d][0], *(const i32x4_t*)a, acc[i], 0, 0, 0);
+          acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(g.w[d][1], *(const i32x4_t*)(a + 64), acc[i], 0, 0, 0);
         }
       }
+    }
+  };
+  // group `at` of unit t from `cur`, with the next one's loads on their way into `nxt`; false where
+  // that one is of other rows, or there is none
+  auto step = [&](Group& cur, Group& nxt) __attribute__((always_inline)) {
+    const bool last = at + 1 == groups;
+    Unit to = u;
+    Cols next{};
+    if (last && t + 1 == u1) {
+      multiply(cur);
+    } else {
+      if (last) {
+        to = decode(t + 1);
+        wrow = weight_row(to);
+        load_cols(next, to);
+      }
+      load(nxt, wrow, last ? 0 : at + 1);
+      multiply(cur);
     }
     if (!last) {
       ++at;
@@ -780,20 +814,20 @@ constexpr int kLdsMost = 156 * 1024;  // dynamic LDS of the narrow kernel
 static bool aligned16(const void* a) { return ((uintptr_t)a & 15) == 0; }
 static int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 
-template <int MODE, int ACT, int WM, int WN, int TM, int TN>
+template <int MODE, int ACT, int WM, int WN, int TM, int TN, int S, int OCC>
 static void launch_tiles(const Params& p, hipStream_t stream) {
   constexpr int BM = 16 * WM * TM, BN = 16 * WN * TN;
   const int64_t nt = MODE == kGateUp ? (p.N + BN / 2 - 1) / (BN / 2) : (p.N + BN - 1) / BN;
   int64_t g = (p.R / BM + (p.R < p.E ? p.R : p.E)) * nt;
-  const int64_t most = (int64_t)cu_count() * (8 / (WM * WN));
+  const int64_t most = (int64_t)cu_count() * OCC;
   if (g > most) g = most;
   if (g >= 8) g -= g % 8;
-  hipLaunchKernelGGL((wide_kernel<MODE, ACT, WM, WN, TM, TN>), dim3((unsigned)g), dim3(64 * WM * WN),
+  hipLaunchKernelGGL((wide_kernel<MODE, ACT, WM, WN, TM, TN, S>), dim3((unsigned)g), dim3(64 * WM * WN),
                      2 * (p.E + 1) * sizeof(int), stream, p);
 }
 template <int MODE, int ACT>
 static void launch_wide(const Params& p, hipStream_t stream) {
-  launch_tiles<MODE, ACT, 4, 2, 4, 8>(p, stream);
+  launch_tiles<MODE, ACT, 4, 2, 4, 8, 2, 1>(p, stream);
 }
 
 static int narrow_blocks(int K, int E) {
