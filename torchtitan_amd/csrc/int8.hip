@@ -230,19 +230,10 @@ struct Params {
 
 __device__ __forceinline__ int64_t count_of(const Params& p, int e) { return p.counts ? p.counts[e] : p.R; }
 
-// sigmoid(z) = 1 / (1 + 2^t), t = -z log2 e, on the hardware's exponential and reciprocal (each
-// within a unit of the last place). t's rounding, which 2^t would magnify by |t|, is made good: the
-// result feeds a rounding to codes, which moves with every unit here.
-__device__ __forceinline__ float sigmoid(float z) {
-  constexpr float kL = -1.44269504088896341f, kLow = -1.44269504088896341 - (double)-1.44269504088896341f;
-  const float t = z * kL, lo = fmaf(z, kL, -t) + z * kLow;
-  const float e = __builtin_amdgcn_exp2f(t);
-  return __builtin_amdgcn_rcpf(1.0f + (e < 1e30f ? fmaf(e * 0.693147180559945309f, lo, e) : e));
-}
 __device__ __forceinline__ float activation(int act, float g, float u, float limit) {
-  if (act == kSwiGLU) return g * sigmoid(g) * u;
+  if (act == kSwiGLU) return g * mx::sigmoid(g) * u;
   const float a = g > limit ? limit : g, b = u < -limit ? -limit : (u > limit ? limit : u);  // NaN passes
-  return a * sigmoid(kOssAlpha * a) * (b + 1.0f);
+  return a * mx::sigmoid(kOssAlpha * a) * (b + 1.0f);
 }
 
 // scales of weight rows n .. n + 3 of expert e (uniform), linear's biases, gpt-oss's of gate and up
@@ -285,7 +276,7 @@ __device__ __forceinline__ void store4(const Params& p, int64_t r, int n, const 
   } else {
     uint16_t* y = (uint16_t*)p.y + r * p.N + n;
     if (p.N % 4 == 0) {
-      if (n < p.N) *(uint2*)y = pack4(v);
+      if (n < p.N) *(uint2*)y = pack4_mid(v);
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) if (n + i < p.N) y[i] = (uint16_t)f2bf(v[i]);
@@ -435,7 +426,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wide_kernel(Params p) {
         for_each<NCOPY>([&](auto c) { copy(c, ik, bi); });
       } else {
         auto frag = [&](const uint8_t* tile, int row, int step) {
-          return *(const i32x4_t*)(tile + row * RB + (((2 * g4 + step) ^ swz(row)) << 4));
+          return *(const i32x4_t*)(tile + row * RB + (((4 * step + g4) ^ swz(row)) << 4));
         };
         i32x4_t af[MB], bq[2];
         // the next stage's copies go between the MFMAs
@@ -513,8 +504,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wide_kernel(Params p) {
         if (n0 >= N) continue;
         col_scales(p.sa, p, cur.e, n0 + 4 * g4, ca);
         col_scales(p.sa, p, cur.e, n0 + 16 + 4 * g4, cb);
-        col_bias(p, cur.e, n0 + 4 * g4, ba);
-        col_bias(p, cur.e, n0 + 16 + 4 * g4, bb);
+        if (p.bias) {
+          col_bias(p, cur.e, n0 + 4 * g4, ba);
+          col_bias(p, cur.e, n0 + 16 + 4 * g4, bb);
+        }
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
           if (i >= tmv) continue;
@@ -522,8 +515,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wide_kernel(Params p) {
           float lo[4], hi[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            lo[k] = (float)acc[i][2 * b][k] * rs[i] * ca[k] + ba[k];
-            hi[k] = (float)acc[i][2 * b + 1][k] * rs[i] * cb[k] + bb[k];
+            lo[k] = (float)acc[i][2 * b][k] * rs[i] * ca[k];
+            hi[k] = (float)acc[i][2 * b + 1][k] * rs[i] * cb[k];
+          }
+          if (p.bias) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) { lo[k] += ba[k]; hi[k] += bb[k]; }
           }
           if (p.y_f32 || N % 8) {
             if (r < end) {
@@ -531,7 +528,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wide_kernel(Params p) {
               store4(p, r, n0 + 16 + 4 * g4, hi);
             }
           } else {
-            const uint4 v = span64(pack4(lo), pack4(hi), lane);
+            const uint4 v = span64(pack4_mid(lo), pack4_mid(hi), lane);
             if (r < end && n0 + 8 * g4 < N) *(uint4*)((uint16_t*)p.y + (int64_t)r * N + n0 + 8 * g4) = v;
           }
         }
