@@ -414,42 +414,64 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wide_kernel(Params p) {
   };
   i32x4_t acc[TM][TN];
   int wave_row = 0;
-  // a tile's stages by a wave with MB blocks of rows
+  // A tile's stages by a wave with MB blocks of rows: 2 TN blocks of 16 columns by 64 k each, the
+  // fragments read two blocks ahead. The barrier between two stages lies ahead of the last two
+  // blocks, whose fragments are there by then, so that MFMAs cover the wait and the next stage's
+  // first reads; copies go between the MFMAs of a stage's first half, to land within it.
   auto stages = [&](auto mb_c) {
-    constexpr int MB = decltype(mb_c)::value;
+    constexpr int MB = decltype(mb_c)::value, NB = 2 * TN;
+    const uint8_t *cP, *cQ;
+    auto enter = [&]() {
+      stage_in();
+      cP = sP[0] + bc * (BM * RB);
+      cQ = sQ[0] + bc * (BN * RB);
+      bc = bc + 1 == S ? 0 : bc + 1;
+    };
+    auto frag = [&](const uint8_t* tile, int row, int step) {
+      return *(const i32x4_t*)(tile + row * RB + (((4 * step + g4) ^ swz(row)) << 4));
+    };
+    i32x4_t af[2][MB > 0 ? MB : 1], bq[4];
+    auto read_q = [&](auto n_c) {
+      constexpr int n = decltype(n_c)::value % NB;
+      bq[n % 4] = frag(cQ, (wn * TN + n % TN) * 16 + ml, n / TN);
+    };
+    auto read_first = [&]() {
+      read_q(std::integral_constant<int, 0>{});
+#pragma unroll
+      for (int i = 0; i < MB; ++i) af[0][i] = frag(cP, (wave_row + i) * 16 + ml, 0);
+      read_q(std::integral_constant<int, 1>{});
+    };
+    enter();
+    if constexpr (MB > 0) read_first();
     for (int kt = 0; kt < nk; ++kt) {
       advance();  // ahead of the MFMAs, which the compiler would otherwise sink behind its branches
-      stage_in();
-      const uint8_t *cP = sP[0] + bc * (BM * RB), *cQ = sQ[0] + bc * (BN * RB);
-      bc = bc + 1 == S ? 0 : bc + 1;
       if constexpr (MB == 0) {
         for_each<NCOPY>([&](auto c) { copy(c, ik, bi); });
+        if (kt + 1 < nk) enter();
       } else {
-        auto frag = [&](const uint8_t* tile, int row, int step) {
-          return *(const i32x4_t*)(tile + row * RB + (((4 * step + g4) ^ swz(row)) << 4));
-        };
-        i32x4_t af[MB], bq[2];
-        // the next stage's copies go between the MFMAs
-        auto step = [&](auto s_c) {
-          constexpr int st = decltype(s_c)::value;
+        for_each<NB>([&](auto n_c) {
+          constexpr int n = decltype(n_c)::value, st = n / TN, j = n % TN, first = TN > MB ? TN - MB : 0;
+          if constexpr (n + 2 < NB) {
+            read_q(std::integral_constant<int, n + 2>{});
+          } else if constexpr (n + 2 == NB) {
+            if (kt + 1 < nk) {
+              enter();
+              read_first();
+            }
+          }
+          if constexpr (st == 0 && j >= first) {
 #pragma unroll
-          for (int i = 0; i < MB; ++i) af[i] = frag(cP, (wave_row + i) * 16 + ml, st);
-          bq[0] = frag(cQ, wn * TN * 16 + ml, st);
-          for_each<TN>([&](auto j_c) {
-            constexpr int j = decltype(j_c)::value;
-            if constexpr (j + 1 < TN) bq[(j + 1) & 1] = frag(cQ, (wn * TN + j + 1) * 16 + ml, st);
+            for (int i = (j - first) * MB / (TN - first); i < (j - first + 1) * MB / (TN - first); ++i)
+              af[1][i] = frag(cP, (wave_row + i) * 16 + ml, 1);
+          }
 #pragma unroll
-            for (int i = 0; i < MB; ++i)
-              acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bq[j & 1], af[i], acc[i][j], 0, 0, 0);
-            constexpr int slot = st * TN + j, slots = 2 * TN;
-            for_each<NCOPY>([&](auto c) {
-              if constexpr (decltype(c)::value * slots / NCOPY == slot) copy(c, ik, bi);
-            });
-            __builtin_amdgcn_sched_barrier(0);
+          for (int i = 0; i < MB; ++i)
+            acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bq[n % 4], af[st][i], acc[i][j], 0, 0, 0);
+          for_each<NCOPY>([&](auto c) {
+            if constexpr (decltype(c)::value * TN / NCOPY == n) copy(c, ik, bi);
           });
-        };
-        step(std::integral_constant<int, 0>{});
-        step(std::integral_constant<int, 1>{});
+          __builtin_amdgcn_sched_barrier(0);
+        });
       }
     }
   };
