@@ -833,12 +833,35 @@ constexpr int kLdsMost = 156 * 1024;  // dynamic LDS of the narrow kernel
 static bool aligned16(const void* a) { return ((uintptr_t)a & 15) == 0; }
 static int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 
-template <int MODE, int ACT, int WM, int WN, int TM, int TN, int S, int OCC>
-static void launch_tiles(const Params& p, hipStream_t stream) {
+// The wide kernel's tiles, with what a stage of 128 k and the rest of a tile take in 10 ns, measured
+// where they fill the chip (16384 rows by 7168 x 7168), and the workgroups a CU holds.
+struct Tile { int bm, bn, per_cu, stage, rest; };
+constexpr Tile kTiles[] = {{256, 256, 1, 145, 550}, {128, 256, 1, 90, 280}, {64, 128, 2, 65, 150}, {64, 64, 2, 43, 100}};
+
+// The tile with the least time by that count: as many rounds of the chip as its tiles take, half a
+// tile more for each expert that can have rows. Measured against the others (us, 256 x 256 / 128 x
+// 256 / 64 x 128 / 64 x 64): 16384 x 7168 x 7168 732 / 808 / 1098 / 1440; 2048 x 2304 x 2304 40 / 29
+// / 36 / 36; 1024 x 2304 x 2304 38 / 27 / 23 / 27; 1003 x 2880 x 1001 59 / 37 / 22 / 19; 131072 rows
+// on 256 experts of 2304 x 1024 564 / 549 / 708 / 834; 8200 on 32 of 7168 x 2048 242 / 210 / 270 / 298.
+static int pick_tile(int64_t R, int64_t E, int64_t K, int64_t cols, int64_t cus) {
+  const int64_t nk = (K + 127) / 128, used = R < E ? R : E;
+  int best = 0;
+  int64_t least = INT64_MAX;
+  for (int i = 0; i < 4; ++i) {
+    const Tile& t = kTiles[i];
+    const int64_t mt = E == 1 ? (R + t.bm - 1) / t.bm : R / t.bm + (used + 1) / 2, tiles = mt * ((cols + t.bn - 1) / t.bn);
+    const int64_t time = (tiles + cus * t.per_cu - 1) / (cus * t.per_cu) * (nk * t.stage + t.rest);
+    if (time < least) { least = time; best = i; }
+  }
+  return best;
+}
+
+template <int MODE, int ACT, int WM, int WN, int TM, int TN, int S>
+static void launch_tiles(const Params& p, int per_cu, hipStream_t stream) {
   constexpr int BM = 16 * WM * TM, BN = 16 * WN * TN;
   const int64_t nt = MODE == kGateUp ? (p.N + BN / 2 - 1) / (BN / 2) : (p.N + BN - 1) / BN;
   int64_t g = (p.R / BM + (p.R < p.E ? p.R : p.E)) * nt;
-  const int64_t most = (int64_t)cu_count() * OCC;
+  const int64_t most = (int64_t)cu_count() * per_cu;
   if (g > most) g = most;
   if (g >= 8) g -= g % 8;
   hipLaunchKernelGGL((wide_kernel<MODE, ACT, WM, WN, TM, TN, S>), dim3((unsigned)g), dim3(64 * WM * WN),
@@ -846,7 +869,14 @@ static void launch_tiles(const Params& p, hipStream_t stream) {
 }
 template <int MODE, int ACT>
 static void launch_wide(const Params& p, hipStream_t stream) {
-  launch_tiles<MODE, ACT, 4, 2, 4, 8, 2, 1>(p, stream);
+  const int tile = pick_tile(p.R, p.E, p.K, MODE == kGateUp ? 2 * (int64_t)p.N : p.N, cu_count());
+  const int per_cu = kTiles[tile].per_cu;
+  switch (tile) {
+    case 0: return launch_tiles<MODE, ACT, 4, 2, 4, 8, 2>(p, per_cu, stream);
+    case 1: return launch_tiles<MODE, ACT, 2, 4, 4, 4, 3>(p, per_cu, stream);
+    case 2: return launch_tiles<MODE, ACT, 2, 2, 2, 4, 3>(p, per_cu, stream);
+    default: return launch_tiles<MODE, ACT, 2, 2, 2, 2, 4>(p, per_cu, stream);
+  }
 }
 
 static int narrow_blocks(int K, int E) {
@@ -863,10 +893,9 @@ static void launch_narrow_of(const Params& p, hipStream_t stream) {
       (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsMost);
     hipLaunchKernelGGL(kernel, dim3((unsigned)std::min(units, most)), dim3(512), (unsigned)lds, stream, p);
   };
-  if (tm == 1 && tiles * nblk < 4 * most) launch(narrow_kernel<MODE, ACT, T, 1, 1, 1>, 1);
-  else if (tiles * nblk < 4 * most) launch(narrow_kernel<MODE, ACT, T, 1, 2, 1>, 1);
-  else if (tm == 1) launch(narrow_kernel<MODE, ACT, T, 4, 1, 1>, 4);
-  else launch(narrow_kernel<MODE, ACT, T, 4, 2, 1>, 4);
+  const bool small = tiles * nblk <= most;
+  if (tm == 1) small ? launch(narrow_kernel<MODE, ACT, T, 1, 1, 1>, 1) : launch(narrow_kernel<MODE, ACT, T, 4, 1, 1>, 4);
+  else small ? launch(narrow_kernel<MODE, ACT, T, 1, 2, 1>, 1) : launch(narrow_kernel<MODE, ACT, T, 4, 2, 1>, 4);
 }
 template <int MODE, int ACT>
 static void launch_narrow(const Params& p, hipStream_t stream) {
