@@ -222,7 +222,7 @@ def stream_of(t: torch.Tensor) -> int:
 
 def require_gpu(*tensors: torch.Tensor | None) -> None:
     for t in tensors:
-        if t is not None and t.device.type != "cuda":
+        if t is not None and not t.is_cuda:
             raise MoEKernelError(
                 "the MI355X MoE kernels run on the GPU only; got a tensor on " f"{t.device}"
             )

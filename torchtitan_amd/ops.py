@@ -1724,23 +1724,23 @@ _I8_BARE = torch.library.Library("moe_mi355x_int8_bare", "FRAGMENT")  # (as _MX_
 INT8_MULTIPLE = 16  # of the products' contractions: weight rows are read in 16-byte pieces
 INT8_MAX_K = 131072  # past it a sum of code products can leave 32 bits
 
+# A generation step's calls take the host as long as the GPU, so what is right is checked in few
+# steps, and a message is put together where something is not.
 
-def _check_int8(op: str, name: str, q: Tensor, scale: Tensor, shape: tuple | None = None) -> None:
-    """A matrix in codes: q [.., K] int8 and scale [..] fp32 on one device, of `shape` where one is given."""
-    if q.dtype != torch.int8 or scale.dtype != torch.float32:
+
+def _check_int8(op: str, name: str, q: Tensor, scale: Tensor, shape: tuple) -> None:
+    """A matrix in codes: q of `shape` int8 and scale of shape[:-1] fp32 on one device."""
+    if q.dtype is torch.int8 and scale.dtype is torch.float32 and q.shape == shape and scale.shape == shape[:-1] \
+            and q.get_device() == scale.get_device():
+        return
+    if q.dtype is not torch.int8 or scale.dtype is not torch.float32:
         raise TypeError(f"{op} expects int8 {name} and float32 scales, got {q.dtype} and {scale.dtype}")
-    qs, ss = q.shape, scale.shape
-    if not qs or ss != qs[:-1] or q.device != scale.device:
-        raise ValueError(f"{op}: {name} {tuple(qs)} on {q.device} and its scales {tuple(ss)} on {scale.device} do not "
-                         "belong together")
-    if shape is not None and qs != shape:
-        raise ValueError(f"{op} expects {name} of {list(shape)}, got {list(qs)}")
+    raise ValueError(f"{op} expects {name} of {list(shape)} with scales of {list(shape[:-1])} on one device, got "
+                     f"{list(q.shape)} on {q.device} and {list(scale.shape)} on {scale.device}")
 
 
-def _check_int8_bias(op: str, bias: Tensor | None, shape: tuple, like: Tensor) -> int:
+def _check_int8_bias(op: str, bias: Tensor, shape: tuple, like: Tensor) -> int:
     """The bias's dtype code."""
-    if bias is None:
-        return 0
     if bias.dtype not in DTYPE_CODES:
         raise TypeError(f"{op} takes biases in bfloat16 and float32, got {bias.dtype}")
     if bias.shape != shape or bias.device != like.device:
@@ -1756,14 +1756,25 @@ def _check_int8_dims(op: str, e: int, *contractions: int) -> None:
             raise ValueError(f"{op} takes contractions that are multiples of {INT8_MULTIPLE} up to {INT8_MAX_K}, got {k}")
 
 
+def _check_int8_devices(op: str, x: Tensor, *others: Tensor) -> None:
+    here = x.get_device()
+    for t in others:
+        if t.get_device() != here:
+            raise ValueError(f"{op}: tensors on more than one device")
+
+
 def _int8_code(op: str, dtype: torch.dtype) -> int:
-    if dtype not in DTYPE_CODES:
+    code = DTYPE_CODES.get(dtype)
+    if code is None:
         raise TypeError(f"{op} supports bfloat16 and float32, got {dtype}")
-    return DTYPE_CODES[dtype]
+    return code
 
 
 def _no_int8_gradients(op: str, *tensors: Tensor | None) -> None:
-    _no_gradients(op, *tensors, instead="codes are not differentiable: train on the bf16 weights")
+    if torch.is_grad_enabled() or forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and (t.requires_grad or forward_ad._current_level >= 0):
+                _no_gradients(op, t, instead="codes are not differentiable: train on the bf16 weights")
 
 
 @_mx_op("int8_quantize(Tensor x) -> (Tensor, Tensor)", _I8)
@@ -1772,14 +1783,15 @@ def _int8_quantize(x: Tensor) -> tuple[Tensor, Tensor]:
     code = _int8_code("int8_quantize", x.dtype)
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"int8_quantize expects rows of at least one column, got {tuple(x.shape)}")
-    *lead, cols = x.shape
-    ld = cols
-    if x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= cols:
-        ld = x.stride(0)  # a slice of wider rows is read where it is
-    else:
-        x = x.contiguous()
-    q = x.new_empty(x.shape, dtype=torch.int8)
-    scale = x.new_empty(lead, dtype=torch.float32)
+    shape = x.shape
+    ld = cols = shape[-1]
+    if not x.is_contiguous():
+        if len(shape) == 2 and x.stride(1) == 1 and x.stride(0) >= cols:
+            ld = x.stride(0)  # a slice of wider rows is read where it is
+        else:
+            x = x.contiguous()
+    q = torch.empty_like(x, dtype=torch.int8) if ld == cols else x.new_empty(shape, dtype=torch.int8)
+    scale = x.new_empty(shape[:-1], dtype=torch.float32)
     with _guard(x):
         call("moe_int8_quant_rows", ptr(x), ld, scale.numel(), cols, code, ptr(q), ptr(scale), stream_of(x))
     return q, scale
@@ -1803,11 +1815,11 @@ def int8_quantize(x: Tensor) -> tuple[Tensor, Tensor]:
 def _int8_dequantize(q: Tensor, scale: Tensor, dtype: torch.dtype) -> Tensor:
     require_gpu(q, scale)
     code = _int8_code("int8_dequantize", dtype)
-    _check_int8("int8_dequantize", "q", q, scale)
-    if q.shape[-1] < 1:
+    if q.dim() < 1 or q.shape[-1] < 1:
         raise ValueError(f"int8_dequantize expects rows of at least one column, got {tuple(q.shape)}")
+    _check_int8("int8_dequantize", "q", q, scale, q.shape)
     q, scale = q.contiguous(), scale.contiguous()
-    x = q.new_empty(q.shape, dtype=dtype)
+    x = torch.empty_like(q, dtype=dtype)
     with _guard(q):
         call("moe_int8_dequant_rows", ptr(q), ptr(scale), scale.numel(), q.shape[-1], code, ptr(x), stream_of(q))
     return x
@@ -1831,35 +1843,41 @@ def _int8_workspace_bytes(r: int, e: int, k: int, hidden: int | None) -> int:
     return int(lib().moe_int8_layer_workspace_bytes(r, e, k, hidden))
 
 
-def _int8_product(op: str, x: Tensor, qw: Tensor, sw: Tensor, counts: Tensor | None, bias: Tensor | None, rows: int) -> Tensor:
+def _int8_product(op: str, x: Tensor, qw: Tensor, sw: Tensor, counts: Tensor | None, bias: Tensor | None, rows: int,
+                  e: int, n: int, k: int) -> Tensor:
     """x [.., K] of `rows` rows by qw [(E,) N, K]."""
     code = _int8_code(op, x.dtype)
-    e, (n, k) = 1 if counts is None else qw.shape[0], qw.shape[-2:]
+    _check_int8(op, "qw", qw, sw, qw.shape)
     _check_int8_dims(op, e, k)
     if n < 1:
         raise ValueError(f"{op} expects at least one output channel, got {tuple(qw.shape)}")
-    bias_code = _check_int8_bias(op, bias, qw.shape[:-1], x)
-    x, qw, sw = _ready(x), _ready(qw), sw.contiguous()
+    bias_code = 0
     if bias is not None:
+        bias_code = _check_int8_bias(op, bias, qw.shape[:-1], x)
         bias = bias.contiguous()
+    x, qw, sw = _ready(x), _ready(qw), sw.contiguous()
     ws_bytes = _int8_workspace_bytes(rows, e, k, None)
     ws = x.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
-    y = x.new_empty(*x.shape[:-1], n)
+    y = x.new_empty((*x.shape[:-1], n))
     with _guard(x):
         call("moe_int8_linear", ptr(x), code, ptr(qw), ptr(sw), ptr(bias), bias_code, ptr(counts), rows, e, k, n, ptr(ws),
              ws_bytes, ptr(y), stream_of(x))
     return y
 
 
+def _rows_of(xs: torch.Size) -> int:
+    return xs[0] if len(xs) == 2 else xs[:-1].numel()
+
+
 @_mx_op("linear_int8(Tensor x, Tensor qw, Tensor sw, Tensor? bias=None) -> Tensor", _I8_BARE)
 def _linear_int8(x, qw, sw, bias=None):
     op = "linear_int8"
     require_gpu(x, qw, sw, bias)
-    _check_int8(op, "qw", qw, sw)
-    if qw.dim() != 2 or x.dim() < 1 or x.shape[-1] != qw.shape[1] or x.device != qw.device:
-        raise ValueError(f"{op} expects x [.., K] and qw [N, K] on one device, got {tuple(x.shape)} on {x.device} and "
-                         f"{tuple(qw.shape)} on {qw.device}")
-    return _int8_product(op, x, qw, sw, None, bias, x.shape[:-1].numel())
+    xs, ws = x.shape, qw.shape
+    if len(ws) != 2 or not xs or xs[-1] != ws[1] or x.get_device() != qw.get_device():
+        raise ValueError(f"{op} expects x [.., K] and qw [N, K] on one device, got {tuple(xs)} on {x.device} and "
+                         f"{tuple(ws)} on {qw.device}")
+    return _int8_product(op, x, qw, sw, None, bias, _rows_of(xs), 1, *ws)
 
 
 @torch.library.register_fake("moe_mi355x_int8_bare::linear_int8", lib=_I8_BARE)
@@ -1879,11 +1897,14 @@ def linear_int8(x: Tensor, qw: Tensor, sw: Tensor, bias: Tensor | None = None) -
 
 def _int8_counts(op: str, x: Tensor, qw: Tensor, counts: Tensor) -> Tensor:
     """The counts of grouped rows as the kernels read them."""
-    if x.dim() != 2 or qw.dim() != 3 or counts.dim() != 1 or counts.shape[0] != qw.shape[0] or x.shape[1] != qw.shape[2]:
-        raise ValueError(f"{op} expects x [R, K], weights [E, .., K] and counts [E], got {tuple(x.shape)}, "
-                         f"{tuple(qw.shape)}, {tuple(counts.shape)}")
-    _check_counts(op, counts, x, qw)
-    return counts.to(torch.int64).contiguous()
+    xs, ws, cs = x.shape, qw.shape, counts.shape
+    if len(xs) != 2 or len(ws) != 3 or len(cs) != 1 or cs[0] != ws[0] or xs[1] != ws[2]:
+        raise ValueError(f"{op} expects x [R, K], weights [E, .., K] and counts [E], got {tuple(xs)}, {tuple(ws)}, {tuple(cs)}")
+    _check_int8_devices(op, x, qw, counts)
+    if counts.dtype is not torch.int64:
+        _check_counts(op, counts)
+        counts = counts.to(torch.int64)
+    return counts.contiguous()
 
 
 @_mx_op("grouped_linear_int8(Tensor x, Tensor qw, Tensor sw, Tensor num_tokens_per_expert, Tensor? bias=None) -> Tensor",
@@ -1891,9 +1912,8 @@ def _int8_counts(op: str, x: Tensor, qw: Tensor, counts: Tensor) -> Tensor:
 def _grouped_linear_int8(x, qw, sw, num_tokens_per_expert, bias=None):
     op = "grouped_linear_int8"
     require_gpu(x, qw, sw, num_tokens_per_expert, bias)
-    _check_int8(op, "qw", qw, sw)
     counts = _int8_counts(op, x, qw, num_tokens_per_expert)
-    return _int8_product(op, x, qw, sw, counts, bias, x.shape[0])
+    return _int8_product(op, x, qw, sw, counts, bias, x.shape[0], *qw.shape)
 
 
 @torch.library.register_fake("moe_mi355x_int8_bare::grouped_linear_int8", lib=_I8_BARE)
@@ -1911,19 +1931,18 @@ def grouped_linear_int8(x: Tensor, qw: Tensor, sw: Tensor, num_tokens_per_expert
 
 def _int8_swiglu(op: str, x, qw1, sw1, qw2, sw2, qw3, sw3, counts, rows) -> Tensor:
     _check_bf16(op, x=x)
-    lead, (h, d) = qw1.shape[:-2], qw1.shape[-2:]
-    _check_int8(op, "w1", qw1, sw1, (*lead, h, d))
-    _check_int8(op, "w2", qw2, sw2, (*lead, d, h))
-    _check_int8(op, "w3", qw3, sw3, (*lead, h, d))
-    if any(t.device != x.device for t in (qw1, qw2, qw3)):
-        raise ValueError(f"{op}: tensors on more than one device")
-    e = lead[0] if lead else 1
+    shape = qw1.shape
+    e, h, d = shape if len(shape) == 3 else (1, *shape)
+    _check_int8(op, "w1", qw1, sw1, shape)
+    _check_int8(op, "w2", qw2, sw2, (e, d, h) if len(shape) == 3 else (d, h))
+    _check_int8(op, "w3", qw3, sw3, shape)
+    _check_int8_devices(op, x, qw1, qw2, qw3)
     _check_int8_dims(op, e, d, h)
-    x, qw1, qw2, qw3 = map(_ready, (x, qw1, qw2, qw3))
+    x, qw1, qw2, qw3 = _ready(x), _ready(qw1), _ready(qw2), _ready(qw3)
     sw1, sw2, sw3 = sw1.contiguous(), sw2.contiguous(), sw3.contiguous()
     ws_bytes = _int8_workspace_bytes(rows, e, d, h)
     ws = x.new_empty(ws_bytes, dtype=torch.uint8)
-    y = x.new_empty(x.shape)
+    y = torch.empty_like(x)
     with _guard(x):
         call("moe_int8_swiglu", ptr(x), ptr(qw1), ptr(sw1), ptr(qw2), ptr(sw2), ptr(qw3), ptr(sw3), ptr(counts), rows, e, d, h,
              ptr(ws), ws_bytes, ptr(y), stream_of(x))
@@ -1936,7 +1955,7 @@ def _swiglu_ffn_int8(x, qw1, sw1, qw2, sw2, qw3, sw3):
     require_gpu(x, qw1, sw1, qw2, sw2, qw3, sw3)
     if qw1.dim() != 2 or x.dim() < 1 or x.shape[-1] != qw1.shape[1]:
         raise ValueError(f"{op} expects x [.., D] and weights [H, D] and [D, H], got {tuple(x.shape)} and {tuple(qw1.shape)}")
-    return _int8_swiglu(op, x, qw1, sw1, qw2, sw2, qw3, sw3, None, x.shape[:-1].numel())
+    return _int8_swiglu(op, x, qw1, sw1, qw2, sw2, qw3, sw3, None, _rows_of(x.shape))
 
 
 @torch.library.register_fake("moe_mi355x_int8_bare::swiglu_ffn_int8", lib=_I8_BARE)
@@ -1989,8 +2008,7 @@ def _grouped_swiglu_oss_int8(x, qmlp1, smlp1, mlp1_bias, qmlp2, smlp2, mlp2_bias
     h = h2 // 2
     _check_int8(op, "mlp1", qmlp1, smlp1, (e, 2 * h, d))
     _check_int8(op, "mlp2", qmlp2, smlp2, (e, d, h))
-    if qmlp2.device != x.device:
-        raise ValueError(f"{op}: tensors on more than one device")
+    _check_int8_devices(op, x, qmlp1, qmlp2)
     _check_int8_dims(op, e, d, h)
     code = _check_int8_bias(op, mlp1_bias, (e, 2 * h), x)
     if _check_int8_bias(op, mlp2_bias, (e, d), x) != code:
@@ -2001,7 +2019,7 @@ def _grouped_swiglu_oss_int8(x, qmlp1, smlp1, mlp1_bias, qmlp2, smlp2, mlp2_bias
     smlp1, smlp2, b1, b2 = (t.contiguous() for t in (smlp1, smlp2, mlp1_bias, mlp2_bias))
     ws_bytes = _int8_workspace_bytes(r, e, d, h)
     ws = x.new_empty(ws_bytes, dtype=torch.uint8)
-    y = x.new_empty(r, d)
+    y = torch.empty_like(x)
     with _guard(x):
         call("moe_int8_oss", ptr(x), ptr(qmlp1), ptr(smlp1), ptr(b1), ptr(qmlp2), ptr(smlp2), ptr(b2), code, ptr(counts), r, e, d,
              h, float(swiglu_limit), ptr(ws), ws_bytes, ptr(y), stream_of(x))
