@@ -30,9 +30,13 @@ typedef int i32x4_t __attribute__((ext_vector_type(4)));
 constexpr int kMaxK = 131072;
 constexpr float kLeast = 127.0f * 0x1p-126f;
 
-// The columns of a row operand: whole stages of 128, so that every copy of a stage lies inside
-// its row, and zeros behind the contraction meet whatever is read of a weight row there.
-__host__ __device__ constexpr int padded(int cols) { return (cols + 127) / 128 * 128; }
+// The columns of a row operand: whole stages of 128, so that every copy of a stage lies inside its
+// row, and zeros behind the contraction meet whatever is read of a weight row there; kLeastStages
+// at least, behind which everything that a tile's first stage asked for has landed.
+constexpr int kLeastStages = 3;
+__host__ __device__ constexpr int padded(int cols) {
+  return cols <= kLeastStages * 128 ? kLeastStages * 128 : (cols + 127) / 128 * 128;
+}
 
 // ---------------------------------------------------------------------------
 // quantization and its inverse
@@ -301,6 +305,7 @@ __device__ __forceinline__ void zero_rest(const Params& p, int from) {
 // in blocks of 16 between gate and up, so that a lane holds both. An expert's rows are shared
 // evenly by its tiles, a tile's by its waves, in blocks of 16, and a wave's stages are compiled for
 // each number of blocks.
+// The scales and biases of a tile come into LDS with its first stage.
 template <int MODE, int ACT, int WM, int WN, int TM, int TN, int S>
 __global__ __launch_bounds__(64 * WM * WN, 2) void wide_kernel(Params p) {
   constexpr int NW = WM * WN, BM = 16 * WM * TM, BN = 16 * WN * TN;
@@ -309,10 +314,15 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wide_kernel(Params p) {
   constexpr int NCOPY = PW + QC, GM = 8;
   static_assert(PW * RPC * NW == BM && QC * RPC * NW == BN && TN % 2 == 0 && 64 * NW >= 256, "whole copies");
   static_assert(NCOPY * (S - 2) < 64, "vmcnt");
+  static_assert(S - 1 <= kLeastStages, "the copies are in the next tile at most");
+  static_assert(BM % 64 == 0 && BN % 64 == 0 && (BM + BN) / 64 <= NW, "a wave's scales");
   __shared__ __attribute__((aligned(1024))) uint8_t sP[S][BM * RB];
   __shared__ __attribute__((aligned(1024))) uint8_t sQ[S][BN * RB];
   __shared__ int4 s_list[kTileList];  // this workgroup's first tiles: first row, end of its rows, expert, column tile
   __shared__ int s_tmp[NW];
+  // of the tile's columns and rows: scales, and biases as they are stored
+  __shared__ __attribute__((aligned(16))) float s_col[BN], s_row[BM];
+  __shared__ __attribute__((aligned(16))) uint32_t s_bias[BN];
   extern __shared__ __attribute__((aligned(16))) int s_dyn_i[];
   int* s_seg = s_dyn_i;           // E + 1
   int* s_tile = s_seg + p.E + 1;  // E + 1
@@ -321,7 +331,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wide_kernel(Params p) {
   const int wm = wv / WN, wn = wv % WN, ml = lane & 15, g4 = lane >> 4;
   const int E = p.E, K = p.K, N = p.N, KC = K / 16;
   const int NT = MODE == kGateUp ? (N + BN / 2 - 1) / (BN / 2) : (N + BN - 1) / BN;
-  const int nk = (K + RB - 1) / RB;
+  const int nk = padded(K) / RB;
   segments(p, s_seg, s_tile, s_tmp, [&](int rows) { return (rows + BM - 1) / BM * NT; });
   const int total_tiles = s_tile[E], G = gridDim.x;
   // each XCD works on a contiguous window of tiles
@@ -338,6 +348,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wide_kernel(Params p) {
     return make_int4(seg0 + 16 * first, min(seg1, seg0 + 16 * end), e, nt);
   };
   if (tid < kTileList && lb + (int64_t)tid * G < total_tiles) s_list[tid] = search(lb + tid * G);
+  if (!p.bias)
+    for (int i = tid; i < BN; i += 64 * NW) s_bias[i] = 0;
   __syncthreads();
   struct TileRef { int row0, end, e, nt; };
   auto decode = [&](int i) {  // this workgroup's i-th tile
@@ -412,13 +424,31 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wide_kernel(Params p) {
   auto stage_in = [&]() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(NCOPY * (S - 2)) : "memory");
   };
+  // scales and biases of tile r, a slot a lane
+  auto bring = [&](const TileRef& r) {
+    if (wv < BN / 64) {
+      const int n = wv * 64 + lane, col0 = r.nt * (MODE == kGateUp ? BN / 2 : BN);
+      const int col = col0 + min(q_col(n), N - 1 - col0), up = MODE == kGateUp ? (n >> 4) & 1 : 0;
+      const int64_t at = r.e * p.e_rows + (int64_t)col * p.r_rows;
+      dma4((up ? p.sb : p.sa) + at, lds_addr((const uint8_t*)&s_col[wv * 64]));
+      if (p.bias) {
+        const uint32_t lds = lds_addr((const uint8_t*)&s_bias[wv * 64]);
+        if (p.bias_f32) dma4((const float*)p.bias + (at + up), lds);
+        else dma2((const uint16_t*)p.bias + (at + up), lds);
+      }
+    } else if (wv < (BM + BN) / 64) {
+      const int w = wv - BN / 64;
+      dma4(p.s + r.row0 + min(w * 64 + lane, r.end - 1 - r.row0), lds_addr((const uint8_t*)&s_row[w * 64]));
+    }
+  };
+
   i32x4_t acc[TM][TN];
   int wave_row = 0;
   // A tile's stages by a wave with MB blocks of rows: 2 TN blocks of 16 columns by 64 k each, the
   // fragments read two blocks ahead. The barrier between two stages lies ahead of the last two
   // blocks, whose fragments are there by then, so that MFMAs cover the wait and the next stage's
   // first reads; copies go between the MFMAs of a stage's first half, to land within it.
-  auto stages = [&](auto mb_c) {
+  auto stages = [&](auto mb_c, const TileRef& cur) {
     constexpr int MB = decltype(mb_c)::value, NB = 2 * TN;
     const uint8_t *cP, *cQ;
     auto enter = [&]() {
@@ -442,6 +472,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wide_kernel(Params p) {
       read_q(std::integral_constant<int, 1>{});
     };
     enter();
+    bring(cur);
     if constexpr (MB > 0) read_first();
     for (int kt = 0; kt < nk; ++kt) {
       advance();  // ahead of the MFMAs, which the compiler would otherwise sink behind its branches
@@ -478,8 +509,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wide_kernel(Params p) {
 
   for (int t = 0; t < my_tiles; ++t) {
     const TileRef cur = decode(t);
-    const int row0 = cur.row0, end = cur.end;
-    const int blocks = (end - row0 + 15) >> 4, each = (blocks + WM - 1) / WM;
+    const int blocks = (cur.end - cur.row0 + 15) >> 4, each = (blocks + WM - 1) / WM;
     wave_row = wm * each;  // this wave's first block, and their number
     const int tmv = max(0, min(each, blocks - wave_row));
 #pragma unroll
@@ -489,70 +519,52 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wide_kernel(Params p) {
     bool done = false;
     for_each<TM + 1>([&](auto mb) {
       if (!done && tmv == decltype(mb)::value) {
-        stages(mb);
+        stages(mb, cur);
         done = true;
       }
     });
-    if (tmv == 0) continue;
 
     // ---- epilogue: lane holds C[m = .. + ml][n = .. + 4 g4 .. + 3] of each 16-column block ----
-    float rs[TM];
-#pragma unroll
-    for (int i = 0; i < TM; ++i) rs[i] = p.s[min(row0 + (wave_row + i) * 16 + ml, end - 1)];
 #pragma unroll
     for (int b = 0; b < TN / 2; ++b) {
-      float ca[4], cb[4], ba[4], bb[4];
-      if (MODE == kGateUp) {
-        const int hc = cur.nt * (BN / 2) + wn * (TN * 8) + b * 16 + 4 * g4;
-        if (hc - 4 * g4 >= N) continue;
-        col_scales(p.sa, p, cur.e, hc, ca);
-        col_scales(p.sb, p, cur.e, hc, cb);
-        if constexpr (ACT == kOssGLU) glu_bias(p, cur.e, hc, ba, bb);
+      const int n0 = cur.nt * (MODE == kGateUp ? BN / 2 : BN) + (wn * TN / 2 + b) * (MODE == kGateUp ? 16 : 32);
+      if (n0 >= N) continue;
+      const int at = (wn * TN + 2 * b) * 16 + 4 * g4;
+      const float4 ca = *(const float4*)&s_col[at], cb = *(const float4*)&s_col[at + 16];
+      float ba[4], bb[4];  // (no biases: zeros)
+      if constexpr (MODE == kLinear || ACT == kOssGLU) {
+        const int sh = p.bias_f32 ? 0 : 16;
 #pragma unroll
-        for (int i = 0; i < TM; ++i) {
-          if (i >= tmv) continue;
-          const int r = row0 + (wave_row + i) * 16 + ml;
-          float v[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            float g = (float)acc[i][2 * b][k] * rs[i] * ca[k], u = (float)acc[i][2 * b + 1][k] * rs[i] * cb[k];
-            if constexpr (ACT == kOssGLU) { g += ba[k]; u += bb[k]; }
-            v[k] = activation(ACT, g, u, p.limit);
-          }
-          if (r < end) *(float4*)(p.h + (int64_t)r * N + hc) = make_float4(v[0], v[1], v[2], v[3]);
+        for (int k = 0; k < 4; ++k) {
+          ba[k] = __uint_as_float(s_bias[at + k] << sh);
+          bb[k] = __uint_as_float(s_bias[at + 16 + k] << sh);
         }
-      } else {
-        const int n0 = cur.nt * BN + wn * TN * 16 + b * 32;
-        if (n0 >= N) continue;
-        col_scales(p.sa, p, cur.e, n0 + 4 * g4, ca);
-        col_scales(p.sa, p, cur.e, n0 + 16 + 4 * g4, cb);
-        if (p.bias) {
-          col_bias(p, cur.e, n0 + 4 * g4, ba);
-          col_bias(p, cur.e, n0 + 16 + 4 * g4, bb);
+      }
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        if (i >= tmv) continue;
+        const int m = (wave_row + i) * 16 + ml, r = cur.row0 + m;
+        const float rs = s_row[m];
+        const i32x4_t sa = acc[i][2 * b], sb = acc[i][2 * b + 1];
+        float lo[4] = {(float)sa[0] * rs * ca.x, (float)sa[1] * rs * ca.y, (float)sa[2] * rs * ca.z, (float)sa[3] * rs * ca.w};
+        float hi[4] = {(float)sb[0] * rs * cb.x, (float)sb[1] * rs * cb.y, (float)sb[2] * rs * cb.z, (float)sb[3] * rs * cb.w};
+        if constexpr (MODE == kLinear || ACT == kOssGLU) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) { lo[k] += ba[k]; hi[k] += bb[k]; }
         }
+        if (MODE == kGateUp) {
+          float h[4];
 #pragma unroll
-        for (int i = 0; i < TM; ++i) {
-          if (i >= tmv) continue;
-          const int r = row0 + (wave_row + i) * 16 + ml;
-          float lo[4], hi[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            lo[k] = (float)acc[i][2 * b][k] * rs[i] * ca[k];
-            hi[k] = (float)acc[i][2 * b + 1][k] * rs[i] * cb[k];
+          for (int k = 0; k < 4; ++k) h[k] = activation(ACT, lo[k], hi[k], p.limit);
+          if (r < cur.end) *(float4*)(p.h + (int64_t)r * N + n0 + 4 * g4) = make_float4(h[0], h[1], h[2], h[3]);
+        } else if (p.y_f32 || N % 8) {
+          if (r < cur.end) {
+            store4(p, r, n0 + 4 * g4, lo);
+            store4(p, r, n0 + 16 + 4 * g4, hi);
           }
-          if (p.bias) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) { lo[k] += ba[k]; hi[k] += bb[k]; }
-          }
-          if (p.y_f32 || N % 8) {
-            if (r < end) {
-              store4(p, r, n0 + 4 * g4, lo);
-              store4(p, r, n0 + 16 + 4 * g4, hi);
-            }
-          } else {
-            const uint4 v = span64(pack4_mid(lo), pack4_mid(hi), lane);
-            if (r < end && n0 + 8 * g4 < N) *(uint4*)((uint16_t*)p.y + (int64_t)r * N + n0 + 8 * g4) = v;
-          }
+        } else {
+          const uint4 v = span64(pack4_mid(lo), pack4_mid(hi), lane);
+          if (r < cur.end && n0 + 8 * g4 < N) *(uint4*)((uint16_t*)p.y + (int64_t)r * N + n0 + 8 * g4) = v;
         }
       }
     }
