@@ -708,6 +708,10 @@ int moe_int8_quant_rows(const void* x, int64_t ld, int64_t rows, int32_t cols, i
 int moe_int8_dequant_rows(const int8_t* q, const float* scale, int64_t rows, int32_t cols, int32_t dtype, void* x,
                           moe_stream_t stream);
 
+/* The kernel that a product of n_rows rows takes: 0 to 3 the one for many rows with tiles of 256 x 256,
+ * 128 x 256, 64 x 128, 64 x 64 (gate and up: columns of both), 4 the one for few. Host only. */
+int moe_int8_tile(int64_t n_rows, int32_t n_experts, int32_t in_features, int32_t columns, int32_t n_cus);
+
 /* Bytes of workspace of moe_int8_linear (0: none is taken). */
 int64_t moe_int8_linear_workspace_bytes(int64_t n_rows, int32_t n_experts, int32_t in_features);
 

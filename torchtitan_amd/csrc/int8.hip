@@ -1031,6 +1031,13 @@ MOE_API int moe_int8_dequant_rows(const int8_t* q, const float* scale, int64_t r
   return launch_status();
 }
 
+MOE_API int moe_int8_tile(int64_t n_rows, int32_t n_experts, int32_t in_features, int32_t columns, int32_t n_cus) {
+  const int st = check_shape(n_rows, n_experts, in_features, columns);
+  if (st) return st;
+  if (n_cus < 1) return kErrInvalidArgument;
+  return takes_narrow(n_rows, n_experts, in_features) ? 4 : pick_tile(n_rows, n_experts, in_features, columns, n_cus);
+}
+
 MOE_API int64_t moe_int8_linear_workspace_bytes(int64_t n_rows, int32_t n_experts, int32_t in_features) {
   if (n_rows < 0 || n_experts < 1 || in_features < 16 || in_features % 16) return kErrInvalidArgument;
   return takes_narrow(n_rows, n_experts, in_features) ? 0 : row_bytes(n_rows, in_features);

@@ -11,11 +11,13 @@ fp32 accumulation, bf16 outputs. Parameters stay bf16/fp32 master weights and
 the state_dict is unchanged; quantization happens inside each forward and
 backward.
 
-Three more, with the same interface and without a counterpart in the reference:
+Four more, with the same interface and without a counterpart in the reference:
 ``MXFP4Converter`` (training with MXFP4 products, gradients straight through),
 ``MXFP8ActivationCheckpointConverter`` (bf16 products, activations kept for the
-backward in MXFP8), and ``MXFP4WeightConverter`` (inference: the experts are
-replaced by ones that hold their weights packed in 4 bits, ``mxfp4.py``).
+backward in MXFP8), ``MXFP4WeightConverter`` (inference: the experts are
+replaced by ones that hold their weights packed in 4 bits, ``mxfp4.py``) and
+``Int8WeightConverter`` (inference: experts, shared experts and projections are
+replaced by ones on 8-bit integers, ``int8.py``).
 """
 
 from __future__ import annotations
@@ -27,11 +29,14 @@ import torch
 from torch import nn
 
 from .configurable import Configurable
+from .feed_forward import FeedForward
 from .gpt_oss import GptOssGroupedExperts
-from .moe import GroupedExperts
+from .int8 import Int8FeedForward, Int8GptOssGroupedExperts, Int8GroupedExperts, Int8Linear
+from .linear import Linear
+from .moe import GroupedExperts, TokenChoiceTopKRouter
 from .mxfp4 import MXFP4GptOssGroupedExperts, MXFP4GroupedExperts
 
-__all__ = ["Float8GroupedMMConverter", "MXFP4Converter", "MXFP4WeightConverter", "MXFP8ActivationCheckpointConverter",
+__all__ = ["Float8GroupedMMConverter", "Int8WeightConverter", "MXFP4Converter", "MXFP4WeightConverter", "MXFP8ActivationCheckpointConverter",
            "MXFP8Converter", "PAD_MULTIPLE_MAP", "find_pad_multiple"]
 
 logger = logging.getLogger(__name__)
@@ -143,6 +148,8 @@ class MXFP8Converter(Configurable):
 
 
 _PACKED = {GroupedExperts: MXFP4GroupedExperts, GptOssGroupedExperts: MXFP4GptOssGroupedExperts}
+_INT8 = {GroupedExperts: Int8GroupedExperts.from_experts, GptOssGroupedExperts: Int8GptOssGroupedExperts.from_experts,
+         FeedForward: Int8FeedForward.from_feed_forward, Linear: Int8Linear.from_linear}
 
 
 class _ExpertsConverter(Configurable):
@@ -168,7 +175,8 @@ class _ExpertsConverter(Configurable):
         """Switches the matching GroupedExperts; returns their names. Matching experts of other
         classes, which have no such recipe, are refused."""
         for name, mod in model.named_modules(remove_duplicate=False):
-            if self._matches(name) and isinstance(mod, (GptOssGroupedExperts, *_PACKED.values())):
+            if self._matches(name) and isinstance(mod, (GptOssGroupedExperts, *_PACKED.values(),
+                                                             Int8GroupedExperts, Int8GptOssGroupedExperts)):
                 raise ValueError(f"{name}: {type(mod).__name__} cannot be converted to {self.attr}")
         return _mark_experts(model, self.fqns, self.attr)
 
@@ -224,6 +232,58 @@ class MXFP4WeightConverter(_ExpertsConverter):
             parent, _, child = name.rpartition(".")
             setattr(model.get_submodule(parent), child, made[mod])
         return [name for name, _mod in matching]
+
+
+def _hooked(mod: nn.Module) -> bool:
+    return bool(mod._forward_hooks or mod._forward_pre_hooks or mod._backward_hooks or mod._backward_pre_hooks)
+
+
+class Int8WeightConverter(_ExpertsConverter):
+    """Inference on 8-bit integers: replaces the matching GroupedExperts, GptOssGroupedExperts,
+    FeedForward and Linear by Int8GroupedExperts, Int8GptOssGroupedExperts, Int8FeedForward and
+    Int8Linear, which hold codes and a scale per output channel in place of the parameters, quantize
+    their inputs by rows and take no gradients. A FeedForward is replaced as a whole, and a router's
+    gate, which decides where tokens go, is left as it is."""
+
+    @dataclass(kw_only=True, slots=True)
+    class Config(_ExpertsConverter.Config):
+        pass
+
+    def convert(self, model: nn.Module) -> list[str]:
+        """Replaces the matching modules; returns their names. Refused are subclasses, which may compute
+        something else, modules with hooks, which would not see the calls any more, feed-forwards
+        with biases, and experts that are marked for another recipe."""
+        kept = set()  # what belongs to a router, or to a module that is replaced as a whole
+        for mod in model.modules():
+            if isinstance(mod, TokenChoiceTopKRouter):
+                kept.update(mod.modules())
+        matching = []
+        for name, mod in model.named_modules(remove_duplicate=False):
+            if self._matches(name) and isinstance(mod, tuple(_INT8)) and mod not in kept:
+                self._check(name, mod)
+                matching.append((name, mod))
+                kept.update(mod.children())
+        made = {}  # of a module that several names share, one
+        for name, mod in matching:
+            if mod not in made:
+                made[mod] = _INT8[type(mod)](mod)
+            parent, _, child = name.rpartition(".")
+            setattr(model.get_submodule(parent), child, made[mod])
+        return [name for name, _mod in matching]
+
+    @staticmethod
+    def _check(name: str, mod: nn.Module) -> None:
+        for part in (mod, *mod.children()):
+            if type(part) not in _INT8:
+                raise ValueError(f"{name}: the subclass {type(part).__name__} has no form on 8-bit integers")
+            if _hooked(part):
+                raise ValueError(f"{name} has hooks, which its form on 8-bit integers would not run: register them after "
+                                 "converting")
+        if isinstance(mod, FeedForward) and any(lin.bias is not None for lin in mod.children()):
+            raise ValueError(f"{name}: a feed-forward with biases has no form on 8-bit integers")
+        marked = [r for r in _RECIPES if getattr(mod, r, False)]
+        if marked:
+            raise ValueError(f"{name} is already converted to {marked[0]}")
 
 
 def find_pad_multiple(converters: list) -> int | None:
