@@ -713,7 +713,7 @@ int moe_int8_dequant_rows(const int8_t* q, const float* scale, int64_t rows, int
 int moe_int8_tile(int64_t n_rows, int32_t n_experts, int32_t in_features, int32_t columns, int32_t n_cus);
 
 /* Bytes of workspace of moe_int8_linear (0: none is taken). */
-int64_t moe_int8_linear_workspace_bytes(int64_t n_rows, int32_t n_experts, int32_t in_features);
+int64_t moe_int8_linear_workspace_bytes(int64_t n_rows, int32_t n_experts, int32_t in_features, int32_t out_features);
 
 /* y [R, out_features] = x.w^T + bias in x's dtype: x [R, in_features] (bf16 or fp32) is
  * quantized on the way; w = qw [E, out, in] with sw [E, out]; bias [E, out] in bias_dtype or

@@ -154,7 +154,7 @@ def test_the_kernel_a_product_takes():
 
         build.build()
     tile = _lib.lib().moe_int8_tile
-    for args, want in (((1, 1, 2304, 2304), 4), ((16, 1, 2304, 2304), 4), ((17, 1, 2304, 2304), 3), ((1, 1, 16384, 2304), 3),
+    for args, want in (((1, 1, 2304, 2304), 4), ((96, 1, 2304, 1024), 4), ((300, 1, 2304, 2304), 3), ((8, 1, 7168, 7168), 3), ((4, 1, 7168, 7168), 4), ((1, 1, 16384, 2304), 3),
                        ((8, 256, 2304, 2048), 4), ((1024, 1, 2304, 2304), 2), ((2048, 1, 2304, 2304), 1), ((4096, 1, 2304, 2304), 0),
                        ((16384, 1, 7168, 7168), 0), ((8200, 32, 7168, 2048), 1)):
         assert tile(*args, 256) == want, args

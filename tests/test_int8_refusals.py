@@ -48,12 +48,12 @@ def test_linear(lib, at):
                       (dict(k=131088), -2), (dict(n=(1 << 22) + 1), -2), (dict(r=2 ** 30), -2), (dict(r=2 ** 27, n=2 ** 12), -2),
                       (dict(dtype=2), -1), (dict(bd=2), -1), (dict(c=None), -1), (dict(x=None), -1), (dict(w=None), -1),
                       (dict(s=None), -1), (dict(y=None), -1), (dict(x=at + 2), -1), (dict(w=at + 8), -1), (dict(y=at + 4), -1),
-                      (dict(r=4000, ws=None), -1), (dict(r=4000, ws=at + 8), -1), (dict(r=4000, size=4000 * 128), -4)):
+                      (dict(r=400000, ws=None), -1), (dict(r=400000, ws=at + 8), -1), (dict(r=400000, size=400000 * 128), -4)):
         assert run(**bad) == want, bad
     ws = lib.moe_int8_linear_workspace_bytes
-    assert ws(-1, 2, 64) == -1 and ws(4, 0, 64) == -1 and ws(4, 2, 72) == -1
-    assert ws(1, 1, 64) == 0  # few rows are quantized on the way
-    assert ws(4000, 2, 2880) == 4000 * 2944 + 16128  # codes of whole stages of 128, and scales
+    assert ws(-1, 2, 64, 64) == -1 and ws(4, 0, 64, 64) == -1 and ws(4, 2, 72, 64) == -2 and ws(4, 2, 64, 0) == -1
+    assert ws(1, 1, 64, 64) == 0  # few rows are quantized on the way
+    assert ws(4000, 2, 2880, 2880) == 4000 * 2944 + 16128  # codes of whole stages of 128, and scales
 
 
 def test_layers(lib, at):
@@ -84,7 +84,7 @@ def _w(*shape):
 def test_arguments(monkeypatch):
     from torchtitan_amd import ops
 
-    monkeypatch.setattr(ops, "require_gpu", lambda *t: None)
+    monkeypatch.setattr(ops, "_int8_device", lambda op, *t: 0)
     bf = torch.bfloat16
     x, w, ws, c = torch.zeros(4, 64, dtype=bf), _w(32, 64), _w(2, 32, 64), torch.tensor([2, 2])
     for call, what in (

@@ -112,7 +112,7 @@ SIGNATURES: dict[str, list] = {
     "moe_int8_quant_rows": [P, I64, I64, I32, I32, P, P, P],
     "moe_int8_dequant_rows": [P, P, I64, I32, I32, P, P],
     "moe_int8_tile": [I64, I32, I32, I32, I32],
-    "moe_int8_linear_workspace_bytes": [I64, I32, I32],
+    "moe_int8_linear_workspace_bytes": [I64, I32, I32, I32],
     "moe_int8_linear": [P, I32, P, P, P, I32, P, I64, I32, I32, I32, P, I64, P, P],
     "moe_int8_layer_workspace_bytes": [I64, I32, I32, I32],
     "moe_int8_swiglu": [P, P, P, P, P, P, P, P, I64, I32, I32, I32, P, I64, P, P],

@@ -861,7 +861,8 @@ static int pick_tile(int64_t R, int64_t E, int64_t K, int64_t cols, int64_t cus)
   int64_t least = INT64_MAX;
   for (int i = 0; i < 4; ++i) {
     const Tile& t = kTiles[i];
-    const int64_t mt = E == 1 ? (R + t.bm - 1) / t.bm : R / t.bm + (used + 1) / 2, tiles = mt * ((cols + t.bn - 1) / t.bn);
+    const int64_t mt = E == 1 ? (R + t.bm - 1) / t.bm : std::max(used, R / t.bm + (used + 1) / 2);
+    const int64_t tiles = mt * ((cols + t.bn - 1) / t.bn);
     const int64_t time = (tiles + cus * t.per_cu - 1) / (cus * t.per_cu) * (nk * t.stage + t.rest);
     if (time < least) { least = time; best = i; }
   }
@@ -915,9 +916,20 @@ static void launch_narrow(const Params& p, hipStream_t stream) {
   else launch_narrow_of<MODE, ACT, uint16_t>(p, stream);
 }
 
-// Whether a product of contraction K goes to the narrow kernel.
-static bool takes_narrow(int64_t R, int64_t E, int K) {
-  return narrow_blocks(K, (int)E) && R <= 16 * (R < E ? R : E);
+// Whether a product with `cols` weight rows (gate_up: of both) goes to the narrow kernel: where it reads
+// little and has up to 128 rows an expert, or where there are up to eight and less work in
+// quantizing them, which every workgroup does, than in its weights (1024 bytes of a row's two in
+// each of 512 workgroups a weight row). us, narrow / wide with its quantization: 16 rows of 7168 x 2048 17 /
+// 19, 48 rows 34 / 21; 96 rows of 2304 x 2304 12 / 13; 48 of 2880 x 2880 14 / 20; 16 of 2304 x 2304 8 / 16; one of 7168 x 7168 20 / 24, eight
+// 29 / 24; experts (both products), one token's 8 of 256 of 2304 / 1024 23 / 29, 64 tokens' 292 / 279; 4, 8,
+// 12 rows each on 32 of 2880 / 2880 157 / 168, 166 / 172, 190 / 174; on 32 of 7168 / 2048 297 / 312, 314 / 317,
+// 359 / 319; 4 on 256 of 2304 / 1024 342 / 325.
+static bool takes_narrow(int64_t R, int64_t E, int K, int64_t cols) {
+  const int tm = narrow_blocks(K, (int)E);
+  if (!tm) return false;
+  const int64_t used = R < E ? R : E, tiles = E == 1 ? (R + 16 * tm - 1) / (16 * tm) : R / (16 * tm) + used;
+  const int64_t bytes = tiles * cols * K;
+  return (R <= 128 * used && bytes <= 30000000) || (R <= 8 * used && 1024 * R <= cols * used * used && bytes <= 900000000);
 }
 
 static int check_shape(int64_t R, int E, int K, int N) {
@@ -949,7 +961,7 @@ static Rows rows_at(uint8_t* ws, int64_t R, int K) { return {(int8_t*)ws, (float
 
 // y = x w^T + b from rows in bf16 or fp32: at x in the workspace or the caller's.
 static void product(Params& p, uint8_t* ws, hipStream_t stream) {
-  if (takes_narrow(p.R, p.E, p.K)) return launch_narrow<kLinear, kSwiGLU>(p, stream);
+  if (takes_narrow(p.R, p.E, p.K, p.N)) return launch_narrow<kLinear, kSwiGLU>(p, stream);
   const Rows rows = rows_at(ws, p.R, p.K);
   if (p.x_f32) launch_quant((const float*)p.x, p.K, p.R, p.K, padded(p.K), rows.q, rows.s, stream);
   else launch_quant((const uint16_t*)p.x, p.K, p.R, p.K, padded(p.K), rows.q, rows.s, stream);
@@ -982,7 +994,7 @@ static int layer(const uint16_t* x, const int8_t* qw1, const float* sw1, const i
   p.r_rows = ACT == kOssGLU ? 2 : 1;
   p.bias = b1; p.bias_f32 = bias_f32; p.limit = limit;
   p.h = h;
-  if (takes_narrow(R, E, D)) {
+  if (takes_narrow(R, E, D, 2 * (int64_t)H)) {
     launch_narrow<kGateUp, ACT>(p, stream);
   } else {
     const Rows rows = rows_at(rows_ws, R, D);
@@ -1035,12 +1047,13 @@ MOE_API int moe_int8_tile(int64_t n_rows, int32_t n_experts, int32_t in_features
   const int st = check_shape(n_rows, n_experts, in_features, columns);
   if (st) return st;
   if (n_cus < 1) return kErrInvalidArgument;
-  return takes_narrow(n_rows, n_experts, in_features) ? 4 : pick_tile(n_rows, n_experts, in_features, columns, n_cus);
+  return takes_narrow(n_rows, n_experts, in_features, columns) ? 4 : pick_tile(n_rows, n_experts, in_features, columns, n_cus);
 }
 
-MOE_API int64_t moe_int8_linear_workspace_bytes(int64_t n_rows, int32_t n_experts, int32_t in_features) {
-  if (n_rows < 0 || n_experts < 1 || in_features < 16 || in_features % 16) return kErrInvalidArgument;
-  return takes_narrow(n_rows, n_experts, in_features) ? 0 : row_bytes(n_rows, in_features);
+MOE_API int64_t moe_int8_linear_workspace_bytes(int64_t n_rows, int32_t n_experts, int32_t in_features, int32_t out_features) {
+  const int st = check_shape(n_rows, n_experts, in_features, out_features);
+  if (st) return st;
+  return takes_narrow(n_rows, n_experts, in_features, out_features) ? 0 : row_bytes(n_rows, in_features);
 }
 
 MOE_API int moe_int8_linear(const void* x, int32_t dtype, const int8_t* qw, const float* sw, const void* bias,
@@ -1055,7 +1068,7 @@ MOE_API int moe_int8_linear(const void* x, int32_t dtype, const int8_t* qw, cons
   if (!x || !qw || !sw || !y) return kErrInvalidArgument;
   for (const void* q : {x, (const void*)qw, (const void*)workspace, (const void*)y})
     if (!aligned16(q)) return kErrInvalidArgument;
-  const int64_t need = moe_int8_linear_workspace_bytes(n_rows, n_experts, in_features);
+  const int64_t need = moe_int8_linear_workspace_bytes(n_rows, n_experts, in_features, out_features);
   if (need && !workspace) return kErrInvalidArgument;
   if (workspace_bytes < need) return kErrWorkspace;
   Params p{};

@@ -1728,23 +1728,44 @@ INT8_MAX_K = 131072  # past it a sum of code products can leave 32 bits
 # steps, and a message is put together where something is not.
 
 
+def _int8_device(op: str, x: Tensor, *others: Tensor | None) -> int:
+    """The GPU that all of them are on."""
+    here = x.get_device()
+    ok = here >= 0
+    for t in others:
+        if t is not None and t.get_device() != here:
+            ok = False
+    if not ok:
+        require_gpu(x, *others)
+        raise ValueError(f"{op}: tensors on more than one device")
+    return here
+
+
+def _int8_launch(here: int, name: str, x: Tensor, *args) -> None:
+    """An entry point on x's device and torch's stream there."""
+    if here == torch._C._cuda_getDevice():
+        call(name, *args, stream_of(x))
+    else:
+        with torch.cuda.device(here):
+            call(name, *args, stream_of(x))
+
+
 def _check_int8(op: str, name: str, q: Tensor, scale: Tensor, shape: tuple) -> None:
-    """A matrix in codes: q of `shape` int8 and scale of shape[:-1] fp32 on one device."""
-    if q.dtype is torch.int8 and scale.dtype is torch.float32 and q.shape == shape and scale.shape == shape[:-1] \
-            and q.get_device() == scale.get_device():
+    """A matrix in codes: q of `shape` int8 and scale of shape[:-1] fp32."""
+    if q.dtype is torch.int8 and scale.dtype is torch.float32 and q.shape == shape and scale.shape == shape[:-1]:
         return
     if q.dtype is not torch.int8 or scale.dtype is not torch.float32:
         raise TypeError(f"{op} expects int8 {name} and float32 scales, got {q.dtype} and {scale.dtype}")
-    raise ValueError(f"{op} expects {name} of {list(shape)} with scales of {list(shape[:-1])} on one device, got "
-                     f"{list(q.shape)} on {q.device} and {list(scale.shape)} on {scale.device}")
+    raise ValueError(f"{op} expects {name} of {list(shape)} with scales of {list(shape[:-1])}, got {list(q.shape)} and "
+                     f"{list(scale.shape)}")
 
 
-def _check_int8_bias(op: str, bias: Tensor, shape: tuple, like: Tensor) -> int:
+def _check_int8_bias(op: str, bias: Tensor, shape: tuple) -> int:
     """The bias's dtype code."""
     if bias.dtype not in DTYPE_CODES:
         raise TypeError(f"{op} takes biases in bfloat16 and float32, got {bias.dtype}")
-    if bias.shape != shape or bias.device != like.device:
-        raise ValueError(f"{op} expects a bias of {list(shape)} on {like.device}, got {list(bias.shape)} on {bias.device}")
+    if bias.shape != shape:
+        raise ValueError(f"{op} expects a bias of {list(shape)}, got {list(bias.shape)}")
     return DTYPE_CODES[bias.dtype]
 
 
@@ -1754,13 +1775,6 @@ def _check_int8_dims(op: str, e: int, *contractions: int) -> None:
     for k in contractions:
         if k < INT8_MULTIPLE or k % INT8_MULTIPLE or k > INT8_MAX_K:
             raise ValueError(f"{op} takes contractions that are multiples of {INT8_MULTIPLE} up to {INT8_MAX_K}, got {k}")
-
-
-def _check_int8_devices(op: str, x: Tensor, *others: Tensor) -> None:
-    here = x.get_device()
-    for t in others:
-        if t.get_device() != here:
-            raise ValueError(f"{op}: tensors on more than one device")
 
 
 def _int8_code(op: str, dtype: torch.dtype) -> int:
@@ -1779,7 +1793,7 @@ def _no_int8_gradients(op: str, *tensors: Tensor | None) -> None:
 
 @_mx_op("int8_quantize(Tensor x) -> (Tensor, Tensor)", _I8)
 def _int8_quantize(x: Tensor) -> tuple[Tensor, Tensor]:
-    require_gpu(x)
+    here = _int8_device("int8_quantize", x)
     code = _int8_code("int8_quantize", x.dtype)
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"int8_quantize expects rows of at least one column, got {tuple(x.shape)}")
@@ -1792,8 +1806,7 @@ def _int8_quantize(x: Tensor) -> tuple[Tensor, Tensor]:
             x = x.contiguous()
     q = torch.empty_like(x, dtype=torch.int8) if ld == cols else x.new_empty(shape, dtype=torch.int8)
     scale = x.new_empty(shape[:-1], dtype=torch.float32)
-    with _guard(x):
-        call("moe_int8_quant_rows", ptr(x), ld, scale.numel(), cols, code, ptr(q), ptr(scale), stream_of(x))
+    _int8_launch(here, "moe_int8_quant_rows", x, x.data_ptr(), ld, scale.numel(), cols, code, q.data_ptr(), scale.data_ptr())
     return q, scale
 
 
@@ -1808,20 +1821,19 @@ def int8_quantize(x: Tensor) -> tuple[Tensor, Tensor]:
     r = 127 / a, scale = a / 127, its codes are x r rounded once to the nearest integer, ties to
     even (|q| <= 127), and stand for q scale. A row with an infinity or a NaN has the scale NaN
     and zero codes. Rows of weights [.., N, K] are output channels, rows of activations tokens."""
-    return _int8_quantize(x.detach())
+    return _int8_quantize(x.detach() if x.requires_grad or forward_ad._current_level >= 0 else x)
 
 
 @_mx_op("int8_dequantize(Tensor q, Tensor scale, ScalarType dtype) -> Tensor", _I8)
 def _int8_dequantize(q: Tensor, scale: Tensor, dtype: torch.dtype) -> Tensor:
-    require_gpu(q, scale)
+    here = _int8_device("int8_dequantize", q, scale)
     code = _int8_code("int8_dequantize", dtype)
     if q.dim() < 1 or q.shape[-1] < 1:
         raise ValueError(f"int8_dequantize expects rows of at least one column, got {tuple(q.shape)}")
     _check_int8("int8_dequantize", "q", q, scale, q.shape)
     q, scale = q.contiguous(), scale.contiguous()
     x = torch.empty_like(q, dtype=dtype)
-    with _guard(q):
-        call("moe_int8_dequant_rows", ptr(q), ptr(scale), scale.numel(), q.shape[-1], code, ptr(x), stream_of(q))
+    _int8_launch(here, "moe_int8_dequant_rows", q, q.data_ptr(), scale.data_ptr(), scale.numel(), q.shape[-1], code, x.data_ptr())
     return x
 
 
@@ -1833,18 +1845,21 @@ def _(q, scale, dtype):
 def int8_dequantize(q: Tensor, scale: Tensor, dtype: torch.dtype = torch.bfloat16) -> Tensor:
     """The values q scale [.., K] of a matrix in codes (int8_quantize), taken in fp32, in bf16 or
     fp32."""
-    return _int8_dequantize(q, scale.detach(), dtype)
+    return _int8_dequantize(q, scale.detach() if scale.requires_grad or forward_ad._current_level >= 0 else scale, dtype)
 
 
 @functools.lru_cache(maxsize=256)
-def _int8_workspace_bytes(r: int, e: int, k: int, hidden: int | None) -> int:
-    if hidden is None:
-        return int(lib().moe_int8_linear_workspace_bytes(r, e, k))
-    return int(lib().moe_int8_layer_workspace_bytes(r, e, k, hidden))
+def _int8_linear_workspace_bytes(r: int, e: int, k: int, n: int) -> int:
+    return max(int(lib().moe_int8_linear_workspace_bytes(r, e, k, n)), 0)  # (what does not fit, the call refuses)
 
 
-def _int8_product(op: str, x: Tensor, qw: Tensor, sw: Tensor, counts: Tensor | None, bias: Tensor | None, rows: int,
-                  e: int, n: int, k: int) -> Tensor:
+@functools.lru_cache(maxsize=256)
+def _int8_layer_workspace_bytes(r: int, e: int, d: int, h: int) -> int:
+    return int(lib().moe_int8_layer_workspace_bytes(r, e, d, h))
+
+
+def _int8_product(op: str, here: int, x: Tensor, qw: Tensor, sw: Tensor, counts: Tensor | None, bias: Tensor | None,
+                  rows: int, e: int, n: int, k: int) -> Tensor:
     """x [.., K] of `rows` rows by qw [(E,) N, K]."""
     code = _int8_code(op, x.dtype)
     _check_int8(op, "qw", qw, sw, qw.shape)
@@ -1853,15 +1868,14 @@ def _int8_product(op: str, x: Tensor, qw: Tensor, sw: Tensor, counts: Tensor | N
         raise ValueError(f"{op} expects at least one output channel, got {tuple(qw.shape)}")
     bias_code = 0
     if bias is not None:
-        bias_code = _check_int8_bias(op, bias, qw.shape[:-1], x)
+        bias_code = _check_int8_bias(op, bias, qw.shape[:-1])
         bias = bias.contiguous()
     x, qw, sw = _ready(x), _ready(qw), sw.contiguous()
-    ws_bytes = _int8_workspace_bytes(rows, e, k, None)
+    ws_bytes = _int8_linear_workspace_bytes(rows, e, k, n)
     ws = x.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
     y = x.new_empty((*x.shape[:-1], n))
-    with _guard(x):
-        call("moe_int8_linear", ptr(x), code, ptr(qw), ptr(sw), ptr(bias), bias_code, ptr(counts), rows, e, k, n, ptr(ws),
-             ws_bytes, ptr(y), stream_of(x))
+    _int8_launch(here, "moe_int8_linear", x, x.data_ptr(), code, qw.data_ptr(), sw.data_ptr(), ptr(bias), bias_code, ptr(counts),
+                 rows, e, k, n, ptr(ws), ws_bytes, y.data_ptr())
     return y
 
 
@@ -1872,12 +1886,11 @@ def _rows_of(xs: torch.Size) -> int:
 @_mx_op("linear_int8(Tensor x, Tensor qw, Tensor sw, Tensor? bias=None) -> Tensor", _I8_BARE)
 def _linear_int8(x, qw, sw, bias=None):
     op = "linear_int8"
-    require_gpu(x, qw, sw, bias)
+    here = _int8_device(op, x, qw, sw, bias)
     xs, ws = x.shape, qw.shape
-    if len(ws) != 2 or not xs or xs[-1] != ws[1] or x.get_device() != qw.get_device():
-        raise ValueError(f"{op} expects x [.., K] and qw [N, K] on one device, got {tuple(xs)} on {x.device} and "
-                         f"{tuple(ws)} on {qw.device}")
-    return _int8_product(op, x, qw, sw, None, bias, _rows_of(xs), 1, *ws)
+    if len(ws) != 2 or not xs or xs[-1] != ws[1]:
+        raise ValueError(f"{op} expects x [.., K] and qw [N, K], got {tuple(xs)} and {tuple(ws)}")
+    return _int8_product(op, here, x, qw, sw, None, bias, _rows_of(xs), 1, *ws)
 
 
 @torch.library.register_fake("moe_mi355x_int8_bare::linear_int8", lib=_I8_BARE)
@@ -1900,7 +1913,6 @@ def _int8_counts(op: str, x: Tensor, qw: Tensor, counts: Tensor) -> Tensor:
     xs, ws, cs = x.shape, qw.shape, counts.shape
     if len(xs) != 2 or len(ws) != 3 or len(cs) != 1 or cs[0] != ws[0] or xs[1] != ws[2]:
         raise ValueError(f"{op} expects x [R, K], weights [E, .., K] and counts [E], got {tuple(xs)}, {tuple(ws)}, {tuple(cs)}")
-    _check_int8_devices(op, x, qw, counts)
     if counts.dtype is not torch.int64:
         _check_counts(op, counts)
         counts = counts.to(torch.int64)
@@ -1911,9 +1923,9 @@ def _int8_counts(op: str, x: Tensor, qw: Tensor, counts: Tensor) -> Tensor:
         _I8_BARE)
 def _grouped_linear_int8(x, qw, sw, num_tokens_per_expert, bias=None):
     op = "grouped_linear_int8"
-    require_gpu(x, qw, sw, num_tokens_per_expert, bias)
+    here = _int8_device(op, x, qw, sw, num_tokens_per_expert, bias)
     counts = _int8_counts(op, x, qw, num_tokens_per_expert)
-    return _int8_product(op, x, qw, sw, counts, bias, x.shape[0], *qw.shape)
+    return _int8_product(op, here, x, qw, sw, counts, bias, x.shape[0], *qw.shape)
 
 
 @torch.library.register_fake("moe_mi355x_int8_bare::grouped_linear_int8", lib=_I8_BARE)
@@ -1929,33 +1941,31 @@ def grouped_linear_int8(x: Tensor, qw: Tensor, sw: Tensor, num_tokens_per_expert
     return _grouped_linear_int8(x, qw, sw, num_tokens_per_expert, bias)
 
 
-def _int8_swiglu(op: str, x, qw1, sw1, qw2, sw2, qw3, sw3, counts, rows) -> Tensor:
+def _int8_swiglu(op: str, here: int, x, qw1, sw1, qw2, sw2, qw3, sw3, counts, rows) -> Tensor:
     _check_bf16(op, x=x)
     shape = qw1.shape
     e, h, d = shape if len(shape) == 3 else (1, *shape)
     _check_int8(op, "w1", qw1, sw1, shape)
     _check_int8(op, "w2", qw2, sw2, (e, d, h) if len(shape) == 3 else (d, h))
     _check_int8(op, "w3", qw3, sw3, shape)
-    _check_int8_devices(op, x, qw1, qw2, qw3)
     _check_int8_dims(op, e, d, h)
     x, qw1, qw2, qw3 = _ready(x), _ready(qw1), _ready(qw2), _ready(qw3)
     sw1, sw2, sw3 = sw1.contiguous(), sw2.contiguous(), sw3.contiguous()
-    ws_bytes = _int8_workspace_bytes(rows, e, d, h)
+    ws_bytes = _int8_layer_workspace_bytes(rows, e, d, h)
     ws = x.new_empty(ws_bytes, dtype=torch.uint8)
     y = torch.empty_like(x)
-    with _guard(x):
-        call("moe_int8_swiglu", ptr(x), ptr(qw1), ptr(sw1), ptr(qw2), ptr(sw2), ptr(qw3), ptr(sw3), ptr(counts), rows, e, d, h,
-             ptr(ws), ws_bytes, ptr(y), stream_of(x))
+    _int8_launch(here, "moe_int8_swiglu", x, x.data_ptr(), qw1.data_ptr(), sw1.data_ptr(), qw2.data_ptr(), sw2.data_ptr(),
+                 qw3.data_ptr(), sw3.data_ptr(), ptr(counts), rows, e, d, h, ws.data_ptr(), ws_bytes, y.data_ptr())
     return y
 
 
 @_mx_op("swiglu_ffn_int8(Tensor x, Tensor qw1, Tensor sw1, Tensor qw2, Tensor sw2, Tensor qw3, Tensor sw3) -> Tensor", _I8_BARE)
 def _swiglu_ffn_int8(x, qw1, sw1, qw2, sw2, qw3, sw3):
     op = "swiglu_ffn_int8"
-    require_gpu(x, qw1, sw1, qw2, sw2, qw3, sw3)
+    here = _int8_device(op, x, qw1, sw1, qw2, sw2, qw3, sw3)
     if qw1.dim() != 2 or x.dim() < 1 or x.shape[-1] != qw1.shape[1]:
         raise ValueError(f"{op} expects x [.., D] and weights [H, D] and [D, H], got {tuple(x.shape)} and {tuple(qw1.shape)}")
-    return _int8_swiglu(op, x, qw1, sw1, qw2, sw2, qw3, sw3, None, _rows_of(x.shape))
+    return _int8_swiglu(op, here, x, qw1, sw1, qw2, sw2, qw3, sw3, None, _rows_of(x.shape))
 
 
 @torch.library.register_fake("moe_mi355x_int8_bare::swiglu_ffn_int8", lib=_I8_BARE)
@@ -1976,9 +1986,9 @@ def swiglu_ffn_int8(x: Tensor, qw1: Tensor, sw1: Tensor, qw2: Tensor, sw2: Tenso
         "Tensor num_tokens_per_expert) -> Tensor", _I8_BARE)
 def _grouped_swiglu_int8(x, qw1, sw1, qw2, sw2, qw3, sw3, num_tokens_per_expert):
     op = "grouped_swiglu_int8"
-    require_gpu(x, qw1, sw1, qw2, sw2, qw3, sw3, num_tokens_per_expert)
+    here = _int8_device(op, x, qw1, sw1, qw2, sw2, qw3, sw3, num_tokens_per_expert)
     counts = _int8_counts(op, x, qw1, num_tokens_per_expert)
-    return _int8_swiglu(op, x, qw1, sw1, qw2, sw2, qw3, sw3, counts, x.shape[0])
+    return _int8_swiglu(op, here, x, qw1, sw1, qw2, sw2, qw3, sw3, counts, x.shape[0])
 
 
 @torch.library.register_fake("moe_mi355x_int8_bare::grouped_swiglu_int8", lib=_I8_BARE)
@@ -2001,28 +2011,27 @@ def grouped_swiglu_int8(
         "Tensor mlp2_bias, Tensor num_tokens_per_expert, float swiglu_limit) -> Tensor", _I8_BARE)
 def _grouped_swiglu_oss_int8(x, qmlp1, smlp1, mlp1_bias, qmlp2, smlp2, mlp2_bias, num_tokens_per_expert, swiglu_limit):
     op = "grouped_swiglu_oss_int8"
-    require_gpu(x, qmlp1, smlp1, mlp1_bias, qmlp2, smlp2, mlp2_bias, num_tokens_per_expert)
+    here = _int8_device(op, x, qmlp1, smlp1, mlp1_bias, qmlp2, smlp2, mlp2_bias, num_tokens_per_expert)
     _check_bf16(op, x=x)
     counts = _int8_counts(op, x, qmlp1, num_tokens_per_expert)
     (r, d), (e, h2, _) = x.shape, qmlp1.shape
     h = h2 // 2
     _check_int8(op, "mlp1", qmlp1, smlp1, (e, 2 * h, d))
     _check_int8(op, "mlp2", qmlp2, smlp2, (e, d, h))
-    _check_int8_devices(op, x, qmlp1, qmlp2)
     _check_int8_dims(op, e, d, h)
-    code = _check_int8_bias(op, mlp1_bias, (e, 2 * h), x)
-    if _check_int8_bias(op, mlp2_bias, (e, d), x) != code:
+    code = _check_int8_bias(op, mlp1_bias, (e, 2 * h))
+    if _check_int8_bias(op, mlp2_bias, (e, d)) != code:
         raise TypeError(f"{op} takes both biases in one dtype, got {mlp1_bias.dtype} and {mlp2_bias.dtype}")
     if not swiglu_limit >= 0:
         raise ValueError(f"{op} expects a clamp limit of at least 0, got {swiglu_limit}")
     x, qmlp1, qmlp2 = map(_ready, (x, qmlp1, qmlp2))
     smlp1, smlp2, b1, b2 = (t.contiguous() for t in (smlp1, smlp2, mlp1_bias, mlp2_bias))
-    ws_bytes = _int8_workspace_bytes(r, e, d, h)
+    ws_bytes = _int8_layer_workspace_bytes(r, e, d, h)
     ws = x.new_empty(ws_bytes, dtype=torch.uint8)
     y = torch.empty_like(x)
-    with _guard(x):
-        call("moe_int8_oss", ptr(x), ptr(qmlp1), ptr(smlp1), ptr(b1), ptr(qmlp2), ptr(smlp2), ptr(b2), code, ptr(counts), r, e, d,
-             h, float(swiglu_limit), ptr(ws), ws_bytes, ptr(y), stream_of(x))
+    _int8_launch(here, "moe_int8_oss", x, x.data_ptr(), qmlp1.data_ptr(), smlp1.data_ptr(), b1.data_ptr(), qmlp2.data_ptr(),
+                 smlp2.data_ptr(), b2.data_ptr(), code, counts.data_ptr(), r, e, d, h, float(swiglu_limit), ws.data_ptr(), ws_bytes,
+                 y.data_ptr())
     return y
 
 
