@@ -892,12 +892,17 @@ static void launch_wide(const Params& p, hipStream_t stream) {
   }
 }
 
-static int narrow_blocks(int K, int E) {
-  return narrow_lds(K, E, 2) <= 80 * 1024 ? 2 : narrow_lds(K, E, 1) <= kLdsMost ? 1 : 0;
+// Blocks of 16 rows in a unit of the narrow kernel: two with more than eight rows an expert, where two
+// workgroups share a CU's LDS still, else one, where that fits; 0: neither does. With few rows the
+// second block is code and LDS for nothing: 16 experts of 2304 / 1024 with 8 rows each 39 us with two in
+// their second product, 35 with one; 64 of 1024 / 512 with two rows 32 / 28.
+static int narrow_blocks(int64_t R, int64_t E, int K) {
+  if (R > 8 * (R < E ? R : E) && narrow_lds(K, (int)E, 2) <= 80 * 1024) return 2;
+  return narrow_lds(K, (int)E, 1) <= kLdsMost ? 1 : 0;
 }
 template <int MODE, int ACT, typename T>
 static void launch_narrow_of(const Params& p, hipStream_t stream) {
-  const int tm = narrow_blocks(p.K, p.E);
+  const int tm = narrow_blocks(p.R, p.E, p.K);
   const int64_t nblk = MODE == kGateUp ? p.N / 8 : (p.N + 15) / 16, tiles = p.R / (16 * tm) + (p.R < p.E ? p.R : p.E);
   const int64_t lds = narrow_lds(p.K, p.E, tm), most = (int64_t)cu_count() * 2;
   auto launch = [&](auto kernel, int nb) {
@@ -925,7 +930,7 @@ static void launch_narrow(const Params& p, hipStream_t stream) {
 // 12 rows each on 32 of 2880 / 2880 157 / 168, 166 / 172, 190 / 174; on 32 of 7168 / 2048 297 / 312, 314 / 317,
 // 359 / 319; 4 on 256 of 2304 / 1024 342 / 325.
 static bool takes_narrow(int64_t R, int64_t E, int K, int64_t cols) {
-  const int tm = narrow_blocks(K, (int)E);
+  const int tm = narrow_blocks(R, E, K);
   if (!tm) return false;
   const int64_t used = R < E ? R : E, tiles = E == 1 ? (R + 16 * tm - 1) / (16 * tm) : R / (16 * tm) + used;
   const int64_t bytes = tiles * cols * K;
