@@ -97,46 +97,47 @@ __device__ __forceinline__ int wave_scan_below(int v, int most) {
   return __builtin_amdgcn_update_dpp(0, wave_scan(v, most), 0x138, 0xf, 0xf, false);  // wave_shr 1
 }
 
-// The same by the first wave alone (lane l the experts l n .. l n + n - 1, n = ceil(E / 64)), where a
-// launch is so short that the barriers of the scans above are a third of it. One barrier.
+// segments() by the first wave alone (lane l the experts l n .. l n + n - 1, n = ceil(E / 64) <= MOST),
+// where a launch is so short that the barriers of the scans above are a third of it. One barrier.
+template <int MOST, typename P, typename F>
+__device__ __forceinline__ void segments_of_lanes(const P& p, int* seg, int* tile, F tiles_of) {
+  const int lane = threadIdx.x, R = (int)p.R, n = (p.E + 63) / 64;
+  int64_t raw[MOST];
+  int cnt[MOST];
+#pragma unroll
+  for (int i = 0; i < MOST; ++i) {  // all of them on their way before the first is used
+    const int e = lane * n + i;
+    raw[i] = i < n && e < p.E ? count_of(p, e) : 0;
+  }
+  int rows = 0;
+#pragma unroll
+  for (int i = 0; i < MOST; ++i) {
+    cnt[i] = raw[i] < 0 ? 0 : (raw[i] > p.R ? R : (int)raw[i]);
+    rows = min(rows + cnt[i], R);
+  }
+  int at = wave_scan_below(rows, R), tiles = 0;
+  const int at0 = at;
+#pragma unroll
+  for (int i = 0; i < MOST; ++i) {
+    cnt[i] = min(cnt[i], R - at);
+    at += cnt[i];
+    tiles += tiles_of(cnt[i]);
+  }
+  int run = at0, tl = wave_scan_below(tiles, 0x3fffffff);
+#pragma unroll
+  for (int i = 0; i < MOST; ++i) {
+    const int e = lane * n + i;
+    if (i < n && e < p.E) { seg[e] = run; tile[e] = tl; }
+    run += cnt[i];
+    tl += tiles_of(cnt[i]);
+  }
+  if (lane == 63) { seg[p.E] = run; tile[p.E] = tl; }
+}
 template <typename P, typename F>
 __device__ __forceinline__ void segments_wave(const P& p, int* seg, int* tile, F tiles_of) {
   if (threadIdx.x < 64) {
-    const int lane = threadIdx.x, R = (int)p.R, n = (p.E + 63) / 64;
-    int64_t raw[kMaxE / 64];
-    int cnt[kMaxE / 64];
-#pragma unroll
-    for (int i = 0; i < kMaxE / 64; ++i) {  // all of them on their way before the first is used
-      if (i >= n) break;
-      const int e = lane * n + i;
-      raw[i] = e < p.E ? count_of(p, e) : 0;
-    }
-    int rows = 0;
-#pragma unroll
-    for (int i = 0; i < kMaxE / 64; ++i) {
-      if (i >= n) break;
-      cnt[i] = raw[i] < 0 ? 0 : (raw[i] > p.R ? R : (int)raw[i]);
-      rows = min(rows + cnt[i], R);
-    }
-    int at = wave_scan_below(rows, R), tiles = 0;
-    const int at0 = at;
-#pragma unroll
-    for (int i = 0; i < kMaxE / 64; ++i) {
-      if (i >= n) break;
-      cnt[i] = min(cnt[i], R - at);
-      at += cnt[i];
-      tiles += tiles_of(cnt[i]);
-    }
-    int run = at0, tl = wave_scan_below(tiles, 0x3fffffff);
-#pragma unroll
-    for (int i = 0; i < kMaxE / 64; ++i) {
-      if (i >= n) break;
-      const int e = lane * n + i;
-      if (e < p.E) { seg[e] = run; tile[e] = tl; }
-      run += cnt[i];
-      tl += tiles_of(cnt[i]);
-    }
-    if (lane == 63) { seg[p.E] = run; tile[p.E] = tl; }
+    if (p.E <= 256) segments_of_lanes<4>(p, seg, tile, tiles_of);
+    else segments_of_lanes<kMaxE / 64>(p, seg, tile, tiles_of);
   }
   __syncthreads();
 }
