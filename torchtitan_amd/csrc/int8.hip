@@ -16,6 +16,7 @@
 // v_mfma_i32_16x16x64_i8: lane (row, q), q = lane / 16, holds 16 consecutive k of its row; the sums
 // are exact (K <= 131072: 2^17 * 127 * 128 < 2^31).
 #include <algorithm>
+#include <atomic>
 
 #include "grouped.h"
 #include "mx.h"
@@ -576,8 +577,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wide_kernel(Params p) {
 // Few rows per expert: the weights are read once and decide the time, so every byte goes straight
 // from memory into the MFMAs' registers. A unit is NB blocks of 16 weight rows (gate_up: 8 gate and
 // 8 up rows each) by up to 16 TM rows of one expert; of eight waves, NB take a block each, and 8 / NB
-// of them share its k, stages of 128 in turn. A wave multiplies a group of DEPTH stages while the
-// next one is on its way, through to the following unit. A workgroup's units are consecutive, so
+// of them share its k, stages of 128 in turn. A wave multiplies a stage while the next one is on its
+// way, through to the following unit. A workgroup's units are consecutive, so
 // the rows, which are quantized on the way into LDS, are prepared once per expert and workgroup.
 // The columns' scales and biases are asked for ahead of the unit's first stages: loads come back in
 // order, so that one asked for where it is used would wait for the stages behind it.
@@ -586,12 +587,15 @@ __host__ __device__ constexpr int64_t narrow_lds(int K, int E, int TM) {  // row
   return 16 * (int64_t)TM * narrow_stride(K) + 2 * 8 * TM * 64 * 16 + 16 * TM * 4 + 8 * 4 + 2 * (E + 1) * (int)sizeof(int);
 }
 
-template <int MODE, int ACT, typename T, int NB, int TM, int DEPTH>
+template <int MODE, int ACT, typename T, int NB, int TM>
 __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
   extern __shared__ __attribute__((aligned(16))) uint8_t s_dyn[];
   constexpr int kRows = 16 * TM, KS = 8 / NB, COLS = MODE == kGateUp ? 8 : 16;  // COLS: columns of a block
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int nb = wv % NB, ks = wv / NB, ml = lane & 15, g4 = lane >> 4;
+  // the arguments in one go: asked for where they are used, each batch of them is a wait of its own
+  asm volatile("" ::"s"(p.counts), "s"(p.R), "s"(p.x), "s"(p.wa), "s"(p.sa), "s"(p.wb), "s"(p.sb), "s"(p.e_rows), "s"(p.r_rows),
+               "s"(p.bias), "s"(p.h), "s"(p.y));
   const int E = p.E, K = p.K, N = p.N, KC = K / 16, nst = (K + 127) / 128;
   const int stride = narrow_stride(K);
   uint8_t* sP = s_dyn;
@@ -612,7 +616,7 @@ __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
   // consecutive units, of which the first workgroups have one more
   const uint32_t total = (uint32_t)__builtin_amdgcn_readfirstlane(s_tile[E]), per = total / gridDim.x, more = total - per * gridDim.x;
   const int u0 = (int)(blockIdx.x * per + min(blockIdx.x, more)), u1 = u0 + (int)per + (blockIdx.x < more ? 1 : 0);
-  const int groups = (nst + KS * DEPTH - 1) / (KS * DEPTH);  // of a wave's stages ks, ks + KS, ...
+  const int mine = (nst + KS - 1) / KS;  // a wave's stages: ks, ks + KS, ...
 
   struct Unit { int e, rt, cb; };
   auto decode = [&](int u) {
@@ -634,15 +638,12 @@ __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
     const int8_t* row = lane_row + (u.e * p.e_rows + (int64_t)first * p.r_rows) * K;
     return MODE == kGateUp ? row : row + (uint32_t)(min(ml, N - 1 - first) * K);
   };
-  struct Group { i32x4_t w[DEPTH][2]; };
+  struct Stage { i32x4_t w[2]; };
   // chunks past a row's end repeat its last one, against zeros in LDS
-  auto load = [&](Group& g, const int8_t* row, int i) {
-#pragma unroll
-    for (int d = 0; d < DEPTH; ++d) {
-      const int c = 8 * (ks + KS * (i * DEPTH + d)) + g4;
-      g.w[d][0] = *(const i32x4_t*)(row + (uint32_t)(min(c, KC - 1) * 16));
-      g.w[d][1] = *(const i32x4_t*)(row + (uint32_t)(min(c + 4, KC - 1) * 16));
-    }
+  auto load = [&](Stage& g, const int8_t* row, int i) {
+    const int c = 8 * (ks + KS * i) + g4;
+    g.w[0] = *(const i32x4_t*)(row + (uint32_t)(min(c, KC - 1) * 16));
+    g.w[1] = *(const i32x4_t*)(row + (uint32_t)(min(c + 4, KC - 1) * 16));
   };
   // A thread's part of a unit's results: columns 4 fc .. of block fb, row fr.
   constexpr int kQuads = MODE == kGateUp ? 2 : 4;
@@ -720,7 +721,7 @@ __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
     return row0;
   };
 
-  Group ga, gb;
+  Stage ga, gb;
   Cols cols{};
   Unit u{};
   const int8_t* wrow = nullptr;
@@ -737,25 +738,21 @@ __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
   i32x4_t acc[TM];
 #pragma unroll
   for (int i = 0; i < TM; ++i) acc[i] = i32x4_t{0, 0, 0, 0};
-  auto multiply = [&](const Group& g) {
+  auto multiply = [&](const Stage& g) {
+    const int st = ks + KS * at;
+    if (st >= nst) return;
 #pragma unroll
-    for (int d = 0; d < DEPTH; ++d) {
-      const int st = ks + KS * (at * DEPTH + d);
-      if (st < nst) {
-#pragma unroll
-        for (int i = 0; i < TM; ++i) {
-          if (i > 0 && rows <= 16 * i) continue;
-          const uint8_t* a = sP + (16 * i + ml) * stride + st * 128 + g4 * 16;
-          acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(g.w[d][0], *(const i32x4_t*)a, acc[i], 0, 0, 0);
-          acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(g.w[d][1], *(const i32x4_t*)(a + 64), acc[i], 0, 0, 0);
-        }
-      }
+    for (int i = 0; i < TM; ++i) {
+      if (i > 0 && rows <= 16 * i) continue;
+      const uint8_t* a = sP + (16 * i + ml) * stride + st * 128 + g4 * 16;
+      acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(g.w[0], *(const i32x4_t*)a, acc[i], 0, 0, 0);
+      acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(g.w[1], *(const i32x4_t*)(a + 64), acc[i], 0, 0, 0);
     }
   };
-  // group `at` of unit t from `cur`, with the next one's loads on their way into `nxt`; false where
+  // stage `at` of unit t from `cur`, with the next one's loads on their way into `nxt`; false where
   // that one is of other rows, or there is none
-  auto step = [&](Group& cur, Group& nxt) __attribute__((always_inline)) {
-    const bool last = at + 1 == groups;
+  auto step = [&](Stage& cur, Stage& nxt) __attribute__((always_inline)) {
+    const bool last = at + 1 == mine;
     Unit to = u;
     Cols next{};
     if (last && t + 1 == u1) {
@@ -900,20 +897,38 @@ static int narrow_blocks(int64_t R, int64_t E, int K) {
   if (R > 8 * (R < E ? R : E) && narrow_lds(K, (int)E, 2) <= 80 * 1024) return 2;
   return narrow_lds(K, (int)E, 1) <= kLdsMost ? 1 : 0;
 }
+// The limit of dynamic LDS is a kernel's on a device: raised at its first launch there that needs it.
+template <auto Kernel>
+static void launch_units(const Params& p, int64_t units, int64_t lds, hipStream_t stream) {
+  static std::atomic<uint64_t> raised{0};
+  if (lds > 64 * 1024) {
+    int dev = 64;
+    const uint64_t bit = hipGetDevice(&dev) == hipSuccess && dev < 64 ? (uint64_t)1 << dev : 0;
+    if (!bit || !(raised.load() & bit)) {
+      if (hipFuncSetAttribute((const void*)Kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsMost) == hipSuccess)
+        raised.fetch_or(bit);
+    }
+  }
+  hipLaunchKernelGGL(Kernel, dim3((unsigned)std::min(units, (int64_t)cu_count() * 2)), dim3(512), (unsigned)lds, stream, p);
+}
 template <int MODE, int ACT, typename T>
 static void launch_narrow_of(const Params& p, hipStream_t stream) {
   const int tm = narrow_blocks(p.R, p.E, p.K);
   const int64_t nblk = MODE == kGateUp ? p.N / 8 : (p.N + 15) / 16, tiles = p.R / (16 * tm) + (p.R < p.E ? p.R : p.E);
-  const int64_t lds = narrow_lds(p.K, p.E, tm), most = (int64_t)cu_count() * 2;
-  auto launch = [&](auto kernel, int nb) {
-    const int64_t units = tiles * ((nblk + nb - 1) / nb);
-    if (lds > 64 * 1024)
-      (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsMost);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)std::min(units, most)), dim3(512), (unsigned)lds, stream, p);
-  };
-  const bool small = tiles * nblk <= most;
-  if (tm == 1) small ? launch(narrow_kernel<MODE, ACT, T, 1, 1, 1>, 1) : launch(narrow_kernel<MODE, ACT, T, 4, 1, 1>, 4);
-  else small ? launch(narrow_kernel<MODE, ACT, T, 1, 2, 1>, 1) : launch(narrow_kernel<MODE, ACT, T, 4, 2, 1>, 4);
+  const int64_t lds = narrow_lds(p.K, p.E, tm);
+  // One block of weight rows a unit, its k shared by all eight waves, where those do not fill the chip
+  // twice (us, one / two / four blocks: 7168 x 2048 9 / 11 / 18, 2304 x 2304 7 / 7 / 9); else four, whose
+  // waves read longer runs (64 tokens' rows on 32 experts of 2880 x 2880 65 / 60 / 58, on 256 of 2304 x 2048
+  // 228 / 190 / 187).
+  const bool small = tiles * nblk <= (int64_t)cu_count() * 2;
+  const int64_t units = small ? tiles * nblk : tiles * ((nblk + 3) / 4);
+  if (tm == 1) {
+    if (small) launch_units<narrow_kernel<MODE, ACT, T, 1, 1>>(p, units, lds, stream);
+    else launch_units<narrow_kernel<MODE, ACT, T, 4, 1>>(p, units, lds, stream);
+  } else {
+    if (small) launch_units<narrow_kernel<MODE, ACT, T, 1, 2>>(p, units, lds, stream);
+    else launch_units<narrow_kernel<MODE, ACT, T, 4, 2>>(p, units, lds, stream);
+  }
 }
 template <int MODE, int ACT>
 static void launch_narrow(const Params& p, hipStream_t stream) {
