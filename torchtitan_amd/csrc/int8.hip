@@ -14,7 +14,10 @@
 //   g' = min(g + b, L), u' = clamp(u + b, -L, L), g' sigmoid(1.702 g') (u' + 1).
 //
 // v_mfma_i32_16x16x64_i8: lane (row, q), q = lane / 16, holds 16 consecutive k of its row; the sums
-// are exact (K <= 131072: 2^17 * 127 * 128 < 2^31).
+// are exact (K <= 131072: 2^17 * 127 * 128 < 2^31), and what is done with them is the same in every
+// kernel and tile, so that a row's results do not depend on which of them it went through. (On
+// random codes that instruction alone runs at 4.1 POP/s on this card, v_mfma_i32_32x32x32_i8 at 3.5: the
+// clock goes by the power they take.)
 #include <algorithm>
 #include <atomic>
 
@@ -103,7 +106,9 @@ __device__ __forceinline__ uint2 codes8(const Eight<T>& e, float r) {
 
 // Rows of cols elements, ld apart, to rows of q_cols >= cols codes, zeros behind. W waves a row,
 // up to 8 chunks of eight elements a lane in registers between the maximum and the codes; longer
-// rows are read again.
+// rows are read again. A code is one fused operation and a byte move. Bound by HBM, 3 bytes an
+// element from bf16: 131072 x 2304 in 150 to 176 us, 5.2 to 6.0 TB/s; 16384 x 7168 (four waves a row) 69 us, 5.1;
+// from fp32 131072 x 1024 115 us, 5.8. 64 x 2304 3.2 us, a launch's latency.
 template <typename T, int W>
 __global__ __launch_bounds__(256) void quant_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int cols,
                                                     int q_cols, int8_t* __restrict__ q, float* __restrict__ scale) {
@@ -173,7 +178,8 @@ __global__ __launch_bounds__(256) void quant_any_kernel(const T* __restrict__ x,
 __device__ __forceinline__ void put(uint16_t* p, float v) { *p = (uint16_t)f2bf(v); }
 __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 
-// Codes back to values: a wave a row, in pieces of eight where they are aligned.
+// Codes back to values: a wave a row, in pieces of eight where they are aligned. Bound by HBM:
+// 131072 x 2304 to bf16 145 us, 6.2 TB/s.
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void dequant_kernel(const int8_t* __restrict__ q, const float* __restrict__ scale,
                                                       int64_t rows, int cols, T* __restrict__ x) {
@@ -305,8 +311,19 @@ __device__ __forceinline__ void zero_rest(const Params& p, int from) {
 // direct-to-LDS copies, S - 1 stages ahead and across tile boundaries. gate_up's columns alternate
 // in blocks of 16 between gate and up, so that a lane holds both. An expert's rows are shared
 // evenly by its tiles, a tile's by its waves, in blocks of 16, and a wave's stages are compiled for
-// each number of blocks.
-// The scales and biases of a tile come into LDS with its first stage.
+// each number of blocks. The scales and biases of a tile come into LDS with its first stage: loads
+// of them behind the sums waited for every copy on its way, 4 % of the whole.
+//
+// What bounds it. Dense, 16384 x 7168 x 7168 on 256 x 256: 684 us, 2.46 POP/s (the library's int8 product of
+// 8192 cubed runs at 1.99, its fp8 one at 2.58): MFMAs 58 % busy at 1.85 GHz, where they alone come to 4.1; no
+// bank conflicts (chunk 4 step + g4 of a row: 2 g4 + step met every bank twice). 131072 rows on 256
+// experts of 2304 / 1024: gate_up 754 us, down 448, 1.6 and 1.4 POP/s: they also move 2.2 and 1.5 GB; without
+// their stores they take 240 us less, without the experts' weights from memory 90.
+// Measured and not kept: a touch of the lines three stages ahead (7 % slower, 64 x 128 tiles 40 %: the
+// copies' path is the narrow place); a tile's results kept in registers and stored between the
+// next one's MFMAs (20 % slower, 250 registers); s_setprio for one of a SIMD's two waves (the same);
+// rows in two, four, eight passes of all kernels so that codes and h stay in the cache (1479, 1531,
+// 1655 us for 1456).
 template <int MODE, int ACT, int WM, int WN, int TM, int TN, int S>
 __global__ __launch_bounds__(64 * WM * WN, 2) void wide_kernel(Params p) {
   constexpr int NW = WM * WN, BM = 16 * WM * TM, BN = 16 * WN * TN;
@@ -582,6 +599,13 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wide_kernel(Params p) {
 // the rows, which are quantized on the way into LDS, are prepared once per expert and workgroup.
 // The columns' scales and biases are asked for ahead of the unit's first stages: loads come back in
 // order, so that one asked for where it is used would wait for the stages behind it.
+//
+// What bounds it: 64 tokens' 256 rows on 32 experts of 2880 x 2880 51 us, 265 MB of weights at 5.2 TB/s. One row
+// of 7168 x 2048 8.5 us, of which the weights are 3: 0.2 until the arguments are there, 0.7 to the first
+// loads, 1.9 until the row is quantized, 4.1 for its weights, 115 KB into each of 128 CUs (28 KB/us is
+// what a CU takes in from memory); one token's 8 experts of 256 of 2304 / 1024 11.3 and 8.6 us. Measured
+// otherwise: two stages in flight 1 to 15 % slower, more spill; x behind the first weights 1 us
+// later; arguments asked for where they are used 0.5 us.
 __host__ __device__ constexpr int narrow_stride(int K) { return padded(K) + 16; }  // rows 16 bytes apart mod 128
 __host__ __device__ constexpr int64_t narrow_lds(int K, int E, int TM) {  // rows, two units' sums, row scales and maxima, segments
   return 16 * (int64_t)TM * narrow_stride(K) + 2 * 8 * TM * 64 * 16 + 16 * TM * 4 + 8 * 4 + 2 * (E + 1) * (int)sizeof(int);
@@ -652,6 +676,7 @@ __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
   struct Cols { float a[4], b[4], ba[4], bb[4]; };  // scales (of gate and up) and biases
   auto first_col = [&](const Unit& u) { return (u.cb * NB + fb) * COLS + 4 * fc; };
   auto load_cols = [&](Cols& c, const Unit& u) {
+    if (fb >= NB) return;  // (whole waves)
     const int n = min(first_col(u), N - 1);
     col_scales(p.sa, p, u.e, n, c.a);
     if (MODE == kGateUp) col_scales(p.sb, p, u.e, n, c.b);
