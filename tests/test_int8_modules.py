@@ -135,6 +135,17 @@ def test_what_cannot_be_converted_is_refused(convert):
     assert isinstance(part, FeedForward) and type(part.w1) is Linear
 
 
+def test_sizes_and_types_are_checked_before_anything_is_replaced(convert):
+    from torchtitan_amd import GroupedExperts
+
+    for bad in (_lin(72, 64).build(), _ffn(h=40).build(), GroupedExperts.Config(dim=24, hidden_dim=48, num_experts=2).build(),
+                _lin(64, 8).build().half(), _lin(64, 8).build().double()):
+        model = torch.nn.ModuleDict({"a": _experts(), "b": bad})
+        with pytest.raises((ValueError, TypeError), match="^b"):
+            convert(model, "a", "b")
+        assert type(model["a"]) is GroupedExperts and model["b"] is bad
+
+
 def test_converter_needs_the_hardware(monkeypatch):
     from torchtitan_amd import quantization as Q
 

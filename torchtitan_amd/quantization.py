@@ -28,6 +28,7 @@ from dataclasses import dataclass, field
 import torch
 from torch import nn
 
+from . import ops
 from .configurable import Configurable
 from .feed_forward import FeedForward
 from .gpt_oss import GptOssGroupedExperts
@@ -284,6 +285,14 @@ class Int8WeightConverter(_ExpertsConverter):
         marked = [r for r in _RECIPES if getattr(mod, r, False)]
         if marked:
             raise ValueError(f"{name} is already converted to {marked[0]}")
+        for part, p in mod.named_parameters():
+            if "bias" in part:
+                continue
+            if p.dtype not in (torch.bfloat16, torch.float32):
+                raise TypeError(f"{name}: 8-bit weights are made of bfloat16 and float32, {part} is {p.dtype}")
+            if p.shape[-1] % ops.INT8_MULTIPLE or not ops.INT8_MULTIPLE <= p.shape[-1] <= ops.INT8_MAX_K:
+                raise ValueError(f"{name}: 8-bit weights take contractions that are multiples of {ops.INT8_MULTIPLE} up to "
+                                 f"{ops.INT8_MAX_K}, {part} is {list(p.shape)}")
 
 
 def find_pad_multiple(converters: list) -> int | None:
