@@ -128,6 +128,49 @@ def test_linear_extremes(dev):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+def test_linear_of_rows_at_the_end_of_the_range(dev, dtype):
+    """Rows that hold the type's lowest value, by weights that bring the result back into its range, as
+    well as rows and weights at the small end: no product of a sum with one scale alone may overflow
+    or lose bits."""
+    banner(f"linear_int8 range {dtype}")
+    from torchtitan_amd import ops
+
+    gen = torch.Generator().manual_seed(8)
+    k, n = 208, 72
+    for r in (1, 3, 150, 700):
+        x = I.rows(gen, r, k, dtype)
+        x[0, 5] = torch.finfo(dtype).min
+        if r > 1:
+            x[1] *= 2.0 ** -80
+            x[2] *= 2.0 ** 105
+        for power in (-30, 0, 10):
+            w = I.weight(gen, n, k, std=2.0 ** power)
+            bias = torch.randn(n, generator=gen).to(dtype)
+            y, tol = I.linear(x, *w, bias, dtype)
+            got = ops.linear_int8(x.to(dev), *(t.to(dev) for t in w), bias.to(dev))
+            inside = (y.abs() + tol < torch.finfo(dtype).max).all(-1)
+            assert inside[1:].all() and (bool(inside[0]) or power >= 0), "range"
+            I.within(got[inside.to(dev)], y[inside], tol[inside], f"{r} rows, weights of 2^{power}")
+
+
+def test_layers_of_rows_at_the_end_of_the_range(dev):
+    banner("layers range")
+    from torchtitan_amd import ops
+
+    gen = torch.Generator().manual_seed(9)
+    e, d, h = 3, 144, 80
+    for per in (1, 3, 200):
+        counts = torch.full((e,), per)
+        x = I.rows(gen, e * per, d, BF)
+        x[::2, 7] = torch.finfo(BF).min
+        x[::2] *= 2.0 ** -10
+        w1, w3 = (I.weight(gen, e, h, d, std=2.0 ** -100) for _ in range(2))
+        w2 = I.weight(gen, e, d, h)
+        got = ops.grouped_swiglu_int8(x.to(dev), *(t.to(dev) for w in (w1, w2, w3) for t in w), counts.to(dev))
+        I.within(got, *I.experts(x, w1, w2, w3, counts), f"{per} rows an expert")
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("e,k,n", [(1, 64, 24), (5, 208, 40), (8, 2304, 136), (40, 320, 260), (3, 96, 1001)])
 def test_grouped_linear(dev, e, k, n, dtype):
     from torchtitan_amd import ops

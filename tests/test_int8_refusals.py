@@ -39,6 +39,30 @@ def test_rows(lib, at):
     assert quant(rows=2 ** 31) == -2 and dequant(rows=2 ** 31) == -2
 
 
+def test_rows_past_the_columns_that_are_counted(lib, at):
+    """Columns are counted in 32 bits, with steps past the last one."""
+    big = 2 ** 30 + 8
+    assert lib.moe_int8_quant_rows(at, big, 1, big, 0, at, at, None) == -2
+    assert lib.moe_int8_dequant_rows(at, at, 1, big, 0, at, None) == -2
+
+
+def test_sizes_that_an_entry_would_cut(monkeypatch):
+    """Sizes past 32 bits are refused before they reach an entry, which would take their low part."""
+    from torchtitan_amd import ops
+
+    monkeypatch.setattr(ops, "_int8_device", lambda *a: 0)
+    monkeypatch.setattr(ops, "_int8_launch", lambda *a: pytest.fail("launched"))
+    x = torch.zeros(1, dtype=torch.bfloat16)
+    for cols in (2 ** 30 + 1, 2 ** 32 + 16):
+        with pytest.raises(ValueError, match="columns"):
+            ops._int8_quantize(x.expand(1, cols))
+        with pytest.raises(ValueError, match="columns"):
+            ops._int8_dequantize(torch.zeros(1, dtype=torch.int8).expand(cols), torch.zeros(()), torch.bfloat16)
+    for n in (2 ** 22 + 1, 2 ** 32 + 8):
+        with pytest.raises(ValueError, match="output channels"):
+            ops._linear_int8(x.expand(1, 16), torch.zeros(1, dtype=torch.int8).expand(n, 16), torch.zeros(1).expand(n))
+
+
 def test_linear(lib, at):
     def run(r=4, e=2, k=64, n=32, x=at, w=at, s=at, b=None, bd=0, c=at, ws=at, size=1 << 40, y=at, dtype=0):
         return lib.moe_int8_linear(x, dtype, w, s, b, bd, c, r, e, k, n, ws, size, y, None)

@@ -32,6 +32,7 @@ using namespace grouped;
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kMaxK = 131072;
+constexpr int kMaxCols = 1 << 30;  // of rows by themselves, so that a column and a step fit 32 bits
 constexpr float kLeast = 127.0f * 0x1p-126f;
 
 // The columns of a row operand: whole stages of 128, so that every copy of a stage lies inside its
@@ -245,6 +246,21 @@ __device__ __forceinline__ float activation(int act, float g, float u, float lim
   if (act == kSwiGLU) return g * mx::sigmoid(g) * u;
   const float a = g > limit ? limit : g, b = u < -limit ? -limit : (u > limit ? limit : u);  // NaN passes
   return a * mx::sigmoid(kOssAlpha * a) * (b + 1.0f);
+}
+
+// Sums s of a row by four columns, in their scales. A sum's product with one scale may leave fp32's
+// range where the whole does not: with the row's first if that is below 2^97 (a sum is below 2^31),
+// else with the column's, which leaves it only where the whole does. Neither goes below the
+// normal range. (Rows of the second kind are rare: a branch of the whole wave, not two choices a sum.)
+__device__ __forceinline__ void scaled(const i32x4_t& s, float rs, const float (&c)[4], float (&v)[4]) {
+#pragma clang fp contract(off)  // (a bias is added to what is rounded here, in every kernel)
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = (float)s[i] * rs * c[i];
+  const bool high = rs >= 0x1p97f;
+  if (__any(high)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = high ? (float)s[i] * c[i] * rs : v[i];
+  }
 }
 
 // scales of weight rows n .. n + 3 of expert e (uniform), linear's biases, gpt-oss's of gate and up
@@ -548,7 +564,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wide_kernel(Params p) {
       const int n0 = cur.nt * (MODE == kGateUp ? BN / 2 : BN) + (wn * TN / 2 + b) * (MODE == kGateUp ? 16 : 32);
       if (n0 >= N) continue;
       const int at = (wn * TN + 2 * b) * 16 + 4 * g4;
-      const float4 ca = *(const float4*)&s_col[at], cb = *(const float4*)&s_col[at + 16];
+      float ca[4], cb[4];
+      *(float4*)ca = *(const float4*)&s_col[at];
+      *(float4*)cb = *(const float4*)&s_col[at + 16];
       float ba[4], bb[4];  // (no biases: zeros)
       if constexpr (MODE == kLinear || ACT == kOssGLU) {
         const int sh = p.bias_f32 ? 0 : 16;
@@ -564,8 +582,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wide_kernel(Params p) {
         const int m = (wave_row + i) * 16 + ml, r = cur.row0 + m;
         const float rs = s_row[m];
         const i32x4_t sa = acc[i][2 * b], sb = acc[i][2 * b + 1];
-        float lo[4] = {(float)sa[0] * rs * ca.x, (float)sa[1] * rs * ca.y, (float)sa[2] * rs * ca.z, (float)sa[3] * rs * ca.w};
-        float hi[4] = {(float)sb[0] * rs * cb.x, (float)sb[1] * rs * cb.y, (float)sb[2] * rs * cb.z, (float)sb[3] * rs * cb.w};
+        float lo[4], hi[4];
+        scaled(sa, rs, ca, lo);
+        scaled(sb, rs, cb, hi);
         if constexpr (MODE == kLinear || ACT == kOssGLU) {
 #pragma unroll
           for (int k = 0; k < 4; ++k) { lo[k] += ba[k]; hi[k] += bb[k]; }
@@ -819,19 +838,19 @@ __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
       };
       const float s = s_scale[fr];
       float v[4];
-      const i32x4_t sg = sum(fl);
+      scaled(sum(fl), s, cols.a, v);
       if (MODE == kGateUp) {
-        const i32x4_t su = sum(fl + 32);
+        float up[4];
+        scaled(sum(fl + 32), s, cols.b, up);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          float gv = (float)sg[q] * s * cols.a[q], uv = (float)su[q] * s * cols.b[q];
-          if constexpr (ACT == kOssGLU) { gv += cols.ba[q]; uv += cols.bb[q]; }
-          v[q] = activation(ACT, gv, uv, p.limit);
+          if constexpr (ACT == kOssGLU) { v[q] += cols.ba[q]; up[q] += cols.bb[q]; }
+          v[q] = activation(ACT, v[q], up[q], p.limit);
         }
         *(float4*)(p.h + (int64_t)(row0 + fr) * N + n) = make_float4(v[0], v[1], v[2], v[3]);
       } else {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) v[q] = (float)sg[q] * s * cols.a[q] + cols.ba[q];
+        for (int q = 0; q < 4; ++q) v[q] += cols.ba[q];
         store4(p, row0 + fr, n, v);
       }
     }
@@ -1064,7 +1083,7 @@ using namespace moe::int8;
 MOE_API int moe_int8_quant_rows(const void* x, int64_t ld, int64_t rows, int32_t cols, int32_t dtype, int8_t* q,
                                 float* scale, hipStream_t stream) {
   if (rows < 0 || cols < 1 || ld < cols || (dtype != 0 && dtype != 1)) return kErrInvalidArgument;
-  if (rows >= kMaxGrid) return kErrUnsupportedShape;
+  if (rows >= kMaxGrid || cols > kMaxCols) return kErrUnsupportedShape;
   if (rows == 0) return kOk;
   if (!x || !q || !scale) return kErrInvalidArgument;
   if (dtype == 0) launch_quant((const uint16_t*)x, ld, rows, cols, cols, q, scale, stream);
@@ -1075,7 +1094,7 @@ MOE_API int moe_int8_quant_rows(const void* x, int64_t ld, int64_t rows, int32_t
 MOE_API int moe_int8_dequant_rows(const int8_t* q, const float* scale, int64_t rows, int32_t cols, int32_t dtype, void* x,
                                   hipStream_t stream) {
   if (rows < 0 || cols < 1 || (dtype != 0 && dtype != 1)) return kErrInvalidArgument;
-  if (rows >= kMaxGrid) return kErrUnsupportedShape;
+  if (rows >= kMaxGrid || cols > kMaxCols) return kErrUnsupportedShape;
   if (rows == 0) return kOk;
   if (!q || !scale || !x) return kErrInvalidArgument;
   const bool vec = cols % 8 == 0 && aligned16(x) && ((uintptr_t)q & 7) == 0;

@@ -1723,6 +1723,8 @@ _I8 = torch.library.Library("moe_mi355x_int8", "FRAGMENT")
 _I8_BARE = torch.library.Library("moe_mi355x_int8_bare", "FRAGMENT")  # (as _MX_BARE)
 INT8_MULTIPLE = 16  # of the products' contractions: weight rows are read in 16-byte pieces
 INT8_MAX_K = 131072  # past it a sum of code products can leave 32 bits
+INT8_MAX_COLUMNS = 2 ** 30  # of rows by themselves
+INT8_MAX_N = 2 ** 22  # output channels
 
 # A generation step's calls take the host as long as the GPU, so what is right is checked in few
 # steps, and a message is put together where something is not.
@@ -1784,6 +1786,11 @@ def _int8_code(op: str, dtype: torch.dtype) -> int:
     return code
 
 
+def _check_int8_columns(op: str, rows: Tensor) -> None:
+    if not rows.dim() or not 1 <= rows.shape[-1] <= INT8_MAX_COLUMNS:
+        raise ValueError(f"{op} expects rows of 1 to {INT8_MAX_COLUMNS} columns, got {tuple(rows.shape)}")
+
+
 def _no_int8_gradients(op: str, *tensors: Tensor | None) -> None:
     if torch.is_grad_enabled() or forward_ad._current_level >= 0:
         for t in tensors:
@@ -1795,8 +1802,7 @@ def _no_int8_gradients(op: str, *tensors: Tensor | None) -> None:
 def _int8_quantize(x: Tensor) -> tuple[Tensor, Tensor]:
     here = _int8_device("int8_quantize", x)
     code = _int8_code("int8_quantize", x.dtype)
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError(f"int8_quantize expects rows of at least one column, got {tuple(x.shape)}")
+    _check_int8_columns("int8_quantize", x)
     shape = x.shape
     ld = cols = shape[-1]
     if not x.is_contiguous():
@@ -1828,8 +1834,7 @@ def int8_quantize(x: Tensor) -> tuple[Tensor, Tensor]:
 def _int8_dequantize(q: Tensor, scale: Tensor, dtype: torch.dtype) -> Tensor:
     here = _int8_device("int8_dequantize", q, scale)
     code = _int8_code("int8_dequantize", dtype)
-    if q.dim() < 1 or q.shape[-1] < 1:
-        raise ValueError(f"int8_dequantize expects rows of at least one column, got {tuple(q.shape)}")
+    _check_int8_columns("int8_dequantize", q)
     _check_int8("int8_dequantize", "q", q, scale, q.shape)
     q, scale = q.contiguous(), scale.contiguous()
     x = torch.empty_like(q, dtype=dtype)
@@ -1864,8 +1869,8 @@ def _int8_product(op: str, here: int, x: Tensor, qw: Tensor, sw: Tensor, counts:
     code = _int8_code(op, x.dtype)
     _check_int8(op, "qw", qw, sw, qw.shape)
     _check_int8_dims(op, e, k)
-    if n < 1:
-        raise ValueError(f"{op} expects at least one output channel, got {tuple(qw.shape)}")
+    if not 1 <= n <= INT8_MAX_N:
+        raise ValueError(f"{op} expects 1 to {INT8_MAX_N} output channels, got {tuple(qw.shape)}")
     bias_code = 0
     if bias is not None:
         bias_code = _check_int8_bias(op, bias, qw.shape[:-1])
