@@ -137,6 +137,81 @@ def test_every_tile(dev, r, e, k, n):
         at += c
 
 
+@pytest.mark.parametrize("r,tile", [(6000, 0), (3000, 1), (1500, 2), (300, 3)])
+def test_layers_on_every_tile(dev, r, tile):
+    """The layers' products on each tile: an expert's first and last rows as they come out alone, the first
+    ones as 64 bits give them. Biases in both types, linear's too."""
+    banner(f"int8 layers on tile {tile}")
+    from torchtitan_amd import _lib, ops
+
+    gen = torch.Generator().manual_seed(11)
+    e, d, h = 4, 1536, 720
+    assert _lib.lib().moe_int8_tile(r, e, d, 2 * h, 256) == tile
+    counts = torch.tensor([r // 4 + 5, 0, r // 2 - 20, r // 4 + 9])
+    x = I.rows(gen, r, d)
+    w1, w2, w3, m1 = (I.weight(gen, e, *s) for s in ((h, d), (d, h), (h, d), (2 * h, d)))
+    b1, b2 = torch.randn(e, 2 * h, generator=gen), torch.randn(e, d, generator=gen)
+    on = lambda *ts: [t.to(dev) for t in ts]  # noqa: E731
+    xd, cd = x.to(dev), counts.to(dev)
+    forms = [(ops.grouped_swiglu_int8, on(*w1, *w2, *w3), (), lambda i, t: I.experts(t, *([q[i:i + 1] for q in w] for w in (w1, w2, w3)),
+                                                                                     torch.tensor([len(t)])))]
+    for dt in (BF, F32):
+        a1, a2 = b1.to(dt), b2.to(dt)
+        forms += [(ops.grouped_swiglu_oss_int8, on(*m1, a1, *w2, a2), (7.0,),
+                   lambda i, t, a1=a1, a2=a2: I.oss(t, [q[i:i + 1] for q in m1], a1[i:i + 1], [q[i:i + 1] for q in w2], a2[i:i + 1],
+                                                    torch.tensor([len(t)]), 7.0)),
+                  (lambda x, qw, sw, b, c: ops.grouped_linear_int8(x, qw, sw, c, b), on(*m1, a1), (),
+                   lambda i, t, a1=a1: I.linear(t, m1[0][i], m1[1][i], a1[i], BF))]
+    for f, weights, rest, want in forms:
+        got = f(xd, *weights, cd, *rest)
+        for i, a, b in I.segments(counts, r):
+            part = [t[i:i + 1] for t in weights]
+            n = min(7, b - a)
+            for at in (a, b - n):
+                alone = f(xd[at:at + n], *part, torch.tensor([n], device=dev), *rest)
+                assert torch.equal(alone, got[at:at + n]), f"expert {i}, rows from {at}"
+            I.within(got[a:a + n], *want(i, x[a:a + n]), f"expert {i}")
+        assert not got[int(counts.sum()):].any()
+
+
+def test_two_threads(dev):
+    """Calls from two threads at once, each on a stream of its own."""
+    banner("int8 threads")
+    from concurrent.futures import ThreadPoolExecutor
+
+    from torchtitan_amd import ops
+
+    gen = torch.Generator().manual_seed(12)
+    w = [t.to(dev) for s in ((8, 256, 512), (8, 512, 256), (8, 256, 512)) for t in I.weight(gen, *s)]
+    xs = [I.rows(gen, n, 512).to(dev) for n in (16, 1600)]
+    cs = [torch.full((8,), len(x) // 8, device=dev) for x in xs]
+    want = [ops.grouped_swiglu_int8(x, *w, c) for x, c in zip(xs, cs)]
+    torch.cuda.synchronize()
+
+    def work(i):
+        s = torch.cuda.Stream()
+        with torch.no_grad(), torch.cuda.stream(s):
+            got = [ops.grouped_swiglu_int8(xs[(i + k) % 2], *w, cs[(i + k) % 2]) for k in range(8)]
+        s.synchronize()
+        return all(torch.equal(g, want[(i + k) % 2]) for k, g in enumerate(got))
+
+    with ThreadPoolExecutor(2) as pool:
+        assert all(pool.map(work, range(4)))
+
+
+def test_operands_on_other_devices_are_refused(dev):
+    from torchtitan_amd import ops
+
+    gen = torch.Generator().manual_seed(13)
+    w = [t.to(dev) for s in ((2, 64, 96), (2, 96, 64), (2, 64, 96)) for t in I.weight(gen, *s)]
+    x, c = I.rows(gen, 8, 96), torch.tensor([4, 4])
+    for call in (lambda: ops.grouped_swiglu_int8(x.to(dev), *w, c), lambda: ops.grouped_swiglu_int8(x, *w, c.to(dev)),
+                 lambda: ops.grouped_linear_int8(x.to(dev), w[0].cpu(), w[1], c.to(dev)), lambda: ops.linear_int8(x.to(dev), w[0][0], w[1][0].cpu()),
+                 lambda: ops.linear_int8(x.to(dev), w[0][0], w[1][0], torch.zeros(64)), lambda: ops.int8_quantize(x)):
+        with pytest.raises((RuntimeError, ValueError, NotImplementedError)):
+            call()
+
+
 def test_many_units_a_workgroup(dev):
     """Few rows on so many wide experts that a workgroup goes through several units and experts."""
     banner("int8 many units")
