@@ -635,7 +635,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wide_kernel(Params p) {
 // The columns' scales and biases are asked for ahead of the unit's first stages: loads come back in
 // order, so that one asked for where it is used would wait for the stages behind it.
 //
-// What bounds it: 64 tokens' 256 rows on 32 experts of 2880 x 2880 51 us, 265 MB of weights at 5.2 TB/s. One row
+// What bounds it: 128 rows on 32 experts of 2880 x 2880 52 us, 265 MB of weights at 5.1 TB/s. One row
 // of 7168 x 2048 8.5 us, of which the weights are 3: 0.2 until the arguments are there, 0.7 to the first
 // loads, 1.9 until the row is quantized, 4.1 for its weights, 115 KB into each of 128 CUs (28 KB/us is
 // what a CU takes in from memory); one token's 8 experts of 256 of 2304 / 1024 11.3 and 8.6 us. Measured
@@ -900,9 +900,9 @@ constexpr Tile kTiles[] = {{256, 256, 1, 145, 550}, {128, 256, 1, 90, 280}, {64,
 
 // The tile with the least time by that count: as many rounds of the chip as its tiles take, half a
 // tile more for each expert that can have rows. Measured against the others (us, 256 x 256 / 128 x
-// 256 / 64 x 128 / 64 x 64): 16384 x 7168 x 7168 732 / 808 / 1098 / 1440; 2048 x 2304 x 2304 40 / 29
-// / 36 / 36; 1024 x 2304 x 2304 38 / 27 / 23 / 27; 1003 x 2880 x 1001 59 / 37 / 22 / 19; 131072 rows
-// on 256 experts of 2304 x 1024 564 / 549 / 708 / 834; 8200 on 32 of 7168 x 2048 242 / 210 / 270 / 298.
+// 256 / 64 x 128 / 64 x 64): 16384 x 7168 x 7168 736 / 796 / 1076 / 1469; 2048 x 2304 x 2304 38 / 27
+// / 33 / 32; 1024 x 2304 x 2304 35 / 24 / 20 / 24; 1003 x 2880 x 1008 41 / 27 / 19 / 16; 131072 rows
+// on 256 experts of 2304 x 1024 548 / 527 / 698 / 848; 8192 on 32 of 7168 x 2048 250 / 204 / 275 / 294.
 static int pick_tile(int64_t R, int64_t E, int64_t K, int64_t cols, int64_t cus) {
   const int64_t nk = (K + 127) / 128, used = R < E ? R : E;
   int best = 0;
@@ -986,19 +986,24 @@ static void launch_narrow(const Params& p, hipStream_t stream) {
 }
 
 // Whether a product with `cols` weight rows (gate_up: of both) goes to the narrow kernel: where it reads
-// little and has up to 128 rows an expert, or where there are up to eight and less work in
-// quantizing them, which every workgroup does, than in its weights (1024 bytes of a row's two in
-// each of 512 workgroups a weight row). us, narrow / wide with its quantization: 16 rows of 7168 x 2048 17 /
-// 19, 48 rows 34 / 21; 96 rows of 2304 x 2304 12 / 13; 48 of 2880 x 2880 14 / 20; 16 of 2304 x 2304 8 / 16; one of 7168 x 7168 20 / 24, eight
-// 29 / 24; experts (both products), one token's 8 of 256 of 2304 / 1024 23 / 29, 64 tokens' 292 / 279; 4, 8,
-// 12 rows each on 32 of 2880 / 2880 157 / 168, 166 / 172, 190 / 174; on 32 of 7168 / 2048 297 / 312, 314 / 317,
-// 359 / 319; 4 on 256 of 2304 / 1024 342 / 325.
+// little and has up to 128 rows an expert, or where there are up to eight, less work in quantizing
+// them, which every workgroup does, than in its weights (1024 bytes of a row's two in each of 512
+// workgroups a weight row), and not so many weights that more bytes on their way count. Where long
+// rows leave a CU one workgroup, half the rows and a fifth of the bytes. us, narrow / wide with its
+// quantization: 16 rows of 7168 x 2048 17.3 / 18.1, 48 rows 34 / 20; 96 rows of 2304 x 2304 11.5 / 11.4;
+// 16 8.2 / 10.2; 32 of 2880 x 2880 13.2 / 12.2, 16 9.0 / 11.5 (a wide call, of two launches, takes the host 4 us
+// more); one of 7168 x 7168 19.8 / 21.8, four 22.1 / 22.1, seven 28.6 / 22.1; on 32 experts of 2880 x 2880 64 rows
+// 48.8 / 51.9, 256 58.1 / 57.4, of 5760 x 2880 8 rows 26.9 / 31.8, 128 112 / 101; on 64 of 2304 x 2048 64 rows 45.6 /
+// 47.5, 256 62.9 / 57.2; on 256 of it 8 10.7 / 12.5, 64 47 / 51, 256 142 / 140; on 256 of 1024 x 2304 64 27 / 30, 256
+// 78 / 74; on 32 of 7168 x 4096 8 rows 57 / 38.
 static bool takes_narrow(int64_t R, int64_t E, int K, int64_t cols) {
   const int tm = narrow_blocks(R, E, K);
   if (!tm) return false;
   const int64_t used = R < E ? R : E, tiles = E == 1 ? (R + 16 * tm - 1) / (16 * tm) : R / (16 * tm) + used;
   const int64_t bytes = tiles * cols * K;
-  return (R <= 128 * used && bytes <= 30000000) || (R <= 8 * used && 1024 * R <= cols * used * used && bytes <= 900000000);
+  const bool two = narrow_lds(K, (int)E, tm) <= 80 * 1024;  // workgroups a CU
+  return (R <= 128 * used && bytes <= 30000000) ||
+         (R <= (two ? 8 : 4) * used && 1024 * R <= cols * used * used && bytes <= (two ? 330000000 : 60000000));
 }
 
 static int check_shape(int64_t R, int E, int K, int N) {
