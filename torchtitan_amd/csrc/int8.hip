@@ -895,15 +895,17 @@ static bool aligned16(const void* a) { return ((uintptr_t)a & 15) == 0; }
 static int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 
 // The wide kernel's tiles, with what a stage of 128 k and the rest of a tile take in 10 ns, measured
-// where they fill the chip (16384 rows by 7168 x 7168), and the workgroups a CU holds.
-struct Tile { int bm, bn, per_cu, stage, rest; };
-constexpr Tile kTiles[] = {{256, 256, 1, 145, 550}, {128, 256, 1, 90, 280}, {64, 128, 2, 65, 150}, {64, 64, 2, 43, 100}};
+// where they fill the chip (16384 rows by 7168 x 7168), and the workgroups a CU holds. Experts' weights
+// come from memory, which the largest tile, with one stage on its way, waits for: `of_experts`.
+struct Tile { int bm, bn, per_cu, stage, of_experts, rest; };
+constexpr Tile kTiles[] = {{256, 256, 1, 145, 165, 550}, {128, 256, 1, 90, 90, 280}, {64, 128, 2, 65, 65, 150}, {64, 64, 2, 43, 43, 100}};
 
 // The tile with the least time by that count: as many rounds of the chip as its tiles take, half a
 // tile more for each expert that can have rows. Measured against the others (us, 256 x 256 / 128 x
 // 256 / 64 x 128 / 64 x 64): 16384 x 7168 x 7168 736 / 796 / 1076 / 1469; 2048 x 2304 x 2304 38 / 27
 // / 33 / 32; 1024 x 2304 x 2304 35 / 24 / 20 / 24; 1003 x 2880 x 1008 41 / 27 / 19 / 16; 131072 rows
-// on 256 experts of 2304 x 1024 548 / 527 / 698 / 848; 8192 on 32 of 7168 x 2048 250 / 204 / 275 / 294.
+// on 256 experts of 2304 x 1024 548 / 527 / 698 / 848; 8192 on 32 of 7168 x 2048 250 / 204 / 275 / 294; 16384 on
+// 32 of 2880 x 2880 213 / 218; layers of experts 131072 on 256 of 2304 / 1024 1480 / 1451, half as many 850 / 798.
 static int pick_tile(int64_t R, int64_t E, int64_t K, int64_t cols, int64_t cus) {
   const int64_t nk = (K + 127) / 128, used = R < E ? R : E;
   int best = 0;
@@ -912,7 +914,7 @@ static int pick_tile(int64_t R, int64_t E, int64_t K, int64_t cols, int64_t cus)
     const Tile& t = kTiles[i];
     const int64_t mt = E == 1 ? (R + t.bm - 1) / t.bm : std::max(used, R / t.bm + (used + 1) / 2);
     const int64_t tiles = mt * ((cols + t.bn - 1) / t.bn);
-    const int64_t time = (tiles + cus * t.per_cu - 1) / (cus * t.per_cu) * (nk * t.stage + t.rest);
+    const int64_t time = (tiles + cus * t.per_cu - 1) / (cus * t.per_cu) * (nk * (E == 1 ? t.stage : t.of_experts) + t.rest);
     if (time < least) { least = time; best = i; }
   }
   return best;
