@@ -346,10 +346,10 @@ __device__ __forceinline__ void zero_rest(const Params& p, int from) {
 // each number of blocks. The scales and biases of a tile come into LDS with its first stage: loads
 // of them behind the sums waited for every copy on its way, 4 % of the whole.
 //
-// What bounds it. Dense, 16384 x 7168 x 7168 on 256 x 256: 684 us, 2.46 POP/s (the library's int8 product of
+// What bounds it. Dense, 16384 x 7168 x 7168 on 256 x 256: 650 to 684 us, 2.46 to 2.59 POP/s (the library's int8 product of
 // 8192 cubed runs at 1.99, its fp8 one at 2.58): MFMAs 58 % busy at 1.85 GHz, where they alone come to 4.1; no
 // bank conflicts (chunk 4 step + g4 of a row: 2 g4 + step met every bank twice). 131072 rows on 256
-// experts of 2304 / 1024: gate_up 754 us, down 448, 1.6 and 1.4 POP/s: they also move 2.2 and 1.5 GB; without
+// experts of 2304 / 1024, on 128 x 256: gate_up 731 us, down 453, 1.7 and 1.4 POP/s: they also move 2.2 and 1.5 GB; without
 // their stores they take 240 us less, without the experts' weights from memory 90.
 // Measured and not kept: a touch of the lines three stages ahead (7 % slower, 64 x 128 tiles 40 %: the
 // copies' path is the narrow place); a tile's results kept in registers and stored between the
