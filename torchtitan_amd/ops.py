@@ -1798,7 +1798,7 @@ def _no_int8_gradients(op: str, *tensors: Tensor | None) -> None:
                 _no_gradients(op, t, instead="codes are not differentiable: train on the bf16 weights")
 
 
-@_mx_op("int8_quantize(Tensor x) -> (Tensor, Tensor)", _I8)
+@_mx_op("int8_quantize(Tensor x) -> (Tensor, Tensor)", _I8_BARE)
 def _int8_quantize(x: Tensor) -> tuple[Tensor, Tensor]:
     here = _int8_device("int8_quantize", x)
     code = _int8_code("int8_quantize", x.dtype)
@@ -1816,21 +1816,24 @@ def _int8_quantize(x: Tensor) -> tuple[Tensor, Tensor]:
     return q, scale
 
 
-@torch.library.register_fake("moe_mi355x_int8::int8_quantize", lib=_I8)
+@torch.library.register_fake("moe_mi355x_int8_bare::int8_quantize", lib=_I8_BARE)
 def _(x):
     return x.new_empty(x.shape, dtype=torch.int8), x.new_empty(x.shape[:-1], dtype=torch.float32)
 
 
+@_inference_op(_int8_quantize, _I8)
 def int8_quantize(x: Tensor) -> tuple[Tensor, Tensor]:
     """x [.., K] (bf16 or fp32) in 8-bit integers with a scale for each row: (q [.., K] int8,
     scale [..] fp32). With a = max(max |x|, 127 * 2^-126) of a row and the fp32 quotients
     r = 127 / a, scale = a / 127, its codes are x r rounded once to the nearest integer, ties to
     even (|q| <= 127), and stand for q scale. A row with an infinity or a NaN has the scale NaN
-    and zero codes. Rows of weights [.., N, K] are output channels, rows of activations tokens."""
-    return _int8_quantize(x.detach() if x.requires_grad or forward_ad._current_level >= 0 else x)
+    and zero codes. Rows of weights [.., N, K] are output channels, rows of activations tokens. For
+    inference: no gradients."""
+    _no_int8_gradients("int8_quantize", x)
+    return _int8_quantize(x)
 
 
-@_mx_op("int8_dequantize(Tensor q, Tensor scale, ScalarType dtype) -> Tensor", _I8)
+@_mx_op("int8_dequantize(Tensor q, Tensor scale, ScalarType dtype) -> Tensor", _I8_BARE)
 def _int8_dequantize(q: Tensor, scale: Tensor, dtype: torch.dtype) -> Tensor:
     here = _int8_device("int8_dequantize", q, scale)
     code = _int8_code("int8_dequantize", dtype)
@@ -1842,15 +1845,17 @@ def _int8_dequantize(q: Tensor, scale: Tensor, dtype: torch.dtype) -> Tensor:
     return x
 
 
-@torch.library.register_fake("moe_mi355x_int8::int8_dequantize", lib=_I8)
+@torch.library.register_fake("moe_mi355x_int8_bare::int8_dequantize", lib=_I8_BARE)
 def _(q, scale, dtype):
     return q.new_empty(q.shape, dtype=dtype)
 
 
+@_inference_op(_int8_dequantize, _I8)
 def int8_dequantize(q: Tensor, scale: Tensor, dtype: torch.dtype = torch.bfloat16) -> Tensor:
     """The values q scale [.., K] of a matrix in codes (int8_quantize), taken in fp32, in bf16 or
-    fp32."""
-    return _int8_dequantize(q, scale.detach() if scale.requires_grad or forward_ad._current_level >= 0 else scale, dtype)
+    fp32. For inference: no gradients."""
+    _no_int8_gradients("int8_dequantize", scale)
+    return _int8_dequantize(q, scale, dtype)
 
 
 @functools.lru_cache(maxsize=256)
