@@ -6,6 +6,11 @@
 ``quantization.Int8WeightConverter`` swaps them into a model. A weight is two buffers: ``*_codes``
 [.., N, K] int8 and ``*_scales`` [.., N] fp32 (``ops.int8_quantize`` of the weight's rows). Activations
 are quantized to 8 bits by rows in the kernels, x and what lies between two products alike.
+
+What computed in fp32 before does so still: a feed-forward, and experts of the for-loop path, give
+rows in fp32 to two products each and their activation to a third, all in fp32. Experts of the
+grouped path round such rows to bf16, as the ones that they stand for do, and gpt-oss's experts their
+biases too.
 """
 
 from __future__ import annotations
@@ -13,6 +18,7 @@ from __future__ import annotations
 from dataclasses import dataclass
 
 import torch
+import torch.nn.functional as F
 
 from . import ops
 from .configurable import Module
@@ -109,11 +115,16 @@ class Int8FeedForward(_Packed):
         return out.train(ffn.training)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if x.dtype == torch.float32:
+            h = F.silu(ops.linear_int8(x, *self.packed("w1"))) * ops.linear_int8(x, *self.packed("w3"))
+            return ops.linear_int8(h, *self.packed("w2"))
         y = ops.swiglu_ffn_int8(x.bfloat16(), *self.packed("w1"), *self.packed("w2"), *self.packed("w3"))
         return y.type_as(x)
 
 
 class Int8GroupedExperts(_Packed):
+    use_grouped_mm = True  # (of the class, for whole modules saved without it)
+
     @dataclass(kw_only=True, slots=True)
     class Config(GroupedExperts.Config):
         pass
@@ -122,6 +133,7 @@ class Int8GroupedExperts(_Packed):
         super().__init__()
         d, h, e = config.dim, config.hidden_dim, config.num_experts
         self.num_experts = e
+        self.use_grouped_mm = config.use_grouped_mm
         self._buffer("w1", e, h, d)
         self._buffer("w2", e, d, h)
         self._buffer("w3", e, h, d)
@@ -129,12 +141,15 @@ class Int8GroupedExperts(_Packed):
     @classmethod
     def from_experts(cls, experts: GroupedExperts) -> "Int8GroupedExperts":
         e, h, d = _local(experts.w1).shape
-        out = _empty(cls.Config(dim=d, hidden_dim=h, num_experts=e))
+        out = _empty(cls.Config(dim=d, hidden_dim=h, num_experts=e, use_grouped_mm=experts.use_grouped_mm))
         for name in ("w1", "w2", "w3"):
             out.pack(name, _local(getattr(experts, name)))
         return out.train(experts.training)
 
     def forward(self, x: torch.Tensor, num_tokens_per_expert: torch.Tensor) -> torch.Tensor:
+        if x.dtype == torch.float32 and not self.use_grouped_mm:
+            g, u = (ops.grouped_linear_int8(x, *self.packed(name), num_tokens_per_expert) for name in ("w1", "w3"))
+            return ops.grouped_linear_int8(F.silu(g) * u, *self.packed("w2"), num_tokens_per_expert)
         y = ops.grouped_swiglu_int8(x.bfloat16(), *self.packed("w1"), *self.packed("w2"), *self.packed("w3"),
                                     num_tokens_per_expert)
         return y.type_as(x)
