@@ -23,6 +23,7 @@ replaced by ones on 8-bit integers, ``int8.py``).
 from __future__ import annotations
 
 import logging
+from collections.abc import Callable
 from dataclasses import dataclass, field
 
 import torch
@@ -107,6 +108,20 @@ def _mark_experts(model: nn.Module, fqns: list[str], attr: str) -> list[str]:
     for mod in matching:
         setattr(mod, attr, True)
     return list(matching.values())
+
+
+def _replace(model: nn.Module, matching: list[tuple[str, nn.Module]], make: Callable) -> list[str]:
+    """Puts make(module) in the place of each of the (name, module), one for a module that several names
+    share; returns the names. All are made before the first is put in place, so that one that cannot be
+    (its weights are not on the GPU, the memory is spent) leaves the model as it was."""
+    made = {}
+    for _name, mod in matching:
+        if mod not in made:
+            made[mod] = make(mod)
+    for name, mod in matching:
+        parent, _, child = name.rpartition(".")
+        setattr(model.get_submodule(parent), child, made[mod])
+    return [name for name, _mod in matching]
 
 
 class MXFP8Converter(Configurable):
@@ -226,13 +241,7 @@ class MXFP4WeightConverter(_ExpertsConverter):
                 raise ValueError(f"{name}: the subclass {type(mod).__name__} has no packed form")
             if mod._forward_hooks or mod._forward_pre_hooks or mod._backward_hooks or mod._backward_pre_hooks:
                 raise ValueError(f"{name} has hooks, which its packed form would not run: register them after packing")
-        made = {}  # of a module that several names share, one
-        for name, mod in matching:
-            if mod not in made:
-                made[mod] = _PACKED[type(mod)].from_experts(mod)
-            parent, _, child = name.rpartition(".")
-            setattr(model.get_submodule(parent), child, made[mod])
-        return [name for name, _mod in matching]
+        return _replace(model, matching, lambda mod: _PACKED[type(mod)].from_experts(mod))
 
 
 def _hooked(mod: nn.Module) -> bool:
@@ -264,13 +273,7 @@ class Int8WeightConverter(_ExpertsConverter):
                 self._check(name, mod)
                 matching.append((name, mod))
                 kept.update(mod.children())
-        made = {}  # of a module that several names share, one
-        for name, mod in matching:
-            if mod not in made:
-                made[mod] = _INT8[type(mod)](mod)
-            parent, _, child = name.rpartition(".")
-            setattr(model.get_submodule(parent), child, made[mod])
-        return [name for name, _mod in matching]
+        return _replace(model, matching, lambda mod: _INT8[type(mod)](mod))
 
     @staticmethod
     def _check(name: str, mod: nn.Module) -> None:
