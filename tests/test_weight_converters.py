@@ -59,3 +59,25 @@ def test_a_later_module_that_cannot_be_packed(converters, monkeypatch, name, op)
     assert {type(m).__name__ for m in model.values()} == {"GroupedExperts"}
     monkeypatch.setattr(ops, op, pack)
     assert converters[name](model, "a", "b", "c") == ["a", "b", "c"] and not list(model.parameters())
+
+
+def test_modules_that_could_not_run(converters):
+    """More experts or output channels than the operators take, and feed-forwards whose widths a layer does not
+    have, are refused by the converter, not by the first call."""
+    from torchtitan_amd import FeedForward, GroupedExperts
+    from torchtitan_amd.gpt_oss import GptOssGroupedExperts
+
+    ffn = lambda w1, w2, w3: FeedForward.Config(w1=_lin(*w1), w2=_lin(*w2), w3=_lin(*w3)).build()  # noqa: E731
+    meta = lambda make: torch.nn.Module.to(make, "meta")  # noqa: E731
+    with torch.device("meta"):
+        wide = _lin(16, 2 ** 22 + 1).build()
+    oss = GptOssGroupedExperts.Config(dim=16, hidden_dim=16, num_experts=1025).build()
+    for bad, what in ((_experts(16, 16, 1025), "experts"), (meta(oss), "experts"), (wide, "output channels"),
+                      (_lin(16, 0).build(), "output channels"), (ffn((64, 32), (32, 48), (64, 32)), "w2"),
+                      (ffn((64, 32), (32, 64), (64, 48)), "w3"), (ffn((64, 32), (32, 64), (48, 32)), "w3")):
+        model = torch.nn.ModuleDict({"a": _experts(), "b": bad})
+        with pytest.raises(ValueError, match=f"^b: .*{what}"):
+            converters["Int8WeightConverter"](model, "a", "b")
+        assert type(model["a"]) is GroupedExperts and model["b"] is bad
+    model = torch.nn.ModuleDict({"a": _experts(16, 16, 1024)})
+    assert converters["Int8WeightConverter"](model, "a") == ["a"]

@@ -35,7 +35,7 @@ from .feed_forward import FeedForward
 from .gpt_oss import GptOssGroupedExperts
 from .int8 import Int8FeedForward, Int8GptOssGroupedExperts, Int8GroupedExperts, Int8Linear
 from .linear import Linear
-from .moe import GroupedExperts, TokenChoiceTopKRouter
+from .moe import GroupedExperts, TokenChoiceTopKRouter, _local
 from .mxfp4 import MXFP4GptOssGroupedExperts, MXFP4GroupedExperts
 
 __all__ = ["Float8GroupedMMConverter", "Int8WeightConverter", "MXFP4Converter", "MXFP4WeightConverter", "MXFP8ActivationCheckpointConverter",
@@ -296,6 +296,15 @@ class Int8WeightConverter(_ExpertsConverter):
             if p.shape[-1] % ops.INT8_MULTIPLE or not ops.INT8_MULTIPLE <= p.shape[-1] <= ops.INT8_MAX_K:
                 raise ValueError(f"{name}: 8-bit weights take contractions that are multiples of {ops.INT8_MULTIPLE} up to "
                                  f"{ops.INT8_MAX_K}, {part} is {list(p.shape)}")
+            *experts, n, _k = _local(p).shape
+            if not 1 <= n <= ops.INT8_MAX_N:
+                raise ValueError(f"{name}: 8-bit weights take 1 to {ops.INT8_MAX_N} output channels, {part} is {list(p.shape)}")
+            if experts and not 1 <= experts[0] <= ops.MAX_GEMM_EXPERTS:
+                raise ValueError(f"{name}: 8-bit weights take 1 to {ops.MAX_GEMM_EXPERTS} experts, {part} is {list(p.shape)}")
+        if isinstance(mod, FeedForward):
+            w1, w2, w3 = (list(lin.weight.shape) for lin in (mod.w1, mod.w2, mod.w3))
+            if w3 != w1 or w2 != w1[::-1]:
+                raise ValueError(f"{name}: 8-bit weights take w1 and w3 of [H, D] and w2 of [D, H], got {w1}, {w3} and {w2}")
 
 
 def find_pad_multiple(converters: list) -> int | None:
