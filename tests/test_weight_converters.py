@@ -81,3 +81,18 @@ def test_modules_that_could_not_run(converters):
         assert type(model["a"]) is GroupedExperts and model["b"] is bad
     model = torch.nn.ModuleDict({"a": _experts(16, 16, 1024)})
     assert converters["Int8WeightConverter"](model, "a") == ["a"]
+
+
+@pytest.mark.parametrize("first", ["ffn", "proj"])
+def test_a_projection_that_a_feed_forward_shares(converters, first):
+    """It is replaced under its own name too, whichever name comes first."""
+    from torchtitan_amd import FeedForward
+
+    ffn = FeedForward.Config(w1=_lin(64, 32), w2=_lin(32, 64), w3=_lin(64, 32)).build()
+    parts = {"ffn": ffn, "proj": ffn.w3}
+    weight = ffn.w3.weight
+    model = torch.nn.ModuleDict({k: parts[k] for k in sorted(parts, key=lambda k: k != first)})
+    assert sorted(converters["Int8WeightConverter"](model, "ffn", "proj")) == ["ffn", "proj"]
+    assert type(model["ffn"]).__name__ == "Int8FeedForward" and type(model["proj"]).__name__ == "Int8Linear"
+    for mod, name in ((model["ffn"], "w3"), (model["proj"], "weight")):
+        assert torch.equal(mod.packed(name)[0], I.pack(weight)[0])

@@ -263,16 +263,17 @@ class Int8WeightConverter(_ExpertsConverter):
         """Replaces the matching modules; returns their names. Refused are subclasses, which may compute
         something else, modules with hooks, which would not see the calls any more, feed-forwards
         with biases, and experts that are marked for another recipe."""
-        kept = set()  # what belongs to a router, or to a module that is replaced as a whole
+        kept = set()  # what belongs to a router
         for mod in model.modules():
             if isinstance(mod, TokenChoiceTopKRouter):
                 kept.update(mod.modules())
-        matching = []
+        matching, whole = [], set()  # whole: the names replaced so far, whose parts (which may have other names too) go with them
         for name, mod in model.named_modules(remove_duplicate=False):
-            if self._matches(name) and isinstance(mod, tuple(_INT8)) and mod not in kept:
+            if (self._matches(name) and isinstance(mod, tuple(_INT8)) and mod not in kept
+                    and name.rpartition(".")[0] not in whole):
                 self._check(name, mod)
                 matching.append((name, mod))
-                kept.update(mod.children())
+                whole.add(name)
         return _replace(model, matching, lambda mod: _INT8[type(mod)](mod))
 
     @staticmethod
