@@ -96,3 +96,46 @@ def test_a_projection_that_a_feed_forward_shares(converters, first):
     assert type(model["ffn"]).__name__ == "Int8FeedForward" and type(model["proj"]).__name__ == "Int8Linear"
     for mod, name in ((model["ffn"], "w3"), (model["proj"], "weight")):
         assert torch.equal(mod.packed(name)[0], I.pack(weight)[0])
+
+
+@pytest.fixture
+def mesh():
+    """Two devices of which this process is the first (nothing is sent)."""
+    import torch.distributed as dist
+    from torch.distributed.device_mesh import init_device_mesh
+    from torch.testing._internal.distributed.fake_pg import FakeStore
+
+    dist.init_process_group("fake", store=FakeStore(), rank=0, world_size=2)
+    try:
+        yield init_device_mesh("cpu", (2,), mesh_dim_names=("tp",))
+    finally:
+        dist.destroy_process_group()
+
+
+@pytest.mark.parametrize("dim", [0, 1])
+def test_projections_sharded_over_devices(converters, mesh, dim):
+    """Half of a weight is not taken for the whole; one that every device holds is."""
+    from torch.distributed.tensor import DTensor, Replicate, Shard
+
+    from torchtitan_amd import FeedForward, Linear
+
+    def place(lin, placement):
+        lin.weight = torch.nn.Parameter(DTensor.from_local(lin.weight.detach(), mesh, [placement], run_check=False))
+        return lin
+
+    def half():
+        lin = place(_lin(32 if dim else 64, 32 if dim == 0 else 64).build(), Shard(dim))
+        lin.in_features, lin.out_features = 64, 64
+        return lin
+
+    ffn = FeedForward.Config(w1=_lin(64, 64), w2=_lin(64, 64), w3=_lin(64, 64)).build()
+    ffn.w3 = half()
+    for bad in (half(), ffn):
+        model = torch.nn.ModuleDict({"a": _experts(), "b": bad})
+        with pytest.raises(ValueError, match="does not fit"):
+            converters["Int8WeightConverter"](model, "a", "b")
+        assert model["b"] is bad and isinstance(bad, (Linear, FeedForward)) and list(model["a"].parameters())
+    lin = place(_lin(64, 32).build(), Replicate())
+    model = torch.nn.ModuleDict({"b": lin})
+    assert converters["Int8WeightConverter"](model, "b") == ["b"]
+    assert torch.equal(model["b"].weight_codes, I.pack(lin.weight.to_local())[0])

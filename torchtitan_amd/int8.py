@@ -43,10 +43,11 @@ class _Packed(Module):
 
     @torch.no_grad()
     def pack(self, name: str, weight: torch.Tensor) -> None:
-        """Takes a weight in bf16 or fp32, on the GPU."""
+        """Takes a weight in bf16 or fp32, on the GPU, whole."""
+        weight = _local(weight).detach()
         if weight.shape != self.packed(name)[0].shape:
             raise ValueError(f"{name} of {list(weight.shape)} does not fit {list(self.packed(name)[0].shape)} codes")
-        q, s = ops.int8_quantize(_local(weight).detach())
+        q, s = ops.int8_quantize(weight)
         setattr(self, name + "_codes", q)
         setattr(self, name + "_scales", s)
 
