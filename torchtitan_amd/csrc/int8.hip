@@ -367,6 +367,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void wide_kernel(Params p) {
   static_assert(NCOPY * (S - 2) < 64, "vmcnt");
   static_assert(S - 1 <= kLeastStages, "the copies are in the next tile at most");
   static_assert(BM % 64 == 0 && BN % 64 == 0 && (BM + BN) / 64 <= NW, "a wave's scales");
+  static_assert(S * (BM + BN) * RB + kTileList * 16 + (2 * BN + BM) * 4 + 2 * (kMaxE + 1) * 4 <= 160 * 1024, "LDS, most experts");
   __shared__ __attribute__((aligned(1024))) uint8_t sP[S][BM * RB];
   __shared__ __attribute__((aligned(1024))) uint8_t sQ[S][BN * RB];
   __shared__ int4 s_list[kTileList];  // this workgroup's first tiles: first row, end of its rows, expert, column tile
