@@ -160,7 +160,9 @@ __global__ __launch_bounds__(256) void quant_kernel(const T* __restrict__ x, int
 __device__ __forceinline__ float element(const uint16_t* p) { return bf2f(*p); }
 __device__ __forceinline__ float element(const float* p) { return *p; }
 
-// Rows whose pieces of eight are not aligned: an element at a time, a wave a row.
+// Rows whose pieces of eight are not aligned: an element at a time, a wave a row, read twice. Far from HBM's
+// rate with 2 or 4 bytes a lane and load: 16384 x 2303 54 us from bf16 and 57 from fp32, where 2304 columns
+// take 19 and 28; 131072 x 2303 568 and 625 (162 and 277); 64 x 8001 35 us, a wave's 126 steps twice.
 template <typename T>
 __global__ __launch_bounds__(256) void quant_any_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int cols,
                                                         int8_t* __restrict__ q, float* __restrict__ scale) {
@@ -180,7 +182,8 @@ __device__ __forceinline__ void put(uint16_t* p, float v) { *p = (uint16_t)f2bf(
 __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 
 // Codes back to values: a wave a row, in pieces of eight where they are aligned. Bound by HBM:
-// 131072 x 2304 to bf16 145 us, 6.2 TB/s.
+// 131072 x 2304 to bf16 145 us, 6.2 TB/s; to fp32 386, 3.9 (16384 rows of it 29 us, 6.5). By elements 131072 x
+// 2303 312 and 521 us, 16384 x 2303 22 and 33.
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void dequant_kernel(const int8_t* __restrict__ q, const float* __restrict__ scale,
                                                       int64_t rows, int cols, T* __restrict__ x) {
@@ -704,7 +707,7 @@ __global__ __launch_bounds__(512, 4) void narrow_kernel(Params p) {
   struct Cols { float a[4], b[4], ba[4], bb[4]; };  // scales (of gate and up) and biases
   auto first_col = [&](const Unit& u) { return (u.cb * NB + fb) * COLS + 4 * fc; };
   auto load_cols = [&](Cols& c, const Unit& u) {
-    if (fb >= NB) return;  // (whole waves)
+    if (fb >= NB) return;  // (whole waves, but for gate and up with one block of each: half of the first)
     const int n = min(first_col(u), N - 1);
     col_scales(p.sa, p, u.e, n, c.a);
     if (MODE == kGateUp) col_scales(p.sb, p, u.e, n, c.b);
@@ -996,10 +999,11 @@ static void launch_narrow(const Params& p, hipStream_t stream) {
 // rows leave a CU one workgroup, half the rows and a fifth of the bytes. us, narrow / wide with its
 // quantization: 16 rows of 7168 x 2048 17.3 / 18.1, 48 rows 34 / 20; 96 rows of 2304 x 2304 11.5 / 11.4;
 // 16 8.2 / 10.2; 32 of 2880 x 2880 13.2 / 12.2, 16 9.0 / 11.5 (a wide call, of two launches, takes the host 4 us
-// more); one of 7168 x 7168 19.8 / 21.8, four 22.1 / 22.1, seven 28.6 / 22.1; on 32 experts of 2880 x 2880 64 rows
-// 48.8 / 51.9, 256 58.1 / 57.4, of 5760 x 2880 8 rows 26.9 / 31.8, 128 112 / 101; on 64 of 2304 x 2048 64 rows 45.6 /
-// 47.5, 256 62.9 / 57.2; on 256 of it 8 10.7 / 12.5, 64 47 / 51, 256 142 / 140; on 256 of 1024 x 2304 64 27 / 30, 256
-// 78 / 74; on 32 of 7168 x 4096 8 rows 57 / 38.
+// more); past 16 rows, weights from memory: 24 rows of 7168 x 2048 16.6 / 19.0, 32 17.5 / 19.0, 40 27.5 / 19.9; 24 of
+// 2880 x 2880 10.4 / 11.6, 32 12.7 / 11.8; 32 of 2304 x 2304 10.3 / 10.4; one of 7168 x 7168 19.8 / 21.8, four 22.1 /
+// 22.1, seven 28.6 / 22.1; on 32 experts of 2880 x 2880 64 rows 48.8 / 51.9, 256 58.1 / 57.4, of 5760 x 2880 8 rows
+// 26.9 / 31.8, 128 112 / 101; on 64 of 2304 x 2048 64 rows 45.6 / 47.5, 256 62.9 / 57.2; on 256 of it 8 10.7 / 12.5, 64
+// 47 / 51, 256 142 / 140; on 256 of 1024 x 2304 64 27 / 30, 256 78 / 74; on 32 of 7168 x 4096 8 rows 57 / 38.
 static bool takes_narrow(int64_t R, int64_t E, int K, int64_t cols) {
   const int tm = narrow_blocks(R, E, K);
   if (!tm) return false;
