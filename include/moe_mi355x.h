@@ -702,7 +702,7 @@ int moe_mxfp4_gemm_down(const uint8_t* qh, const uint8_t* sh, const uint8_t* qw2
 /* x [rows, cols] (dtype MOE_DTYPE_BF16 or MOE_DTYPE_FP32), rows ld >= cols elements
  * apart -> q [rows, cols], scale [rows], and back (x [rows, cols] in dtype). Any cols
  * and alignment; 16-byte aligned rows of a multiple of 8 columns are read in wide
- * pieces, others an element at a time, which takes two to four times as long. */
+ * pieces, others an element at a time, which takes up to four times as long. */
 int moe_int8_quant_rows(const void* x, int64_t ld, int64_t rows, int32_t cols, int32_t dtype, int8_t* q, float* scale,
                         moe_stream_t stream);
 int moe_int8_dequant_rows(const int8_t* q, const float* scale, int64_t rows, int32_t cols, int32_t dtype, void* x,
